@@ -266,7 +266,9 @@ def _calls(s):
             return P.ragged_fwd(s["q"], s["k"], s["v"], s["cu_q"], s["cu_k"], causal=s["causal"])
         out = P.attention_ragged(s["q"], s["k"], s["v"], s["cu_q"], s["cu_k"], causal=s["causal"])
         return (out.detach(), *torch.autograd.grad(out, (s["q"], s["k"], s["v"]), s["do"]))
-    cache = P.KVCache(*s["parts"])
+    cache = s.get("cache")
+    if cache is None:           # (a program makes it once)
+        cache = s["cache"] = P.KVCache(*s["parts"])
     if s["op"] == "decode":
         if s["write"]:
             P.cache_write(cache, *s["fresh"], s["table"], s["lens"])
