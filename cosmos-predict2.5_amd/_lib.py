@@ -245,6 +245,49 @@ class GemmDesc(ctypes.Structure):
     ]
 
 
+class RaggedDesc(ctypes.Structure):
+    """Mirror of ``struct cosmos_attn_ragged_desc``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("n_seq", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("causal", ctypes.c_int32), ("fill", ctypes.c_int32),
+        ("Tq", ctypes.c_int64), ("Tk", ctypes.c_int64),
+        ("sm_scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p),
+        ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("dout", ctypes.c_void_p), ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 2), ("k_stride", ctypes.c_int64 * 2), ("v_stride", ctypes.c_int64 * 2), ("o_stride", ctypes.c_int64 * 2),
+        ("dout_stride", ctypes.c_int64 * 2), ("dq_stride", ctypes.c_int64 * 2), ("dk_stride", ctypes.c_int64 * 2), ("dv_stride", ctypes.c_int64 * 2),
+    ]
+
+
+class CacheDesc(ctypes.Structure):
+    """Mirror of ``struct cosmos_attn_cache_desc``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32), ("dtype", ctypes.c_int32), ("kind", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("pages", ctypes.c_int64),
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("k_scale_stride", ctypes.c_int64 * 2), ("v_scale_stride", ctypes.c_int64 * 2),
+        ("B", ctypes.c_int32), ("width", ctypes.c_int32),
+        ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("lens", ctypes.c_void_p), ("cu", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("k_rows", ctypes.c_void_p), ("v_rows", ctypes.c_void_p),
+        ("k_rows_stride", ctypes.c_int64 * 2), ("v_rows_stride", ctypes.c_int64 * 2),
+        ("fill", ctypes.c_int32), ("Hq", ctypes.c_int32), ("sm_scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("o", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 2), ("o_stride", ctypes.c_int64 * 2),
+        ("lse", ctypes.c_void_p),
+    ]
+
+
+CACHE_SAME, CACHE_E4M3, CACHE_INT8 = 0, 1, 2
 GEMM_XWT, GEMM_XW, GEMM_XTX = 0, 1, 2
 GEMM_SUM = 1
 
@@ -279,6 +322,14 @@ EXPORTS = {
     "cosmos_attn_gemm": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),               # (a descriptor, also as packed bytes)
     "cosmos_attn_gemm_preferred": (ctypes.c_int, [ctypes.c_void_p]),                      # (as well)
     "cosmos_gelu": (ctypes.c_int, [ctypes.POINTER(GeluDesc), ctypes.c_void_p]),
+    # (descriptors, also as packed bytes)
+    "cosmos_attn_ragged": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "cosmos_attn_ragged_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "cosmos_attn_ragged_bwd": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "cosmos_attn_cache_write": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "cosmos_attn_cache_read": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "cosmos_attn_cache_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "cosmos_attn_cache_attention": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,705 @@
+// Attention over packed sequences of different lengths with grouped heads, forward and backward, for gfx950: kernels and C ABI (cosmos_attn_ragged, cosmos_attn_ragged_bwd).
+//
+// Sequence i has the rows cu_q[i] .. cu_q[i + 1] - 1 of q and the rows cu_k[i] .. of k and v.  With c the scale, t and j counted from the sequence's start, Lq and Lk its lengths:
+//     s_tj = c q_t k_j,   visible: j <= t + Lk - Lq (causal, aligned at the ends) or all,   p = exp(s - lse),   o_t = sum_j p_tj v_j,   lse_t = log sum_j exp(s_tj)
+//     dp_tj = do_t v_j,   delta_t = sum_d do_t o_t,   ds = p (dp - delta),   dq_t = c sum_j ds_tj k_j,   dk_j = c sum_t ds_tj q_t,   dv_j = sum_t p_tj do_t
+// A row that sees no key: o = 0, lse = -inf, no gradient.
+//
+// Grouped heads.  The `group` query heads of a key head are rows of one matrix: row r of sequence i and key head h is token r / group, query head h group + r % group.  A tile of
+// rows then shares K and V among the heads, few tokens still fill a tile, a causal tile's diagonal is `group` times shorter, and the sums over the group that dk and dv need
+// are part of the contraction over rows.
+//
+// Who does what.  Lengths stay on the device: the grid is what the tensors' row counts allow at most, and every workgroup finds its sequence by a scan over the offsets
+// (64 sequences a step, each wavefront for itself).  No work list, no copy to the host, nothing to prepare, and a captured call follows its offsets.
+//
+// Offsets are not trusted: a sequence whose offsets do not ascend within the tensors has no rows; one whose keys' offsets do not has rows of NaN (no gradients: zeros).
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+#include <math.h>
+#include <mutex>
+#include <set>
+#include <utility>
+
+#include "cosmos_attn_hip.h"
+
+namespace {
+
+#include "attn_common_gfx950.h"
+
+constexpr int kThreads = 256;      // four wavefronts of 32 rows (or keys) each
+constexpr int kRows = 128;         // of a workgroup
+constexpr int kStep = 64;          // keys (or rows) that are in LDS at a time, twice
+
+struct RaggedParams {
+    const char *q, *k, *v, *o_in, *dout;
+    char *o, *dq, *dk, *dv;
+    float* lse;                    // [Hq, Tq]; written by the forward (may be null), read by the backward
+    float* delta;                  // [Hq, Tq]: of the backward's first kernel for its second
+    const int *cu_q, *cu_k;
+    // bytes between rows and between heads
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+    int n_seq, Tq, Tk, Hkv, group, causal, fill;
+    float scale, scale_log2;       // scale_log2 >= 0: `flip` says that q's signs are turned instead
+    unsigned flip;
+};
+
+// ---- a tile in LDS: kStep rows of D 16-bit elements, as chunks of 16 bytes.  Chunk c of row r lies at c XOR mix(r): what a wavefront reads at once, 16 bytes of each of 32 rows (a fragment
+// with lane = row) or, transposing, 64 bytes of each of 8 rows, then lies in different banks, and a load to LDS still takes whole rows.
+template <int D> struct Tile {
+    static constexpr int ROW = 2 * D, BYTES = kStep * ROW, CHUNKS = D / 8, ROWS_PER_LOAD = 1024 / ROW, LOADS = kStep / 4 / ROWS_PER_LOAD;
+    static __device__ __forceinline__ int mix(int r) { return D == 128 ? 4 * (r & 3) | ((r >> 2) & 3) : 4 * ((r >> 1) & 1) | ((r >> 2) & 3); }
+    // where lane reads chunk 2 c + lane / 32 of row lane % 32
+    static __device__ __forceinline__ int at(int lane, int c) { return (lane & 31) * ROW + ((((2 * c) | (lane >> 5)) ^ mix(lane & 31)) << 4); }
+    // where lane passes the address for channels 32 db .. + 31, rows 4 (lane / 32) .. + 3 + 8 s, transposing
+    static __device__ __forceinline__ int at_transposed(int lane, int db, int s) {
+        const int row = 8 * s + 4 * (lane >> 5) + ((lane & 15) >> 2), chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        return row * ROW + ((chunk ^ mix(row)) << 4) + 8 * (lane & 1);
+    }
+    // the row (of the tile) and the byte in that row that this lane loads with load i of wavefront `wave`
+    static __device__ __forceinline__ int load_row(int lane, int wave, int i) { return 16 * wave + i * ROWS_PER_LOAD + lane / CHUNKS; }
+    static __device__ __forceinline__ int load_byte(int lane, int wave, int i) { return ((lane % CHUNKS) ^ mix(load_row(lane, wave, i))) << 4; }
+    static __device__ __forceinline__ int load_to(int wave, int i) { return (16 * wave + i * ROWS_PER_LOAD) * ROW; }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, char* dst, int offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)dst, 16, offset, 0, 0, 0);
+}
+template <typename V8> __device__ __forceinline__ V8 read_rows(const char* part, int at) { return *reinterpret_cast<const V8*>(part + at); }
+// the 16 rows 16 c .. + 15 of 32 channels as an operand with lane = channel: slot s of a lane is row 16 c + 8 (s / 4) + 4 (lane / 32) + s % 4, the order of a product's result registers
+template <typename V8> __device__ __forceinline__ V8 read_channels(const char* part, int at0, int at1) {
+    typedef __attribute__((address_space(3))) s16x4* P;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(part + at0)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(part + at1));
+    return __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+// all loads to LDS have landed and all reads have returned; then the workgroup meets
+__device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// `rows_left` rows from `at` on (at most kStep are read), what lies behind them reads as zeros
+template <int D> __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char* at, int64_t row_bytes, int rows_left) {
+    const int rows = rows_left < kStep ? rows_left : kStep;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, rows > 0 ? (int)((rows - 1) * row_bytes) + 2 * D : 0, 0x00020000);
+}
+template <typename T> __device__ __forceinline__ unsigned round2(float a, float b) {
+    typedef T V2 __attribute__((ext_vector_type(2)));
+    const V2 two = {(T)a, (T)b};
+    return __builtin_bit_cast(unsigned, two);
+}
+__device__ __forceinline__ float over_halves_sum(float x) { float lo, hi; both_halves(x, lo, hi); return lo + hi; }
+__device__ __forceinline__ float over_halves_max(float x) { float lo, hi; both_halves(x, lo, hi); return fmaxf(lo, hi); }
+
+// ---- which sequence
+struct Range { int start, length; };
+__device__ __forceinline__ Range range_of(const int* cu, int i, int total) {
+    const int a = cu[i], b = cu[i + 1];
+    return a >= 0 && a <= b && b <= total ? Range{a, b - a} : Range{0, -1};
+}
+struct Found { int seq, tile, of; };     // seq < 0: behind the last tile, `tile` of them
+// Tile `index` of the sequences' tiles of `rows` of length x `group`, in the sequences' order.
+__device__ __forceinline__ Found find(const int* cu, int n, int total, int group, int rows, int index) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int base = 0; base < n; base += 64) {
+        const int i = base + lane;
+        int tiles = 0;
+        if (i < n) {
+            const Range r = range_of(cu, i, total);
+            tiles = r.length > 0 ? (int)(((int64_t)r.length * group + rows - 1) / rows) : 0;
+        }
+        int sum = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) { const int up = __shfl_up(sum, d); sum += lane >= d ? up : 0; }
+        const unsigned long long past = __ballot(before + sum > index);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            const int ends = __builtin_amdgcn_readlane(sum, at), of = __builtin_amdgcn_readlane(tiles, at);
+            return {base + at, index - (before + ends - of), of};
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return {-1, index - before, 0};
+}
+
+// ---- rows of no sequence: zeros, lse = -inf
+template <int D> __device__ __forceinline__ void clear_rows(char* out, int64_t row, int64_t head, const int* cu, int n, int total, int heads, int first_head, int rows, int tile, float* lse) {
+    int lead = cu[0], from = cu[n];
+    lead = lead < 0 ? 0 : lead > total ? total : lead;
+    from = from < lead ? lead : from > total ? total : from;
+    const int64_t count = (int64_t)(lead + total - from) * heads;
+    constexpr int CHUNKS = D / 8;
+    for (int i = threadIdx.x; i < rows * CHUNKS; i += kThreads) {
+        const int64_t r = (int64_t)tile * rows + i / CHUNKS;
+        if (r >= count) continue;
+        int t = (int)(r / heads);
+        const int h = first_head + (int)(r % heads);
+        t = t < lead ? t : from + (t - lead);
+        *reinterpret_cast<u32x4*>(out + t * row + h * head + 16 * (i % CHUNKS)) = u32x4{0, 0, 0, 0};
+        if (lse && i % CHUNKS == 0) lse[(int64_t)h * total + t] = -INFINITY;
+    }
+}
+
+constexpr float kLowest = -3.0e38f;      // a max that no score has moved yet: exponentials of masked scores stay 0 and those of the sums so far too
+
+// ---- forward.  A workgroup: kRows rows of one sequence and key head; a wavefront 32 of them, one a lane and its other half: S^T = K Q^T has the keys in registers, so that the softmax
+// needs one exchange between the halves, and P^T, rounded, is the next product's operand where it lies.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef typename VecOf<T>::v8 V8;
+    typedef Tile<D> L;
+    constexpr int NC = D / 16, NB = D / 32;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int head = blockIdx.x % p.Hkv;
+    const Found f = find(p.cu_q, p.n_seq, p.Tq, p.group, kRows, blockIdx.x / p.Hkv);
+    if (f.seq < 0) {
+        if (p.fill) clear_rows<D>(p.o, p.o_row, p.o_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f.tile, p.lse);
+        return;
+    }
+    const int tile = f.of - 1 - f.tile;             // (causal: the longest first)
+    const Range rq = range_of(p.cu_q, f.seq, p.Tq), rk = range_of(p.cu_k, f.seq, p.Tk);
+    const int rows = rq.length * p.group, lk = rk.length > 0 ? rk.length : 0, shift = lk - rq.length;
+    const int row = tile * kRows + 32 * wave + (lane & 31);
+    const bool live = row < rows;
+    const int token = row / p.group, hq = head * p.group + (row - token * p.group);
+    // keys that this lane's row sees, the most of this wavefront's and of the workgroup's rows, the fewest of this wavefront's
+    auto keys_of = [&](int t) { const int e = t + shift + 1; return !p.causal || e > lk ? lk : e < 0 ? 0 : e; };
+    const int end = live ? keys_of(token) : 0;
+    const int first = tile * kRows + 32 * wave;
+    auto token_at = [&](int r) { return __builtin_amdgcn_readfirstlane((r < rows ? r : rows - 1) / p.group); };
+    const int wave_end = first < rows ? keys_of(token_at(first + 31)) : 0, wave_all = keys_of(token_at(first));
+    const int n = (keys_of(token_at(tile * kRows + kRows - 1)) + kStep - 1) / kStep;
+
+    const char* const kp = p.k + rk.start * p.k_row + head * p.k_head;
+    const char* const vp = p.v + rk.start * p.v_row + head * p.v_head;
+    int k_off[L::LOADS], v_off[L::LOADS];
+#pragma unroll
+    for (int i = 0; i < L::LOADS; ++i) {
+        k_off[i] = L::load_row(lane, wave, i) * (int)p.k_row + L::load_byte(lane, wave, i);
+        v_off[i] = L::load_row(lane, wave, i) * (int)p.v_row + L::load_byte(lane, wave, i);
+    }
+    auto fill = [&](int t) {
+        const auto kr = rows_of<D>(kp + (int64_t)t * kStep * p.k_row, p.k_row, lk - t * kStep), vr = rows_of<D>(vp + (int64_t)t * kStep * p.v_row, p.v_row, lk - t * kStep);
+        char* const to = smem + (t & 1) * 2 * L::BYTES;
+#pragma unroll
+        for (int i = 0; i < L::LOADS; ++i) load_to_lds(kr, to + L::load_to(wave, i), k_off[i]);
+#pragma unroll
+        for (int i = 0; i < L::LOADS; ++i) load_to_lds(vr, to + L::BYTES + L::load_to(wave, i), v_off[i]);
+    };
+    if (n > 0) fill(0);
+
+    // Q as an operand: channels 16 c + 8 half .. + 7 of this lane's row
+    V8 qf[NC];
+    {
+        const char* const at = p.q + (rq.start + token) * p.q_row + hq * p.q_head + 16 * half;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            u32x4 w = {0, 0, 0, 0};
+            if (live) w = *reinterpret_cast<const u32x4*>(at + 32 * c);
+            w ^= p.flip;
+            qf[c] = __builtin_bit_cast(V8, w);
+        }
+    }
+    int k_at[NC], v_at[NB][2];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) k_at[c] = L::at(lane, c);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) { v_at[b][0] = L::at_transposed(lane, b, 0); v_at[b][1] = L::at_transposed(lane, b, 1); }
+
+    f32x16 acc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
+    float m = kLowest, l = 0.f;       // (l: of this lane's half of the keys)
+
+    for (int t = 0; t < n; ++t) {
+        meet();
+        if (t + 1 < n) fill(t + 1);
+        const int key0 = t * kStep;
+        if (key0 >= wave_end) continue;
+        const char* const kt = smem + (t & 1) * 2 * L::BYTES;
+        const char* const vt = kt + L::BYTES;
+        f32x16 s[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) s[h] = mfma32(read_rows<V8>(kt + 32 * h * L::ROW, k_at[c]), qf[c], s[h]);
+        if (key0 + kStep > wave_all) {          // (some row of the wavefront does not see all of these keys)
+            const int left = end - key0 - 4 * half;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[h][e] = 32 * h + 8 * (e >> 2) + (e & 3) < left ? s[h][e] : -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[h][e]);
+        top = over_halves_max(top) * p.scale_log2;
+        if (__any(top > m + kMaxSlack)) {
+            const float to = fmaxf(m, top), by = __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= by;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[b] *= by;
+        }
+        V8 pf[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                u32x4 w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 8 * c + 2 * i;
+                    const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][e], p.scale_log2, -m)), b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][e + 1], p.scale_log2, -m));
+                    l += a;
+                    l += b;
+                    w[i] = round2<T>(a, b);
+                }
+                pf[2 * h + c] = __builtin_bit_cast(V8, w);
+            }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[b] = mfma32(read_channels<V8>(vt + 16 * c * L::ROW, v_at[b][0], v_at[b][1]), pf[c], acc[b]);
+    }
+    if (!live) return;
+    l = over_halves_sum(l);
+    float by = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    float lse = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * 0.693147180559945309f : l == 0.f ? -INFINITY : l;
+    if (rk.length < 0) by = lse = NAN;
+    char* const at = p.o + (rq.start + token) * p.o_row + hq * p.o_head + 8 * half;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<u32x2*>(at + 64 * b + 16 * i) = u32x2{round2<T>(acc[b][4 * i] * by, acc[b][4 * i + 1] * by), round2<T>(acc[b][4 * i + 2] * by, acc[b][4 * i + 3] * by)};
+    if (p.lse && half == 0) p.lse[(int64_t)hq * p.Tq + rq.start + token] = lse;
+#endif
+}
+
+// ---- backward, first kernel: delta and dq.  The forward's rows and tiles, with P from lse, dP^T = V dO^T beside S^T, and dQ^T = K^T dS^T.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef typename VecOf<T>::v8 V8;
+    typedef Tile<D> L;
+    constexpr int NC = D / 16, NB = D / 32;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int head = blockIdx.x % p.Hkv;
+    const Found f = find(p.cu_q, p.n_seq, p.Tq, p.group, kRows, blockIdx.x / p.Hkv);
+    if (f.seq < 0) {
+        clear_rows<D>(p.dq, p.dq_row, p.dq_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f.tile, nullptr);
+        return;
+    }
+    const int tile = f.of - 1 - f.tile;
+    const Range rq = range_of(p.cu_q, f.seq, p.Tq), rk = range_of(p.cu_k, f.seq, p.Tk);
+    const int rows = rq.length * p.group, lk = rk.length > 0 ? rk.length : 0, shift = lk - rq.length;
+    const int row = tile * kRows + 32 * wave + (lane & 31);
+    const bool live = row < rows;
+    const int token = row / p.group, hq = head * p.group + (row - token * p.group);
+    auto keys_of = [&](int t) { const int e = t + shift + 1; return !p.causal || e > lk ? lk : e < 0 ? 0 : e; };
+    const int end = live ? keys_of(token) : 0;
+    const int first = tile * kRows + 32 * wave;
+    auto token_at = [&](int r) { return __builtin_amdgcn_readfirstlane((r < rows ? r : rows - 1) / p.group); };
+    const int wave_end = first < rows ? keys_of(token_at(first + 31)) : 0, wave_all = keys_of(token_at(first));
+    const int n = (keys_of(token_at(tile * kRows + kRows - 1)) + kStep - 1) / kStep;
+
+    const char* const kp = p.k + rk.start * p.k_row + head * p.k_head;
+    const char* const vp = p.v + rk.start * p.v_row + head * p.v_head;
+    int k_off[L::LOADS], v_off[L::LOADS];
+#pragma unroll
+    for (int i = 0; i < L::LOADS; ++i) {
+        k_off[i] = L::load_row(lane, wave, i) * (int)p.k_row + L::load_byte(lane, wave, i);
+        v_off[i] = L::load_row(lane, wave, i) * (int)p.v_row + L::load_byte(lane, wave, i);
+    }
+    auto fill = [&](int t) {
+        const auto kr = rows_of<D>(kp + (int64_t)t * kStep * p.k_row, p.k_row, lk - t * kStep), vr = rows_of<D>(vp + (int64_t)t * kStep * p.v_row, p.v_row, lk - t * kStep);
+        char* const to = smem + (t & 1) * 2 * L::BYTES;
+#pragma unroll
+        for (int i = 0; i < L::LOADS; ++i) load_to_lds(kr, to + L::load_to(wave, i), k_off[i]);
+#pragma unroll
+        for (int i = 0; i < L::LOADS; ++i) load_to_lds(vr, to + L::BYTES + L::load_to(wave, i), v_off[i]);
+    };
+    if (n > 0) fill(0);
+
+    V8 qf[NC], gf[NC];
+    float delta = 0.f;
+    {
+        const char* const qa = p.q + (rq.start + token) * p.q_row + hq * p.q_head + 16 * half;
+        const char* const ga = p.dout + (rq.start + token) * p.do_row + hq * p.do_head + 16 * half;
+        const char* const oa = p.o_in + (rq.start + token) * p.o_row + hq * p.o_head + 16 * half;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            u32x4 a = {0, 0, 0, 0}, b = a, o = a;
+            if (live) {
+                a = *reinterpret_cast<const u32x4*>(qa + 32 * c);
+                b = *reinterpret_cast<const u32x4*>(ga + 32 * c);
+                o = *reinterpret_cast<const u32x4*>(oa + 32 * c);
+            }
+            a ^= p.flip;
+            qf[c] = __builtin_bit_cast(V8, a);
+            gf[c] = __builtin_bit_cast(V8, b);
+            const V8 of = __builtin_bit_cast(V8, o);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)gf[c][i], (float)of[i], delta);
+        }
+        delta = over_halves_sum(delta);
+    }
+    const int64_t stat = (int64_t)hq * p.Tq + rq.start + token;
+    float lse2 = INFINITY;            // (P = 0 where there is no row, or nothing that it sees)
+    if (live) {
+        const float x = p.lse[stat];
+        lse2 = x == -INFINITY ? INFINITY : x * 1.44269504088896341f;
+        if (half == 0) p.delta[stat] = delta;
+    }
+    int k_at[NC], k_tr[NB][2];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) k_at[c] = L::at(lane, c);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) { k_tr[b][0] = L::at_transposed(lane, b, 0); k_tr[b][1] = L::at_transposed(lane, b, 1); }
+    f32x16 acc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
+
+    for (int t = 0; t < n; ++t) {
+        meet();
+        if (t + 1 < n) fill(t + 1);
+        const int key0 = t * kStep;
+        if (key0 >= wave_end) continue;
+        const char* const kt = smem + (t & 1) * 2 * L::BYTES;
+        const char* const vt = kt + L::BYTES;
+        const bool masked = key0 + kStep > wave_all;
+        const int left = end - key0 - 4 * half;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            f32x16 s = f32x16{}, g = f32x16{};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s = mfma32(read_rows<V8>(kt + 32 * h * L::ROW, k_at[c]), qf[c], s);
+                g = mfma32(read_rows<V8>(vt + 32 * h * L::ROW, k_at[c]), gf[c], g);
+            }
+            V8 df[2];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], p.scale_log2, -lse2));
+                s[e] = pe * (g[e] - delta);
+            }
+            if (masked)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = 32 * h + 8 * (e >> 2) + (e & 3) < left ? s[e] : 0.f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                u32x4 w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = round2<T>(s[8 * c + 2 * i], s[8 * c + 2 * i + 1]);
+                df[c] = __builtin_bit_cast(V8, w);
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) acc[b] = mfma32(read_channels<V8>(kt + (32 * h + 16 * c) * L::ROW, k_tr[b][0], k_tr[b][1]), df[c], acc[b]);
+        }
+    }
+    if (!live) return;
+    const float by = p.scale;
+    char* const at = p.dq + (rq.start + token) * p.dq_row + hq * p.dq_head + 8 * half;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<u32x2*>(at + 64 * b + 16 * i) = u32x2{round2<T>(acc[b][4 * i] * by, acc[b][4 * i + 1] * by), round2<T>(acc[b][4 * i + 2] * by, acc[b][4 * i + 3] * by)};
+#endif
+}
+
+// ---- backward, second kernel: dk and dv.  A workgroup: 128 keys of one sequence and key head, a wavefront 32 of them, one a lane; the sequence's rows (of all heads of the group) go by in
+// steps of kStep.  S = Q K^T has the rows in registers: P and dS, rounded, are operands of dV^T += dO^T P and dK^T += Q^T dS where they lie.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, D == 128 ? 1 : 2) ragged_dkdv_kernel(const RaggedParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef typename VecOf<T>::v8 V8;
+    typedef Tile<D> L;
+    constexpr int NC = D / 16, NB = D / 32;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    float* const stats = reinterpret_cast<float*>(smem + 4 * L::BYTES);       // [2][lse, delta][kStep]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int head = blockIdx.x % p.Hkv;
+    const Found f = find(p.cu_k, p.n_seq, p.Tk, 1, kRows, blockIdx.x / p.Hkv);
+    if (f.seq < 0) {
+        clear_rows<D>(p.dk, p.dk_row, p.dk_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f.tile, nullptr);
+        clear_rows<D>(p.dv, p.dv_row, p.dv_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f.tile, nullptr);
+        return;
+    }
+    const Range rq = range_of(p.cu_q, f.seq, p.Tq), rk = range_of(p.cu_k, f.seq, p.Tk);
+    const int lq = rq.length > 0 ? rq.length : 0, rows = lq * p.group, shift = rk.length - lq;
+    const int key = f.tile * kRows + 32 * wave + (lane & 31);
+    const bool live = key < rk.length;
+    // the first row that sees a key
+    auto first_of = [&](int j) { const int t = j - shift; return !p.causal || t <= 0 ? 0 : t >= lq ? rows : t * p.group; };
+    const int from = first_of(key);
+    const int wave_first = __builtin_amdgcn_readfirstlane(first_of(f.tile * kRows + 32 * wave)), wave_all = __builtin_amdgcn_readfirstlane(first_of(f.tile * kRows + 32 * wave + 31));
+    const int t0 = __builtin_amdgcn_readfirstlane(first_of(f.tile * kRows)) / kStep, n = (rows + kStep - 1) / kStep;
+
+    V8 kf[NC], vf[NC];
+    {
+        const char* const ka = p.k + (rk.start + (live ? key : 0)) * p.k_row + head * p.k_head + 16 * half;
+        const char* const va = p.v + (rk.start + (live ? key : 0)) * p.v_row + head * p.v_head + 16 * half;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            kf[c] = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(ka + 32 * c) ^ p.flip);
+            vf[c] = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(va + 32 * c));
+        }
+    }
+    // this lane's row of each load: the token in the step's first, and the head; both go on by kStep rows a step
+    const int step_tokens = kStep / p.group, step_heads = kStep - step_tokens * p.group;
+    int token[L::LOADS], hd[L::LOADS], byte[L::LOADS];
+#pragma unroll
+    for (int i = 0; i < L::LOADS; ++i) {
+        const int r = t0 * kStep + L::load_row(lane, wave, i);
+        token[i] = r / p.group;
+        hd[i] = r - token[i] * p.group;
+        byte[i] = L::load_byte(lane, wave, i);
+    }
+    const int stat_row = threadIdx.x & (kStep - 1);
+    int stat_token = (t0 * kStep + stat_row) / p.group, stat_head = t0 * kStep + stat_row - stat_token * p.group;
+    float stat = 0.f;
+    const char* const qp = p.q + rq.start * p.q_row + (int64_t)head * p.group * p.q_head;
+    const char* const gp = p.dout + rq.start * p.do_row + (int64_t)head * p.group * p.do_head;
+    auto next = [&](int& t, int& h) { t += step_tokens; h += step_heads; const bool over = h >= p.group; t += over; h -= over ? p.group : 0; };
+    auto fill = [&](int t) {
+        const int base = t * kStep / p.group;      // (uniform) token that offsets are counted from
+        const auto qr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(qp + base * p.q_row), 0, 0x7FFFFFFF, 0x00020000);
+        const auto gr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(gp + base * p.do_row), 0, 0x7FFFFFFF, 0x00020000);
+        char* const to = smem + (t & 1) * 2 * L::BYTES;
+#pragma unroll
+        for (int i = 0; i < L::LOADS; ++i) {
+            const bool in = token[i] < lq;
+            load_to_lds(qr, to + L::load_to(wave, i), in ? (token[i] - base) * (int)p.q_row + hd[i] * (int)p.q_head + byte[i] : (int)0x80000000);
+            load_to_lds(gr, to + L::BYTES + L::load_to(wave, i), in ? (token[i] - base) * (int)p.do_row + hd[i] * (int)p.do_head + byte[i] : (int)0x80000000);
+            next(token[i], hd[i]);
+        }
+        if (threadIdx.x < 2 * kStep) {             // lse (threads 0 ..) and delta (threads kStep ..) of the step's rows
+            const bool in = stat_token < lq;
+            const float* const of = threadIdx.x < kStep ? p.lse : p.delta;
+            stat = threadIdx.x < kStep ? -INFINITY : 0.f;
+            if (in) stat = of[(int64_t)(head * p.group + stat_head) * p.Tq + rq.start + stat_token];
+            next(stat_token, stat_head);
+        }
+    };
+    int q_at[NC], q_tr[NB][2];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) q_at[c] = L::at(lane, c);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) { q_tr[b][0] = L::at_transposed(lane, b, 0); q_tr[b][1] = L::at_transposed(lane, b, 1); }
+    f32x16 dk[NB], dv[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) dk[b] = dv[b] = f32x16{};
+
+    if (t0 < n) fill(t0);
+    for (int t = t0; t < n; ++t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // (P = 0 where there is no row, or nothing that it sees)
+        if (threadIdx.x < 2 * kStep) stats[(t & 1) * 2 * kStep + threadIdx.x] = threadIdx.x >= kStep ? stat : stat == -INFINITY ? INFINITY : stat * 1.44269504088896341f;
+        meet();
+        if (t + 1 < n) fill(t + 1);
+        const int row0 = t * kStep;
+        if (row0 + kStep <= wave_first) continue;
+        const char* const qt = smem + (t & 1) * 2 * L::BYTES;
+        const char* const gt = qt + L::BYTES;
+        const float* const st = stats + (t & 1) * 2 * kStep;
+        const bool masked = row0 < wave_all;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            f32x16 s = f32x16{}, g = f32x16{};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s = mfma32(read_rows<V8>(qt + 32 * h * L::ROW, q_at[c]), kf[c], s);
+                g = mfma32(read_rows<V8>(gt + 32 * h * L::ROW, q_at[c]), vf[c], g);
+            }
+            // element e: row 8 (e / 4) + 4 half + e % 4
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 32 * h + 8 * i + 4 * half), delta = *reinterpret_cast<const f32x4*>(st + kStep + 32 * h + 8 * i + 4 * half);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[4 * i + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + j], p.scale_log2, -lse[j]));
+                    g[4 * i + j] -= delta[j];
+                }
+            }
+            if (masked) {
+                const int left = from - row0 - 32 * h - 4 * half;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) >= left ? s[e] : 0.f;
+            }
+            V8 pf[2], df[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                u32x4 w, x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 8 * c + 2 * i;
+                    w[i] = round2<T>(s[e], s[e + 1]);
+                    x[i] = round2<T>(s[e] * g[e], s[e + 1] * g[e + 1]);
+                }
+                pf[c] = __builtin_bit_cast(V8, w);
+                df[c] = __builtin_bit_cast(V8, x);
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    dv[b] = mfma32(read_channels<V8>(gt + (32 * h + 16 * c) * L::ROW, q_tr[b][0], q_tr[b][1]), pf[c], dv[b]);
+                    dk[b] = mfma32(read_channels<V8>(qt + (32 * h + 16 * c) * L::ROW, q_tr[b][0], q_tr[b][1]), df[c], dk[b]);
+                }
+        }
+    }
+    if (!live) return;
+    char* const ka = p.dk + (rk.start + key) * p.dk_row + head * p.dk_head + 8 * half;
+    char* const va = p.dv + (rk.start + key) * p.dv_row + head * p.dv_head + 8 * half;
+    const float by = p.scale;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            *reinterpret_cast<u32x2*>(ka + 64 * b + 16 * i) = u32x2{round2<T>(dk[b][4 * i] * by, dk[b][4 * i + 1] * by), round2<T>(dk[b][4 * i + 2] * by, dk[b][4 * i + 3] * by)};
+            *reinterpret_cast<u32x2*>(va + 64 * b + 16 * i) = u32x2{round2<T>(dv[b][4 * i], dv[b][4 * i + 1]), round2<T>(dv[b][4 * i + 2], dv[b][4 * i + 3])};
+        }
+#endif
+}
+
+// ---- C ABI
+constexpr int64_t kMost = 0x7FFFFFFF;
+// rows of a step and a token's heads are addressed with 32 bits
+constexpr int64_t kMostRowBytes = (int64_t)1 << 23;
+
+int check_tensor(const void* at, const int64_t* stride, int64_t rows, int heads, int D) {
+    if (!at) return COSMOS_ATTN_BAD_ARG;
+    if (!aligned16(at) || stride[0] % 8 || stride[1] % 8) return COSMOS_ATTN_BAD_STRIDE;
+    if (rows > 1 && stride[0] < D) return COSMOS_ATTN_BAD_STRIDE;
+    if (stride[0] * 2 > kMostRowBytes || stride[1] < 0 || (heads > 1 && stride[1] * 2 * heads > ((int64_t)1 << 30))) return COSMOS_ATTN_BAD_STRIDE;
+    return COSMOS_ATTN_OK;
+}
+// rows or heads that share memory can be read, not written
+int check_output(const void* at, const int64_t* stride, int64_t rows, int heads, int D) {
+    const int st = check_tensor(at, stride, rows, heads, D);
+    if (st != COSMOS_ATTN_OK) return st;
+    if (heads > 1 && stride[1] < D) return COSMOS_ATTN_BAD_STRIDE;
+    // one of the two dims holds the other
+    const bool by_row = rows <= 1 || stride[0] >= (heads - 1) * stride[1] + D, by_head = heads <= 1 || stride[1] >= (rows - 1) * stride[0] + D;
+    return by_row || by_head ? COSMOS_ATTN_OK : COSMOS_ATTN_BAD_STRIDE;
+}
+
+int check(const cosmos_attn_ragged_desc* d, bool backward) {
+    if (!d || d->abi_version != COSMOS_ATTN_ABI_VERSION) return COSMOS_ATTN_BAD_ARG;
+    if (d->dtype != COSMOS_ATTN_BF16 && d->dtype != COSMOS_ATTN_FP16) return COSMOS_ATTN_UNSUPPORTED;
+    if (d->n_seq < 0 || d->Hq < 1 || d->Hkv < 1 || d->Tq < 0 || d->Tk < 0 || !(fabsf(d->sm_scale) <= 3.0e38f)) return COSMOS_ATTN_BAD_ARG;
+    if (d->Hq % d->Hkv) return COSMOS_ATTN_BAD_SHAPE;
+    if (d->D != 64 && d->D != 128) return COSMOS_ATTN_UNSUPPORTED;
+    const int64_t group = d->Hq / d->Hkv;
+    // (tile counts and rows are 32-bit numbers)
+    if (d->Tq * group > kMost / 2 || d->Tk > kMost / 2) return COSMOS_ATTN_UNSUPPORTED;
+    if (((d->Tq * group + d->Tk) / kRows + d->n_seq + 1) * d->Hkv > kMost) return COSMOS_ATTN_UNSUPPORTED;
+    if (!d->cu_q || !d->cu_k) return COSMOS_ATTN_BAD_ARG;
+    if ((reinterpret_cast<uintptr_t>(d->cu_q) | reinterpret_cast<uintptr_t>(d->cu_k)) & 3) return COSMOS_ATTN_BAD_STRIDE;
+    int st = COSMOS_ATTN_OK;
+    auto in = [&](const void* at, const int64_t* stride, int64_t rows, int heads) { if (st == COSMOS_ATTN_OK && rows) st = check_tensor(at, stride, rows, heads, d->D); };
+    auto out = [&](const void* at, const int64_t* stride, int64_t rows, int heads) { if (st == COSMOS_ATTN_OK && rows) st = check_output(at, stride, rows, heads, d->D); };
+    in(d->q, d->q_stride, d->Tq, d->Hq);
+    in(d->k, d->k_stride, d->Tk, d->Hkv);
+    in(d->v, d->v_stride, d->Tk, d->Hkv);
+    if (!backward) {
+        out(d->o, d->o_stride, d->Tq, d->Hq);
+    } else {
+        in(d->o, d->o_stride, d->Tq, d->Hq);
+        in(d->dout, d->dout_stride, d->Tq, d->Hq);
+        out(d->dq, d->dq_stride, d->Tq, d->Hq);
+        out(d->dk, d->dk_stride, d->Tk, d->Hkv);
+        out(d->dv, d->dv_stride, d->Tk, d->Hkv);
+        if (st == COSMOS_ATTN_OK && d->Tq && !d->lse) st = COSMOS_ATTN_BAD_ARG;
+    }
+    return st;
+}
+
+RaggedParams params_of(const cosmos_attn_ragged_desc* d) {
+    RaggedParams p = {};
+    p.q = (const char*)d->q; p.k = (const char*)d->k; p.v = (const char*)d->v;
+    p.o = (char*)d->o; p.o_in = (const char*)d->o; p.dout = (const char*)d->dout;
+    p.dq = (char*)d->dq; p.dk = (char*)d->dk; p.dv = (char*)d->dv;
+    p.lse = d->lse;
+    p.cu_q = d->cu_q; p.cu_k = d->cu_k;
+    p.q_row = 2 * d->q_stride[0]; p.q_head = 2 * d->q_stride[1];
+    p.k_row = 2 * d->k_stride[0]; p.k_head = 2 * d->k_stride[1];
+    p.v_row = 2 * d->v_stride[0]; p.v_head = 2 * d->v_stride[1];
+    p.o_row = 2 * d->o_stride[0]; p.o_head = 2 * d->o_stride[1];
+    p.do_row = 2 * d->dout_stride[0]; p.do_head = 2 * d->dout_stride[1];
+    p.dq_row = 2 * d->dq_stride[0]; p.dq_head = 2 * d->dq_stride[1];
+    p.dk_row = 2 * d->dk_stride[0]; p.dk_head = 2 * d->dk_stride[1];
+    p.dv_row = 2 * d->dv_stride[0]; p.dv_head = 2 * d->dv_stride[1];
+    p.n_seq = d->n_seq; p.Tq = (int)d->Tq; p.Tk = (int)d->Tk; p.Hkv = d->Hkv; p.group = d->Hq / d->Hkv;
+    p.causal = d->causal != 0; p.fill = d->fill != 0;
+    p.scale = d->sm_scale;
+    p.scale_log2 = fmaxf(fabsf(d->sm_scale) * 1.44269504088896341f, 1e-37f);      // (a masked score of -inf stays that)
+    p.flip = signbit(d->sm_scale) ? 0x80008000u : 0u;
+    return p;
+}
+
+template <typename P> int launch(void (*kernel)(P), int64_t blocks, size_t lds, const P& p, hipStream_t stream) {
+    if (blocks <= 0) return COSMOS_ATTN_OK;
+    if (!allow_lds((const void*)kernel, lds)) return COSMOS_ATTN_LAUNCH_FAILED;
+    kernel<<<dim3((unsigned)blocks), dim3(kThreads), lds, stream>>>(p);
+    return hipGetLastError() == hipSuccess ? COSMOS_ATTN_OK : COSMOS_ATTN_LAUNCH_FAILED;
+}
+template <typename F> int with_type(int dtype, int D, F&& f) {
+    if (dtype == COSMOS_ATTN_BF16) return D == 128 ? f((__bf16*)nullptr, Int<128>{}) : f((__bf16*)nullptr, Int<64>{});
+    return D == 128 ? f((_Float16*)nullptr, Int<128>{}) : f((_Float16*)nullptr, Int<64>{});
+}
+// at most so many tiles are there: each sequence rounds up once, and so do the rows of none
+int64_t most_tiles(int64_t rows, int n_seq) { return rows / kRows + n_seq + 1; }
+
+}  // namespace
+
+extern "C" {
+
+int cosmos_attn_ragged(const cosmos_attn_ragged_desc* desc, void* stream) {
+    const int st = check(desc, false);
+    if (st != COSMOS_ATTN_OK) return st;
+    if (!desc->Tq) return COSMOS_ATTN_OK;
+    if (!device_is_whole_mi355x()) return COSMOS_ATTN_WRONG_DEVICE;
+    const RaggedParams p = params_of(desc);
+    return with_type(desc->dtype, desc->D, [&](auto* t, auto d) {
+        constexpr int D = decltype(d)::value;
+        return launch(ragged_fwd_kernel<std::remove_pointer_t<decltype(t)>, D>, most_tiles((int64_t)p.Tq * p.group, p.n_seq) * p.Hkv, 4 * Tile<D>::BYTES, p, (hipStream_t)stream);
+    });
+}
+
+size_t cosmos_attn_ragged_bwd_workspace_bytes(const cosmos_attn_ragged_desc* desc) {
+    return check(desc, true) == COSMOS_ATTN_OK ? (size_t)desc->Tq * desc->Hq * sizeof(float) : 0;
+}
+
+int cosmos_attn_ragged_bwd(const cosmos_attn_ragged_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
+    const int st = check(desc, true);
+    if (st != COSMOS_ATTN_OK) return st;
+    if (workspace_bytes < cosmos_attn_ragged_bwd_workspace_bytes(desc) || (desc->Tq && !workspace)) return COSMOS_ATTN_WORKSPACE_TOO_SMALL;
+    if (!device_is_whole_mi355x()) return COSMOS_ATTN_WRONG_DEVICE;
+    RaggedParams p = params_of(desc);
+    p.delta = (float*)workspace;
+    return with_type(desc->dtype, desc->D, [&](auto* t, auto d) {
+        constexpr int D = decltype(d)::value;
+        typedef std::remove_pointer_t<decltype(t)> T;
+        const int done = desc->Tq ? launch(ragged_dq_kernel<T, D>, most_tiles((int64_t)p.Tq * p.group, p.n_seq) * p.Hkv, 4 * Tile<D>::BYTES, p, (hipStream_t)stream) : COSMOS_ATTN_OK;
+        if (done != COSMOS_ATTN_OK || !desc->Tk) return done;
+        return launch(ragged_dkdv_kernel<T, D>, most_tiles(p.Tk, p.n_seq) * p.Hkv, 4 * Tile<D>::BYTES + 4 * kStep * sizeof(float), p, (hipStream_t)stream);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,166 @@
+"""Attention over packed sequences of different lengths with grouped heads, and its gradients (``cosmos_attn_ragged``, ``cosmos_attn_ragged_bwd``).
+
+All sequences of a batch lie one behind the other, ``[rows, heads, D]``, and int32 offsets on the device say where each begins: no padding, no copy of the lengths to the host, and a captured
+call follows offsets that change between replays.  Each ``Hq / Hkv`` query heads in a row share a key head.  With ``causal`` the masks are aligned at the sequences' ends: the last query sees
+every key, so queries may be the last few of a prompt whose first keys come from elsewhere (``kv_cache.cache_read``).
+
+The reference has no counterpart: its attention takes one length for the batch (cosmos_predict2/_src/predict2/networks/attention.py:90-181 ignores ``q_lens`` / ``k_lens``).
+"""
+from __future__ import annotations
+
+import struct
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import _DTYPES, _on_device
+
+HEAD_DIMS = (64, 128)
+_MOST_ROW_BYTES = 1 << 23
+
+# struct cosmos_attn_ragged_desc in one go
+_RAGGED_DESC = struct.Struct("@8i2qfi11Q16q")
+
+
+def packed_ready(x: torch.Tensor) -> bool:
+    """Can the kernels read ``[rows, heads, D]`` as it is: elements of a row of a head side by side, 16-byte steps, rows behind each other?"""
+    rows, heads, D = x.shape
+    row, head, last = x.stride()
+    return (last == 1 and row % 8 == 0 and head % 8 == 0 and x.data_ptr() % 16 == 0 and (rows <= 1 or row >= D) and head >= 0
+            and 2 * row <= _MOST_ROW_BYTES and (heads <= 1 or 2 * heads * head <= 1 << 30))
+
+
+def packed(x: torch.Tensor) -> torch.Tensor:
+    return x if packed_ready(x) else x.clone(memory_format=torch.contiguous_format)
+
+
+def check_rows(x: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
+    """A GPU's 16-bit ``[rows, heads, D]`` of a head dim that is built, on the device and of the type of ``like``."""
+    assert x.dim() == 3, f"{name} must be [rows, heads, D]"
+    if not x.is_cuda:
+        raise RuntimeError("cosmos attention (HIP) needs tensors on a GPU; there is no CPU path")
+    if x.dtype not in _DTYPES:
+        raise NotImplementedError(f"{name}: dtype={x.dtype} is not supported (bf16 / fp16)")
+    if x.shape[2] not in HEAD_DIMS:
+        raise NotImplementedError(f"{name}: head dim {x.shape[2]}: the HIP kernels are built for {HEAD_DIMS}")
+    if like is not None:
+        assert x.dtype == like.dtype and x.device == like.device, f"{name} must have the type and device of the others"
+
+
+def int32_on(x: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """Offsets, lengths and tables as the kernels take them: int32 on the device, elements of the last dim side by side."""
+    assert not x.is_floating_point() and not x.is_complex() and x.dtype != torch.bool, "offsets, lengths and tables are whole numbers"
+    if x.dtype != torch.int32 or x.device != device:
+        x = x.to(device=device, dtype=torch.int32)
+    return x if x.dim() == 0 or x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+def _check(q, k, v, cu_q, cu_k):
+    check_rows(q, "q")
+    check_rows(k, "k", q)
+    check_rows(v, "v", q)
+    assert k.shape == v.shape and k.shape[2] == q.shape[2], "k and v have one shape, and q their head dim"
+    assert q.shape[1] >= 1 and k.shape[1] >= 1 and q.shape[1] % k.shape[1] == 0, "the query heads are a multiple of the key heads"
+    cu_q = int32_on(cu_q, q.device)
+    cu_k = cu_q if cu_k is None else int32_on(cu_k, q.device)
+    assert cu_q.dim() == 1 and cu_q.shape == cu_k.shape and cu_q.shape[0] >= 1, "cu_q and cu_k hold one offset more than there are sequences"
+    return cu_q, cu_k
+
+
+def _strides(*tensors):
+    return [s for x in tensors for s in ((0, 0) if x is None else x.stride()[:2])]
+
+
+def _pointers(*tensors):
+    return [0 if x is None else x.data_ptr() for x in tensors]
+
+
+def _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, fill, dout=None, dq=None, dk=None, dv=None) -> bytes:
+    return _RAGGED_DESC.pack(
+        _lib.ABI_VERSION, _DTYPES[q.dtype], cu_q.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2], 1 if causal else 0, 1 if fill else 0, q.shape[0], k.shape[0],
+        q.shape[2] ** -0.5 if sm_scale is None else sm_scale, 0, *_pointers(q, k, v, cu_q, cu_k, o, lse, dout, dq, dk, dv), *_strides(q, k, v, o, dout, dq, dk, dv))
+
+
+def ragged_fwd(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_q: torch.Tensor,
+    cu_k: Optional[torch.Tensor] = None,
+    causal: bool = False,
+    sm_scale: Optional[float] = None,
+    need_lse: bool = True,
+    out: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``(o, lse)``: ``q [Tq, Hq, D]``, ``k``, ``v`` ``[Tk, Hkv, D]``; sequence i has the rows ``cu_q[i] .. cu_q[i + 1] - 1`` of q and ``cu_k[i] ..`` of k and v
+    (``cu_k`` None: the same).  ``causal``: query t of Lq sees the keys up to ``t + Lk - Lq``.  ``lse``: fp32 ``[Hq, Tq]``.
+
+    A row that sees no key: o = 0, lse = -inf.  Rows of no sequence (before ``cu_q[0]``, from the last offset on) become zeros, and -inf; in ``out``, a tensor that is given for o, they are
+    left as they are.  Offsets that do not ascend within the tensors: such ``cu_q`` leaves the sequence's rows unwritten, such ``cu_k`` makes them NaN.  ``out`` must not overlap the inputs.  No gradients:
+    :func:`attention_ragged` has them."""
+    cu_q, cu_k = _check(q, k, v, cu_q, cu_k)
+    q, k, v = packed(q), packed(k), packed(v)
+    if out is None:
+        o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    else:
+        assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out must have q's shape, type and device"
+        if not packed_ready(out):
+            raise ValueError("out: rows of 16-byte steps are written in place, this view cannot be")
+        o = out
+    lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32) if need_lse else None
+    desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, out is None)
+    run = _lib.load_library().cosmos_attn_ragged
+    _lib.raise_for_status(_on_device(q.device, lambda stream: run(desc, stream)))
+    return o, lse
+
+
+def ragged_bwd(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    o: torch.Tensor,
+    lse: torch.Tensor,
+    dout: torch.Tensor,
+    cu_q: torch.Tensor,
+    cu_k: Optional[torch.Tensor] = None,
+    causal: bool = False,
+    sm_scale: Optional[float] = None,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(dq, dk, dv)`` of :func:`ragged_fwd` for the gradient ``dout`` of o, from its o and lse.  Rows of no sequence get zeros.  The same results every time (no atomics)."""
+    cu_q, cu_k = _check(q, k, v, cu_q, cu_k)
+    for x, name in ((o, "o"), (dout, "dout")):
+        assert x.shape == q.shape and x.dtype == q.dtype and x.device == q.device, f"{name} must have q's shape, type and device"
+    assert lse.shape == (q.shape[1], q.shape[0]) and lse.dtype == torch.float32 and lse.device == q.device, "lse is the forward's, fp32 [Hq, Tq]"
+    q, k, v, o, dout, lse = packed(q), packed(k), packed(v), packed(o), packed(dout), lse.contiguous()
+    dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
+    desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, True, dout, dq, dk, dv)
+    lib = _lib.load_library()
+    ws_bytes = lib.cosmos_attn_ragged_bwd_workspace_bytes(desc)
+    workspace = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8)
+    _lib.raise_for_status(_on_device(q.device, lambda stream: lib.cosmos_attn_ragged_bwd(desc, workspace.data_ptr(), ws_bytes, stream)))
+    return dq, dk, dv
+
+
+class _RaggedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, causal, softmax_scale):
+        o, lse = ragged_fwd(q, k, v, cu_q, cu_k, causal=causal, sm_scale=softmax_scale)
+        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k)
+        ctx.causal, ctx.softmax_scale = causal, softmax_scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, o, lse, cu_q, cu_k = ctx.saved_tensors
+        return (*ragged_bwd(q, k, v, o, lse, dout, cu_q, cu_k, causal=ctx.causal, sm_scale=ctx.softmax_scale), None, None, None, None)
+
+
+def attention_ragged(q, k, v, cu_q, cu_k=None, softmax_scale=None, causal=False):
+    """Differentiable attention over packed sequences: o of :func:`ragged_fwd`, gradients by :func:`ragged_bwd`.  The offsets must not change between the two."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        cu_q = int32_on(cu_q, q.device)
+        return _RaggedFn.apply(q, k, v, cu_q, cu_q if cu_k is None else int32_on(cu_k, q.device), causal, softmax_scale)
+    return ragged_fwd(q, k, v, cu_q, cu_k, causal=causal, sm_scale=softmax_scale, need_lse=False)[0]

@@ -401,6 +401,87 @@ COSMOS_ATTN_API int cosmos_attn_gemm(const cosmos_attn_gemm_desc *desc, void *st
 /* 1 where cosmos_attn_gemm takes the call and is faster than the vendor library's product (or products and additions), 0 elsewhere.  Looks at sizes only. */
 COSMOS_ATTN_API int cosmos_attn_gemm_preferred(const cosmos_attn_gemm_desc *desc);
 
+/*
+ * Attention over packed sequences of different lengths with grouped heads (no counterpart in the reference, whose attention has one length for the batch and as many key as query heads).
+ * q, o [Tq, Hq, D], k, v [Tk, Hkv, D]; query head h reads key head h / (Hq / Hkv).  Sequence i: rows cu_q[i] .. cu_q[i + 1] - 1 of q and cu_k[i] .. cu_k[i + 1] - 1 of k and v; the
+ * offsets stay on the device and may change between replays of a captured call.  With t and j counted from the sequence's start and Lq, Lk its lengths:
+ *     o_t = sum_j softmax_j(sm_scale q_t k_j) v_j over the visible keys: all, or (causal) j <= t + Lk - Lq: the last query sees all keys
+ *     lse_t = log sum_j exp(sm_scale q_t k_j)
+ * A row that sees no key: o = 0, lse = -inf, and no gradient.  Rows of no sequence (before cu_q[0], from cu_q[n_seq] on) are left as they are, or with `fill` become zeros (lse -inf).
+ * Offsets that do not ascend within the tensors: a sequence of such cu_q has no rows, one of such cu_k rows of NaN; neither reads or writes outside of the tensors.
+ * What a row does not see has no influence on it as long as it is finite within the row's own sequence; what lies outside of the sequences may be anything.
+ *
+ * cosmos_attn_ragged_bwd: dq, dk, dv for the gradient dout of o, from the forward's o and lse; rows of no sequence become zeros.  No atomics: the same results every time.
+ * The workspace holds a number per row and head.  Outputs must not overlap inputs or each other.
+ */
+typedef struct cosmos_attn_ragged_desc {
+    int32_t abi_version, dtype;
+    int32_t n_seq, Hq, Hkv, D;         /* Hq % Hkv == 0; D 64 or 128 */
+    int32_t causal, fill;
+    int64_t Tq, Tk;                    /* Tq * Hq / Hkv and Tk below 2^30 */
+    float sm_scale;
+    int32_t reserved;
+    const void *q, *k, *v;
+    const int32_t *cu_q, *cu_k;        /* [n_seq + 1] */
+    void *o;                           /* (backward: read) */
+    float *lse;                        /* [Hq, Tq] fp32; the forward's may be NULL */
+    const void *dout;                  /* from here on: backward alone */
+    void *dq, *dk, *dv;
+    int64_t q_stride[2], k_stride[2], v_stride[2], o_stride[2];   /* (row, head) element strides, multiples of 8; a row at most 2^22 elements */
+    int64_t dout_stride[2], dq_stride[2], dk_stride[2], dv_stride[2];
+} cosmos_attn_ragged_desc;
+
+COSMOS_ATTN_API int cosmos_attn_ragged(const cosmos_attn_ragged_desc *desc, void *stream);
+COSMOS_ATTN_API size_t cosmos_attn_ragged_bwd_workspace_bytes(const cosmos_attn_ragged_desc *desc);
+COSMOS_ATTN_API int cosmos_attn_ragged_bwd(const cosmos_attn_ragged_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * A paged key-value cache (no counterpart in the reference).  k and v: pages of page_size rows of D elements for each of Hkv heads, [pages, Hkv, page_size, D] through (page, head, row)
+ * element strides, of the 16-bit type `dtype` or of 8 bits with an fp32 scale for each row, [pages, Hkv, page_size] through (page, head) strides:
+ *     scale = max |x| * fp32(1 / 448) (e4m3) or * fp32(1 / 127) (int8), code = round(x / scale), all in fp32;  a row with a value that is not finite has the scale NaN
+ * Position j of sequence i lies in page table[i][j / page_size], place j % page_size.  Tables and lengths stay on the device and may change between replays of a captured call; entries
+ * behind a sequence's last page are not looked at.  They are not trusted: a page outside of the cache or a length that the table does not hold writes nothing, reads back as NaN and
+ * makes the sequence's attention NaN.  What pages hold behind a sequence's end may be anything.
+ *
+ * cosmos_attn_cache_write: packed rows k_rows, v_rows [rows, Hkv, D]; sequence i's are cu[i] .. cu[i + 1] - 1 (cu NULL: one for each sequence), its last positions: lens[i], which counts
+ *     them, is where they end.  Rows of no sequence, and sequences with lens[i] below their rows, write nothing.  Two rows of a call must not have one place (two sequences sharing a page).
+ * cosmos_attn_cache_read: the first cu[i + 1] - cu[i] positions of sequence i to the rows cu[i] .. of k_rows and v_rows, code * scale rounded to `dtype`; rows of no sequence are left as
+ *     they are, or with `fill` become zeros.
+ * cosmos_attn_cache_attention: o[i] = softmax(sm_scale q[i] K^T) V over the first lens[i] positions, q, o [B, Hq, D], query head h on key head h / (Hq / Hkv); lse [B, Hq] fp32 or NULL.
+ *     lens[i] == 0: o = 0, lse = -inf.  The workspace holds sums of the sequences that several workgroups share; the bytes follow from the sizes alone.
+ */
+enum cosmos_attn_cache_kind { COSMOS_ATTN_CACHE_SAME = 0, COSMOS_ATTN_CACHE_E4M3 = 1, COSMOS_ATTN_CACHE_INT8 = 2 };
+typedef struct cosmos_attn_cache_desc {
+    int32_t abi_version, dtype;
+    int32_t kind;                      /* enum cosmos_attn_cache_kind */
+    int32_t Hkv, D, page_size;         /* D 64 or 128; page_size a power of two, 16 .. 1024 */
+    int64_t pages;                     /* at least 1 */
+    void *k, *v;
+    int64_t k_stride[3], v_stride[3];  /* multiples of 16 bytes */
+    float *k_scale, *v_scale;          /* 8 bits alone */
+    int64_t k_scale_stride[2], v_scale_stride[2];   /* multiples of 4 */
+    int32_t B, width;                  /* sequences; entries of a row of the table: width * page_size below 2^31 */
+    const int32_t *table;              /* [B, width], rows table_stride elements apart */
+    int64_t table_stride;
+    const int32_t *lens;               /* [B]; not read by cosmos_attn_cache_read */
+    const int32_t *cu;                 /* [B + 1]; not read by cosmos_attn_cache_attention */
+    int64_t rows;
+    void *k_rows, *v_rows;             /* written by cosmos_attn_cache_read alone */
+    int64_t k_rows_stride[2], v_rows_stride[2];   /* (row, head), multiples of 8 */
+    int32_t fill, Hq;
+    float sm_scale;
+    int32_t reserved;
+    const void *q;
+    void *o;
+    int64_t q_stride[2], o_stride[2];
+    float *lse;
+} cosmos_attn_cache_desc;
+
+COSMOS_ATTN_API int cosmos_attn_cache_write(const cosmos_attn_cache_desc *desc, void *stream);
+COSMOS_ATTN_API int cosmos_attn_cache_read(const cosmos_attn_cache_desc *desc, void *stream);
+COSMOS_ATTN_API size_t cosmos_attn_cache_attention_workspace_bytes(const cosmos_attn_cache_desc *desc);
+COSMOS_ATTN_API int cosmos_attn_cache_attention(const cosmos_attn_cache_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -41,6 +41,11 @@ def net_oracle():
 
 
 @pytest.fixture(scope="session")
+def ragged_oracle():
+    return entry.load_ragged_oracle()
+
+
+@pytest.fixture(scope="session")
 def pkg():
     """The package with its HIP library loaded; fails loudly when the library is not built."""
     return entry.load_package()

@@ -1,0 +1,287 @@
+"""Attention over packed sequences, forward and gradients, against the oracle in 64 bits; bounds count roundings (oracle/ragged_oracle.py)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def cu(lens, first=0):
+    return [first + sum(lens[:i]) for i in range(len(lens) + 1)]
+
+
+def offsets(values, gpu):
+    return torch.tensor(values, dtype=torch.int32, device=gpu)
+
+
+def rows(n, heads, D, dtype, gpu, seed, size=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (size * torch.randn(n, heads, D, generator=g)).to(dtype).to(gpu)
+
+
+def near(got, want, tol, what):
+    got = got.double().cpu()
+    same = (got == want) | (got.isnan() & want.isnan())
+    off = torch.where(same, torch.zeros_like(want), (got - want).abs())
+    bad = ~(off <= tol)
+    at = tuple(int(i) for i in bad.nonzero()[0]) if bad.any() else ()
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, at {at}: {float(got[at])} for {float(want[at])}, bound {float(tol[at])}"
+
+
+def both(pkg, oracle, gpu, ql, kl, Hq, Hkv, D, dtype, causal, scale=None, size=1.0, seed=0, backward=True):
+    q, k, v = rows(sum(ql), Hq, D, dtype, gpu, seed, size), rows(sum(kl), Hkv, D, dtype, gpu, seed + 1, size), rows(sum(kl), Hkv, D, dtype, gpu, seed + 2)
+    c = D ** -0.5 if scale is None else scale
+    at = (cu(ql), cu(kl))
+    on = [offsets(x, gpu) for x in at]
+    o, lse = pkg.ragged_fwd(q, k, v, *on, causal=causal, sm_scale=scale)
+    O, L, o_tol, l_tol = oracle.ragged_fwd(q, k, v, *at, causal, c, dtype)
+    near(o, O, o_tol, "o")
+    near(lse, L, l_tol, "lse")
+    if not backward:
+        return
+    g = rows(sum(ql), Hq, D, dtype, gpu, seed + 3)
+    got = pkg.ragged_bwd(q, k, v, o, lse, g, *on, causal=causal, sm_scale=scale)
+    want, tols = oracle.ragged_bwd(q, k, v, g, *at, causal, c, dtype)
+    for name, a, b, t in zip(("dq", "dk", "dv"), got, want, tols):
+        near(a, b, t, name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens", [[1], [33], [64], [65], [128], [129], [300], [1, 0, 63, 2, 200, 0, 127]])
+def test_lengths(pkg, ragged_oracle, gpu, lens, causal, D, dtype):
+    both(pkg, ragged_oracle, gpu, lens, lens, 4, 2, D, dtype, causal)
+
+
+@pytest.mark.parametrize("Hq, Hkv", [(1, 1), (3, 3), (3, 1), (5, 1), (14, 2), (16, 1), (8, 4), (40, 8), (67, 1)])
+def test_heads(pkg, ragged_oracle, gpu, Hq, Hkv):
+    both(pkg, ragged_oracle, gpu, [70, 1, 150], [70, 1, 150], Hq, Hkv, 64, BF16, True)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("ql, kl", [([5], [300]), ([1, 1, 1], [1, 64, 129]), ([70, 3, 9], [10, 3, 200]), ([4, 0, 6], [0, 7, 5]), ([200], [131]), ([130, 40], [1, 0])])
+@pytest.mark.parametrize("causal", [False, True])
+def test_queries_and_keys_of_different_numbers(pkg, ragged_oracle, gpu, ql, kl, causal, D):
+    both(pkg, ragged_oracle, gpu, ql, kl, 6, 2, D, BF16, causal)
+
+
+def test_many_sequences(pkg, ragged_oracle, gpu):
+    lens = [(7 * i * i) % 23 for i in range(150)]
+    both(pkg, ragged_oracle, gpu, lens, lens, 2, 1, 64, FP16, True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1.0])
+def test_scales(pkg, ragged_oracle, gpu, scale, dtype):
+    both(pkg, ragged_oracle, gpu, [90, 200], [90, 200], 4, 2, 64, dtype, True, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_scores_that_spread(pkg, ragged_oracle, gpu, dtype):
+    """The running max moves late and often."""
+    both(pkg, ragged_oracle, gpu, [257, 90], [257, 90], 4, 2, 128, dtype, True, size=6.0, backward=False)
+
+
+def test_max_that_moves_in_the_last_tile(pkg, ragged_oracle, gpu):
+    q, k, v = (rows(500, 2, 64, BF16, gpu, i) for i in range(3))
+    k[450:] *= 20
+    at = [0, 500]
+    o, lse = pkg.ragged_fwd(q, k, v, offsets(at, gpu))
+    O, L, o_tol, l_tol = ragged_oracle.ragged_fwd(q, k, v, at, at, False, 0.125, BF16)
+    near(o, O, o_tol, "o")
+    near(lse, L, l_tol, "lse")
+
+
+def test_strides(pkg, ragged_oracle, gpu):
+    """q, k and v as the projection's output has them, shared heads without a copy, a gradient that is broadcast, rows that are taken apart."""
+    lens, Hq, Hkv, D = [50, 130], 6, 2, 64
+    at = cu(lens)
+    qkv = rows(180, Hq + 2 * Hkv, D, BF16, gpu, 5)
+    q, k, v = qkv[:, :Hq], qkv[:, Hq:Hq + Hkv], qkv[:, Hq + Hkv:]
+    on = offsets(at, gpu)
+    want = pkg.ragged_fwd(q.clone(), k.clone(), v.clone(), on, causal=True)
+    got = pkg.ragged_fwd(q, k, v, on, causal=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    shared = pkg.ragged_fwd(q, k[:, :1].expand(-1, 2, -1), v[:, :1].expand(-1, 2, -1), on, causal=True)
+    assert torch.equal(shared[0], pkg.ragged_fwd(q, k[:, :1], v[:, :1], on, causal=True)[0])
+    heads_first = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(pkg.ragged_fwd(heads_first, k, v, on, causal=True)[0], want[0])
+    apart = torch.randn(180, Hkv, D, 2, device=gpu).to(BF16)[..., 0]
+    assert torch.equal(pkg.ragged_fwd(q, apart, v, on)[0], pkg.ragged_fwd(q, apart.contiguous(), v, on)[0])
+    g = torch.ones(1, 1, 1, dtype=BF16, device=gpu).expand(180, Hq, D)
+    a = pkg.ragged_bwd(q, k, v, *want, g, on, causal=True)
+    b = pkg.ragged_bwd(q.clone(), k.clone(), v.clone(), *want, g.contiguous(), on, causal=True)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_rows_of_no_sequence(pkg, ragged_oracle, gpu):
+    """In front of the first sequence and behind the last one: not read, whatever they hold; left alone in a given output, zeros in a new one."""
+    lens, first = [40, 100], 7
+    at, n = cu(lens, first), 7 + 140 + 9
+    q, k, v, g = (rows(n, h, 128, BF16, gpu, i) for i, h in enumerate((4, 2, 2, 4)))
+    outside = torch.ones(n, dtype=torch.bool, device=gpu)
+    outside[7:147] = False
+    for x in (q, k, v, g):
+        x[outside] = math.nan
+    on = offsets(at, gpu)
+    o, lse = pkg.ragged_fwd(q, k, v, on, causal=True)
+    assert (o[outside] == 0).all() and (lse[:, outside] == -math.inf).all()
+    inside = [x[~outside] for x in (q, k, v, g)]
+    O, L, o_tol, l_tol = ragged_oracle.ragged_fwd(*inside[:3], cu(lens), cu(lens), True, 128 ** -0.5, BF16)
+    near(o[~outside], O, o_tol, "o")
+    given = torch.full_like(q, 3.0)
+    assert pkg.ragged_fwd(q, k, v, on, causal=True, out=given)[0] is given
+    assert (given[outside] == 3).all() and torch.equal(given[~outside], o[~outside])
+    grads = pkg.ragged_bwd(q, k, v, o, lse, g, on, causal=True)
+    want, tols = ragged_oracle.ragged_bwd(*inside, cu(lens), cu(lens), True, 128 ** -0.5, BF16)
+    for x, w, t in zip(grads, want, tols):
+        assert (x[outside] == 0).all()
+        near(x[~outside], w, t, "a gradient")
+
+
+def test_no_sequences_and_no_rows(pkg, gpu):
+    q, k = rows(5, 4, 64, BF16, gpu, 0), rows(3, 2, 64, BF16, gpu, 1)
+    o, lse = pkg.ragged_fwd(q, k, k, offsets([0], gpu), offsets([0], gpu))
+    assert (o == 0).all() and (lse == -math.inf).all()
+    o, lse = pkg.ragged_fwd(q[:0], k, k, offsets([0, 0], gpu), offsets([0, 3], gpu))
+    assert o.shape == (0, 4, 64)
+    grads = pkg.ragged_bwd(q[:0], k, k, o, lse, q[:0], offsets([0, 0], gpu), offsets([0, 3], gpu))
+    assert (grads[1] == 0).all() and (grads[2] == 0).all()
+    o, lse = pkg.ragged_fwd(q, k[:0], k[:0], offsets([0, 5], gpu), offsets([0, 0], gpu))
+    assert (o == 0).all() and (lse == -math.inf).all()
+    grads = pkg.ragged_bwd(q, k[:0], k[:0], o, lse, q, offsets([0, 5], gpu), offsets([0, 0], gpu))
+    assert (grads[0] == 0).all()
+
+
+def test_offsets_that_do_not_ascend_within_the_tensors(pkg, gpu):
+    """The kernels' own checks: such rows are not there, such keys make NaN; the other sequences are as ever."""
+    q, k = rows(100, 4, 64, BF16, gpu, 0), rows(100, 2, 64, BF16, gpu, 1)
+    good = pkg.ragged_fwd(q, k, k, offsets([0, 30, 100], gpu), causal=True)[0]
+    out = torch.full_like(q, 3.0)
+    pkg.ragged_fwd(q, k, k, offsets([0, 30, 101], gpu), offsets([0, 30, 100], gpu), causal=True, out=out)
+    assert torch.equal(out[:30], good[:30]) and (out[30:] == 3).all()
+    o, lse = pkg.ragged_fwd(q, k, k, offsets([0, 30, 100], gpu), offsets([0, 30, 1 << 30], gpu), causal=True)
+    assert torch.equal(o[:30], good[:30]) and o[30:].isnan().all() and lse[:, 30:].isnan().all()
+    o, _ = pkg.ragged_fwd(q, k, k, offsets([0, 30, 100], gpu), offsets([-5, 30, 20], gpu))
+    assert o.isnan().all()
+    grads = pkg.ragged_bwd(q, k, k, good, lse, q, offsets([0, 30, 100], gpu), offsets([-5, 30, 20], gpu))
+    assert (grads[0] == 0).all()
+
+
+def test_values_that_are_not_finite_stay_in_their_rows(pkg, gpu):
+    """NaN in one sequence says nothing in another, and a masked score nothing at all."""
+    q, k, v = (rows(200, 2, 64, BF16, gpu, i) for i in range(3))
+    on = offsets([0, 100, 200], gpu)
+    clean = pkg.ragged_fwd(q, k, v, on, causal=True)[0]
+    k2, v2 = k.clone(), v.clone()
+    k2[100:] = math.nan
+    v2[100:] = math.inf
+    o = pkg.ragged_fwd(q, k2, v2, on, causal=True)[0]
+    assert torch.equal(o[:100], clean[:100]) and o[100:].isnan().all()
+    k2 = k.clone()
+    k2[60] = math.nan                # keys that a query does not see yet
+    o = pkg.ragged_fwd(q, k2, v, on, causal=True)[0]
+    assert torch.equal(o[:60], clean[:60]) and o[60:100].isnan().all() and torch.equal(o[100:], clean[100:])
+
+
+def test_gradients_through_autograd(pkg, ragged_oracle, gpu):
+    lens = [37, 90]
+    at = cu(lens)
+    leaves = [rows(127, h, 64, FP16, gpu, i).requires_grad_() for i, h in enumerate((6, 2, 2))]
+    g = rows(127, 6, 64, FP16, gpu, 9)
+    o = pkg.attention_ragged(*leaves, offsets(at, gpu), causal=True, softmax_scale=0.2)
+    o.backward(g)
+    want, tols = ragged_oracle.ragged_bwd(*(x.detach() for x in leaves), g, at, at, True, 0.2, FP16)
+    for x, w, t in zip(leaves, want, tols):
+        near(x.grad, w, t, "a gradient")
+    plain = pkg.attention_ragged(*(x.detach() for x in leaves), offsets(at, gpu), causal=True, softmax_scale=0.2)
+    assert torch.equal(o, plain) and not plain.requires_grad
+    with pytest.raises(RuntimeError):
+        a = torch.autograd.grad(pkg.attention_ragged(*leaves, offsets(at, gpu)), leaves[0], g.clone().requires_grad_(), create_graph=True)[0]
+        torch.autograd.grad(a.sum(), leaves[1])
+
+
+def test_gradients_of_shared_and_of_frozen_tensors(pkg, gpu):
+    """One tensor as key and value gets both gradients; heads shared by expansion their sum; a frozen one none."""
+    q, k = rows(90, 4, 64, BF16, gpu, 0), rows(90, 1, 64, BF16, gpu, 1).requires_grad_()
+    on, g = offsets([0, 90], gpu), rows(90, 4, 64, BF16, gpu, 2)
+    pkg.attention_ragged(q, k, k, on, causal=True).backward(g)
+    o, lse = pkg.ragged_fwd(q, k.detach(), k.detach(), on, causal=True)
+    _, dk, dv = pkg.ragged_bwd(q, k.detach(), k.detach(), o, lse, g, on, causal=True)
+    assert torch.equal(k.grad, dk + dv) and q.grad is None
+    k2 = k.detach().clone().requires_grad_()
+    pkg.attention_ragged(q, k2.expand(-1, 2, -1), k.detach().expand(-1, 2, -1), on, causal=True).backward(g)
+    # Two key heads of two query heads each: their gradients are rounded (half a step, 2^-8, of each: they may be far larger than their sum), their sum is, and the shared head's is.
+    two = pkg.ragged_bwd(q, k.detach().expand(-1, 2, -1), k.detach().expand(-1, 2, -1), o, lse, g, on, causal=True)[1].double()
+    assert ((k2.grad.double() - dk.double()).abs() <= 2.0 ** -8 * (1 + 2.0 ** -7) * (two.abs().sum(1, keepdim=True) + k2.grad.double().abs() + dk.double().abs()) + 1e-5).all()
+
+
+def test_same_results_every_time(pkg, gpu):
+    q, k, v, g = (rows(1000, h, 128, BF16, gpu, i) for i, h in enumerate((8, 2, 2, 8)))
+    on = offsets([0, 300, 301, 1000], gpu)
+    o, lse = pkg.ragged_fwd(q, k, v, on, causal=True)
+    first = pkg.ragged_bwd(q, k, v, o, lse, g, on, causal=True)
+    for _ in range(5):
+        again = pkg.ragged_fwd(q, k, v, on, causal=True)
+        assert torch.equal(again[0], o) and torch.equal(again[1], lse)
+        assert all(torch.equal(a, b) for a, b in zip(pkg.ragged_bwd(q, k, v, o, lse, g, on, causal=True), first))
+
+
+def test_captured_calls_follow_their_offsets(pkg, gpu):
+    q, k, v, g = (rows(400, h, 64, BF16, gpu, i) for i, h in enumerate((4, 2, 2, 4)))
+    on = offsets([0, 100, 400], gpu)
+
+    def step():
+        o, lse = pkg.ragged_fwd(q, k, v, on, causal=True)
+        return (o, lse, *pkg.ragged_bwd(q, k, v, o, lse, g, on, causal=True))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        made = step()
+    for at in ([0, 100, 400], [0, 399, 400], [0, 0, 250], [0, 100, 400]):
+        on.copy_(offsets(at, gpu))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in made]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_another_stream(pkg, gpu):
+    q, k, v = (rows(300, 4, 128, BF16, gpu, i) for i in range(3))
+    on = offsets([0, 300], gpu)
+    want = pkg.ragged_fwd(q, k, v, on, causal=True)[0]
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        got = pkg.ragged_fwd(q, k, v, on, causal=True)[0]
+    other.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_rows_behind_32_bits(pkg, ragged_oracle, gpu):
+    """Rows 4 MiB apart: 700 of them span more than 2^31 bytes (and elements)."""
+    n, step = 1100, 1 << 21
+    pool = torch.zeros(n * step, dtype=BF16, device=gpu)
+    views = []
+    for i, h in enumerate((4, 2, 2)):
+        view = pool.as_strided((n, h, 64), (step, 64, 1), i * 1024)
+        view.copy_(rows(n, h, 64, BF16, gpu, i))
+        views.append(view)
+    lens = [300, 800]
+    on, at = offsets(cu(lens), gpu), cu(lens)
+    want = pkg.ragged_fwd(*(x.contiguous() for x in views), on, causal=True)
+    out = pool.as_strided((n, 4, 64), (step, 64, 1), 8192)
+    got = pkg.ragged_fwd(*views, on, causal=True, out=out)
+    assert torch.equal(out, want[0]) and torch.equal(got[1], want[1])
+    g = rows(n, 4, 64, BF16, gpu, 7)
+    a = pkg.ragged_bwd(*views, out, got[1], g, on, causal=True)
+    b = pkg.ragged_bwd(*(x.contiguous() for x in views), want[0], want[1], g, on, causal=True)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
