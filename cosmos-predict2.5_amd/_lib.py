@@ -323,7 +323,8 @@ EXPORTS = {
     "cosmos_attn_gemm_preferred": (ctypes.c_int, [ctypes.c_void_p]),                      # (as well)
     "cosmos_gelu": (ctypes.c_int, [ctypes.POINTER(GeluDesc), ctypes.c_void_p]),
     # (descriptors, also as packed bytes)
-    "cosmos_attn_ragged": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "cosmos_attn_ragged_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "cosmos_attn_ragged": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "cosmos_attn_ragged_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p]),
     "cosmos_attn_ragged_bwd": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "cosmos_attn_cache_write": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),

@@ -9,8 +9,9 @@
 // rows then shares K and V among the heads, few tokens still fill a tile, a causal tile's diagonal is `group` times shorter, and the sums over the group that dk and dv need
 // are part of the contraction over rows.
 //
-// Who does what.  Lengths stay on the device: the grid is what the tensors' row counts allow at most, and every workgroup finds its sequence by a scan over the offsets
-// (64 sequences a step, each wavefront for itself).  No work list, no copy to the host, nothing to prepare, and a captured call follows its offsets.
+// Who does what.  Lengths stay on the device: the grid is what the tensors' row counts allow at most, and every workgroup finds its tile from the offsets (each wavefront for itself).  No work
+// list, no copy to the host, nothing to prepare, and a captured call follows its offsets.  Where a call has few tiles, those with more than an equal share of all steps are cut along
+// their keys (rows), and a second kernel adds the parts up, in their order.
 //
 // Offsets are not trusted: a sequence whose offsets do not ascend within the tensors has no rows; one whose keys' offsets do not has rows of NaN (no gradients: zeros).
 #include <hip/hip_runtime.h>
@@ -40,14 +41,16 @@ struct RaggedParams {
     // bytes between rows and between heads
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
     int n_seq, Tq, Tk, Hkv, group, causal, fill;
+    int tiles, most_parts, least;  // tiles that there may be, parts that one may be cut into, steps of a part
+    float* parts;                  // what they leave: of part s of tile i and key head h, at (i Hkv + h) most_parts + s
     float scale, scale_log2;       // scale_log2 >= 0: `flip` says that q's signs are turned instead
     unsigned flip;
 };
 
-// ---- a tile in LDS: kStep rows of D 16-bit elements, as chunks of 16 bytes.  Chunk c of row r lies at c XOR mix(r): what a wavefront reads at once, 16 bytes of each of 32 rows (a fragment
+// ---- a tile in LDS: N rows of D 16-bit elements, as chunks of 16 bytes.  Chunk c of row r lies at c XOR mix(r): what a wavefront reads at once, 16 bytes of each of 32 rows (a fragment
 // with lane = row) or, transposing, 64 bytes of each of 8 rows, then lies in different banks, and a load to LDS still takes whole rows.
-template <int D> struct Tile {
-    static constexpr int ROW = 2 * D, BYTES = kStep * ROW, CHUNKS = D / 8, ROWS_PER_LOAD = 1024 / ROW, LOADS = kStep / 4 / ROWS_PER_LOAD;
+template <int D, int N = kStep> struct Tile {
+    static constexpr int ROW = 2 * D, BYTES = N * ROW, CHUNKS = D / 8, ROWS_PER_LOAD = 1024 / ROW, LOADS = N / 4 / ROWS_PER_LOAD;
     static __device__ __forceinline__ int mix(int r) { return D == 128 ? 4 * (r & 3) | ((r >> 2) & 3) : 4 * ((r >> 1) & 1) | ((r >> 2) & 3); }
     // where lane reads chunk 2 c + lane / 32 of row lane % 32
     static __device__ __forceinline__ int at(int lane, int c) { return (lane & 31) * ROW + ((((2 * c) | (lane >> 5)) ^ mix(lane & 31)) << 4); }
@@ -57,15 +60,18 @@ template <int D> struct Tile {
         return row * ROW + ((chunk ^ mix(row)) << 4) + 8 * (lane & 1);
     }
     // the row (of the tile) and the byte in that row that this lane loads with load i of wavefront `wave`
-    static __device__ __forceinline__ int load_row(int lane, int wave, int i) { return 16 * wave + i * ROWS_PER_LOAD + lane / CHUNKS; }
+    static __device__ __forceinline__ int load_row(int lane, int wave, int i) { return N / 4 * wave + i * ROWS_PER_LOAD + lane / CHUNKS; }
     static __device__ __forceinline__ int load_byte(int lane, int wave, int i) { return ((lane % CHUNKS) ^ mix(load_row(lane, wave, i))) << 4; }
-    static __device__ __forceinline__ int load_to(int wave, int i) { return (16 * wave + i * ROWS_PER_LOAD) * ROW; }
+    static __device__ __forceinline__ int load_to(int wave, int i) { return (N / 4 * wave + i * ROWS_PER_LOAD) * ROW; }
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+// of a tile's part: its rows' max, sum of exponentials and D sums
+template <int D> constexpr int kPartFloats = kRows * (D + 2);
 
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, char* dst, int offset) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)dst, 16, offset, 0, 0, 0);
@@ -77,15 +83,19 @@ template <typename V8> __device__ __forceinline__ V8 read_channels(const char* p
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(part + at0)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(part + at1));
     return __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-// all loads to LDS have landed and all reads have returned; then the workgroup meets
+// Two pairs of tiles, the one read while the other is loaded.  Arrays of their own: the compiler waits for loads to LDS in front of a read that may be of the same array.
+#define LDS_TILES(L) __shared__ __attribute__((aligned(1024))) char tile0[L::BYTES], tile1[L::BYTES], tile2[L::BYTES], tile3[L::BYTES]
+// all loads to LDS have landed and all reads have returned; then the workgroup meets.  (Through the builtin, which the compiler counts with: it then waits for nothing else in front of reads.)
+constexpr int kNothingUnderWay = 0x0070;      // vmcnt 0, lgkmcnt 0
 __device__ __forceinline__ void meet() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(kNothingUnderWay);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
-// `rows_left` rows from `at` on (at most kStep are read), what lies behind them reads as zeros
-template <int D> __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char* at, int64_t row_bytes, int rows_left) {
-    const int rows = rows_left < kStep ? rows_left : kStep;
+// `rows_left` rows from `at` on (at most N are read), what lies behind them reads as zeros
+template <int D, int N = kStep> __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char* at, int64_t row_bytes, int rows_left) {
+    const int rows = rows_left < N ? rows_left : N;
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, rows > 0 ? (int)((rows - 1) * row_bytes) + 2 * D : 0, 0x00020000);
 }
 template <typename T> __device__ __forceinline__ unsigned round2(float a, float b) {
@@ -102,30 +112,101 @@ __device__ __forceinline__ Range range_of(const int* cu, int i, int total) {
     const int a = cu[i], b = cu[i + 1];
     return a >= 0 && a <= b && b <= total ? Range{a, b - a} : Range{0, -1};
 }
-struct Found { int seq, tile, of; };     // seq < 0: behind the last tile, `tile` of them
-// Tile `index` of the sequences' tiles of `rows` of length x `group`, in the sequences' order.
-__device__ __forceinline__ Found find(const int* cu, int n, int total, int group, int rows, int index) {
+// sums over the wavefront's lanes up to each one (data-parallel-primitive moves: within rows of 16, then the rows' ends)
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+__device__ __forceinline__ int sums_up_to(int v) {
+    v = dpp_add<0x111, 0xF>(v);      // row_shr 1, 2, 4, 8
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);      // row_bcast 15 to rows 1 and 3
+    return dpp_add<0x143, 0xC>(v);   // row_bcast 31 to rows 2 and 3
+}
+__device__ __forceinline__ int sum_of(int v) { return __builtin_amdgcn_readlane(sums_up_to(v), 63); }
+
+// The tiles of a kernel: kRows rows (or keys) of a sequence each, with `steps` of kStep keys (kRowStep rows) that go by.  Rank 0 of a sequence's tiles is the longest one; the last rows
+// see the most keys, the first keys are seen by the most rows.
+constexpr int kRowStep = 32;
+struct Lengths { int lq, lk; };      // lq < 0 or lk < 0: bad offsets
+template <bool KEYS> struct Tiles {
+    const RaggedParams& p;
+    __device__ __forceinline__ Lengths lengths(int i) const { return {range_of(p.cu_q, i, p.Tq).length, range_of(p.cu_k, i, p.Tk).length}; }
+    __device__ __forceinline__ int count(Lengths n) const {
+        const int64_t rows = KEYS ? n.lk : (int64_t)n.lq * p.group;
+        return rows > 0 ? (int)((rows + kRows - 1) / kRows) : 0;
+    }
+    static __device__ __forceinline__ int at(int rank, int tiles) { return KEYS ? rank : tiles - 1 - rank; }
+    // first row that sees key j, in rows; (rounded up to steps where none does)
+    __device__ __forceinline__ int first_row(Lengths n, int j) const {
+        const int lq = n.lq > 0 ? n.lq : 0, t = j - (n.lk - lq);
+        return !p.causal || t <= 0 ? 0 : t >= lq ? (lq * p.group + kRowStep - 1) / kRowStep * kRowStep : t * p.group;
+    }
+    // keys that row r's token sees
+    __device__ __forceinline__ int keys(Lengths n, int r) const {
+        const int lk = n.lk > 0 ? n.lk : 0, e = r / p.group + lk - n.lq + 1;
+        return !p.causal || e > lk ? lk : e < 0 ? 0 : e;
+    }
+    __device__ __forceinline__ int first_step(Lengths n, int tile) const { return KEYS ? first_row(n, tile * kRows) / kRowStep : 0; }
+    __device__ __forceinline__ int end_step(Lengths n, int tile) const {
+        if (KEYS) return n.lq > 0 ? (n.lq * p.group + kRowStep - 1) / kRowStep : 0;
+        const int rows = n.lq * p.group, last = tile * kRows + kRows - 1;
+        return (keys(n, last < rows ? last : rows - 1) + kStep - 1) / kStep;
+    }
+    __device__ __forceinline__ int steps(Lengths n, int tile) const { return end_step(n, tile) - first_step(n, tile); }
+};
+
+// Parts are written and read in fp32 and joined by a launch of its own, so they have `least` steps at least.  dk and dv, and where shares are large: parts of three fifths of a workgroup's
+// share of all steps, as 512 causal tiles are dealt out evenly only if the long ones are in pieces that short ones fit beside (gradients of 16384 positions, 16 heads on 4, us, parts of a
+// share / of 3/5 / of 2/5: 4558 / 3973 / 3890).  Else five quarters, which are all on the chip at once: a few more than fit take a second round (512 queries, 8 heads each, on 8192 keys: 704
+// parts 72, 520 75, 455 63).
+constexpr int kAtOnce = 2 * kNumCUs;      // workgroups
+constexpr int least_steps(bool keys, int D) { return keys ? D == 128 ? 16 : 64 : D == 128 ? 12 : 24; }
+struct Found { int seq, tile, parts; Lengths n; };     // seq < 0: behind the last tile, `tile` of them
+// Tile `index` of all sequences', in the sequences' order and the longest of each first, and how many parts it is cut into.
+// (The longest of all first, by counts of the tiles longer than some length, for which the length is searched: 5 % slower on 12 prompts and on four documents.  Short tiles, which are mostly
+// waiting, then run beside each other at the end instead of beside long ones.)
+template <bool KEYS> __device__ __forceinline__ Found find(const RaggedParams& p, int index) {
+    const Tiles<KEYS> T{p};
     const int lane = threadIdx.x & 63;
+    Found f = {-1, 0, 1, {0, 0}};
+    // (a sequence's: all of its tiles times the mean of the longest and the shortest; no more than 64 of them add up to in 32 bits)
+    auto share_of = [&](Lengths n, int tiles) {
+        const int64_t sum = tiles ? (int64_t)tiles * (T.steps(n, T.at(0, tiles)) + T.steps(n, T.at(tiles - 1, tiles))) / 2 : 0;
+        return (int)(sum < (1 << 25) ? sum : (1 << 25) - 1);
+    };
     int before = 0;
-    for (int base = 0; base < n; base += 64) {
-        const int i = base + lane;
+    int64_t all = 0;                 // steps
+    for (int base = 0; base < p.n_seq; base += 64) {
+        Lengths n = {-1, -1};
         int tiles = 0;
-        if (i < n) {
-            const Range r = range_of(cu, i, total);
-            tiles = r.length > 0 ? (int)(((int64_t)r.length * group + rows - 1) / rows) : 0;
-        }
-        int sum = tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) { const int up = __shfl_up(sum, d); sum += lane >= d ? up : 0; }
+        if (base + lane < p.n_seq) { n = T.lengths(base + lane); tiles = T.count(n); }
+        const int sum = sums_up_to(tiles);
         const unsigned long long past = __ballot(before + sum > index);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            const int ends = __builtin_amdgcn_readlane(sum, at), of = __builtin_amdgcn_readlane(tiles, at);
-            return {base + at, index - (before + ends - of), of};
+        if (past && f.seq < 0) {
+            const int at = __builtin_ctzll(past), of = __builtin_amdgcn_readlane(tiles, at);
+            f.seq = base + at;
+            f.n = {__builtin_amdgcn_readlane(n.lq, at), __builtin_amdgcn_readlane(n.lk, at)};
+            f.tile = T.at(index - (before + __builtin_amdgcn_readlane(sum, at) - of), of);
+            if (p.most_parts <= 1) return f;
         }
         before += __builtin_amdgcn_readlane(sum, 63);
+        if (p.most_parts > 1) all += sum_of(share_of(n, tiles));
     }
-    return {-1, index - before, 0};
+    if (f.seq < 0) { f.tile = index - before; return f; }
+    const int64_t share = (all * p.Hkv + kAtOnce - 1) / kAtOnce;
+    const int steps = T.steps(f.n, f.tile);
+    const int64_t wish = KEYS || share >= 2 * p.least ? 3 * share / 5 : 5 * share / 4;
+    const int per = wish > p.least ? (int)wish : p.least, parts = (steps + per - 1) / per;
+    f.parts = __builtin_amdgcn_readfirstlane(parts < 1 ? 1 : parts < p.most_parts ? parts : p.most_parts);
+    return f;
+}
+// Of block `b`: the key head, the tile's place among all, the part.  Last parts first, which only long tiles have, and all tiles' first parts at the end, so that short tiles end the call.
+// Parts of one number lie together: a die hands workgroups to its four shader engines in turn, and parts that are
+// not there (their workgroups end at once) among the others leave some engines with nothing else: 37 us became 54 on 368 tiles of 25 steps.
+struct Block { int head, index, part; };
+__device__ __forceinline__ Block block_of(const RaggedParams& p, int b) {
+    const int rest = b / p.Hkv, before = p.most_parts > 1 ? rest / p.tiles : 0;
+    return {b - rest * p.Hkv, rest - before * p.tiles, p.most_parts - 1 - before};
 }
 
 // ---- rows of no sequence: zeros, lse = -inf
@@ -156,15 +237,17 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
     typedef typename VecOf<T>::v8 V8;
     typedef Tile<D> L;
     constexpr int NC = D / 16, NB = D / 32;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    LDS_TILES(L);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int head = blockIdx.x % p.Hkv;
-    const Found f = find(p.cu_q, p.n_seq, p.Tq, p.group, kRows, blockIdx.x / p.Hkv);
+    const Block block = block_of(p, blockIdx.x);
+    const int head = block.head;
+    const Found f = find<false>(p, block.index);
     if (f.seq < 0) {
-        if (p.fill) clear_rows<D>(p.o, p.o_row, p.o_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f.tile, p.lse);
+        if (p.fill && block.part == 0) clear_rows<D>(p.o, p.o_row, p.o_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f.tile, p.lse);
         return;
     }
-    const int tile = f.of - 1 - f.tile;             // (causal: the longest first)
+    if (block.part >= f.parts) return;
+    const int tile = f.tile;
     const Range rq = range_of(p.cu_q, f.seq, p.Tq), rk = range_of(p.cu_k, f.seq, p.Tk);
     const int rows = rq.length * p.group, lk = rk.length > 0 ? rk.length : 0, shift = lk - rq.length;
     const int row = tile * kRows + 32 * wave + (lane & 31);
@@ -176,7 +259,9 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
     const int first = tile * kRows + 32 * wave;
     auto token_at = [&](int r) { return __builtin_amdgcn_readfirstlane((r < rows ? r : rows - 1) / p.group); };
     const int wave_end = first < rows ? keys_of(token_at(first + 31)) : 0, wave_all = keys_of(token_at(first));
-    const int n = (keys_of(token_at(tile * kRows + kRows - 1)) + kStep - 1) / kStep;
+    // steps of this part
+    const int steps = Tiles<false>{p}.end_step(f.n, tile);
+    const int t0 = (int)((int64_t)block.part * steps / f.parts), n = (int)((int64_t)(block.part + 1) * steps / f.parts);
 
     const char* const kp = p.k + rk.start * p.k_row + head * p.k_head;
     const char* const vp = p.v + rk.start * p.v_row + head * p.v_head;
@@ -186,15 +271,14 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
         k_off[i] = L::load_row(lane, wave, i) * (int)p.k_row + L::load_byte(lane, wave, i);
         v_off[i] = L::load_row(lane, wave, i) * (int)p.v_row + L::load_byte(lane, wave, i);
     }
-    auto fill = [&](int t) {
+    auto fill = [&](int t, char* kt, char* vt) __attribute__((always_inline)) {
         const auto kr = rows_of<D>(kp + (int64_t)t * kStep * p.k_row, p.k_row, lk - t * kStep), vr = rows_of<D>(vp + (int64_t)t * kStep * p.v_row, p.v_row, lk - t * kStep);
-        char* const to = smem + (t & 1) * 2 * L::BYTES;
 #pragma unroll
-        for (int i = 0; i < L::LOADS; ++i) load_to_lds(kr, to + L::load_to(wave, i), k_off[i]);
+        for (int i = 0; i < L::LOADS; ++i) load_to_lds(kr, kt + L::load_to(wave, i), k_off[i]);
 #pragma unroll
-        for (int i = 0; i < L::LOADS; ++i) load_to_lds(vr, to + L::BYTES + L::load_to(wave, i), v_off[i]);
+        for (int i = 0; i < L::LOADS; ++i) load_to_lds(vr, vt + L::load_to(wave, i), v_off[i]);
     };
-    if (n > 0) fill(0);
+    if (t0 < n) fill(t0, tile0, tile1);
 
     // Q as an operand: channels 16 c + 8 half .. + 7 of this lane's row
     V8 qf[NC];
@@ -219,13 +303,9 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
     float m = kLowest, l = 0.f;       // (l: of this lane's half of the keys)
 
-    for (int t = 0; t < n; ++t) {
-        meet();
-        if (t + 1 < n) fill(t + 1);
+    auto step = [&](int t, const char* kt, const char* vt) __attribute__((always_inline)) {
         const int key0 = t * kStep;
-        if (key0 >= wave_end) continue;
-        const char* const kt = smem + (t & 1) * 2 * L::BYTES;
-        const char* const vt = kt + L::BYTES;
+        if (key0 >= wave_end) return;
         f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
         for (int c = 0; c < NC; ++c)
@@ -271,9 +351,27 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[b] = mfma32(read_channels<V8>(vt + 16 * c * L::ROW, v_at[b][0], v_at[b][1]), pf[c], acc[b]);
+    };
+    for (int t = t0; t < n; t += 2) {
+        meet();
+        if (t + 1 < n) fill(t + 1, tile2, tile3);
+        step(t, tile0, tile1);
+        if (t + 1 == n) break;
+        meet();
+        if (t + 2 < n) fill(t + 2, tile0, tile1);
+        step(t + 1, tile2, tile3);
     }
     if (!live) return;
     l = over_halves_sum(l);
+    if (f.parts > 1) {
+        float* const part = p.parts + (((int64_t)block.index * p.Hkv + head) * p.most_parts + block.part) * kPartFloats<D> + (32 * wave + (lane & 31)) * (D + 2);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x2*>(part + 2 + 32 * b + 8 * i + 4 * half) = f32x2{acc[b][4 * i], acc[b][4 * i + 1]}, *reinterpret_cast<f32x2*>(part + 4 + 32 * b + 8 * i + 4 * half) = f32x2{acc[b][4 * i + 2], acc[b][4 * i + 3]};
+        if (half == 0) *reinterpret_cast<f32x2*>(part) = f32x2{m, l};
+        return;
+    }
     float by = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
     float lse = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * 0.693147180559945309f : l == 0.f ? -INFINITY : l;
     if (rk.length < 0) by = lse = NAN;
@@ -294,15 +392,17 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
     typedef typename VecOf<T>::v8 V8;
     typedef Tile<D> L;
     constexpr int NC = D / 16, NB = D / 32;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    LDS_TILES(L);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int head = blockIdx.x % p.Hkv;
-    const Found f = find(p.cu_q, p.n_seq, p.Tq, p.group, kRows, blockIdx.x / p.Hkv);
+    const Block block = block_of(p, blockIdx.x);
+    const int head = block.head;
+    const Found f = find<false>(p, block.index);
     if (f.seq < 0) {
-        clear_rows<D>(p.dq, p.dq_row, p.dq_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f.tile, nullptr);
+        if (block.part == 0) clear_rows<D>(p.dq, p.dq_row, p.dq_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f.tile, nullptr);
         return;
     }
-    const int tile = f.of - 1 - f.tile;
+    if (block.part >= f.parts) return;
+    const int tile = f.tile;
     const Range rq = range_of(p.cu_q, f.seq, p.Tq), rk = range_of(p.cu_k, f.seq, p.Tk);
     const int rows = rq.length * p.group, lk = rk.length > 0 ? rk.length : 0, shift = lk - rq.length;
     const int row = tile * kRows + 32 * wave + (lane & 31);
@@ -313,7 +413,9 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
     const int first = tile * kRows + 32 * wave;
     auto token_at = [&](int r) { return __builtin_amdgcn_readfirstlane((r < rows ? r : rows - 1) / p.group); };
     const int wave_end = first < rows ? keys_of(token_at(first + 31)) : 0, wave_all = keys_of(token_at(first));
-    const int n = (keys_of(token_at(tile * kRows + kRows - 1)) + kStep - 1) / kStep;
+    // steps of this part
+    const int steps = Tiles<false>{p}.end_step(f.n, tile);
+    const int t0 = (int)((int64_t)block.part * steps / f.parts), n = (int)((int64_t)(block.part + 1) * steps / f.parts);
 
     const char* const kp = p.k + rk.start * p.k_row + head * p.k_head;
     const char* const vp = p.v + rk.start * p.v_row + head * p.v_head;
@@ -323,15 +425,14 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
         k_off[i] = L::load_row(lane, wave, i) * (int)p.k_row + L::load_byte(lane, wave, i);
         v_off[i] = L::load_row(lane, wave, i) * (int)p.v_row + L::load_byte(lane, wave, i);
     }
-    auto fill = [&](int t) {
+    auto fill = [&](int t, char* kt, char* vt) __attribute__((always_inline)) {
         const auto kr = rows_of<D>(kp + (int64_t)t * kStep * p.k_row, p.k_row, lk - t * kStep), vr = rows_of<D>(vp + (int64_t)t * kStep * p.v_row, p.v_row, lk - t * kStep);
-        char* const to = smem + (t & 1) * 2 * L::BYTES;
 #pragma unroll
-        for (int i = 0; i < L::LOADS; ++i) load_to_lds(kr, to + L::load_to(wave, i), k_off[i]);
+        for (int i = 0; i < L::LOADS; ++i) load_to_lds(kr, kt + L::load_to(wave, i), k_off[i]);
 #pragma unroll
-        for (int i = 0; i < L::LOADS; ++i) load_to_lds(vr, to + L::BYTES + L::load_to(wave, i), v_off[i]);
+        for (int i = 0; i < L::LOADS; ++i) load_to_lds(vr, vt + L::load_to(wave, i), v_off[i]);
     };
-    if (n > 0) fill(0);
+    if (t0 < n) fill(t0, tile0, tile1);
 
     V8 qf[NC], gf[NC];
     float delta = 0.f;
@@ -361,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
     if (live) {
         const float x = p.lse[stat];
         lse2 = x == -INFINITY ? INFINITY : x * 1.44269504088896341f;
-        if (half == 0) p.delta[stat] = delta;
+        if (half == 0 && block.part == 0) p.delta[stat] = delta;
     }
     int k_at[NC], k_tr[NB][2];
 #pragma unroll
@@ -372,13 +473,9 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
 
-    for (int t = 0; t < n; ++t) {
-        meet();
-        if (t + 1 < n) fill(t + 1);
+    auto step = [&](int t, const char* kt, const char* vt) __attribute__((always_inline)) {
         const int key0 = t * kStep;
-        if (key0 >= wave_end) continue;
-        const char* const kt = smem + (t & 1) * 2 * L::BYTES;
-        const char* const vt = kt + L::BYTES;
+        if (key0 >= wave_end) return;
         const bool masked = key0 + kStep > wave_all;
         const int left = end - key0 - 4 * half;
 #pragma unroll
@@ -410,8 +507,25 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
 #pragma unroll
                 for (int b = 0; b < NB; ++b) acc[b] = mfma32(read_channels<V8>(kt + (32 * h + 16 * c) * L::ROW, k_tr[b][0], k_tr[b][1]), df[c], acc[b]);
         }
+    };
+    for (int t = t0; t < n; t += 2) {
+        meet();
+        if (t + 1 < n) fill(t + 1, tile2, tile3);
+        step(t, tile0, tile1);
+        if (t + 1 == n) break;
+        meet();
+        if (t + 2 < n) fill(t + 2, tile0, tile1);
+        step(t + 1, tile2, tile3);
     }
     if (!live) return;
+    if (f.parts > 1) {
+        float* const part = p.parts + (((int64_t)block.index * p.Hkv + head) * p.most_parts + block.part) * (kRows * D) + (32 * wave + (lane & 31)) * D;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(part + 32 * b + 8 * i + 4 * half) = f32x4{acc[b][4 * i], acc[b][4 * i + 1], acc[b][4 * i + 2], acc[b][4 * i + 3]};
+        return;
+    }
     const float by = p.scale;
     char* const at = p.dq + (rq.start + token) * p.dq_row + hq * p.dq_head + 8 * half;
 #pragma unroll
@@ -423,33 +537,47 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
 }
 
 // ---- backward, second kernel: dk and dv.  A workgroup: 128 keys of one sequence and key head, a wavefront 32 of them, one a lane; the sequence's rows (of all heads of the group) go by in
-// steps of kStep.  S = Q K^T has the rows in registers: P and dS, rounded, are operands of dV^T += dO^T P and dK^T += Q^T dS where they lie.
+// steps of kRowStep.  S = Q K^T has the rows in registers: P and dS, rounded, are operands of dV^T += dO^T P and dK^T += Q^T dS where they lie.  K stays in registers, V too at head dim 64 and in
+// LDS at 128: with both in registers there are too many for two wavefronts on a SIMD, whose matrix products and other arithmetic go on beside each other (head dim 64, 1560 + 880 + 390 positions,
+// 16 heads, us, dq with it, V in LDS / in registers: 95 / 87).
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, D == 128 ? 1 : 2) ragged_dkdv_kernel(const RaggedParams p) {
+__global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef typename VecOf<T>::v8 V8;
-    typedef Tile<D> L;
+    typedef Tile<D, kRowStep> L;
+    typedef Tile<D, kRows> LV;
     constexpr int NC = D / 16, NB = D / 32;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
-    float* const stats = reinterpret_cast<float*>(smem + 4 * L::BYTES);       // [2][lse, delta][kStep]
+    LDS_TILES(L);
+    constexpr bool V_IN_LDS = D == 128;
+    __shared__ __attribute__((aligned(1024))) char values[V_IN_LDS ? LV::BYTES : 16];
+    __shared__ __attribute__((aligned(16))) float stats0[2 * kRowStep], stats1[2 * kRowStep];      // lse, delta of a step's rows
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int head = blockIdx.x % p.Hkv;
-    const Found f = find(p.cu_k, p.n_seq, p.Tk, 1, kRows, blockIdx.x / p.Hkv);
+    const Block block = block_of(p, blockIdx.x);
+    const int head = block.head;
+    const Found f = find<true>(p, block.index);
     if (f.seq < 0) {
+        if (block.part) return;
         clear_rows<D>(p.dk, p.dk_row, p.dk_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f.tile, nullptr);
         clear_rows<D>(p.dv, p.dv_row, p.dv_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f.tile, nullptr);
         return;
     }
+    if (block.part >= f.parts) return;
     const Range rq = range_of(p.cu_q, f.seq, p.Tq), rk = range_of(p.cu_k, f.seq, p.Tk);
-    const int lq = rq.length > 0 ? rq.length : 0, rows = lq * p.group, shift = rk.length - lq;
-    const int key = f.tile * kRows + 32 * wave + (lane & 31);
+    const int lq = rq.length > 0 ? rq.length : 0;
+    const int key0 = f.tile * kRows, key = key0 + 32 * wave + (lane & 31);
     const bool live = key < rk.length;
-    // the first row that sees a key
-    auto first_of = [&](int j) { const int t = j - shift; return !p.causal || t <= 0 ? 0 : t >= lq ? rows : t * p.group; };
-    const int from = first_of(key);
-    const int wave_first = __builtin_amdgcn_readfirstlane(first_of(f.tile * kRows + 32 * wave)), wave_all = __builtin_amdgcn_readfirstlane(first_of(f.tile * kRows + 32 * wave + 31));
-    const int t0 = __builtin_amdgcn_readfirstlane(first_of(f.tile * kRows)) / kStep, n = (rows + kStep - 1) / kStep;
+    const Tiles<true> tiles{p};
+    const int from = tiles.first_row(f.n, key);
+    const int wave_first = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave)), wave_all = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave + 31));
+    // steps of this part
+    const int begin = tiles.first_step(f.n, f.tile), steps = tiles.end_step(f.n, f.tile) - begin;
+    const int t0 = begin + (int)((int64_t)block.part * steps / f.parts), n = begin + (int)((int64_t)(block.part + 1) * steps / f.parts);
 
+    if constexpr (V_IN_LDS) {
+        const auto vr = rows_of<D, kRows>(p.v + (rk.start + (int64_t)key0) * p.v_row + head * p.v_head, p.v_row, rk.length - key0);
+#pragma unroll
+        for (int i = 0; i < LV::LOADS; ++i) load_to_lds(vr, values + LV::load_to(wave, i), LV::load_row(lane, wave, i) * (int)p.v_row + LV::load_byte(lane, wave, i));
+    }
     V8 kf[NC], vf[NC];
     {
         const char* const ka = p.k + (rk.start + (live ? key : 0)) * p.k_row + head * p.k_head + 16 * half;
@@ -457,41 +585,40 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 1 : 2) ragged_dkdv_kernel
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             kf[c] = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(ka + 32 * c) ^ p.flip);
-            vf[c] = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(va + 32 * c));
+            if constexpr (!V_IN_LDS) vf[c] = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(va + 32 * c));
         }
     }
-    // this lane's row of each load: the token in the step's first, and the head; both go on by kStep rows a step
-    const int step_tokens = kStep / p.group, step_heads = kStep - step_tokens * p.group;
+    // this lane's row of each load: the token and the head; both go on by kRowStep rows a step
+    const int step_tokens = kRowStep / p.group, step_heads = kRowStep - step_tokens * p.group;
     int token[L::LOADS], hd[L::LOADS], byte[L::LOADS];
 #pragma unroll
     for (int i = 0; i < L::LOADS; ++i) {
-        const int r = t0 * kStep + L::load_row(lane, wave, i);
+        const int r = t0 * kRowStep + L::load_row(lane, wave, i);
         token[i] = r / p.group;
         hd[i] = r - token[i] * p.group;
         byte[i] = L::load_byte(lane, wave, i);
     }
-    const int stat_row = threadIdx.x & (kStep - 1);
-    int stat_token = (t0 * kStep + stat_row) / p.group, stat_head = t0 * kStep + stat_row - stat_token * p.group;
+    const int stat_row = threadIdx.x & (kRowStep - 1);
+    int stat_token = (t0 * kRowStep + stat_row) / p.group, stat_head = t0 * kRowStep + stat_row - stat_token * p.group;
     float stat = 0.f;
     const char* const qp = p.q + rq.start * p.q_row + (int64_t)head * p.group * p.q_head;
     const char* const gp = p.dout + rq.start * p.do_row + (int64_t)head * p.group * p.do_head;
     auto next = [&](int& t, int& h) { t += step_tokens; h += step_heads; const bool over = h >= p.group; t += over; h -= over ? p.group : 0; };
-    auto fill = [&](int t) {
-        const int base = t * kStep / p.group;      // (uniform) token that offsets are counted from
+    auto fill = [&](int t, char* qt, char* gt) __attribute__((always_inline)) {
+        const int base = t * kRowStep / p.group;      // (uniform) token that offsets are counted from
         const auto qr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(qp + base * p.q_row), 0, 0x7FFFFFFF, 0x00020000);
         const auto gr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(gp + base * p.do_row), 0, 0x7FFFFFFF, 0x00020000);
-        char* const to = smem + (t & 1) * 2 * L::BYTES;
 #pragma unroll
         for (int i = 0; i < L::LOADS; ++i) {
             const bool in = token[i] < lq;
-            load_to_lds(qr, to + L::load_to(wave, i), in ? (token[i] - base) * (int)p.q_row + hd[i] * (int)p.q_head + byte[i] : (int)0x80000000);
-            load_to_lds(gr, to + L::BYTES + L::load_to(wave, i), in ? (token[i] - base) * (int)p.do_row + hd[i] * (int)p.do_head + byte[i] : (int)0x80000000);
+            load_to_lds(qr, qt + L::load_to(wave, i), in ? (token[i] - base) * (int)p.q_row + hd[i] * (int)p.q_head + byte[i] : (int)0x80000000);
+            load_to_lds(gr, gt + L::load_to(wave, i), in ? (token[i] - base) * (int)p.do_row + hd[i] * (int)p.do_head + byte[i] : (int)0x80000000);
             next(token[i], hd[i]);
         }
-        if (threadIdx.x < 2 * kStep) {             // lse (threads 0 ..) and delta (threads kStep ..) of the step's rows
+        if (threadIdx.x < 2 * kRowStep) {             // lse (threads 0 ..) and delta (threads kRowStep ..) of the step's rows
             const bool in = stat_token < lq;
-            const float* const of = threadIdx.x < kStep ? p.lse : p.delta;
-            stat = threadIdx.x < kStep ? -INFINITY : 0.f;
+            const float* const of = threadIdx.x < kRowStep ? p.lse : p.delta;
+            stat = threadIdx.x < kRowStep ? -INFINITY : 0.f;
             if (in) stat = of[(int64_t)(head * p.group + stat_head) * p.Tq + rq.start + stat_token];
             next(stat_token, stat_head);
         }
@@ -501,69 +628,85 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 1 : 2) ragged_dkdv_kernel
     for (int c = 0; c < NC; ++c) q_at[c] = L::at(lane, c);
 #pragma unroll
     for (int b = 0; b < NB; ++b) { q_tr[b][0] = L::at_transposed(lane, b, 0); q_tr[b][1] = L::at_transposed(lane, b, 1); }
+    const char* const mine = values + 32 * wave * L::ROW;
     f32x16 dk[NB], dv[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) dk[b] = dv[b] = f32x16{};
 
-    if (t0 < n) fill(t0);
-    for (int t = t0; t < n; ++t) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        // (P = 0 where there is no row, or nothing that it sees)
-        if (threadIdx.x < 2 * kStep) stats[(t & 1) * 2 * kStep + threadIdx.x] = threadIdx.x >= kStep ? stat : stat == -INFINITY ? INFINITY : stat * 1.44269504088896341f;
-        meet();
-        if (t + 1 < n) fill(t + 1);
-        const int row0 = t * kStep;
-        if (row0 + kStep <= wave_first) continue;
-        const char* const qt = smem + (t & 1) * 2 * L::BYTES;
-        const char* const gt = qt + L::BYTES;
-        const float* const st = stats + (t & 1) * 2 * kStep;
-        const bool masked = row0 < wave_all;
+    auto step = [&](int t, const char* qt, const char* gt, const float* st) __attribute__((always_inline)) {
+        const int row0 = t * kRowStep;
+        if (row0 + kRowStep <= wave_first) return;
+        f32x16 s = f32x16{}, g = f32x16{};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            f32x16 s = f32x16{}, g = f32x16{};
+        for (int c = 0; c < NC; ++c) {
+            s = mfma32(read_rows<V8>(qt, q_at[c]), kf[c], s);
+            if constexpr (V_IN_LDS) g = mfma32(read_rows<V8>(gt, q_at[c]), read_rows<V8>(mine, q_at[c]), g);
+            else g = mfma32(read_rows<V8>(gt, q_at[c]), vf[c], g);
+        }
+        // element e: row 8 (e / 4) + 4 half + e % 4
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                s = mfma32(read_rows<V8>(qt + 32 * h * L::ROW, q_at[c]), kf[c], s);
-                g = mfma32(read_rows<V8>(gt + 32 * h * L::ROW, q_at[c]), vf[c], g);
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 8 * i + 4 * half), delta = *reinterpret_cast<const f32x4*>(st + kRowStep + 8 * i + 4 * half);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[4 * i + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + j], p.scale_log2, -lse[j]));
+                g[4 * i + j] -= delta[j];
             }
-            // element e: row 8 (e / 4) + 4 half + e % 4
+        }
+        if (row0 < wave_all) {
+            const int left = from - row0 - 4 * half;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) >= left ? s[e] : 0.f;
+        }
+        V8 pf[2], df[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            u32x4 w, x;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 32 * h + 8 * i + 4 * half), delta = *reinterpret_cast<const f32x4*>(st + kStep + 32 * h + 8 * i + 4 * half);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[4 * i + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + j], p.scale_log2, -lse[j]));
-                    g[4 * i + j] -= delta[j];
-                }
+                const int e = 8 * c + 2 * i;
+                w[i] = round2<T>(s[e], s[e + 1]);
+                x[i] = round2<T>(s[e] * g[e], s[e + 1] * g[e + 1]);
             }
-            if (masked) {
-                const int left = from - row0 - 32 * h - 4 * half;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) >= left ? s[e] : 0.f;
-            }
-            V8 pf[2], df[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                u32x4 w, x;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int e = 8 * c + 2 * i;
-                    w[i] = round2<T>(s[e], s[e + 1]);
-                    x[i] = round2<T>(s[e] * g[e], s[e + 1] * g[e + 1]);
-                }
-                pf[c] = __builtin_bit_cast(V8, w);
-                df[c] = __builtin_bit_cast(V8, x);
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    dv[b] = mfma32(read_channels<V8>(gt + (32 * h + 16 * c) * L::ROW, q_tr[b][0], q_tr[b][1]), pf[c], dv[b]);
-                    dk[b] = mfma32(read_channels<V8>(qt + (32 * h + 16 * c) * L::ROW, q_tr[b][0], q_tr[b][1]), df[c], dk[b]);
-                }
+            pf[c] = __builtin_bit_cast(V8, w);
+            df[c] = __builtin_bit_cast(V8, x);
         }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                dv[b] = mfma32(read_channels<V8>(gt + 16 * c * L::ROW, q_tr[b][0], q_tr[b][1]), pf[c], dv[b]);
+                dk[b] = mfma32(read_channels<V8>(qt + 16 * c * L::ROW, q_tr[b][0], q_tr[b][1]), df[c], dk[b]);
+            }
+    };
+    // (P = 0 where there is no row, or nothing that it sees)
+    auto keep = [&](float* st) __attribute__((always_inline)) {
+        if (threadIdx.x < 2 * kRowStep) st[threadIdx.x] = threadIdx.x >= kRowStep ? stat : stat == -INFINITY ? INFINITY : stat * 1.44269504088896341f;
+    };
+    if (t0 < n) fill(t0, tile0, tile1);
+    for (int t = t0; t < n; t += 2) {
+        keep(stats0);
+        meet();
+        if (t + 1 < n) fill(t + 1, tile2, tile3);
+        step(t, tile0, tile1, stats0);
+        if (t + 1 == n) break;
+        keep(stats1);
+        meet();
+        if (t + 2 < n) fill(t + 2, tile0, tile1);
+        step(t + 1, tile2, tile3, stats1);
     }
     if (!live) return;
+    if (f.parts > 1) {
+        float* const part = p.parts + (((int64_t)block.index * p.Hkv + head) * p.most_parts + block.part) * (2 * kRows * D) + (32 * wave + (lane & 31)) * D;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                *reinterpret_cast<f32x4*>(part + 32 * b + 8 * i + 4 * half) = f32x4{dk[b][4 * i], dk[b][4 * i + 1], dk[b][4 * i + 2], dk[b][4 * i + 3]};
+                *reinterpret_cast<f32x4*>(part + kRows * D + 32 * b + 8 * i + 4 * half) = f32x4{dv[b][4 * i], dv[b][4 * i + 1], dv[b][4 * i + 2], dv[b][4 * i + 3]};
+            }
+        return;
+    }
     char* const ka = p.dk + (rk.start + key) * p.dk_row + head * p.dk_head + 8 * half;
     char* const va = p.dv + (rk.start + key) * p.dv_row + head * p.dv_head + 8 * half;
     const float by = p.scale;
@@ -574,6 +717,61 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 1 : 2) ragged_dkdv_kernel
             *reinterpret_cast<u32x2*>(ka + 64 * b + 16 * i) = u32x2{round2<T>(dk[b][4 * i] * by, dk[b][4 * i + 1] * by), round2<T>(dk[b][4 * i + 2] * by, dk[b][4 * i + 3] * by)};
             *reinterpret_cast<u32x2*>(va + 64 * b + 16 * i) = u32x2{round2<T>(dv[b][4 * i], dv[b][4 * i + 1]), round2<T>(dv[b][4 * i + 2], dv[b][4 * i + 3])};
         }
+#endif
+}
+
+// ---- the tiles that were cut: their parts added up, D / 4 lanes to a row.  WHICH: 0 o and lse, 1 dq, 2 dk and dv
+constexpr int kJoinThreads = 1024;
+template <int D> constexpr int kJoinBlocks = kRows * (D / 4) / kJoinThreads;      // of a tile
+template <typename T, int D, int WHICH>
+__global__ void __launch_bounds__(kJoinThreads) ragged_join_kernel(const RaggedParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr bool KEYS = WHICH == 2;
+    constexpr int LANES = D / 4, AT_ONCE = kJoinThreads / LANES;
+    const int head = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv % p.tiles;
+    const Found f = find<KEYS>(p, index);
+    if (f.seq < 0 || f.parts <= 1) return;
+    const int c = 4 * (threadIdx.x % LANES);
+    const Range r = range_of(KEYS ? p.cu_k : p.cu_q, f.seq, KEYS ? p.Tk : p.Tq);
+    const int rows = KEYS ? r.length : r.length * p.group;
+    const float* const from = p.parts + ((int64_t)index * p.Hkv + head) * p.most_parts * (WHICH == 0 ? kPartFloats<D> : WHICH * kRows * D);
+    auto store = [&](char* to, f32x4 x) { *reinterpret_cast<u32x2*>(to + 2 * c) = u32x2{round2<T>(x[0], x[1]), round2<T>(x[2], x[3])}; };
+    const int i = blockIdx.x / (p.Hkv * p.tiles) * AT_ONCE + threadIdx.x / LANES;
+    const int row = f.tile * kRows + i;
+    if (row >= rows) return;
+    const int token = KEYS ? row : row / p.group, h = KEYS ? head : head * p.group + (row - token * p.group);
+    if constexpr (WHICH == 0) {
+        const float* const at = from + i * (D + 2);
+        float m = kLowest, l = 0.f;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = 0; s < f.parts; ++s) m = fmaxf(m, at[s * kPartFloats<D>]);
+#pragma unroll 4
+        for (int s = 0; s < f.parts; ++s) {
+            const float* const a = at + s * kPartFloats<D>;
+            const float by = __builtin_amdgcn_exp2f(a[0] - m);
+            const f32x2 lo = *reinterpret_cast<const f32x2*>(a + 2 + c), hi = *reinterpret_cast<const f32x2*>(a + 4 + c);
+            l += by * a[1];
+            sum += by * f32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+        const float by = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+        store(p.o + (r.start + token) * p.o_row + h * p.o_head, sum * by);
+        if (p.lse && c == 0) p.lse[(int64_t)h * p.Tq + r.start + token] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * 0.693147180559945309f : l == 0.f ? -INFINITY : l;
+    } else {
+        f32x4 sum[WHICH];
+#pragma unroll
+        for (int w = 0; w < WHICH; ++w) {
+            sum[w] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int s = 0; s < f.parts; ++s) sum[w] += *reinterpret_cast<const f32x4*>(from + (WHICH * s + w) * (kRows * D) + i * D + c);
+        }
+        if constexpr (WHICH == 1) {
+            store(p.dq + (r.start + token) * p.dq_row + h * p.dq_head, sum[0] * p.scale);
+        } else {
+            store(p.dk + (r.start + token) * p.dk_row + h * p.dk_head, sum[0] * p.scale);
+            store(p.dv + (r.start + token) * p.dv_row + h * p.dv_head, sum[1]);
+        }
+    }
 #endif
 }
 
@@ -608,7 +806,7 @@ int check(const cosmos_attn_ragged_desc* d, bool backward) {
     const int64_t group = d->Hq / d->Hkv;
     // (tile counts and rows are 32-bit numbers)
     if (d->Tq * group > kMost / 2 || d->Tk > kMost / 2) return COSMOS_ATTN_UNSUPPORTED;
-    if (((d->Tq * group + d->Tk) / kRows + d->n_seq + 1) * d->Hkv > kMost) return COSMOS_ATTN_UNSUPPORTED;
+    if (((d->Tq * group + d->Tk) / kRows + d->n_seq + 1) * d->Hkv > kMost / 32) return COSMOS_ATTN_UNSUPPORTED;
     if (!d->cu_q || !d->cu_k) return COSMOS_ATTN_BAD_ARG;
     if ((reinterpret_cast<uintptr_t>(d->cu_q) | reinterpret_cast<uintptr_t>(d->cu_k)) & 3) return COSMOS_ATTN_BAD_STRIDE;
     int st = COSMOS_ATTN_OK;
@@ -653,10 +851,9 @@ RaggedParams params_of(const cosmos_attn_ragged_desc* d) {
     return p;
 }
 
-template <typename P> int launch(void (*kernel)(P), int64_t blocks, size_t lds, const P& p, hipStream_t stream) {
+int launch(void (*kernel)(RaggedParams), int64_t blocks, const RaggedParams& p, void* stream, int threads = kThreads) {
     if (blocks <= 0) return COSMOS_ATTN_OK;
-    if (!allow_lds((const void*)kernel, lds)) return COSMOS_ATTN_LAUNCH_FAILED;
-    kernel<<<dim3((unsigned)blocks), dim3(kThreads), lds, stream>>>(p);
+    kernel<<<dim3((unsigned)blocks), dim3(threads), 0, (hipStream_t)stream>>>(p);
     return hipGetLastError() == hipSuccess ? COSMOS_ATTN_OK : COSMOS_ATTN_LAUNCH_FAILED;
 }
 template <typename F> int with_type(int dtype, int D, F&& f) {
@@ -665,40 +862,78 @@ template <typename F> int with_type(int dtype, int D, F&& f) {
 }
 // at most so many tiles are there: each sequence rounds up once, and so do the rows of none
 int64_t most_tiles(int64_t rows, int n_seq) { return rows / kRows + n_seq + 1; }
+// Parts that a tile may be cut into.  A call with fewer tiles than some rounds of workgroups ends with its longest tiles on a few compute units; one with more is dealt out evenly as it is.
+// (The workgroups of parts that a tile does not have end at once.)
+constexpr int64_t kFullGrid = 6 * kNumCUs;
+int most_parts(int64_t tiles, int64_t longest, int least) {
+    int64_t parts = (kFullGrid + tiles - 1) / tiles;
+    parts = parts < 16 ? parts : 16;
+    const int64_t of_length = longest / least;
+    parts = parts < of_length ? parts : of_length;
+    return parts > 1 ? (int)parts : 1;
+}
+struct Cut { int64_t tiles; int parts, least; size_t bytes; };
+Cut cut_of(const cosmos_attn_ragged_desc* d, int which) {
+    const int64_t group = d->Hq / d->Hkv, rows = d->Tq * group, tiles = which == 2 ? most_tiles(d->Tk, d->n_seq) : most_tiles(rows, d->n_seq);
+    const int64_t longest = which == 2 ? (rows + kRowStep - 1) / kRowStep : (d->Tk + kStep - 1) / kStep;
+    const int least = least_steps(which == 2, d->D), parts = most_parts(tiles * d->Hkv, longest, least);
+    return {tiles, parts, least, parts > 1 ? (size_t)tiles * d->Hkv * parts * kRows * (which == 0 ? d->D + 2 : which * d->D) * sizeof(float) : 0};
+}
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 
 extern "C" {
 
-int cosmos_attn_ragged(const cosmos_attn_ragged_desc* desc, void* stream) {
+size_t cosmos_attn_ragged_workspace_bytes(const cosmos_attn_ragged_desc* desc) { return check(desc, false) == COSMOS_ATTN_OK ? cut_of(desc, 0).bytes : 0; }
+
+int cosmos_attn_ragged(const cosmos_attn_ragged_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
     const int st = check(desc, false);
     if (st != COSMOS_ATTN_OK) return st;
     if (!desc->Tq) return COSMOS_ATTN_OK;
+    const Cut cut = cut_of(desc, 0);
+    if (workspace_bytes < cut.bytes || (cut.bytes && !workspace)) return COSMOS_ATTN_WORKSPACE_TOO_SMALL;
+    if (cut.bytes && !aligned16(workspace)) return COSMOS_ATTN_BAD_STRIDE;
     if (!device_is_whole_mi355x()) return COSMOS_ATTN_WRONG_DEVICE;
-    const RaggedParams p = params_of(desc);
+    RaggedParams p = params_of(desc);
+    p.tiles = (int)cut.tiles; p.most_parts = cut.parts; p.least = cut.least;
+    p.parts = (float*)workspace;
     return with_type(desc->dtype, desc->D, [&](auto* t, auto d) {
         constexpr int D = decltype(d)::value;
-        return launch(ragged_fwd_kernel<std::remove_pointer_t<decltype(t)>, D>, most_tiles((int64_t)p.Tq * p.group, p.n_seq) * p.Hkv, 4 * Tile<D>::BYTES, p, (hipStream_t)stream);
+        typedef std::remove_pointer_t<decltype(t)> T;
+        const int done = launch(ragged_fwd_kernel<T, D>, cut.tiles * p.Hkv * cut.parts, p, stream);
+        return done != COSMOS_ATTN_OK || cut.parts == 1 ? done : launch(ragged_join_kernel<T, D, 0>, cut.tiles * p.Hkv * kJoinBlocks<D>, p, stream, kJoinThreads);
     });
 }
 
 size_t cosmos_attn_ragged_bwd_workspace_bytes(const cosmos_attn_ragged_desc* desc) {
-    return check(desc, true) == COSMOS_ATTN_OK ? (size_t)desc->Tq * desc->Hq * sizeof(float) : 0;
+    if (check(desc, true) != COSMOS_ATTN_OK) return 0;
+    const size_t a = cut_of(desc, 1).bytes, b = cut_of(desc, 2).bytes;
+    return up((size_t)desc->Tq * desc->Hq * sizeof(float)) + (a > b ? a : b);
 }
 
 int cosmos_attn_ragged_bwd(const cosmos_attn_ragged_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
     const int st = check(desc, true);
     if (st != COSMOS_ATTN_OK) return st;
-    if (workspace_bytes < cosmos_attn_ragged_bwd_workspace_bytes(desc) || (desc->Tq && !workspace)) return COSMOS_ATTN_WORKSPACE_TOO_SMALL;
+    const size_t wanted = cosmos_attn_ragged_bwd_workspace_bytes(desc);
+    if (workspace_bytes < wanted || (wanted && !workspace)) return COSMOS_ATTN_WORKSPACE_TOO_SMALL;
+    if (wanted && !aligned16(workspace)) return COSMOS_ATTN_BAD_STRIDE;
     if (!device_is_whole_mi355x()) return COSMOS_ATTN_WRONG_DEVICE;
     RaggedParams p = params_of(desc);
     p.delta = (float*)workspace;
+    p.parts = (float*)((char*)workspace + up((size_t)desc->Tq * desc->Hq * sizeof(float)));      // (of dq, then of dk and dv)
     return with_type(desc->dtype, desc->D, [&](auto* t, auto d) {
         constexpr int D = decltype(d)::value;
         typedef std::remove_pointer_t<decltype(t)> T;
-        const int done = desc->Tq ? launch(ragged_dq_kernel<T, D>, most_tiles((int64_t)p.Tq * p.group, p.n_seq) * p.Hkv, 4 * Tile<D>::BYTES, p, (hipStream_t)stream) : COSMOS_ATTN_OK;
-        if (done != COSMOS_ATTN_OK || !desc->Tk) return done;
-        return launch(ragged_dkdv_kernel<T, D>, most_tiles(p.Tk, p.n_seq) * p.Hkv, 4 * Tile<D>::BYTES + 4 * kStep * sizeof(float), p, (hipStream_t)stream);
+        int done = COSMOS_ATTN_OK;
+        auto run = [&](const Cut& cut, auto kernel, auto join) {
+            p.tiles = (int)cut.tiles; p.most_parts = cut.parts; p.least = cut.least;
+            if (done == COSMOS_ATTN_OK) done = launch(kernel, cut.tiles * p.Hkv * cut.parts, p, stream);
+            if (done == COSMOS_ATTN_OK && cut.parts > 1) done = launch(join, cut.tiles * p.Hkv * kJoinBlocks<D>, p, stream, kJoinThreads);
+        };
+        if (desc->Tq) run(cut_of(desc, 1), ragged_dq_kernel<T, D>, ragged_join_kernel<T, D, 1>);
+        if (desc->Tk) run(cut_of(desc, 2), ragged_dkdv_kernel<T, D>, ragged_join_kernel<T, D, 2>);
+        return done;
     });
 }
 

@@ -111,8 +111,11 @@ def ragged_fwd(
         o = out
     lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32) if need_lse else None
     desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, out is None)
-    run = _lib.load_library().cosmos_attn_ragged
-    _lib.raise_for_status(_on_device(q.device, lambda stream: run(desc, stream)))
+    lib = _lib.load_library()
+    ws_bytes = lib.cosmos_attn_ragged_workspace_bytes(desc)
+    workspace = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
+    at = 0 if workspace is None else workspace.data_ptr()
+    _lib.raise_for_status(_on_device(q.device, lambda stream: lib.cosmos_attn_ragged(desc, at, ws_bytes, stream)))
     return o, lse
 
 

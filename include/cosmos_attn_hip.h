@@ -412,7 +412,8 @@ COSMOS_ATTN_API int cosmos_attn_gemm_preferred(const cosmos_attn_gemm_desc *desc
  * What a row does not see has no influence on it as long as it is finite within the row's own sequence; what lies outside of the sequences may be anything.
  *
  * cosmos_attn_ragged_bwd: dq, dk, dv for the gradient dout of o, from the forward's o and lse; rows of no sequence become zeros.  No atomics: the same results every time.
- * The workspace holds a number per row and head.  Outputs must not overlap inputs or each other.
+ * The workspaces hold a number per row and head (backward) and the parts of tiles that are cut where there are few; the bytes follow from the sizes alone, and may be 0.  Outputs must not
+ * overlap inputs or each other.
  */
 typedef struct cosmos_attn_ragged_desc {
     int32_t abi_version, dtype;
@@ -431,7 +432,8 @@ typedef struct cosmos_attn_ragged_desc {
     int64_t dout_stride[2], dq_stride[2], dk_stride[2], dv_stride[2];
 } cosmos_attn_ragged_desc;
 
-COSMOS_ATTN_API int cosmos_attn_ragged(const cosmos_attn_ragged_desc *desc, void *stream);
+COSMOS_ATTN_API size_t cosmos_attn_ragged_workspace_bytes(const cosmos_attn_ragged_desc *desc);
+COSMOS_ATTN_API int cosmos_attn_ragged(const cosmos_attn_ragged_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
 COSMOS_ATTN_API size_t cosmos_attn_ragged_bwd_workspace_bytes(const cosmos_attn_ragged_desc *desc);
 COSMOS_ATTN_API int cosmos_attn_ragged_bwd(const cosmos_attn_ragged_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
 

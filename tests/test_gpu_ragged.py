@@ -74,6 +74,20 @@ def test_many_sequences(pkg, ragged_oracle, gpu):
     both(pkg, ragged_oracle, gpu, lens, lens, 2, 1, 64, FP16, True)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("ql, kl", [([1], [9000]), ([3, 1, 0, 40], [700, 5000, 300, 1100]), ([1500], [1500]), ([900, 1300, 17], [900, 1300, 17]), ([600] + [1] * 70, [2000] + [3] * 70), ([1200, 64], [500, 1100])])
+def test_few_tiles_that_are_cut(pkg, ragged_oracle, gpu, ql, kl, causal):
+    """Fewer tiles than workgroups fit on the chip: long ones are cut along their keys, or rows, and joined."""
+    both(pkg, ragged_oracle, gpu, ql, kl, 2, 1, 64, BF16, causal)
+
+
+def test_lengths_that_are_nearly_one(pkg, ragged_oracle, gpu):
+    """The longest tiles first: as many of one length as sequences, lengths that differ by a step."""
+    for lens in ([65, 64, 63, 129, 128, 127, 1, 193], [128] * 5, [300, 1, 300, 1, 299], [0, 0, 500, 0]):
+        both(pkg, ragged_oracle, gpu, lens, lens, 3, 1, 64, BF16, True)
+        both(pkg, ragged_oracle, gpu, lens, [n + 70 * (i % 3) for i, n in enumerate(lens)], 3, 1, 64, BF16, True)
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 1.0])
 def test_scales(pkg, ragged_oracle, gpu, scale, dtype):

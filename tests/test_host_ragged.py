@@ -35,20 +35,20 @@ def test_ragged_desc_layout_and_status_codes(pkg):
         (dict(o_stride=(128, 64)), L.ST_BAD_STRIDE),
     ]
     for over, want in cases:
-        assert lib.cosmos_attn_ragged(ctypes.byref(ragged_desc(pkg, **over)), None) == want, over
+        assert lib.cosmos_attn_ragged(ctypes.byref(ragged_desc(pkg, **over)), P, 1 << 40, None) == want, over
         if "o_stride" not in over:
             assert lib.cosmos_attn_ragged_bwd(ctypes.byref(ragged_desc(pkg, **over)), P, 1 << 40, None) == want, over
         assert lib.cosmos_attn_ragged_bwd_workspace_bytes(ctypes.byref(ragged_desc(pkg, **over))) == 0 or "o_stride" in over
     # outputs whose rows share memory
     for over in (dict(o_stride=(1024, 0)), dict(o_stride=(512, 128))):
-        assert lib.cosmos_attn_ragged(ctypes.byref(ragged_desc(pkg, **over)), None) == L.ST_BAD_STRIDE
+        assert lib.cosmos_attn_ragged(ctypes.byref(ragged_desc(pkg, **over)), P, 1 << 40, None) == L.ST_BAD_STRIDE
     for over in (dict(dq_stride=(1024, 0)), dict(dk_stride=(128, 128)), dict(dv=None), dict(dout=None), dict(lse=None)):
         assert lib.cosmos_attn_ragged_bwd(ctypes.byref(ragged_desc(pkg, **over)), P, 1 << 40, None) in (L.ST_BAD_STRIDE, L.ST_BAD_ARG), over
     D = ragged_desc(pkg)
     assert lib.cosmos_attn_ragged_bwd_workspace_bytes(ctypes.byref(D)) >= 100 * 8 * 4
     assert lib.cosmos_attn_ragged_bwd(ctypes.byref(D), None, 0, None) == L.ST_WORKSPACE
     # nothing to do: no launch, whatever the addresses are
-    assert lib.cosmos_attn_ragged(ctypes.byref(ragged_desc(pkg, Tq=0, q=None, o=None)), None) == L.ST_OK
+    assert lib.cosmos_attn_ragged(ctypes.byref(ragged_desc(pkg, Tq=0, q=None, o=None)), None, 0, None) == L.ST_OK
 
 
 def cache_desc(pkg, **over):
