@@ -46,7 +46,7 @@ struct CacheParams {
     char* o;
     float* lse;
     int64_t q_row, q_head, o_row, o_head;
-    int group, row_blocks, slots;                 // slots: workgroups per head and block of rows
+    int group, row_blocks, slots, whole;          // slots: workgroups for the shares, per head and block of rows; whole: a workgroup has all of a sequence
     float scale_log2;
     unsigned flip;
     float* parts;
@@ -77,90 +77,172 @@ template <typename T, int KIND, bool H> __device__ __forceinline__ unsigned code
     }
 }
 
-// max over the LANES (8 or 16) neighbouring lanes of a row
-template <int CTRL> __device__ __forceinline__ float dpp_max(float v) {
-    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false)));
+// max over the LANES (4 or 8) neighbouring lanes of a row
+template <int CTRL> __device__ __forceinline__ unsigned dpp_max(unsigned v) {
+    const unsigned moved = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+    return v > moved ? v : moved;
 }
-template <int LANES> __device__ __forceinline__ float row_max(float v) {
+template <int LANES> __device__ __forceinline__ unsigned row_max(unsigned v) {
     v = dpp_max<0xB1>(v);       // quad_perm [1, 0, 3, 2]
     v = dpp_max<0x4E>(v);       // quad_perm [2, 3, 0, 1]
-    v = dpp_max<0x141>(v);      // row_half_mirror
-    return LANES == 16 ? dpp_max<0x140>(v) : v;      // row_mirror
+    return LANES == 8 ? dpp_max<0x141>(v) : v;      // row_half_mirror
 }
 
-// ---- packed rows: which sequence a row is of, and its place there; false: of none
-__device__ __forceinline__ bool place_of(const int* cu, int n, int64_t row, int64_t rows, int& seq, int& place, int& length) {
-    int lo = 0, hi = n;                           // the last offset at or below the row
+// ---- packed rows: which sequence a row is of, and its place there
+struct Place { int seq, at, length; bool in; };
+// the last offset of lo .. hi at or below the row (or lo)
+__device__ __forceinline__ int last_below(const int* cu, int lo, int hi, int64_t row) {
     while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
+        const int mid = (int)(((unsigned)lo + (unsigned)hi + 1) >> 1);
         if (cu[mid] <= row) lo = mid;
         else hi = mid - 1;
     }
-    const int64_t a = cu[lo], b = lo < n ? cu[lo + 1] : a;
-    seq = lo;
-    place = (int)(row - a);
-    length = (int)(b - a);
-    return lo < n && a >= 0 && row >= a && row < b && b <= rows;
+    return lo;
+}
+// `near`: the offset found for the workgroup's first row, most often this one's too
+__device__ __forceinline__ Place place_of(const int* cu, int n, int near, int64_t row, int64_t rows) {
+    int at = near;
+    if (at < n && cu[at + 1] <= row) at = last_below(cu, at + 1, n, row);
+    const int64_t a = cu[at], b = at < n ? cu[at + 1] : a;
+    return {at, (int)(row - a), (int)(b - a), at < n && a >= 0 && row >= a && row < b && b <= rows};
 }
 
-constexpr int kRowsPerThread = 4;      // rows that a thread has under way
+// Both kernels: a lane has EACH elements of a row of a head, 8 where pages hold 16 bits and 16 where they hold codes: 16 bytes of the narrower side.  A workgroup has kUnits times
+// kThreads EACH / D rows, in the packed rows' order, the keys' heads and then the values'.  A thread's rows are looked up, loaded and worked on side by side: one by one, each behind the one
+// before, and with 8 elements, 16384 + 9999 + 1 + 4096 rows of 8 heads in e4m3 took 95 us to write (now 49) and 53 to read back (now 42); 189 MB each way at the rate of a large copy
+// are 37.
+constexpr int kUnits = 2;
+constexpr int each_of(int kind) { return kind == SAME16 ? 8 : 16; }
+template <int D, int EACH> struct Rows {
+    static constexpr int LANES = D / EACH, ROWS = kThreads / LANES;
+    int64_t row[kUnits];          // packed row
+    int head[kUnits];
+    bool value[kUnits], in[kUnits];      // a row of V; there is such a row
+    int first;                    // offset of the first row's sequence
+    __device__ __forceinline__ Rows(const CacheParams& p) {
+        const unsigned both = 2u * (unsigned)p.Hkv;
+        const int64_t unit = (int64_t)blockIdx.x * (kUnits * ROWS), row0 = unit / both;
+        const unsigned over = (unsigned)(unit - row0 * both) + threadIdx.x / LANES;
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const unsigned u = over + i * ROWS, r = u / both, h = u - r * both;
+            row[i] = row0 + r;
+            in[i] = row[i] < p.rows;
+            value[i] = h >= (unsigned)p.Hkv;
+            head[i] = (int)(value[i] ? h - p.Hkv : h);
+        }
+        first = p.cu ? last_below(p.cu, 0, p.B, row0) : 0;
+    }
+    __device__ __forceinline__ char* packed(const CacheParams& p, int i) const {
+        return (value[i] ? p.v_rows + row[i] * p.vr_row + head[i] * p.vr_head : p.k_rows + row[i] * p.kr_row + head[i] * p.kr_head) + 2 * EACH * (threadIdx.x % LANES);
+    }
+    __device__ __forceinline__ char* cached(const CacheParams& p, int i, int page, int at) const {
+        return (value[i] ? p.v + page * p.v_page + head[i] * p.v_head + (int64_t)at * p.v_row : p.k + page * p.k_page + head[i] * p.k_head + (int64_t)at * p.k_row) + 16 * (threadIdx.x % LANES);
+    }
+    __device__ __forceinline__ float* scale(const CacheParams& p, int i, int page, int at) const {
+        return (value[i] ? p.v_scale + page * p.vs_page + head[i] * p.vs_head : p.k_scale + page * p.ks_page + head[i] * p.ks_head) + at;
+    }
+};
 
-// ---- writing: D / 8 lanes to a row, its max by exchanges among them
+// x / s as IEEE division rounds it, for |x / s| up to some hundreds: x r corrected by the remainder, which fma gives exactly (Markstein's division), with r = 1 / s good to an ulp.  (That one
+// correction is enough has been seen for all there is: a 16-bit x has 2^7 or 2^10 significands and s, which follows from another one, as many.)  Rows whose scale would leave the range
+// in which all of that is exact are multiplied with a power of two first, as their scale is.
+struct Divide {
+    float s, r, by;
+    __device__ __forceinline__ explicit Divide(float scale) {
+        by = scale < 0x1p-60f ? 0x1p64f : 1.f;
+        s = scale * by;
+        r = __builtin_amdgcn_rcpf(s);
+        r = __builtin_fmaf(__builtin_fmaf(-s, r, 1.f), r, r);
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        const float q = x * r;
+        return __builtin_fmaf(__builtin_fmaf(-s, q, x), r, q);
+    }
+};
+
+// ---- writing
 template <typename T, int KIND, int D>
 __global__ void __launch_bounds__(kThreads) cache_write_kernel(const CacheParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int LANES = D / 8, ROWS = kThreads / LANES;
-    const int part = threadIdx.x % LANES;
-    const int64_t units = p.rows * 2 * p.Hkv;
+    constexpr int EACH = each_of(KIND);
+    typedef Rows<D, EACH> R;
+    const R rows(p);
+    const int part = threadIdx.x % R::LANES, mask = (1 << p.page_shift) - 1;
+    int page[kUnits], at[kUnits];
+    u32x4 x[kUnits][EACH / 8];
+    bool in[kUnits];
 #pragma unroll
-    for (int i = 0; i < kRowsPerThread; ++i) {
-        const int64_t u = ((int64_t)blockIdx.x * kRowsPerThread + i) * ROWS + threadIdx.x / LANES;
-        if (u >= units) return;
-        const int64_t row = u / (2 * p.Hkv);
-        const int which = (int)(u - row * 2 * p.Hkv), value = which >= p.Hkv, h = value ? which - p.Hkv : which;
-        int seq = (int)row, place = 0, fresh = 1;
-        if (p.cu && !place_of(p.cu, p.B, row, p.rows, seq, place, fresh)) continue;
-        const int at = p.lens[seq] - fresh + place;
-        if (at < 0 || p.lens[seq] < fresh || (at >> p.page_shift) >= p.width) continue;
-        const int page = p.table[seq * p.table_row + (at >> p.page_shift)];
-        if (page < 0 || page >= p.pages) continue;
-        const int in_page = at & ((1 << p.page_shift) - 1);
-        const u32x4 x = *reinterpret_cast<const u32x4*>((value ? p.v_rows + row * p.vr_row + h * p.vr_head : p.k_rows + row * p.kr_row + h * p.kr_head) + 16 * part);
-        char* const to = value ? p.v + page * p.v_page + h * p.v_head + (int64_t)in_page * p.v_row : p.k + page * p.k_page + h * p.k_head + (int64_t)in_page * p.k_row;
+    for (int i = 0; i < kUnits; ++i)
+#pragma unroll
+        for (int j = 0; j < EACH / 8; ++j) {
+            x[i][j] = u32x4{0, 0, 0, 0};
+            if (rows.in[i]) x[i][j] = *reinterpret_cast<const u32x4*>(rows.packed(p, i) + 16 * j);
+        }
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        Place w = {(int)rows.row[i], 0, 1, true};
+        in[i] = rows.in[i];
+        if (in[i] && p.cu) w = place_of(p.cu, p.B, rows.first, rows.row[i], p.rows);
+        in[i] = in[i] && w.in;
+        at[i] = page[i] = 0;
+        if (in[i]) {
+            const int len = p.lens[w.seq], to = len - w.length + w.at;
+            in[i] = len >= w.length && (to >> p.page_shift) < p.width;
+            if (in[i]) page[i] = p.table[w.seq * p.table_row + (to >> p.page_shift)];
+            at[i] = to & mask;
+            in[i] = in[i] && page[i] >= 0 && page[i] < p.pages;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
         if constexpr (KIND == SAME16) {
-            *reinterpret_cast<u32x4*>(to + 16 * part) = x;
+            if (in[i]) *reinterpret_cast<u32x4*>(rows.cached(p, i, page[i], at[i])) = x[i][0];
         } else {
-            float f[8], top = 0.f, nan = 0.f;
+            // the largest magnitude: of 16-bit floats without their signs as whole numbers, in whose order NaN comes behind infinity and that behind all others
+            typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 most = {0, 0};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f[2 * j] = low<T>(x[j]);
-                f[2 * j + 1] = high<T>(x[j]);
-            }
+            for (int j = 0; j < 8; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[i][j / 4][j % 4] & 0x7FFF7FFFu));
+            const unsigned top = row_max<R::LANES>(most[0] > most[1] ? most[0] : most[1]);
+            // (a row of zeros: divided by 1; one that is not finite: codes of no meaning)
+            const float scale = top < (__is_same(T, __bf16) ? 0x7F80u : 0x7C00u) ? low<T>(top) * (KIND == E4M3 ? 1.f / 448.f : 1.f / 127.f) : NAN;
+            const Divide over(scale > 0.f ? scale : 1.f);
+            float f[16];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                top = fmaxf(top, fabsf(f[j]));
-                nan = f[j] == f[j] ? nan : INFINITY;           // (a max passes over NaN)
+                f[2 * j] = low<T>(x[i][j / 4][j % 4]);
+                f[2 * j + 1] = high<T>(x[i][j / 4][j % 4]);
             }
-            top = row_max<LANES>(fmaxf(top, nan));
-            const bool finite = top < INFINITY;
-            const float scale = finite ? top * (KIND == E4M3 ? 1.f / 448.f : 1.f / 127.f) : NAN;
-            const bool some = finite && scale > 0.f;
-            u32x2 codes = {0, 0};
+            if (__any(over.by != 1.f)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = some ? f[j] / scale : 0.f;
+                for (int j = 0; j < 16; ++j) f[j] *= over.by;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) f[j] = over(f[j]);
+            u32x4 codes = {0, 0, 0, 0};
             if constexpr (KIND == E4M3) {
                 // (scale's own rounding may leave a quotient just above 448; the conversion's largest code takes those below 464)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j], f[4 * j + 1], 0, false);
+                for (int j = 0; j < 4; ++j) {
+                    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j], f[4 * j + 1], 0, false);
                     codes[j] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j + 2], f[4 * j + 3], w, true);
                 }
             } else {
+                // 2^23 + 2^22 + f: f rounded to a whole number, ties to even, in the low bits
 #pragma unroll
-                for (int j = 0; j < 8; ++j) codes[j / 4] |= ((unsigned)(int)__builtin_rintf(fminf(fmaxf(f[j], -127.f), 127.f)) & 0xFFu) << 8 * (j % 4);
+                for (int j = 0; j < 4; ++j) {
+                    unsigned w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = __builtin_bit_cast(unsigned, f[4 * j + k] + 12582912.f);
+                    const unsigned lo = __builtin_amdgcn_perm(w[1], w[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(w[3], w[2], 0x04000C0Cu);
+                    codes[j] = lo | hi;
+                }
             }
-            *reinterpret_cast<u32x2*>(to + 8 * part) = codes;
-            if (part == 0) (value ? p.v_scale + page * p.vs_page + h * p.vs_head : p.k_scale + page * p.ks_page + h * p.ks_head)[in_page] = scale;
+            if (in[i]) {
+                *reinterpret_cast<u32x4*>(rows.cached(p, i, page[i], at[i])) = codes;
+                if (part == 0) *rows.scale(p, i, page[i], at[i]) = scale;
+            }
         }
     }
 #endif
@@ -170,78 +252,117 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const CacheParams
 template <typename T, int KIND, int D>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const CacheParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int LANES = D / 8, ROWS = kThreads / LANES;
-    const int part = threadIdx.x % LANES;
-    const int64_t units = p.rows * 2 * p.Hkv;
+    constexpr int EACH = each_of(KIND);
+    typedef Rows<D, EACH> R;
+    const R rows(p);
+    const int mask = (1 << p.page_shift) - 1;
+    int page[kUnits], at[kUnits];
+    bool of[kUnits];              // a row of some sequence
 #pragma unroll
-    for (int i = 0; i < kRowsPerThread; ++i) {
-        const int64_t u = ((int64_t)blockIdx.x * kRowsPerThread + i) * ROWS + threadIdx.x / LANES;
-        if (u >= units) return;
-        const int64_t row = u / (2 * p.Hkv);
-        const int which = (int)(u - row * 2 * p.Hkv), value = which >= p.Hkv, h = value ? which - p.Hkv : which;
-        u32x4* const to = reinterpret_cast<u32x4*>((value ? p.v_rows + row * p.vr_row + h * p.vr_head : p.k_rows + row * p.kr_row + h * p.kr_head) + 16 * part);
-        int seq, at, length;
-        if (!place_of(p.cu, p.B, row, p.rows, seq, at, length)) {
-            if (p.fill) *to = u32x4{0, 0, 0, 0};
-            continue;
+    for (int i = 0; i < kUnits; ++i) {
+        at[i] = 0;
+        page[i] = -1;
+        of[i] = false;
+        if (rows.in[i]) {
+            const Place w = place_of(p.cu, p.B, rows.first, rows.row[i], p.rows);
+            of[i] = w.in;
+            if (w.in && (w.at >> p.page_shift) < p.width) page[i] = p.table[w.seq * p.table_row + (w.at >> p.page_shift)];
+            at[i] = w.at & mask;
+            page[i] = page[i] < p.pages ? page[i] : -1;
         }
-        int page = -1;
-        if ((at >> p.page_shift) < p.width) page = p.table[seq * p.table_row + (at >> p.page_shift)];
-        if (page < 0 || page >= p.pages) {
-            const unsigned nan = round2<T>(NAN, NAN);
-            *to = u32x4{nan, nan, nan, nan};
-            continue;
+    }
+    u32x4 w[kUnits];
+    float scale[kUnits];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        scale[i] = 1.f;
+        w[i] = u32x4{0, 0, 0, 0};
+        if (page[i] >= 0) {
+            w[i] = *reinterpret_cast<const u32x4*>(rows.cached(p, i, page[i], at[i]));
+            if constexpr (KIND != SAME16) scale[i] = *rows.scale(p, i, page[i], at[i]);
         }
-        const int in_page = at & ((1 << p.page_shift) - 1);
-        const char* const from = value ? p.v + page * p.v_page + h * p.v_head + (int64_t)in_page * p.v_row : p.k + page * p.k_page + h * p.k_head + (int64_t)in_page * p.k_row;
+    }
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        if (!rows.in[i] || !(of[i] || p.fill)) continue;
+        const bool there = page[i] >= 0;
+        const unsigned other = of[i] ? round2<T>(NAN, NAN) : 0u;      // (of no sequence: zeros; of a page that is not there: NaN)
+        u32x4* const to = reinterpret_cast<u32x4*>(rows.packed(p, i));
         if constexpr (KIND == SAME16) {
-            *to = *reinterpret_cast<const u32x4*>(from + 16 * part);
+            *to = there ? w[i] : u32x4{other, other, other, other};
         } else {
-            const u32x2 codes = *reinterpret_cast<const u32x2*>(from + 8 * part);
-            const float scale = (value ? p.v_scale + page * p.vs_page + h * p.vs_head : p.k_scale + page * p.ks_page + h * p.ks_head)[in_page];
-            u32x4 w;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const unsigned a = code_pair<T, KIND, false>(codes[j]), b = code_pair<T, KIND, true>(codes[j]);
-                w[2 * j] = round2<T>(low<T>(a) * scale, high<T>(a) * scale);
-                w[2 * j + 1] = round2<T>(low<T>(b) * scale, high<T>(b) * scale);
+                u32x4 x;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const unsigned a = code_pair<T, KIND, false>(w[i][2 * j + k]), b = code_pair<T, KIND, true>(w[i][2 * j + k]);
+                    x[2 * k] = round2<T>(low<T>(a) * scale[i], high<T>(a) * scale[i]);
+                    x[2 * k + 1] = round2<T>(low<T>(b) * scale[i], high<T>(b) * scale[i]);
+                }
+                to[j] = there ? x : u32x4{other, other, other, other};
             }
-            *to = w;
         }
     }
 #endif
 }
 
 // ---- attention of one token over the pages
-// The keys of all sequences, in tiles of kTile (each sequence rounded up), are one list per key head, dealt out to `slots` workgroups in equal runs.  A workgroup writes the sequences
-// that lie in its run whole; of one that its neighbours share it leaves sums of its part, which cache_join_kernel adds up.
+// A workgroup's share is an equal part of all sequences' keys, in tiles of kTile.  A sequence of more is cut into parts, of which each has a workgroup for each key head; one in one part
+// has its rows written at once, the others' parts leave sums, which cache_join_kernel adds up.  (Equal runs of one list of all sequences' tiles: a workgroup then waits for the first keys of each
+// of many short sequences in turn, 32 sequences of 1 to 2817 keys in int8 25 us instead of 19, though 48 of 1 to 7817 97 instead of 100.)
 constexpr int kTile = 128;           // keys: 32 of each wavefront
-constexpr int kLeast = 1;            // tiles of a workgroup
 constexpr float kLowest = -3.0e38f;
 
 __device__ __forceinline__ int tiles_of(const CacheParams& p, int i) {
     const int n = p.lens[i];
     return n > 0 && n <= (int64_t)p.width << p.page_shift ? (n + kTile - 1) / kTile : 0;
 }
-// the tiles in front of sequence i (or all of them, i = B) and those of sequences up to 64 on: sums over 64 sequences a step
-struct Scan { int before, sum, tiles; };
-__device__ __forceinline__ int scan64(int tiles) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) { const int up = __shfl_up(tiles, d); tiles += lane >= d ? up : 0; }
-    return tiles;
+// sums over the wavefront's lanes up to each one (data-parallel-primitive moves: within rows of 16, then the rows' ends)
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+__device__ __forceinline__ int sums_up_to(int v) {
+    v = dpp_add<0x111, 0xF>(v);      // row_shr 1, 2, 4, 8
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);      // row_bcast 15 to rows 1 and 3
+    return dpp_add<0x143, 0xC>(v);   // row_bcast 31 to rows 2 and 3
 }
-__device__ __forceinline__ int total_tiles(const CacheParams& p) {
+__device__ __forceinline__ int sum_of(int v) { return __builtin_amdgcn_readlane(sums_up_to(v), 63); }
+// A sequence's parts have a share at most; three quarters of one where shares are large and most sequences have only a few parts, which rounding up leaves far from equal (48 sequences of 1 to
+// 7817 keys, us, a share / three quarters: 106 / 100; but 131072 + 70001 + 99 keys in e4m3 84 / 88, 32 of 1 to 2817 in int8 18.9 / 20.5).
+struct Share {
+    int per, most;
+    __device__ __forceinline__ int parts(int tiles) const { return tiles > per ? (tiles + most - 1) / most : 1; }
+    __device__ __forceinline__ bool is_long(int tiles) const { return 2 * tiles > per; }
+};
+__device__ __forceinline__ Share share_of(const CacheParams& p) {
     const int lane = threadIdx.x & 63;
     int mine = 0;
     for (int base = 0; base < p.B; base += 64) mine += base + lane < p.B ? tiles_of(p, base + lane) : 0;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) mine += __shfl_xor(mine, d);
-    return __builtin_amdgcn_readfirstlane(mine);
+    int per = (sum_of(mine) + p.slots - 1) / p.slots;
+    per = per > 1 ? per : 1;
+    return {per, per >= 8 && 4 * (int64_t)p.B > p.slots ? (3 * per + 3) / 4 : per};
 }
-__device__ __forceinline__ int run_length(int total, int slots) {
-    const int per = (total + slots - 1) / slots;
-    return per > kLeast ? per : kLeast;
+// The part `slot`: first come the parts of sequences of more than half a share, in order, then the shorter ones, which end the call on what those leave (without keys: one part too).
+// seq < 0: behind the last.
+struct Part { int seq, part, parts, tiles; };
+__device__ __forceinline__ Part part_of(const CacheParams& p, int slot) {
+    const int lane = threadIdx.x & 63;
+    const Share share = share_of(p);
+    int before = 0;
+    for (int shorter = 0; shorter < 2; ++shorter)
+        for (int base = 0; base < p.B; base += 64) {
+            const int tiles = base + lane < p.B ? tiles_of(p, base + lane) : 0;
+            const int parts = base + lane < p.B && share.is_long(tiles) != (bool)shorter ? share.parts(tiles) : 0, sum = sums_up_to(parts);
+            const unsigned long long past = __ballot(before + sum > slot);
+            if (past) {
+                const int at = __builtin_ctzll(past), of = __builtin_amdgcn_readlane(parts, at);
+                return {base + at, slot - (before + __builtin_amdgcn_readlane(sum, at) - of), of, __builtin_amdgcn_readlane(tiles, at)};
+            }
+            before += __builtin_amdgcn_readlane(sum, 63);
+        }
+    return {-1, 0, 0, 0};
 }
 // floats of a part: D sums, the max they refer to, the sum of the exponentials, for each of 16 NR rows
 template <int D, int NR> constexpr int kPartFloats = 16 * NR * (D + 2);
@@ -265,298 +386,303 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
     const int head = blockIdx.x % p.Hkv, block = blockIdx.x / p.Hkv % p.row_blocks, slot = blockIdx.x / (p.Hkv * p.row_blocks);
     const int row0 = block * 16 * NR;
 
-    const int total = total_tiles(p), per = run_length(total, p.slots);
-    const int first = slot * per, last = first + per < total ? first + per : total;
-    // (sequences of nothing are whole wherever they lie: the first workgroup's)
-    if (slot == 0) {
-        for (int i = wave; i < p.B; i += kThreads / 64) {
-            if (tiles_of(p, i)) continue;
-            const bool bad = p.lens[i] != 0;
-            for (int r = 0; r < 16 * NR && row0 + r < p.group; ++r) {
-                const int hq = head * p.group + row0 + r;
-                const unsigned w = bad ? round2<T>(NAN, NAN) : 0u;
-                if (lane < D / 8) *reinterpret_cast<u32x4*>(p.o + i * p.o_row + hq * p.o_head + 16 * lane) = u32x4{w, w, w, w};
-                if (p.lse && lane == 0) p.lse[(int64_t)i * p.group * p.Hkv + hq] = bad ? NAN : -INFINITY;
-            }
+    // rows of a sequence without keys: zeros, or NaN where its length is none
+    auto write_empty = [&](int i) {
+        const bool bad = p.lens[i] != 0;
+        const unsigned w = bad ? round2<T>(NAN, NAN) : 0u;
+        for (int r = 0; r < 16 * NR && row0 + r < p.group; ++r) {
+            const int hq = head * p.group + row0 + r;
+            if (lane < D / 8) *reinterpret_cast<u32x4*>(p.o + i * p.o_row + hq * p.o_head + 16 * lane) = u32x4{w, w, w, w};
+            if (p.lse && lane == 0) p.lse[(int64_t)i * p.group * p.Hkv + hq] = bad ? NAN : -INFINITY;
         }
+    };
+    Part mine = {slot, 0, 1, 0};
+    if (p.whole) mine.tiles = __builtin_amdgcn_readfirstlane(tiles_of(p, slot));
+    else mine = part_of(p, slot);
+    if (mine.seq < 0) return;
+    const int seq = mine.seq;
+    if (!mine.tiles) {
+        if (wave == 0) write_empty(seq);
+        return;
     }
-    if (first >= last) return;
-
-    // the first sequence of the run
-    int seq = 0, begin = 0;                       // (begin: of its tiles in the list)
-    for (int base = 0, before = 0; base < p.B; base += 64) {
-        const int sum = scan64(base + lane < p.B ? tiles_of(p, base + lane) : 0);
-        const unsigned long long past = __ballot(before + sum > first);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            seq = base + at;
-            begin = before + __builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readfirstlane(tiles_of(p, seq));
-            break;
-        }
-        before += __builtin_amdgcn_readlane(sum, 63);
-    }
-
+    const int len = __builtin_amdgcn_readfirstlane(p.lens[seq]), from = (int)((int64_t)mine.part * mine.tiles / mine.parts), to = (int)((int64_t)(mine.part + 1) * mine.tiles / mine.parts);
+    const int* const table = p.table + seq * p.table_row;
     const char* const kh = p.k + head * p.k_head;
     const char* const vh = p.v + head * p.v_head;
     const int mask = (1 << p.page_shift) - 1;
-    for (int tile = first; tile < last;) {
-        const int len = __builtin_amdgcn_readfirstlane(p.lens[seq]), tiles = __builtin_amdgcn_readfirstlane(tiles_of(p, seq));
-        if (!tiles) { ++seq; continue; }
-        const int from = tile - begin, to = last - begin < tiles ? last - begin : tiles;      // of this sequence's tiles
-        const int* const table = p.table + seq * p.table_row;
-
-        // Q: row n16 of each block of 16, the channels that this lane's K holds
-        V8 qf[NR][NC];
+    // Q: row n16 of each block of 16, the channels that this lane's K holds
+    V8 qf[NR][NC];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const int row = row0 + 16 * r + n16;
-            const char* const at = p.q + (int64_t)seq * p.q_row + (int64_t)(head * p.group + (row < p.group ? row : 0)) * p.q_head;
+    for (int r = 0; r < NR; ++r) {
+        const int row = row0 + 16 * r + n16;
+        const char* const at = p.q + (int64_t)seq * p.q_row + (int64_t)(head * p.group + (row < p.group ? row : 0)) * p.q_head;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int channel = CODES ? 64 * (c / 2) + 16 * g + 8 * (c % 2) : 32 * c + 8 * g;
-                u32x4 w = *reinterpret_cast<const u32x4*>(at + 2 * channel);
-                w ^= p.flip;
-                qf[r][c] = __builtin_bit_cast(V8, row < p.group ? w : u32x4{0, 0, 0, 0});
-            }
+        for (int c = 0; c < NC; ++c) {
+            const int channel = CODES ? 64 * (c / 2) + 16 * g + 8 * (c % 2) : 32 * c + 8 * g;
+            u32x4 w = *reinterpret_cast<const u32x4*>(at + 2 * channel);
+            w ^= p.flip;
+            qf[r][c] = __builtin_bit_cast(V8, row < p.group ? w : u32x4{0, 0, 0, 0});
         }
-        f32x4 acc[NR][NB];
-        float m[NR], l[NR], R = 0.f;
-        bool bad = false;
+    }
+    f32x4 acc[NR][NB];
+    float m[NR], l[NR], R = 0.f;
+    bool bad = false;
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            m[r] = kLowest;
-            l[r] = 0.f;
+    for (int r = 0; r < NR; ++r) {
+        m[r] = kLowest;
+        l[r] = 0.f;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) acc[r][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < NB; ++b) acc[r][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // Steps of 32 keys.  A step's K is loaded behind the products of the one before, its V behind that one's, and its pages are looked up a step earlier still: nothing waits for
+    // addresses, and little for what they point at.  Keys past the end are the last one's, with weights of 0: whatever else the page holds is not looked at.
+    constexpr int KLOADS = CODES ? NC / 2 : NC, VWORDS = NB * BYTES / 4;
+    const int most = len - 1, first_key = 32 * wave;
+    int end = (len - first_key + kTile - 1) / kTile;                  // this wavefront's steps
+    end = to < end ? to : end;
+    u32x4 kw[2][KLOADS];
+    unsigned vw[8][VWORDS];
+    float ks[8], vs[8];
+    // K: row n16 of key half u is key 8 (n16 / 4) + 4 u + n16 % 4, so that a lane's results of the two halves are those of 8 keys in order, 8 g .. 8 g + 7
+    auto k_key = [&](int t, int u) { const int key = t * kTile + first_key + 8 * (n16 >> 2) + 4 * u + (n16 & 3); return key < most ? key : most; };
+    // V: keys 8 g .. 8 g + 7, channels NB n16 .. NB n16 + NB - 1; 8 keys in order share a page
+    auto v_key = [&](int t) { const int key = t * kTile + first_key + 8 * g; return key < (most & ~7) ? key : (most & ~7); };
+    int kp[2], vp;
+    auto look_up = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) kp[u] = table[k_key(t, u) >> p.page_shift];
+        vp = table[v_key(t) >> p.page_shift];
+    };
+    auto checked = [&](int page) { const bool in = page >= 0 && page < p.pages; bad |= !in; return in ? page : 0; };
+    auto load_k = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const char* const at = kh + checked(kp[u]) * p.k_page + (int64_t)(k_key(t, u) & mask) * p.k_row + 16 * g;
+#pragma unroll
+            for (int c = 0; c < KLOADS; ++c) kw[u][c] = *reinterpret_cast<const u32x4*>(at + 64 * c);
         }
-        for (int t = from; t < to; ++t) {
-            const int key0 = t * kTile + 32 * wave;
-            if (key0 >= len) break;
-            // Keys past the end are the last one's, with weights of 0: whatever else the page holds is not looked at.
-            const int most = len - 1;
-            auto page_at = [&](int key) {
-                const int page = table[key >> p.page_shift];
-                const bool in = page >= 0 && page < p.pages;
-                bad |= !in;
-                return in ? page : 0;
-            };
-            // K: row n16 of key half u is key 8 (n16 / 4) + 4 u + n16 % 4, so that a lane's results of the two halves are those of 8 keys in order, 8 g .. 8 g + 7
-            unsigned kw[2][CODES ? NC / 2 : NC][4];
+    };
+    auto load_v = [&](int t, int page) __attribute__((always_inline)) {
+        const int key8 = v_key(t), in8 = key8 & mask;
+        const char* const at = vh + page * p.v_page + (int64_t)in8 * p.v_row + NB * BYTES * n16;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) __builtin_memcpy(vw[i], __builtin_assume_aligned(at + (int64_t)(key8 + i < most ? i : most - key8) * p.v_row, 4 * VWORDS), 4 * VWORDS);
+        if constexpr (CODES) {
+            __builtin_memcpy(ks, __builtin_assume_aligned(p.k_scale + page * p.ks_page + head * p.ks_head + in8, 16), 32);
+            __builtin_memcpy(vs, __builtin_assume_aligned(p.v_scale + page * p.vs_page + head * p.vs_head + in8, 16), 32);
+        }
+    };
+    if (from < end) {
+        look_up(from);
+        load_k(from);
+        load_v(from, checked(vp));
+        look_up(from + 1);
+    }
+    // (the last step loads nothing: a condition around the loads would have the compiler wait for all of them at the next use of any)
+    auto step = [&](int t, auto more) __attribute__((always_inline)) {
+        f32x4 s[NR][2];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) s[r][0] = s[r][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                int key = key0 + 8 * (n16 >> 2) + 4 * u + (n16 & 3);
-                key = key < most ? key : most;
-                const char* const at = kh + page_at(key) * p.k_page + (int64_t)(key & mask) * p.k_row;
-#pragma unroll
-                for (int c = 0; c < (CODES ? NC / 2 : NC); ++c) {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(at + 64 * c + 16 * g);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) kw[u][c][i] = w[i];
-                }
-            }
-            // V: keys 8 g .. 8 g + 7, channels NB n16 .. NB n16 + NB - 1
-            unsigned vw[8][NB / 2];
-            float ks[8], vs[8];
-            const int key8 = key0 + 8 * g < (most & ~7) ? key0 + 8 * g : (most & ~7);
-            const int page8 = page_at(key8), in8 = key8 & mask;
-            {
-                const char* const at = vh + page8 * p.v_page + (int64_t)in8 * p.v_row + NB * BYTES * n16;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const char* const a = at + (int64_t)(key8 + i < most ? i : most - key8) * p.v_row;
-                    constexpr int WORDS = NB * BYTES / 4;
-                    unsigned w[WORDS];
-                    __builtin_memcpy(w, __builtin_assume_aligned(a, 4 * WORDS), 4 * WORDS);
-                    if constexpr (CODES) {
-#pragma unroll
-                        for (int j = 0; j < WORDS; ++j) {
-                            vw[i][2 * j] = code_pair<T, KIND, false>(w[j]);
-                            vw[i][2 * j + 1] = code_pair<T, KIND, true>(w[j]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < WORDS; ++j) vw[i][j] = w[j];
-                    }
-                }
-            }
-            if constexpr (CODES) {
-                const float* const a = p.k_scale + page8 * p.ks_page + head * p.ks_head + in8;
-                const float* const b = p.v_scale + page8 * p.vs_page + head * p.vs_head + in8;
-                __builtin_memcpy(ks, __builtin_assume_aligned(a, 16), 32);
-                __builtin_memcpy(vs, __builtin_assume_aligned(b, 16), 32);
-            }
-            const int left = len - key0 - 8 * g;
-            float by[8];                            // what V's weights are multiplied with
-            if constexpr (CODES) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) by[i] = i < left ? vs[i] : 0.f;
-                if constexpr (__is_same(T, _Float16)) {
-                    // Weights p scale in fp16 would leave its range where values are small.  They are held relative to the largest scale so far, but for a factor of up to 64.
-                    float top = by[0];
-#pragma unroll
-                    for (int i = 1; i < 8; ++i) top = fmaxf(top, by[i]);
-                    if (__any(top > 64.f * R)) {
-                        top = fmaxf(R, over_quarters_max(top));
-                        const float f = R / top;
-#pragma unroll
-                        for (int r = 0; r < NR; ++r)
-#pragma unroll
-                            for (int b = 0; b < NB; ++b) acc[r][b] *= f;
-                        R = top;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) by[i] = R > 0.f ? by[i] / R : by[i];
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-                for (int c = 0; c < NC; ++c)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        u32x4 w;
-                        if constexpr (CODES) {
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                w[2 * i] = code_pair<T, KIND, false>(kw[u][c / 2][2 * (c % 2) + i]);
-                                w[2 * i + 1] = code_pair<T, KIND, true>(kw[u][c / 2][2 * (c % 2) + i]);
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) w[i] = kw[u][c][i];
-                        }
-                        s[u] = mfma16(__builtin_bit_cast(V8, w), qf[r][c], s[u]);
-                    }
-                float x[8], top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    x[i] = s[i / 4][i % 4] * p.scale_log2;
-                    if constexpr (CODES) x[i] *= ks[i];
-                    x[i] = i < left ? x[i] : -INFINITY;
-                    top = fmaxf(top, x[i]);
-                }
-                if (__any(top > m[r] + kMaxSlack)) {
-                    top = fmaxf(m[r], over_quarters_max(top));
-                    const float f = __builtin_amdgcn_exp2f(m[r] - top);
-                    m[r] = top;
-                    l[r] *= f;
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) acc[r][b] *= f;
-                }
                 u32x4 w;
+                if constexpr (CODES) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    x[i] = __builtin_amdgcn_exp2f(x[i] - m[r]);
-                    l[r] += x[i];
-                    if constexpr (CODES) x[i] *= by[i];
+                    for (int i = 0; i < 2; ++i) {
+                        w[2 * i] = code_pair<T, KIND, false>(kw[u][c / 2][2 * (c % 2) + i]);
+                        w[2 * i + 1] = code_pair<T, KIND, true>(kw[u][c / 2][2 * (c % 2) + i]);
+                    }
+                } else {
+                    w = kw[u][c];
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = round2<T>(x[2 * i], x[2 * i + 1]);
-                const V8 pf = __builtin_bit_cast(V8, w);
-                // output rows NB n + b, n = 0 .. 15: what lane n16 holds of V, transposed in its registers
+                for (int r = 0; r < NR; ++r) s[r][u] = mfma16(__builtin_bit_cast(V8, w), qf[r][c], s[r][u]);
+            }
+        int vnext = 0;
+        if constexpr (decltype(more)::value) {
+            load_k(t + 1);
+            vnext = checked(vp);
+            look_up(t + 2);
+        }
+        const int left = len - t * kTile - first_key - 8 * g;
+        float by[8];                            // what V's weights are multiplied with
+        if constexpr (CODES) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    u32x4 vt;
+            for (int i = 0; i < 8; ++i) by[i] = i < left ? vs[i] : 0.f;
+            if constexpr (__is_same(T, _Float16)) {
+                // Weights p scale in fp16 would leave its range where values are small.  They are held relative to the largest scale so far, but for a factor of up to 64.
+                float top = by[0];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) vt[i] = __builtin_amdgcn_perm(vw[2 * i + 1][b / 2], vw[2 * i][b / 2], b % 2 ? 0x07060302u : 0x05040100u);
-                    acc[r][b] = mfma16(__builtin_bit_cast(V8, vt), pf, acc[r][b]);
+                for (int i = 1; i < 8; ++i) top = fmaxf(top, by[i]);
+                if (__any(top > 64.f * R)) {
+                    top = fmaxf(R, over_quarters_max(top));
+                    const float f = R / top;
+#pragma unroll
+                    for (int r = 0; r < NR; ++r)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) acc[r][b] *= f;
+                    R = top;
                 }
+                const float over = R > 0.f ? 1.f / R : 1.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) by[i] *= over;
             }
         }
-        // ---- join the wavefronts: [wave][row][channel], then [wave][row] of max, sum
-        float* const sums = smem;
-        float* const stat = smem + 4 * 16 * NR * D;
-        const float back = CODES && __is_same(T, _Float16) ? R : 1.f;
-        const bool any_bad = __any(bad);
+        V8 pf[NR];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            float lr = l[r];
-            lr += __shfl_xor(lr, 16);
-            lr += __shfl_xor(lr, 32);
-            if (any_bad) lr = NAN;
-            if (g == 0) {
-                stat[2 * (wave * 16 * NR + 16 * r + n16)] = m[r];
-                stat[2 * (wave * 16 * NR + 16 * r + n16) + 1] = lr;
+            float x[8], top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = s[r][i / 4][i % 4] * p.scale_log2;
+                if constexpr (CODES) x[i] *= ks[i];
+                x[i] = i < left ? x[i] : -INFINITY;
+                top = fmaxf(top, x[i]);
+            }
+            if (__any(top > m[r] + kMaxSlack)) {
+                top = fmaxf(m[r], over_quarters_max(top));
+                const float f = __builtin_amdgcn_exp2f(m[r] - top);
+                m[r] = top;
+                l[r] *= f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) acc[r][b] *= f;
+            }
+            u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(x[i] - m[r]);
+                l[r] += x[i];
+                if constexpr (CODES) x[i] *= by[i];
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int b = 0; b < NB; b += 4)
-                    *reinterpret_cast<f32x4*>(sums + (wave * 16 * NR + 16 * r + n16) * D + NB * (4 * g + e) + b) = f32x4{acc[r][b][e], acc[r][b + 1][e], acc[r][b + 2][e], acc[r][b + 3][e]} * back;
+            for (int i = 0; i < 4; ++i) w[i] = round2<T>(x[2 * i], x[2 * i + 1]);
+            pf[r] = __builtin_bit_cast(V8, w);
         }
-        __syncthreads();
-        const bool whole = from == 0 && to == tiles;
-        constexpr int LANES = D / 8, AT_ONCE = kThreads / LANES;
-        for (int r = threadIdx.x / LANES; r < 16 * NR && row0 + r < p.group; r += AT_ONCE) {
-            const int c = 8 * (threadIdx.x % LANES);
-            float top = kLowest, sum = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        // output rows NB n + b, n = 0 .. 15: what lane n16 holds of V, transposed in its registers
+        unsigned vx[8][NB / 2];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[2 * (w * 16 * NR + r)]);
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float by = __builtin_amdgcn_exp2f(stat[2 * (w * 16 * NR + r)] - top);
-                sum += by * stat[2 * (w * 16 * NR + r) + 1];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] += by * sums[(w * 16 * NR + r) * D + c + i];
+            for (int j = 0; j < VWORDS; ++j) {
+                if constexpr (CODES) {
+                    vx[i][2 * j] = code_pair<T, KIND, false>(vw[i][j]);
+                    vx[i][2 * j + 1] = code_pair<T, KIND, true>(vw[i][j]);
+                } else {
+                    vx[i][j] = vw[i][j];
+                }
             }
-            const int hq = head * p.group + row0 + r;
-            if (whole) {
-                const float by = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-                *reinterpret_cast<u32x4*>(p.o + (int64_t)seq * p.o_row + hq * p.o_head + 2 * c) = u32x4{round2<T>(f[0] * by, f[1] * by), round2<T>(f[2] * by, f[3] * by), round2<T>(f[4] * by, f[5] * by), round2<T>(f[6] * by, f[7] * by)};
-                if (p.lse && c == 0) p.lse[(int64_t)seq * p.group * p.Hkv + hq] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f : sum == 0.f ? -INFINITY : sum;
-            } else {
-                // a run's first sequence may be its predecessors' too (part 0), its last one its successors' (part 1, unless it is the first as well)
-                float* const part = p.parts + ((((int64_t)slot * p.row_blocks + block) * p.Hkv + head) * 2 + (from == 0)) * kPartFloats<D, NR>;
-                *reinterpret_cast<f32x4*>(part + r * D + c) = f32x4{f[0], f[1], f[2], f[3]};
-                *reinterpret_cast<f32x4*>(part + r * D + c + 4) = f32x4{f[4], f[5], f[6], f[7]};
-                if (c == 0) { part[16 * NR * D + 2 * r] = top; part[16 * NR * D + 2 * r + 1] = sum; }
-            }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            u32x4 vt;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vt[i] = __builtin_amdgcn_perm(vx[2 * i + 1][b / 2], vx[2 * i][b / 2], b % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int r = 0; r < NR; ++r) acc[r][b] = mfma16(__builtin_bit_cast(V8, vt), pf[r], acc[r][b]);
         }
-        __syncthreads();
-        tile = begin + to;
-        begin += tiles;
-        ++seq;
+        if constexpr (decltype(more)::value) load_v(t + 1, vnext);
+    };
+    if (from < end) {
+        for (int t = from; t + 1 < end; ++t) step(t, Int<1>{});
+        step(end - 1, Int<0>{});
+    }
+    // ---- join the wavefronts: [wave][row][channel], then [wave][row] of max, sum
+    float* const sums = smem;
+    float* const stat = smem + 4 * 16 * NR * D;
+    const float back = CODES && __is_same(T, _Float16) ? R : 1.f;
+    const bool any_bad = __any(bad);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        float lr = l[r];
+        lr += __shfl_xor(lr, 16);
+        lr += __shfl_xor(lr, 32);
+        if (any_bad) lr = NAN;
+        if (g == 0) {
+            stat[2 * (wave * 16 * NR + 16 * r + n16)] = m[r];
+            stat[2 * (wave * 16 * NR + 16 * r + n16) + 1] = lr;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int b = 0; b < NB; b += 4)
+                *reinterpret_cast<f32x4*>(sums + (wave * 16 * NR + 16 * r + n16) * D + NB * (4 * g + e) + b) = f32x4{acc[r][b][e], acc[r][b + 1][e], acc[r][b + 2][e], acc[r][b + 3][e]} * back;
+    }
+    __syncthreads();
+    constexpr int LANES = D / 8, AT_ONCE = kThreads / LANES;
+    for (int r = threadIdx.x / LANES; r < 16 * NR && row0 + r < p.group; r += AT_ONCE) {
+        const int c = 8 * (threadIdx.x % LANES);
+        float top = kLowest, sum = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[2 * (w * 16 * NR + r)]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float by = __builtin_amdgcn_exp2f(stat[2 * (w * 16 * NR + r)] - top);
+            sum += by * stat[2 * (w * 16 * NR + r) + 1];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] += by * sums[(w * 16 * NR + r) * D + c + i];
+        }
+        const int hq = head * p.group + row0 + r;
+        if (mine.parts == 1) {
+            const float by = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+            *reinterpret_cast<u32x4*>(p.o + (int64_t)seq * p.o_row + hq * p.o_head + 2 * c) = u32x4{round2<T>(f[0] * by, f[1] * by), round2<T>(f[2] * by, f[3] * by), round2<T>(f[4] * by, f[5] * by), round2<T>(f[6] * by, f[7] * by)};
+            if (p.lse && c == 0) p.lse[(int64_t)seq * p.group * p.Hkv + hq] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f : sum == 0.f ? -INFINITY : sum;
+        } else {
+            float* const part = p.parts + (((int64_t)slot * p.row_blocks + block) * p.Hkv + head) * kPartFloats<D, NR>;
+            *reinterpret_cast<f32x4*>(part + r * D + c) = f32x4{f[0], f[1], f[2], f[3]};
+            *reinterpret_cast<f32x4*>(part + r * D + c + 4) = f32x4{f[4], f[5], f[6], f[7]};
+            if (c == 0) { part[16 * NR * D + 2 * r] = top; part[16 * NR * D + 2 * r + 1] = sum; }
+        }
     }
 #endif
 }
 
-// ---- the sequences that several workgroups have parts of: one workgroup for each sequence, key head and block of rows
+// ---- the sequences that several workgroups have parts of: a workgroup for each sequence and query head, D / 4 lanes to a part, kThreads / (D / 4) parts at a time
 template <typename T, int D, int NR>
 __global__ void __launch_bounds__(kThreads) cache_join_kernel(const CacheParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const int head = blockIdx.x % p.Hkv, block = blockIdx.x / p.Hkv % p.row_blocks, seq = blockIdx.x / (p.Hkv * p.row_blocks), lane = threadIdx.x & 63;
-    const int tiles = tiles_of(p, seq);
-    if (!tiles) return;
-    int all = 0, before = 0;
-    for (int base = 0; base < p.B; base += 64) {
-        const int n = base + lane < p.B ? tiles_of(p, base + lane) : 0;
-        all += n;
-        before += base + lane < seq ? n : 0;
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) { all += __shfl_xor(all, d); before += __shfl_xor(before, d); }
-    const int per = run_length(all, p.slots), w0 = before / per, w1 = (before + tiles - 1) / per;
-    if (w0 == w1) return;
     constexpr int LANES = D / 4, AT_ONCE = kThreads / LANES;
-    const int row0 = block * 16 * NR;
-    auto part = [&](int w) { return p.parts + ((((int64_t)w * p.row_blocks + block) * p.Hkv + head) * 2 + (w == w0)) * kPartFloats<D, NR>; };
-    for (int r = threadIdx.x / LANES; r < 16 * NR && row0 + r < p.group; r += AT_ONCE) {
-        const int c = 4 * (threadIdx.x % LANES);
-        float top = kLowest, sum = 0.f;
-        f32x4 f = {0.f, 0.f, 0.f, 0.f};
-        for (int w = w0; w <= w1; ++w) top = fmaxf(top, part(w)[16 * NR * D + 2 * r]);
-        for (int w = w0; w <= w1; ++w) {
-            const float* const a = part(w);
-            const float by = __builtin_amdgcn_exp2f(a[16 * NR * D + 2 * r] - top);
-            sum += by * a[16 * NR * D + 2 * r + 1];
-            f += by * *reinterpret_cast<const f32x4*>(a + r * D + c);
-        }
-        const float by = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-        const int hq = head * p.group + row0 + r;
-        *reinterpret_cast<u32x2*>(p.o + (int64_t)seq * p.o_row + hq * p.o_head + 2 * c) = u32x2{round2<T>(f[0] * by, f[1] * by), round2<T>(f[2] * by, f[3] * by)};
-        if (p.lse && c == 0) p.lse[(int64_t)seq * p.group * p.Hkv + hq] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f : sum == 0.f ? -INFINITY : sum;
+    __shared__ __attribute__((aligned(16))) float smem[AT_ONCE][D + 4];
+    const int heads = p.group * p.Hkv, seq = blockIdx.x / heads, hq = blockIdx.x - seq * heads, head = hq / p.group, row = hq - head * p.group, block = row / (16 * NR), r = row % (16 * NR);
+    const int lane = threadIdx.x & 63;
+    const Share share = share_of(p);
+    const int parts = share.parts(__builtin_amdgcn_readfirstlane(tiles_of(p, seq)));
+    if (parts == 1) return;
+    int before = 0;
+    for (int base = 0; base < seq; base += 64) {
+        const int n = base + lane < seq ? tiles_of(p, base + lane) : 0;
+        before += share.is_long(n) ? share.parts(n) : 0;
     }
+    const int w0 = sum_of(before), w1 = w0 + parts - 1;
+    const int c = 4 * (threadIdx.x % LANES), slice = threadIdx.x / LANES;
+    float top = kLowest, sum = 0.f;
+    f32x4 f = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int w = w0 + slice; w <= w1; w += AT_ONCE) {
+        const float* const a = p.parts + (((int64_t)w * p.row_blocks + block) * p.Hkv + head) * kPartFloats<D, NR>;
+        const float m = a[16 * NR * D + 2 * r], l = a[16 * NR * D + 2 * r + 1];
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a + r * D + c);
+        const float to = fmaxf(top, m), was = __builtin_amdgcn_exp2f(top - to), is = __builtin_amdgcn_exp2f(m - to);
+        top = to;
+        sum = sum * was + l * is;
+        f = f * was + x * is;
+    }
+    *reinterpret_cast<f32x4*>(&smem[slice][c]) = f;
+    if (c == 0) { smem[slice][D] = top; smem[slice][D + 1] = sum; }
+    __syncthreads();
+    if (slice) return;
+    for (int i = 0; i < AT_ONCE; ++i) top = fmaxf(top, smem[i][D]);
+    sum = 0.f;
+    f = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+        const float is = __builtin_amdgcn_exp2f(smem[i][D] - top);
+        sum += smem[i][D + 1] * is;
+        f += *reinterpret_cast<const f32x4*>(&smem[i][c]) * is;
+    }
+    const float by = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    *reinterpret_cast<u32x2*>(p.o + (int64_t)seq * p.o_row + hq * p.o_head + 2 * c) = u32x2{round2<T>(f[0] * by, f[1] * by), round2<T>(f[2] * by, f[3] * by)};
+    if (p.lse && c == 0) p.lse[(int64_t)seq * heads + hq] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f : sum == 0.f ? -INFINITY : sum;
 #endif
 }
 
@@ -653,7 +779,7 @@ int check_packed(const cosmos_attn_cache_desc* d, bool out) {
     return st;
 }
 int64_t packed_blocks(const cosmos_attn_cache_desc* d) {
-    const int64_t per = (int64_t)kRowsPerThread * (kThreads / (d->D / 8));
+    const int64_t per = (int64_t)kUnits * (kThreads / (d->D / each_of(d->kind)));
     return (d->rows * 2 * d->Hkv + per - 1) / per;
 }
 
@@ -669,16 +795,21 @@ int check_attention(const cosmos_attn_cache_desc* d) {
     st = check_rows(d->q, d->q_stride);
     return st != COSMOS_ATTN_OK ? st : check_out(d->o, d->o_stride, d->B, d->Hq, d->D);
 }
+// Tables of few tiles: a workgroup for each sequence, and nothing to join, which a second launch would be for (333 keys of 4 heads: 6.3 us, as parts 5.8 and 3.8 for the join).
+constexpr int kWholeTiles = 4;
 struct Shape { int row_blocks, rows16, slots; bool whole; };
 Shape shape_of(const cosmos_attn_cache_desc* d) {
     const int group = d->Hq / d->Hkv, rows16 = group <= 16 ? 1 : 2, row_blocks = (group + 16 * rows16 - 1) / (16 * rows16);
     const int64_t capacity = ((int64_t)d->width * d->page_size + kTile - 1) / kTile, most = (int64_t)d->B * capacity;
-    // as many workgroups as fit on the chip at once, if the tables hold that many tiles
+    if (capacity <= kWholeTiles) return {row_blocks, rows16, 1, true};
+    // two workgroups a compute unit, if the tables hold that many tiles
     int64_t slots = 2 * kNumCUs / ((int64_t)d->Hkv * row_blocks);
     slots = slots < 1 ? 1 : slots;
-    slots = slots > most ? most : slots;
-    return {row_blocks, rows16, (int)(slots < 1 ? 1 : slots), capacity <= 1};
+    return {row_blocks, rows16, (int)(slots > most ? most : slots), false};
 }
+
+// parts of all sequences, for a head: each rounds up once (parts are three quarters of a share, rounded up, at least)
+int64_t most_parts(int64_t B, int64_t slots) { return 4 * slots / 3 + 1 + B; }
 
 }  // namespace
 
@@ -707,7 +838,7 @@ int cosmos_attn_cache_read(const cosmos_attn_cache_desc* desc, void* stream) {
 size_t cosmos_attn_cache_attention_workspace_bytes(const cosmos_attn_cache_desc* desc) {
     if (check_attention(desc) != COSMOS_ATTN_OK || !desc->B) return 0;
     const Shape s = shape_of(desc);
-    return s.whole ? 0 : (size_t)s.slots * s.row_blocks * desc->Hkv * 2 * 16 * s.rows16 * (desc->D + 2) * sizeof(float);
+    return s.whole ? 0 : (size_t)most_parts(desc->B, s.slots) * s.row_blocks * desc->Hkv * 16 * s.rows16 * (desc->D + 2) * sizeof(float);
 }
 
 int cosmos_attn_cache_attention(const cosmos_attn_cache_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
@@ -721,7 +852,7 @@ int cosmos_attn_cache_attention(const cosmos_attn_cache_desc* desc, void* worksp
     CacheParams p = params_of(desc);
     p.q = (const char*)desc->q; p.o = (char*)desc->o; p.lse = desc->lse;
     p.q_row = 2 * desc->q_stride[0]; p.q_head = 2 * desc->q_stride[1]; p.o_row = 2 * desc->o_stride[0]; p.o_head = 2 * desc->o_stride[1];
-    p.group = desc->Hq / desc->Hkv; p.row_blocks = s.row_blocks; p.slots = s.slots;
+    p.group = desc->Hq / desc->Hkv; p.row_blocks = s.row_blocks; p.slots = s.slots; p.whole = s.whole;
     p.scale_log2 = fmaxf(fabsf(desc->sm_scale) * 1.44269504088896341f, 1e-37f);
     p.flip = signbit(desc->sm_scale) ? 0x80008000u : 0u;
     p.parts = (float*)workspace;
@@ -730,8 +861,8 @@ int cosmos_attn_cache_attention(const cosmos_attn_cache_desc* desc, void* worksp
         constexpr int D = decltype(dim)::value, K = decltype(kind)::value;
         auto run = [&](auto blocks16) {
             constexpr int NR = decltype(blocks16)::value;
-            const int done = launch(cache_attention_kernel<T, K, D, NR>, (int64_t)p.Hkv * p.row_blocks * p.slots, 4 * 16 * NR * (D + 2) * sizeof(float), p, stream);
-            return done != COSMOS_ATTN_OK || s.whole ? done : launch(cache_join_kernel<T, D, NR>, (int64_t)p.Hkv * p.row_blocks * p.B, 0, p, stream);
+            const int done = launch(cache_attention_kernel<T, K, D, NR>, (int64_t)p.Hkv * p.row_blocks * (s.whole ? p.B : most_parts(p.B, p.slots)), 4 * 16 * NR * (D + 2) * sizeof(float), p, stream);
+            return done != COSMOS_ATTN_OK || s.whole ? done : launch(cache_join_kernel<T, D, NR>, (int64_t)desc->Hq * p.B, 0, p, stream);
         };
         return s.rows16 == 1 ? run(Int<1>{}) : run(Int<2>{});
     });

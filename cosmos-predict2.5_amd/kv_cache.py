@@ -20,8 +20,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _on_device
-from .ragged import HEAD_DIMS, check_rows, int32_on, packed, packed_ready
+from .ops import _DTYPES
+from .ragged import HEAD_DIMS, check_rows, int32_on, on_device, packed, packed_ready, plain_int32
 
 KINDS = {torch.bfloat16: _lib.CACHE_SAME, torch.float16: _lib.CACHE_SAME, torch.float8_e4m3fn: _lib.CACHE_E4M3, torch.int8: _lib.CACHE_INT8}
 
@@ -34,7 +34,7 @@ class KVCache:
     """Pages of keys and values, ``[pages, heads, page_size, head_dim]`` each: bf16, fp16, or 8 bits (float8_e4m3fn, int8) with an fp32 scale for each row of a head,
     ``[pages, heads, page_size]``.  Takes the tensors as they are (any page, head and row strides of 16-byte steps) and writes into them."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page_size", "head_dim", "dtype", "device", "kind", "_parts")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page_size", "head_dim", "dtype", "device", "kind", "_parts", "_index")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
         assert k.dim() == 4 and v.shape == k.shape, "k and v must be [pages, heads, page_size, head_dim]"
@@ -59,6 +59,7 @@ class KVCache:
                 assert x is not None and x.shape == k.shape[:3] and x.dtype == torch.float32 and x.device == k.device, "8 bits need fp32 scales [pages, heads, page_size]"
                 assert x.stride(2) == 1 and x.stride(0) % 4 == 0 and x.stride(1) % 4 == 0 and x.data_ptr() % 16 == 0, "scales of a head's page lie side by side"
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._index = k.get_device()
         at = lambda x: 0 if x is None else x.data_ptr()
         steps = lambda x, n: (0,) * n if x is None else x.stride()[:n]
         self._parts = {
@@ -82,22 +83,32 @@ class KVCache:
 
 
 def _check_table(cache: KVCache, table: torch.Tensor) -> torch.Tensor:
+    if plain_int32(table, 2, cache._index):
+        return table
     table = int32_on(table, cache.device)
     assert table.dim() == 2, "table must be [sequences, pages of a sequence at most]"
     return table if table.shape[0] <= 1 or table.stride(0) >= 0 else table.contiguous()
 
 
-def _check_numbers(x: torch.Tensor, count: int, device: torch.device, what: str) -> torch.Tensor:
-    x = int32_on(x, device)
+def _check_numbers(x: torch.Tensor, count: int, cache: KVCache, what: str) -> torch.Tensor:
+    if plain_int32(x, 1, cache._index) and x.shape[0] == count:
+        return x
+    x = int32_on(x, cache.device)
     assert x.dim() == 1 and x.shape[0] == count, f"{what} numbers are needed"
     return x
 
 
-def _call(table, lens=None, cu=None, rows=0, k=None, v=None, fill=False, Hq=0, sm_scale=0.0, q=None, o=None, lse=None) -> bytes:
-    at = lambda x: 0 if x is None else x.data_ptr()
-    steps = lambda x: (0, 0) if x is None else x.stride()[:2]
-    return _CALL_PART.pack(table.shape[0], table.shape[1], at(table), table.stride(0), at(lens), at(cu), rows, at(k), at(v), *steps(k), *steps(v), 1 if fill else 0, Hq, sm_scale, 0,
-                           at(q), at(o), *steps(q), *steps(o), at(lse))
+def _call(table, lens=0, cu=0, rows=0, k=0, v=0, k_stride=(0, 0), v_stride=(0, 0), fill=0, Hq=0, sm_scale=0.0, q=0, o=0, q_stride=(0, 0), o_stride=(0, 0), lse=0) -> bytes:
+    B, width = table.shape
+    return _CALL_PART.pack(B, width, table.data_ptr(), table.stride()[0], lens, cu, rows, k, v, *k_stride, *v_stride, fill, Hq, sm_scale, 0, q, o, *q_stride, *o_stride, lse)
+
+
+def _check_rows(x: torch.Tensor, name: str, cache: KVCache, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rows of the cache's head dim and device, as the kernels take them."""
+    if not (x.is_cuda and x.dim() == 3 and x.dtype in _DTYPES and x.get_device() == cache._index and (like is None or x.dtype is like.dtype)):
+        check_rows(x, name, like)
+    assert x.device == cache.device and x.shape[2] == cache.head_dim, f"{name} must be [rows, heads, D] of the cache's head dim, on its device"
+    return x if packed_ready(x) else packed(x)
 
 
 def cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, cu: Optional[torch.Tensor] = None) -> None:
@@ -106,19 +117,18 @@ def cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, table: torch.T
     8 bits: ``scale = max |x| * fp32(1 / 448)`` (e4m3) or ``* fp32(1 / 127)`` (int8), ``code = round(x / scale)``, all in fp32; a row with a value that is not finite reads back as NaN.
     Rows of no sequence, sequences whose ``lens`` is below their rows or more than the table holds, and pages outside of the cache: nothing is written.  No two rows of a call may have
     one place."""
-    check_rows(k, "k")
-    check_rows(v, "v", k)
-    assert k.shape == v.shape and k.shape[1:] == (cache.heads, cache.head_dim) and k.device == cache.device, "k and v must be [rows, heads, D] of the cache"
+    k = _check_rows(k, "k", cache)
+    v = _check_rows(v, "v", cache, k)
+    assert k.shape == v.shape and k.shape[1] == cache.heads, "k and v must be [rows, heads, D] of the cache"
     part, table = cache._part(k.dtype), _check_table(cache, table)
-    lens = _check_numbers(lens, table.shape[0], cache.device, "as many lengths as the table has sequences: its")
+    B, rows = table.shape[0], k.shape[0]
+    lens = _check_numbers(lens, B, cache, "as many lengths as the table has sequences: its")
     if cu is None:
-        assert k.shape[0] == table.shape[0], "one row for each sequence, or offsets"
+        assert rows == B, "one row for each sequence, or offsets"
     else:
-        cu = _check_numbers(cu, table.shape[0] + 1, cache.device, "one offset more than the table has sequences: its")
-    k, v = packed(k), packed(v)
-    desc = part + _call(table, lens, cu, k.shape[0], k, v)
-    run = _lib.load_library().cosmos_attn_cache_write
-    _lib.raise_for_status(_on_device(cache.device, lambda stream: run(desc, stream)))
+        cu = _check_numbers(cu, B + 1, cache, "one offset more than the table has sequences: its")
+    desc = part + _call(table, lens.data_ptr(), 0 if cu is None else cu.data_ptr(), rows, k.data_ptr(), v.data_ptr(), k.stride()[:2], v.stride()[:2])
+    on_device(cache._index, _lib.load_library().cosmos_attn_cache_write, desc)
 
 
 def cache_read(cache: KVCache, table: torch.Tensor, cu: torch.Tensor, rows: int, dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -130,11 +140,12 @@ def cache_read(cache: KVCache, table: torch.Tensor, cu: torch.Tensor, rows: int,
         raise NotImplementedError(f"dtype={dtype} is not supported (bf16 / fp16)")
     assert rows >= 0
     part, table = cache._part(dtype), _check_table(cache, table)
-    cu = _check_numbers(cu, table.shape[0] + 1, cache.device, "one offset more than the table has sequences: its")
-    k, v = (torch.empty((rows, cache.heads, cache.head_dim), dtype=dtype, device=cache.device) for _ in range(2))
-    desc = part + _call(table, None, cu, rows, k, v, True)
-    run = _lib.load_library().cosmos_attn_cache_read
-    _lib.raise_for_status(_on_device(cache.device, lambda stream: run(desc, stream)))
+    cu = _check_numbers(cu, table.shape[0] + 1, cache, "one offset more than the table has sequences: its")
+    heads, D = cache.heads, cache.head_dim
+    k = torch.empty((rows, heads, D), dtype=dtype, device=cache.device)
+    v = torch.empty_like(k)
+    desc = part + _call(table, 0, cu.data_ptr(), rows, k.data_ptr(), v.data_ptr(), (heads * D, D), (heads * D, D), 1)
+    on_device(cache._index, _lib.load_library().cosmos_attn_cache_read, desc)
     return k, v
 
 
@@ -158,24 +169,23 @@ def cache_attention(
     """``(o, lse)``: attention of one token of each sequence, ``q [B, Hq, D]``, over the first ``lens[i]`` positions that its row of ``table`` holds; ``lse``: fp32 ``[B, Hq]``.
 
     ``lens[i] == 0``: o = 0, lse = -inf.  A length that the table does not hold, or a page outside of the cache among a sequence's: NaN.  ``out``: a tensor for o."""
-    check_rows(q, "q")
+    q = _check_rows(q, "q", cache)
     B, Hq, D = q.shape
-    assert D == cache.head_dim and Hq >= 1 and Hq % cache.heads == 0 and q.device == cache.device, "q must be [B, Hq, D], Hq a multiple of the cache's heads"
+    assert Hq >= 1 and Hq % cache.heads == 0, "q must be [B, Hq, D], Hq a multiple of the cache's heads"
     part, table = cache._part(q.dtype), _check_table(cache, table)
     assert table.shape[0] == B, "a row of the table for each sequence"
-    lens = _check_numbers(lens, B, cache.device, "as many lengths as there are sequences: their")
-    q = packed(q)
+    lens = _check_numbers(lens, B, cache, "as many lengths as there are sequences: their")
     if out is None:
-        o = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+        o = torch.empty_like(q) if q.is_contiguous() else torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
     else:
         assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out must have q's shape, type and device"
         if not packed_ready(out):
             raise ValueError("out: rows of 16-byte steps are written in place, this view cannot be")
         o = out
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if need_lse else None
-    desc = part + _call(table, lens, None, 0, None, None, False, Hq, D ** -0.5 if sm_scale is None else sm_scale, q, o, lse)
+    lse = q.new_empty((B, Hq), dtype=torch.float32) if need_lse else None
     ws_bytes = _workspace_bytes(cache.heads, D, cache.page_size, B, table.shape[1], Hq)
-    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    run, at = _lib.load_library().cosmos_attn_cache_attention, 0 if workspace is None else workspace.data_ptr()
-    _lib.raise_for_status(_on_device(q.device, lambda stream: run(desc, at, ws_bytes, stream)))
+    workspace = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    desc = part + _call(table, lens.data_ptr(), 0, 0, 0, 0, (0, 0), (0, 0), 0, Hq, D ** -0.5 if sm_scale is None else sm_scale, q.data_ptr(), o.data_ptr(), q.stride()[:2], o.stride()[:2],
+                        0 if lse is None else lse.data_ptr())
+    on_device(cache._index, _lib.load_library().cosmos_attn_cache_attention, desc, 0 if workspace is None else workspace.data_ptr(), ws_bytes)
     return o, lse

@@ -88,6 +88,30 @@ def test_codes_of_all_sizes(pkg, ragged_oracle, gpu, kind, dtype):
         assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.nan_to_num(), want.nan_to_num())
 
 
+@pytest.mark.parametrize("dtype, bits", [(BF16, 7), (FP16, 10)])
+@pytest.mark.parametrize("kind", [E4M3, INT8])
+def test_every_quotient(pkg, ragged_oracle, gpu, kind, dtype, bits):
+    """All significands of a value, over two binades, over all significands of its row's largest: codes next to a border are those of IEEE division."""
+    n = 1 << bits
+    tops = 1 + torch.arange(n) / n
+    values = torch.cat([1 + torch.arange(n) / n, (1 + torch.arange(n) / n) / 2])
+    values = torch.cat([values, values.new_zeros(-len(values) % 127)]).reshape(-1, 127)
+    x = torch.empty(n, len(values), 128)
+    x[:, :, :127] = torch.minimum(values[None], tops[:, None, None])
+    x[:, :, 1:127:2] *= -1
+    x[:, :, 127] = tops[:, None]
+    x = x.reshape(1, -1, 128).transpose(0, 1).to(dtype)
+    table, pages = tables([len(x)], 64, gpu)
+    cache = empty(pkg, pages, 1, 64, 128, kind, gpu)
+    on = offsets([0, len(x)], gpu)
+    pkg.cache_write(cache, x.to(gpu), (x * 2.0 ** 3).to(gpu), table, offsets([len(x)], gpu), on)
+    codes, scale = ragged_oracle.quantise(x, kind)
+    at = torch.arange(len(x), device=gpu)
+    for got, got_scale, by in ((cache.k, cache.k_scale, 1.0), (cache.v, cache.v_scale, 8.0)):
+        assert torch.equal(got_scale[table[0, at // 64].long(), 0, at % 64].cpu(), scale[:, 0] * by)
+        assert torch.equal(got.view(torch.uint8)[table[0, at // 64].long(), 0, at % 64].cpu().view(kind).float(), codes[:, 0].float())      # (zeros of either sign)
+
+
 def test_only_new_tokens_are_written(pkg, gpu):
     lens, new = [20, 5, 1], [3, 5, 0]
     table, pages = tables(lens, 16, gpu)
@@ -155,7 +179,7 @@ def check_decode(pkg, oracle, gpu, lens, page, Hq, Hkv, D, dtype, kind, scale=No
 
 @pytest.mark.parametrize("dtype, kind", TYPES)
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("lens, page", [([1], 16), ([33, 0, 128, 129, 5], 16), ([1000, 1, 257], 64), ([700], 1024)])
+@pytest.mark.parametrize("lens, page", [([1], 16), ([33, 0, 128, 129, 5], 16), ([495, 0, 384], 16), ([1000, 1, 257], 64), ([700], 1024), ([0, 600, 1], 16)])
 def test_one_token(pkg, ragged_oracle, gpu, lens, page, D, dtype, kind):
     check_decode(pkg, ragged_oracle, gpu, lens, page, 4, 2, D, dtype, kind)
 
@@ -207,7 +231,7 @@ def test_what_cannot_be_looked_up_is_nan(pkg, ragged_oracle, gpu):
 
 def test_a_table_of_one_page_takes_one_kernel(pkg, ragged_oracle, gpu):
     """No workspace, nothing to join."""
-    assert pkg.kv_cache._workspace_bytes(2, 64, 128, 3, 1, 4) == 0
+    assert pkg.kv_cache._workspace_bytes(2, 64, 128, 3, 1, 4) == 0 == pkg.kv_cache._workspace_bytes(2, 64, 128, 3, 4, 4) < pkg.kv_cache._workspace_bytes(2, 64, 128, 3, 5, 4)
     cache = empty(pkg, 3, 2, 128, 64, BF16, gpu)
     k, v = rows(200, 2, 64, BF16, gpu, 0), rows(200, 2, 64, BF16, gpu, 1)
     table, lens = offsets([2, 0, 1], gpu)[:, None], [128, 0, 72]

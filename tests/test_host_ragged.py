@@ -92,17 +92,17 @@ def test_cache_desc_layout_and_status_codes(pkg):
     for over, want in [(dict(Hq=0), L.ST_BAD_ARG), (dict(Hq=7), L.ST_BAD_SHAPE), (dict(lens=None), L.ST_BAD_ARG), (dict(q=None), L.ST_BAD_ARG), (dict(o_stride=(512, 0)), L.ST_BAD_STRIDE),
                        (dict(o_stride=(64, 64)), L.ST_BAD_STRIDE), (dict(q=P + 2), L.ST_BAD_STRIDE), (dict(sm_scale=float("inf")), L.ST_BAD_ARG)]:
         assert attend(cache_desc(pkg, **over)) == want, over
-    D = cache_desc(pkg)
+    D = cache_desc(pkg, width=100, table_stride=100)
     assert lib.cosmos_attn_cache_attention_workspace_bytes(ctypes.byref(D)) > 0
     assert lib.cosmos_attn_cache_attention(ctypes.byref(D), None, 0, None) == L.ST_WORKSPACE
     assert write(cache_desc(pkg, rows=0, k_rows=None)) == L.ST_OK and attend(cache_desc(pkg, B=0)) == L.ST_OK
 
 
 def test_attention_workspace_does_not_grow_with_the_table(pkg):
-    """Parts are kept for each workgroup, not for each piece of a sequence."""
+    """Parts are kept for each workgroup, one of a share of all keys or of a sequence's last ones."""
     of = lambda B, width: pkg.kv_cache._workspace_bytes(8, 128, 64, B, width, 32)
-    assert of(1, 1 << 14) == of(64, 1 << 14) > 0
-    assert pkg.kv_cache._workspace_bytes(8, 128, 16, 64, 8, 32) == 0          # tables of one tile: nothing is shared
+    assert of(3, 1 << 14) == of(3, 1 << 12) > 0 and of(64, 1 << 14) < 2 * of(1, 1 << 14)
+    assert pkg.kv_cache._workspace_bytes(8, 128, 16, 64, 32, 32) == 0          # tables of few tiles: nothing is shared
 
 
 def test_python_argument_checks(pkg, monkeypatch):
@@ -131,7 +131,7 @@ def test_refusals_before_a_launch(pkg, monkeypatch):
         raise AssertionError("launched")
 
     for module in (pkg.ragged, pkg.kv_cache):
-        monkeypatch.setattr(module, "_on_device", no_launch)
+        monkeypatch.setattr(module, "on_device", no_launch)
     new = lambda *shape, dtype=torch.bfloat16: on(torch.zeros(*shape, dtype=dtype))
     q, k, cu = new(4, 6, 64), new(4, 2, 64), new(2, dtype=torch.int32)
     for call, error in [
