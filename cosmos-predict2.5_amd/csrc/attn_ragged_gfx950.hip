@@ -20,6 +20,7 @@
 #include <math.h>
 #include <mutex>
 #include <set>
+#include <type_traits>
 #include <utility>
 
 #include "cosmos_attn_hip.h"
@@ -103,6 +104,20 @@ template <typename T> __device__ __forceinline__ unsigned round2(float a, float 
     const V2 two = {(T)a, (T)b};
     return __builtin_bit_cast(unsigned, two);
 }
+// The order of a block's LDS reads and matrix products, READS to PRODUCTS: AHEAD reads first, then each product with its share of the others.  (Left alone the compiler reads the operands of two
+// products and waits for them: 2 % of the forward, and of the dK/dV kernel, where no more registers are free for it.)
+template <int READS, int PRODUCTS, int AHEAD> __device__ __forceinline__ void reads_ahead() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int FIRST = AHEAD < READS ? AHEAD : READS, PER = READS / PRODUCTS, WITH = (READS - FIRST) / PER;
+    __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
+#pragma unroll
+    for (int i = 0; i < WITH; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - WITH, 0);
+#endif
+}
 __device__ __forceinline__ float over_halves_sum(float x) { float lo, hi; both_halves(x, lo, hi); return lo + hi; }
 __device__ __forceinline__ float over_halves_max(float x) { float lo, hi; both_halves(x, lo, hi); return fmaxf(lo, hi); }
 
@@ -124,35 +139,35 @@ __device__ __forceinline__ int sums_up_to(int v) {
 }
 __device__ __forceinline__ int sum_of(int v) { return __builtin_amdgcn_readlane(sums_up_to(v), 63); }
 
-// The tiles of a kernel: kRows rows (or keys) of a sequence each, with `steps` of kStep keys (kRowStep rows) that go by.  Rank 0 of a sequence's tiles is the longest one; the last rows
+// The tiles of a kernel: ROWS rows (or keys) of a sequence each, with `steps` of STEP keys (rows) that go by.  Rank 0 of a sequence's tiles is the longest one; the last rows
 // see the most keys, the first keys are seen by the most rows.
-constexpr int kRowStep = 32;
 struct Lengths { int lq, lk; };      // lq < 0 or lk < 0: bad offsets
-template <bool KEYS> struct Tiles {
+template <bool KEYS, int ROWS, int STEP> struct Tiles {
     const RaggedParams& p;
     __device__ __forceinline__ Lengths lengths(int i) const { return {range_of(p.cu_q, i, p.Tq).length, range_of(p.cu_k, i, p.Tk).length}; }
     __device__ __forceinline__ int count(Lengths n) const {
         const int64_t rows = KEYS ? n.lk : (int64_t)n.lq * p.group;
-        return rows > 0 ? (int)((rows + kRows - 1) / kRows) : 0;
+        return rows > 0 ? (int)((rows + ROWS - 1) / ROWS) : 0;
     }
     static __device__ __forceinline__ int at(int rank, int tiles) { return KEYS ? rank : tiles - 1 - rank; }
     // first row that sees key j, in rows; (rounded up to steps where none does)
     __device__ __forceinline__ int first_row(Lengths n, int j) const {
         const int lq = n.lq > 0 ? n.lq : 0, t = j - (n.lk - lq);
-        return !p.causal || t <= 0 ? 0 : t >= lq ? (lq * p.group + kRowStep - 1) / kRowStep * kRowStep : t * p.group;
+        return !p.causal || t <= 0 ? 0 : t >= lq ? (lq * p.group + STEP - 1) / STEP * STEP : t * p.group;
     }
     // keys that row r's token sees
     __device__ __forceinline__ int keys(Lengths n, int r) const {
         const int lk = n.lk > 0 ? n.lk : 0, e = r / p.group + lk - n.lq + 1;
         return !p.causal || e > lk ? lk : e < 0 ? 0 : e;
     }
-    __device__ __forceinline__ int first_step(Lengths n, int tile) const { return KEYS ? first_row(n, tile * kRows) / kRowStep : 0; }
+    __device__ __forceinline__ int first_step(Lengths n, int tile) const { return KEYS ? first_row(n, tile * ROWS) / STEP : 0; }
     __device__ __forceinline__ int end_step(Lengths n, int tile) const {
-        if (KEYS) return n.lq > 0 ? (n.lq * p.group + kRowStep - 1) / kRowStep : 0;
-        const int rows = n.lq * p.group, last = tile * kRows + kRows - 1;
-        return (keys(n, last < rows ? last : rows - 1) + kStep - 1) / kStep;
+        if (KEYS) return n.lq > 0 ? (n.lq * p.group + STEP - 1) / STEP : 0;
+        const int rows = n.lq * p.group, last = tile * ROWS + ROWS - 1;
+        return (keys(n, last < rows ? last : rows - 1) + STEP - 1) / STEP;
     }
     __device__ __forceinline__ int steps(Lengths n, int tile) const { return end_step(n, tile) - first_step(n, tile); }
+    static constexpr bool OF_KEYS = KEYS;
 };
 
 // Parts are written and read in fp32 and joined by a launch of its own, so they have `least` steps at least.  dk and dv, and where shares are large: parts of three fifths of a workgroup's
@@ -160,13 +175,19 @@ template <bool KEYS> struct Tiles {
 // share / of 3/5 / of 2/5: 4558 / 3973 / 3890).  Else five quarters, which are all on the chip at once: a few more than fit take a second round (512 queries, 8 heads each, on 8192 keys: 704
 // parts 72, 520 75, 455 63).
 constexpr int kAtOnce = 2 * kNumCUs;      // workgroups
-constexpr int least_steps(bool keys, int D) { return keys ? D == 128 ? 16 : 64 : D == 128 ? 12 : 24; }
+constexpr int least_steps(int D) { return D == 128 ? 12 : 24; }
+constexpr int least_rows(int D) { return D == 128 ? 512 : 2048; }       // (of dk and dv, in rows)
+typedef Tiles<false, kRows, kStep> RowTiles;
+// of dk and dv
+constexpr int row_step(int D) { return D == 128 ? 32 : 64; }
+template <int D> using KeyTiles = Tiles<true, kRows, row_step(D)>;
 struct Found { int seq, tile, parts; Lengths n; };     // seq < 0: behind the last tile, `tile` of them
 // Tile `index` of all sequences', in the sequences' order and the longest of each first, and how many parts it is cut into.
 // (The longest of all first, by counts of the tiles longer than some length, for which the length is searched: 5 % slower on 12 prompts and on four documents.  Short tiles, which are mostly
 // waiting, then run beside each other at the end instead of beside long ones.)
-template <bool KEYS> __device__ __forceinline__ Found find(const RaggedParams& p, int index) {
-    const Tiles<KEYS> T{p};
+template <typename Kind> __device__ __forceinline__ Found find(const RaggedParams& p, int index) {
+    constexpr bool KEYS = Kind::OF_KEYS;
+    const Kind T{p};
     const int lane = threadIdx.x & 63;
     Found f = {-1, 0, 1, {0, 0}};
     // (a sequence's: all of its tiles times the mean of the longest and the shortest; no more than 64 of them add up to in 32 bits)
@@ -241,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Block block = block_of(p, blockIdx.x);
     const int head = block.head;
-    const Found f = find<false>(p, block.index);
+    const Found f = find<RowTiles>(p, block.index);
     if (f.seq < 0) {
         if (p.fill && block.part == 0) clear_rows<D>(p.o, p.o_row, p.o_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f.tile, p.lse);
         return;
@@ -260,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
     auto token_at = [&](int r) { return __builtin_amdgcn_readfirstlane((r < rows ? r : rows - 1) / p.group); };
     const int wave_end = first < rows ? keys_of(token_at(first + 31)) : 0, wave_all = keys_of(token_at(first));
     // steps of this part
-    const int steps = Tiles<false>{p}.end_step(f.n, tile);
+    const int steps = RowTiles{p}.end_step(f.n, tile);
     const int t0 = (int)((int64_t)block.part * steps / f.parts), n = (int)((int64_t)(block.part + 1) * steps / f.parts);
 
     const char* const kp = p.k + rk.start * p.k_row + head * p.k_head;
@@ -311,6 +332,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int h = 0; h < 2; ++h) s[h] = mfma32(read_rows<V8>(kt + 32 * h * L::ROW, k_at[c]), qf[c], s[h]);
+        reads_ahead<2 * NC, 2 * NC, 8>();
         if (key0 + kStep > wave_all) {          // (some row of the wavefront does not see all of these keys)
             const int left = end - key0 - 4 * half;
 #pragma unroll
@@ -331,6 +353,8 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[b] *= by;
         }
+        // (at head dim 64, with twice the exponentials to a product, the second half of a step goes before another wavefront's first: 321 us become 309 on 8192 positions, 16 heads; at 128 1 % slower)
+        if constexpr (D == 64) __builtin_amdgcn_s_setprio(1);
         V8 pf[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -351,6 +375,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[b] = mfma32(read_channels<V8>(vt + 16 * c * L::ROW, v_at[b][0], v_at[b][1]), pf[c], acc[b]);
+        if constexpr (D == 64) __builtin_amdgcn_s_setprio(0);
     };
     for (int t = t0; t < n; t += 2) {
         meet();
@@ -396,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Block block = block_of(p, blockIdx.x);
     const int head = block.head;
-    const Found f = find<false>(p, block.index);
+    const Found f = find<RowTiles>(p, block.index);
     if (f.seq < 0) {
         if (block.part == 0) clear_rows<D>(p.dq, p.dq_row, p.dq_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f.tile, nullptr);
         return;
@@ -414,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
     auto token_at = [&](int r) { return __builtin_amdgcn_readfirstlane((r < rows ? r : rows - 1) / p.group); };
     const int wave_end = first < rows ? keys_of(token_at(first + 31)) : 0, wave_all = keys_of(token_at(first));
     // steps of this part
-    const int steps = Tiles<false>{p}.end_step(f.n, tile);
+    const int steps = RowTiles{p}.end_step(f.n, tile);
     const int t0 = (int)((int64_t)block.part * steps / f.parts), n = (int)((int64_t)(block.part + 1) * steps / f.parts);
 
     const char* const kp = p.k + rk.start * p.k_row + head * p.k_head;
@@ -506,6 +531,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int b = 0; b < NB; ++b) acc[b] = mfma32(read_channels<V8>(kt + (32 * h + 16 * c) * L::ROW, k_tr[b][0], k_tr[b][1]), df[c], acc[b]);
+            reads_ahead<4 * NB, 2 * NB, 8>();
         }
     };
     for (int t = t0; t < n; t += 2) {
@@ -537,24 +563,24 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
 }
 
 // ---- backward, second kernel: dk and dv.  A workgroup: 128 keys of one sequence and key head, a wavefront 32 of them, one a lane; the sequence's rows (of all heads of the group) go by in
-// steps of kRowStep.  S = Q K^T has the rows in registers: P and dS, rounded, are operands of dV^T += dO^T P and dK^T += Q^T dS where they lie.  K stays in registers, V too at head dim 64 and in
+// steps of STEP.  S = Q K^T has the rows in registers: P and dS, rounded, are operands of dV^T += dO^T P and dK^T += Q^T dS where they lie.  K stays in registers, V too at head dim 64 and in
 // LDS at 128: with both in registers there are too many for two wavefronts on a SIMD, whose matrix products and other arithmetic go on beside each other (head dim 64, 1560 + 880 + 390 positions,
 // 16 heads, us, dq with it, V in LDS / in registers: 95 / 87).
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef typename VecOf<T>::v8 V8;
-    typedef Tile<D, kRowStep> L;
+    constexpr int STEP = row_step(D), NC = D / 16, NB = D / 32;
+    typedef Tile<D, STEP> L;
     typedef Tile<D, kRows> LV;
-    constexpr int NC = D / 16, NB = D / 32;
     LDS_TILES(L);
     constexpr bool V_IN_LDS = D == 128;
     __shared__ __attribute__((aligned(1024))) char values[V_IN_LDS ? LV::BYTES : 16];
-    __shared__ __attribute__((aligned(16))) float stats0[2 * kRowStep], stats1[2 * kRowStep];      // lse, delta of a step's rows
+    __shared__ __attribute__((aligned(16))) float stats0[2 * STEP], stats1[2 * STEP];      // lse, delta of a step's rows
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Block block = block_of(p, blockIdx.x);
     const int head = block.head;
-    const Found f = find<true>(p, block.index);
+    const Found f = find<KeyTiles<D>>(p, block.index);
     if (f.seq < 0) {
         if (block.part) return;
         clear_rows<D>(p.dk, p.dk_row, p.dk_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f.tile, nullptr);
@@ -566,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     const int lq = rq.length > 0 ? rq.length : 0;
     const int key0 = f.tile * kRows, key = key0 + 32 * wave + (lane & 31);
     const bool live = key < rk.length;
-    const Tiles<true> tiles{p};
+    const KeyTiles<D> tiles{p};
     const int from = tiles.first_row(f.n, key);
     const int wave_first = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave)), wave_all = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave + 31));
     // steps of this part
@@ -588,24 +614,24 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
             if constexpr (!V_IN_LDS) vf[c] = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(va + 32 * c));
         }
     }
-    // this lane's row of each load: the token and the head; both go on by kRowStep rows a step
-    const int step_tokens = kRowStep / p.group, step_heads = kRowStep - step_tokens * p.group;
+    // this lane's row of each load: the token and the head; both go on by STEP rows a step
+    const int step_tokens = STEP / p.group, step_heads = STEP - step_tokens * p.group;
     int token[L::LOADS], hd[L::LOADS], byte[L::LOADS];
 #pragma unroll
     for (int i = 0; i < L::LOADS; ++i) {
-        const int r = t0 * kRowStep + L::load_row(lane, wave, i);
+        const int r = t0 * STEP + L::load_row(lane, wave, i);
         token[i] = r / p.group;
         hd[i] = r - token[i] * p.group;
         byte[i] = L::load_byte(lane, wave, i);
     }
-    const int stat_row = threadIdx.x & (kRowStep - 1);
-    int stat_token = (t0 * kRowStep + stat_row) / p.group, stat_head = t0 * kRowStep + stat_row - stat_token * p.group;
+    const int stat_row = threadIdx.x & (STEP - 1);
+    int stat_token = (t0 * STEP + stat_row) / p.group, stat_head = t0 * STEP + stat_row - stat_token * p.group;
     float stat = 0.f;
     const char* const qp = p.q + rq.start * p.q_row + (int64_t)head * p.group * p.q_head;
     const char* const gp = p.dout + rq.start * p.do_row + (int64_t)head * p.group * p.do_head;
     auto next = [&](int& t, int& h) { t += step_tokens; h += step_heads; const bool over = h >= p.group; t += over; h -= over ? p.group : 0; };
     auto fill = [&](int t, char* qt, char* gt) __attribute__((always_inline)) {
-        const int base = t * kRowStep / p.group;      // (uniform) token that offsets are counted from
+        const int base = t * STEP / p.group;      // (uniform) token that offsets are counted from
         const auto qr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(qp + base * p.q_row), 0, 0x7FFFFFFF, 0x00020000);
         const auto gr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(gp + base * p.do_row), 0, 0x7FFFFFFF, 0x00020000);
 #pragma unroll
@@ -615,10 +641,10 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
             load_to_lds(gr, gt + L::load_to(wave, i), in ? (token[i] - base) * (int)p.do_row + hd[i] * (int)p.do_head + byte[i] : (int)0x80000000);
             next(token[i], hd[i]);
         }
-        if (threadIdx.x < 2 * kRowStep) {             // lse (threads 0 ..) and delta (threads kRowStep ..) of the step's rows
+        if (threadIdx.x < 2 * STEP) {             // lse (threads 0 ..) and delta (threads STEP ..) of the step's rows
             const bool in = stat_token < lq;
-            const float* const of = threadIdx.x < kRowStep ? p.lse : p.delta;
-            stat = threadIdx.x < kRowStep ? -INFINITY : 0.f;
+            const float* const of = threadIdx.x < STEP ? p.lse : p.delta;
+            stat = threadIdx.x < STEP ? -INFINITY : 0.f;
             if (in) stat = of[(int64_t)(head * p.group + stat_head) * p.Tq + rq.start + stat_token];
             next(stat_token, stat_head);
         }
@@ -634,54 +660,59 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     for (int b = 0; b < NB; ++b) dk[b] = dv[b] = f32x16{};
 
     auto step = [&](int t, const char* qt, const char* gt, const float* st) __attribute__((always_inline)) {
-        const int row0 = t * kRowStep;
-        if (row0 + kRowStep <= wave_first) return;
-        f32x16 s = f32x16{}, g = f32x16{};
+        const int row0 = t * STEP;
+        if (row0 + STEP <= wave_first) return;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            s = mfma32(read_rows<V8>(qt, q_at[c]), kf[c], s);
-            if constexpr (V_IN_LDS) g = mfma32(read_rows<V8>(gt, q_at[c]), read_rows<V8>(mine, q_at[c]), g);
-            else g = mfma32(read_rows<V8>(gt, q_at[c]), vf[c], g);
-        }
-        // element e: row 8 (e / 4) + 4 half + e % 4
+        for (int h = 0; h < STEP / 32; ++h) {
+            if constexpr (D == 128) SCHED_FENCE();      // (both halves at once need more registers than there are)
+            f32x16 s = f32x16{}, g = f32x16{};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 8 * i + 4 * half), delta = *reinterpret_cast<const f32x4*>(st + kRowStep + 8 * i + 4 * half);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[4 * i + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + j], p.scale_log2, -lse[j]));
-                g[4 * i + j] -= delta[j];
+            for (int c = 0; c < NC; ++c) {
+                s = mfma32(read_rows<V8>(qt + 32 * h * L::ROW, q_at[c]), kf[c], s);
+                if constexpr (V_IN_LDS) g = mfma32(read_rows<V8>(gt + 32 * h * L::ROW, q_at[c]), read_rows<V8>(mine, q_at[c]), g);
+                else g = mfma32(read_rows<V8>(gt + 32 * h * L::ROW, q_at[c]), vf[c], g);
             }
-        }
-        if (row0 < wave_all) {
-            const int left = from - row0 - 4 * half;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) >= left ? s[e] : 0.f;
-        }
-        V8 pf[2], df[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            u32x4 w, x;
+            // element e: row 8 (e / 4) + 4 half + e % 4
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int e = 8 * c + 2 * i;
-                w[i] = round2<T>(s[e], s[e + 1]);
-                x[i] = round2<T>(s[e] * g[e], s[e + 1] * g[e + 1]);
+                const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 32 * h + 8 * i + 4 * half), delta = *reinterpret_cast<const f32x4*>(st + STEP + 32 * h + 8 * i + 4 * half);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[4 * i + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + j], p.scale_log2, -lse[j]));
+                    g[4 * i + j] -= delta[j];
+                }
             }
-            pf[c] = __builtin_bit_cast(V8, w);
-            df[c] = __builtin_bit_cast(V8, x);
+            if (row0 < wave_all) {
+                const int left = from - row0 - 32 * h - 4 * half;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) >= left ? s[e] : 0.f;
+            }
+            V8 pf[2], df[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                u32x4 w, x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 8 * c + 2 * i;
+                    w[i] = round2<T>(s[e], s[e + 1]);
+                    x[i] = round2<T>(s[e] * g[e], s[e + 1] * g[e + 1]);
+                }
+                pf[c] = __builtin_bit_cast(V8, w);
+                df[c] = __builtin_bit_cast(V8, x);
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    dv[b] = mfma32(read_channels<V8>(gt + (32 * h + 16 * c) * L::ROW, q_tr[b][0], q_tr[b][1]), pf[c], dv[b]);
+                    dk[b] = mfma32(read_channels<V8>(qt + (32 * h + 16 * c) * L::ROW, q_tr[b][0], q_tr[b][1]), df[c], dk[b]);
+                }
+            reads_ahead<8 * NB, 4 * NB, 8>();
         }
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                dv[b] = mfma32(read_channels<V8>(gt + 16 * c * L::ROW, q_tr[b][0], q_tr[b][1]), pf[c], dv[b]);
-                dk[b] = mfma32(read_channels<V8>(qt + 16 * c * L::ROW, q_tr[b][0], q_tr[b][1]), df[c], dk[b]);
-            }
     };
     // (P = 0 where there is no row, or nothing that it sees)
     auto keep = [&](float* st) __attribute__((always_inline)) {
-        if (threadIdx.x < 2 * kRowStep) st[threadIdx.x] = threadIdx.x >= kRowStep ? stat : stat == -INFINITY ? INFINITY : stat * 1.44269504088896341f;
+        if (threadIdx.x < 2 * STEP) st[threadIdx.x] = threadIdx.x >= STEP ? stat : stat == -INFINITY ? INFINITY : stat * 1.44269504088896341f;
     };
     if (t0 < n) fill(t0, tile0, tile1);
     for (int t = t0; t < n; t += 2) {
@@ -729,7 +760,7 @@ __global__ void __launch_bounds__(kJoinThreads) ragged_join_kernel(const RaggedP
     constexpr bool KEYS = WHICH == 2;
     constexpr int LANES = D / 4, AT_ONCE = kJoinThreads / LANES;
     const int head = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv % p.tiles;
-    const Found f = find<KEYS>(p, index);
+    const Found f = find<std::conditional_t<KEYS, KeyTiles<D>, RowTiles>>(p, index);
     if (f.seq < 0 || f.parts <= 1) return;
     const int c = 4 * (threadIdx.x % LANES);
     const Range r = range_of(KEYS ? p.cu_k : p.cu_q, f.seq, KEYS ? p.Tk : p.Tq);
@@ -874,9 +905,10 @@ int most_parts(int64_t tiles, int64_t longest, int least) {
 }
 struct Cut { int64_t tiles; int parts, least; size_t bytes; };
 Cut cut_of(const cosmos_attn_ragged_desc* d, int which) {
+    const int step = row_step(d->D);
     const int64_t group = d->Hq / d->Hkv, rows = d->Tq * group, tiles = which == 2 ? most_tiles(d->Tk, d->n_seq) : most_tiles(rows, d->n_seq);
-    const int64_t longest = which == 2 ? (rows + kRowStep - 1) / kRowStep : (d->Tk + kStep - 1) / kStep;
-    const int least = least_steps(which == 2, d->D), parts = most_parts(tiles * d->Hkv, longest, least);
+    const int64_t longest = which == 2 ? (rows + step - 1) / step : (d->Tk + kStep - 1) / kStep;
+    const int least = which == 2 ? least_rows(d->D) / step : least_steps(d->D), parts = most_parts(tiles * d->Hkv, longest, least);
     return {tiles, parts, least, parts > 1 ? (size_t)tiles * d->Hkv * parts * kRows * (which == 0 ? d->D + 2 : which * d->D) * sizeof(float) : 0};
 }
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
