@@ -29,18 +29,21 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kThreads = 256;
 enum Kind { SAME16 = COSMOS_ATTN_CACHE_SAME, E4M3 = COSMOS_ATTN_CACHE_E4M3, INT8 = COSMOS_ATTN_CACHE_INT8 };
 
+// keys, or values
+struct Side {
+    char* pages;                                  // bytes between pages, heads and rows
+    int64_t page, head, row;
+    float* scales;                                // elements between pages and heads
+    int64_t scale_page, scale_head;
+    char* packed;                                 // rows outside of the cache: bytes between rows and heads
+    int64_t packed_row, packed_head;
+};
 struct CacheParams {
-    char *k, *v;                                  // bytes between pages, heads and rows
-    int64_t k_page, k_head, v_page, v_head;
-    int k_row, v_row;
-    float *k_scale, *v_scale;                     // elements between pages and heads
-    int64_t ks_page, ks_head, vs_page, vs_head;
+    Side side[2];                                 // keys, values
     const int *table, *lens, *cu;
     int64_t table_row;
     int width, B, pages, page_shift, Hkv, fill;
     int64_t rows;                                 // packed rows
-    char *k_rows, *v_rows;                        // bytes between rows and heads
-    int64_t kr_row, kr_head, vr_row, vr_head;
     // attention
     const char* q;
     char* o;
@@ -89,7 +92,6 @@ template <int LANES> __device__ __forceinline__ unsigned row_max(unsigned v) {
 }
 
 // ---- packed rows: which sequence a row is of, and its place there
-struct Place { int seq, at, length; bool in; };
 // the last offset of lo .. hi at or below the row (or lo)
 __device__ __forceinline__ int last_below(const int* cu, int lo, int hi, int64_t row) {
     while (lo < hi) {
@@ -99,49 +101,51 @@ __device__ __forceinline__ int last_below(const int* cu, int lo, int hi, int64_t
     }
     return lo;
 }
-// `near`: the offset found for the workgroup's first row, most often this one's too
-__device__ __forceinline__ Place place_of(const int* cu, int n, int near, int64_t row, int64_t rows) {
-    int at = near;
-    if (at < n && cu[at + 1] <= row) at = last_below(cu, at + 1, n, row);
-    const int64_t a = cu[at], b = at < n ? cu[at + 1] : a;
-    return {at, (int)(row - a), (int)(b - a), at < n && a >= 0 && row >= a && row < b && b <= rows};
-}
+struct Place {
+    int seq, start, end, len;     // its offsets; keys in the cache (writing)
+    __device__ __forceinline__ Place(const CacheParams& p, int at, bool lens) : seq(at), start(0), end(0), len(0) {
+        if (!p.cu) {              // one row to a sequence
+            start = at;
+            end = at + 1;
+        } else {
+            start = p.cu[at];
+            end = at < p.B ? p.cu[at + 1] : start;
+        }
+        if (lens && at < p.B) len = p.lens[at];
+    }
+    __device__ __forceinline__ bool has(const CacheParams& p, int row) const { return seq < p.B && start >= 0 && row >= start && row < end && end <= p.rows; }
+};
 
-// Both kernels: a lane has EACH elements of a row of a head, 8 where pages hold 16 bits and 16 where they hold codes: 16 bytes of the narrower side.  A workgroup has kUnits times
-// kThreads EACH / D rows, in the packed rows' order, the keys' heads and then the values'.  A thread's rows are looked up, loaded and worked on side by side: one by one, each behind the one
-// before, and with 8 elements, 16384 + 9999 + 1 + 4096 rows of 8 heads in e4m3 took 95 us to write (now 49) and 53 to read back (now 42); 189 MB each way at the rate of a large copy
-// are 37.
-constexpr int kUnits = 2;
+// Both kernels: a lane has EACH elements of a row of a head, 8 where pages hold 16 bits and 16 where they hold codes: 16 bytes of the narrower side.  A workgroup has kThreads EACH / D rows,
+// in the packed rows' order, of the keys or of the values (even and odd workgroups), so that their addresses are the scalar unit's to form, and so is the place of the first row's sequence,
+// most often that of all.  16384 + 9999 + 1 + 4096 rows of 8 heads in e4m3: 42 us to write and 32 to read back; with all of that in each thread 54 and 34, with 8 elements of a code to a
+// lane 95 and 53; two rows to a thread 44 and 33, four 48 and 35 (and 4.5 us instead of 3.4 for a few rows).  189 MB each way at the rate of a large copy are 37: a write forms 3 quotients,
+// products and codes to a lane's element, the vector unit's work of about as long.
 constexpr int each_of(int kind) { return kind == SAME16 ? 8 : 16; }
 template <int D, int EACH> struct Rows {
     static constexpr int LANES = D / EACH, ROWS = kThreads / LANES;
-    int64_t row[kUnits];          // packed row
-    int head[kUnits];
-    bool value[kUnits], in[kUnits];      // a row of V; there is such a row
-    int first;                    // offset of the first row's sequence
-    __device__ __forceinline__ Rows(const CacheParams& p) {
-        const unsigned both = 2u * (unsigned)p.Hkv;
-        const int64_t unit = (int64_t)blockIdx.x * (kUnits * ROWS), row0 = unit / both;
-        const unsigned over = (unsigned)(unit - row0 * both) + threadIdx.x / LANES;
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-            const unsigned u = over + i * ROWS, r = u / both, h = u - r * both;
-            row[i] = row0 + r;
-            in[i] = row[i] < p.rows;
-            value[i] = h >= (unsigned)p.Hkv;
-            head[i] = (int)(value[i] ? h - p.Hkv : h);
-        }
-        first = p.cu ? last_below(p.cu, 0, p.B, row0) : 0;
+    const Side& side;
+    int64_t row0;                 // the workgroup's first packed row
+    int row, head;                // row: counted from there
+    bool in;                      // there is such a row
+    __device__ __forceinline__ Rows(const CacheParams& p) : side(p.side[blockIdx.x & 1]) {
+        const int64_t unit = (int64_t)(blockIdx.x >> 1) * ROWS;
+        row0 = unit / p.Hkv;
+        const unsigned u = (unsigned)(unit - row0 * p.Hkv) + threadIdx.x / LANES, r = u / (unsigned)p.Hkv;
+        row = (int)r;
+        head = (int)(u - r * p.Hkv);
+        in = row0 + r < p.rows;
     }
-    __device__ __forceinline__ char* packed(const CacheParams& p, int i) const {
-        return (value[i] ? p.v_rows + row[i] * p.vr_row + head[i] * p.vr_head : p.k_rows + row[i] * p.kr_row + head[i] * p.kr_head) + 2 * EACH * (threadIdx.x % LANES);
+    // where the row is (if there is one)
+    __device__ __forceinline__ Place place(const CacheParams& p, bool lens) const {
+        Place w(p, p.cu ? last_below(p.cu, 0, p.B, row0) : (int)row0, lens);
+        if (in && this->at() >= w.end && w.seq < p.B) w = Place(p, p.cu ? last_below(p.cu, w.seq + 1, p.B, this->at()) : this->at(), lens);
+        return w;
     }
-    __device__ __forceinline__ char* cached(const CacheParams& p, int i, int page, int at) const {
-        return (value[i] ? p.v + page * p.v_page + head[i] * p.v_head + (int64_t)at * p.v_row : p.k + page * p.k_page + head[i] * p.k_head + (int64_t)at * p.k_row) + 16 * (threadIdx.x % LANES);
-    }
-    __device__ __forceinline__ float* scale(const CacheParams& p, int i, int page, int at) const {
-        return (value[i] ? p.v_scale + page * p.vs_page + head[i] * p.vs_head : p.k_scale + page * p.ks_page + head[i] * p.ks_head) + at;
-    }
+    __device__ __forceinline__ int at() const { return (int)row0 + row; }       // of all
+    __device__ __forceinline__ char* packed() const { return side.packed + row0 * side.packed_row + row * side.packed_row + head * side.packed_head + 2 * EACH * (threadIdx.x % LANES); }
+    __device__ __forceinline__ char* cached(int page, int key) const { return side.pages + page * side.page + head * side.head + key * side.row + 16 * (threadIdx.x % LANES); }
+    __device__ __forceinline__ float* scale(int page, int key) const { return side.scales + page * side.scale_page + head * side.scale_head + key; }
 };
 
 // x / s as IEEE division rounds it, for |x / s| up to some hundreds: x r corrected by the remainder, which fma gives exactly (Markstein's division), with r = 1 / s good to an ulp.  (That one
@@ -168,81 +172,63 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const CacheParams
     constexpr int EACH = each_of(KIND);
     typedef Rows<D, EACH> R;
     const R rows(p);
-    const int part = threadIdx.x % R::LANES, mask = (1 << p.page_shift) - 1;
-    int page[kUnits], at[kUnits];
-    u32x4 x[kUnits][EACH / 8];
-    bool in[kUnits];
+    u32x4 x[EACH / 8];
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i)
-#pragma unroll
-        for (int j = 0; j < EACH / 8; ++j) {
-            x[i][j] = u32x4{0, 0, 0, 0};
-            if (rows.in[i]) x[i][j] = *reinterpret_cast<const u32x4*>(rows.packed(p, i) + 16 * j);
-        }
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-        Place w = {(int)rows.row[i], 0, 1, true};
-        in[i] = rows.in[i];
-        if (in[i] && p.cu) w = place_of(p.cu, p.B, rows.first, rows.row[i], p.rows);
-        in[i] = in[i] && w.in;
-        at[i] = page[i] = 0;
-        if (in[i]) {
-            const int len = p.lens[w.seq], to = len - w.length + w.at;
-            in[i] = len >= w.length && (to >> p.page_shift) < p.width;
-            if (in[i]) page[i] = p.table[w.seq * p.table_row + (to >> p.page_shift)];
-            at[i] = to & mask;
-            in[i] = in[i] && page[i] >= 0 && page[i] < p.pages;
-        }
+    for (int j = 0; j < EACH / 8; ++j) {
+        x[j] = u32x4{0, 0, 0, 0};
+        if (rows.in) x[j] = *reinterpret_cast<const u32x4*>(rows.packed() + 16 * j);
     }
+    const Place w = rows.place(p, true);
+    const int to = w.len - (w.end - rows.at()), key = to & ((1 << p.page_shift) - 1);
+    int page = -1;
+    if (rows.in && w.has(p, rows.at()) && w.len >= w.end - w.start && (to >> p.page_shift) < p.width) page = p.table[w.seq * p.table_row + (to >> p.page_shift)];
+    const bool in = page >= 0 && page < p.pages;
+    if constexpr (KIND == SAME16) {
+        if (in) *reinterpret_cast<u32x4*>(rows.cached(page, key)) = x[0];
+    } else {
+        // the largest magnitude: of 16-bit floats without their signs as whole numbers, in whose order NaN comes behind infinity and that behind all others
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 most = {0, 0};
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-        if constexpr (KIND == SAME16) {
-            if (in[i]) *reinterpret_cast<u32x4*>(rows.cached(p, i, page[i], at[i])) = x[i][0];
+        for (int j = 0; j < 8; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[j / 4][j % 4] & 0x7FFF7FFFu));
+        const unsigned top = row_max<R::LANES>(most[0] > most[1] ? most[0] : most[1]);
+        // (a row of zeros: divided by 1; one that is not finite: codes of no meaning)
+        const float scale = top < (__is_same(T, __bf16) ? 0x7F80u : 0x7C00u) ? low<T>(top) * (KIND == E4M3 ? 1.f / 448.f : 1.f / 127.f) : NAN;
+        const Divide over(scale > 0.f ? scale : 1.f);
+        float f[16];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            f[2 * j] = low<T>(x[j / 4][j % 4]);
+            f[2 * j + 1] = high<T>(x[j / 4][j % 4]);
+        }
+        if (__any(over.by != 1.f)) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) f[j] *= over.by;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) f[j] = over(f[j]);
+        u32x4 codes = {0, 0, 0, 0};
+        if constexpr (KIND == E4M3) {
+            // (scale's own rounding may leave a quotient just above 448; the conversion's largest code takes those below 464)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j], f[4 * j + 1], 0, false);
+                codes[j] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j + 2], f[4 * j + 3], w, true);
+            }
         } else {
-            // the largest magnitude: of 16-bit floats without their signs as whole numbers, in whose order NaN comes behind infinity and that behind all others
-            typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-            u16x2 most = {0, 0};
+            // 2^23 + 2^22 + f: f rounded to a whole number, ties to even, in the low bits
 #pragma unroll
-            for (int j = 0; j < 8; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[i][j / 4][j % 4] & 0x7FFF7FFFu));
-            const unsigned top = row_max<R::LANES>(most[0] > most[1] ? most[0] : most[1]);
-            // (a row of zeros: divided by 1; one that is not finite: codes of no meaning)
-            const float scale = top < (__is_same(T, __bf16) ? 0x7F80u : 0x7C00u) ? low<T>(top) * (KIND == E4M3 ? 1.f / 448.f : 1.f / 127.f) : NAN;
-            const Divide over(scale > 0.f ? scale : 1.f);
-            float f[16];
+            for (int j = 0; j < 4; ++j) {
+                unsigned w[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                f[2 * j] = low<T>(x[i][j / 4][j % 4]);
-                f[2 * j + 1] = high<T>(x[i][j / 4][j % 4]);
+                for (int k = 0; k < 4; ++k) w[k] = __builtin_bit_cast(unsigned, f[4 * j + k] + 12582912.f);
+                const unsigned lo = __builtin_amdgcn_perm(w[1], w[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(w[3], w[2], 0x04000C0Cu);
+                codes[j] = lo | hi;
             }
-            if (__any(over.by != 1.f)) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) f[j] *= over.by;
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) f[j] = over(f[j]);
-            u32x4 codes = {0, 0, 0, 0};
-            if constexpr (KIND == E4M3) {
-                // (scale's own rounding may leave a quotient just above 448; the conversion's largest code takes those below 464)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j], f[4 * j + 1], 0, false);
-                    codes[j] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j + 2], f[4 * j + 3], w, true);
-                }
-            } else {
-                // 2^23 + 2^22 + f: f rounded to a whole number, ties to even, in the low bits
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    unsigned w[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) w[k] = __builtin_bit_cast(unsigned, f[4 * j + k] + 12582912.f);
-                    const unsigned lo = __builtin_amdgcn_perm(w[1], w[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(w[3], w[2], 0x04000C0Cu);
-                    codes[j] = lo | hi;
-                }
-            }
-            if (in[i]) {
-                *reinterpret_cast<u32x4*>(rows.cached(p, i, page[i], at[i])) = codes;
-                if (part == 0) *rows.scale(p, i, page[i], at[i]) = scale;
-            }
+        }
+        if (in) {
+            *reinterpret_cast<u32x4*>(rows.cached(page, key)) = codes;
+            if (threadIdx.x % R::LANES == 0) *rows.scale(page, key) = scale;
         }
     }
 #endif
@@ -252,56 +238,35 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const CacheParams
 template <typename T, int KIND, int D>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const CacheParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int EACH = each_of(KIND);
-    typedef Rows<D, EACH> R;
-    const R rows(p);
-    const int mask = (1 << p.page_shift) - 1;
-    int page[kUnits], at[kUnits];
-    bool of[kUnits];              // a row of some sequence
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-        at[i] = 0;
-        page[i] = -1;
-        of[i] = false;
-        if (rows.in[i]) {
-            const Place w = place_of(p.cu, p.B, rows.first, rows.row[i], p.rows);
-            of[i] = w.in;
-            if (w.in && (w.at >> p.page_shift) < p.width) page[i] = p.table[w.seq * p.table_row + (w.at >> p.page_shift)];
-            at[i] = w.at & mask;
-            page[i] = page[i] < p.pages ? page[i] : -1;
-        }
+    const Rows<D, each_of(KIND)> rows(p);
+    const Place w = rows.place(p, false);
+    const int from = rows.at() - w.start, key = from & ((1 << p.page_shift) - 1);
+    const bool of = rows.in && w.has(p, rows.at());      // a row of some sequence
+    if (!rows.in || !(of || p.fill)) return;
+    int page = -1;
+    if (of && (from >> p.page_shift) < p.width) page = p.table[w.seq * p.table_row + (from >> p.page_shift)];
+    const bool there = page >= 0 && page < p.pages;
+    const unsigned other = of ? round2<T>(NAN, NAN) : 0u;      // (of no sequence: zeros; of a page that is not there: NaN)
+    float scale = 1.f;
+    u32x4 codes = {0, 0, 0, 0};
+    if (there) {
+        codes = *reinterpret_cast<const u32x4*>(rows.cached(page, key));
+        if constexpr (KIND != SAME16) scale = *rows.scale(page, key);
     }
-    u32x4 w[kUnits];
-    float scale[kUnits];
+    u32x4* const to = reinterpret_cast<u32x4*>(rows.packed());
+    if constexpr (KIND == SAME16) {
+        *to = there ? codes : u32x4{other, other, other, other};
+    } else {
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-        scale[i] = 1.f;
-        w[i] = u32x4{0, 0, 0, 0};
-        if (page[i] >= 0) {
-            w[i] = *reinterpret_cast<const u32x4*>(rows.cached(p, i, page[i], at[i]));
-            if constexpr (KIND != SAME16) scale[i] = *rows.scale(p, i, page[i], at[i]);
-        }
-    }
+        for (int j = 0; j < 2; ++j) {
+            u32x4 x;
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-        if (!rows.in[i] || !(of[i] || p.fill)) continue;
-        const bool there = page[i] >= 0;
-        const unsigned other = of[i] ? round2<T>(NAN, NAN) : 0u;      // (of no sequence: zeros; of a page that is not there: NaN)
-        u32x4* const to = reinterpret_cast<u32x4*>(rows.packed(p, i));
-        if constexpr (KIND == SAME16) {
-            *to = there ? w[i] : u32x4{other, other, other, other};
-        } else {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                u32x4 x;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const unsigned a = code_pair<T, KIND, false>(w[i][2 * j + k]), b = code_pair<T, KIND, true>(w[i][2 * j + k]);
-                    x[2 * k] = round2<T>(low<T>(a) * scale[i], high<T>(a) * scale[i]);
-                    x[2 * k + 1] = round2<T>(low<T>(b) * scale[i], high<T>(b) * scale[i]);
-                }
-                to[j] = there ? x : u32x4{other, other, other, other};
+            for (int k = 0; k < 2; ++k) {
+                const unsigned a = code_pair<T, KIND, false>(codes[2 * j + k]), b = code_pair<T, KIND, true>(codes[2 * j + k]);
+                x[2 * k] = round2<T>(low<T>(a) * scale, high<T>(a) * scale);
+                x[2 * k + 1] = round2<T>(low<T>(b) * scale, high<T>(b) * scale);
             }
+            to[j] = there ? x : u32x4{other, other, other, other};
         }
     }
 #endif
@@ -407,8 +372,8 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
     }
     const int len = __builtin_amdgcn_readfirstlane(p.lens[seq]), from = (int)((int64_t)mine.part * mine.tiles / mine.parts), to = (int)((int64_t)(mine.part + 1) * mine.tiles / mine.parts);
     const int* const table = p.table + seq * p.table_row;
-    const char* const kh = p.k + head * p.k_head;
-    const char* const vh = p.v + head * p.v_head;
+    const char* const kh = p.side[0].pages + head * p.side[0].head;
+    const char* const vh = p.side[1].pages + head * p.side[1].head;
     const int mask = (1 << p.page_shift) - 1;
     // Q: row n16 of each block of 16, the channels that this lane's K holds
     V8 qf[NR][NC];
@@ -457,19 +422,19 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
     auto load_k = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const char* const at = kh + checked(kp[u]) * p.k_page + (int64_t)(k_key(t, u) & mask) * p.k_row + 16 * g;
+            const char* const at = kh + checked(kp[u]) * p.side[0].page + (k_key(t, u) & mask) * p.side[0].row + 16 * g;
 #pragma unroll
             for (int c = 0; c < KLOADS; ++c) kw[u][c] = *reinterpret_cast<const u32x4*>(at + 64 * c);
         }
     };
     auto load_v = [&](int t, int page) __attribute__((always_inline)) {
         const int key8 = v_key(t), in8 = key8 & mask;
-        const char* const at = vh + page * p.v_page + (int64_t)in8 * p.v_row + NB * BYTES * n16;
+        const char* const at = vh + page * p.side[1].page + in8 * p.side[1].row + NB * BYTES * n16;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) __builtin_memcpy(vw[i], __builtin_assume_aligned(at + (int64_t)(key8 + i < most ? i : most - key8) * p.v_row, 4 * VWORDS), 4 * VWORDS);
+        for (int i = 0; i < 8; ++i) __builtin_memcpy(vw[i], __builtin_assume_aligned(at + (key8 + i < most ? i : most - key8) * p.side[1].row, 4 * VWORDS), 4 * VWORDS);
         if constexpr (CODES) {
-            __builtin_memcpy(ks, __builtin_assume_aligned(p.k_scale + page * p.ks_page + head * p.ks_head + in8, 16), 32);
-            __builtin_memcpy(vs, __builtin_assume_aligned(p.v_scale + page * p.vs_page + head * p.vs_head + in8, 16), 32);
+            __builtin_memcpy(ks, __builtin_assume_aligned(p.side[0].scales + page * p.side[0].scale_page + head * p.side[0].scale_head + in8, 16), 32);
+            __builtin_memcpy(vs, __builtin_assume_aligned(p.side[1].scales + page * p.side[1].scale_page + head * p.side[1].scale_head + in8, 16), 32);
         }
     };
     if (from < end) {
@@ -735,16 +700,14 @@ int check(const cosmos_attn_cache_desc* d) {
 CacheParams params_of(const cosmos_attn_cache_desc* d) {
     CacheParams p = {};
     const int bytes = d->kind == COSMOS_ATTN_CACHE_SAME ? 2 : 1;
-    p.k = (char*)d->k; p.v = (char*)d->v;
-    p.k_page = bytes * d->k_stride[0]; p.k_head = bytes * d->k_stride[1]; p.k_row = (int)(bytes * d->k_stride[2]);
-    p.v_page = bytes * d->v_stride[0]; p.v_head = bytes * d->v_stride[1]; p.v_row = (int)(bytes * d->v_stride[2]);
-    p.k_scale = d->k_scale; p.v_scale = d->v_scale;
-    p.ks_page = d->k_scale_stride[0]; p.ks_head = d->k_scale_stride[1]; p.vs_page = d->v_scale_stride[0]; p.vs_head = d->v_scale_stride[1];
+    auto side = [&](void* pages, const int64_t* stride, float* scales, const int64_t* scale_stride, void* packed, const int64_t* packed_stride) {
+        return Side{(char*)pages, bytes * stride[0], bytes * stride[1], bytes * stride[2], scales, scale_stride[0], scale_stride[1], (char*)packed, 2 * packed_stride[0], 2 * packed_stride[1]};
+    };
+    p.side[0] = side(d->k, d->k_stride, d->k_scale, d->k_scale_stride, d->k_rows, d->k_rows_stride);
+    p.side[1] = side(d->v, d->v_stride, d->v_scale, d->v_scale_stride, d->v_rows, d->v_rows_stride);
     p.table = d->table; p.lens = d->lens; p.cu = d->cu; p.table_row = d->table_stride;
     p.width = d->width; p.B = d->B; p.pages = (int)d->pages; p.page_shift = __builtin_ctz(d->page_size); p.Hkv = d->Hkv; p.fill = d->fill != 0;
     p.rows = d->rows;
-    p.k_rows = (char*)d->k_rows; p.v_rows = (char*)d->v_rows;
-    p.kr_row = 2 * d->k_rows_stride[0]; p.kr_head = 2 * d->k_rows_stride[1]; p.vr_row = 2 * d->v_rows_stride[0]; p.vr_head = 2 * d->v_rows_stride[1];
     return p;
 }
 
@@ -779,8 +742,8 @@ int check_packed(const cosmos_attn_cache_desc* d, bool out) {
     return st;
 }
 int64_t packed_blocks(const cosmos_attn_cache_desc* d) {
-    const int64_t per = (int64_t)kUnits * (kThreads / (d->D / each_of(d->kind)));
-    return (d->rows * 2 * d->Hkv + per - 1) / per;
+    const int64_t per = (int64_t)(kThreads / (d->D / each_of(d->kind)));
+    return 2 * ((d->rows * d->Hkv + per - 1) / per);
 }
 
 int check_attention(const cosmos_attn_cache_desc* d) {
