@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(kThreads) cache_join_kernel(const CacheParams 
 }
 
 // ---- C ABI
-constexpr int64_t kMost = 0x7FFFFFFF;
+constexpr int64_t kMost = 0x7FFFFFFF, kMostBlocks = 0xFFFFFFFF / kThreads;      // (the threads of a launch are a 32-bit number)
 constexpr int64_t kMostRowBytes = (int64_t)1 << 23;
 
 int check_half(const void* at, const int64_t* stride, int bytes, int D) {
@@ -720,12 +720,16 @@ template <typename F> int with_type(const cosmos_attn_cache_desc* d, F&& f) {
 }
 int launch(void (*kernel)(CacheParams), int64_t blocks, size_t lds, const CacheParams& p, void* stream) {
     if (blocks <= 0) return COSMOS_ATTN_OK;
-    if (blocks > kMost) return COSMOS_ATTN_UNSUPPORTED;
+    if (blocks > kMostBlocks) return COSMOS_ATTN_UNSUPPORTED;
     if (lds && !allow_lds((const void*)kernel, lds)) return COSMOS_ATTN_LAUNCH_FAILED;
     kernel<<<dim3((unsigned)blocks), dim3(kThreads), lds, (hipStream_t)stream>>>(p);
     return hipGetLastError() == hipSuccess ? COSMOS_ATTN_OK : COSMOS_ATTN_LAUNCH_FAILED;
 }
 
+int64_t packed_blocks(const cosmos_attn_cache_desc* d) {
+    const int64_t per = kThreads / (d->D / each_of(d->kind));
+    return 2 * ((d->rows * d->Hkv + per - 1) / per);
+}
 int check_packed(const cosmos_attn_cache_desc* d, bool out) {
     int st = check(d);
     if (st != COSMOS_ATTN_OK) return st;
@@ -733,6 +737,7 @@ int check_packed(const cosmos_attn_cache_desc* d, bool out) {
     if (!d->rows) return COSMOS_ATTN_OK;
     if (d->B && !(out ? (const void*)d->cu : (const void*)d->lens)) return COSMOS_ATTN_BAD_ARG;
     if (!out && !d->cu && d->rows != d->B) return COSMOS_ATTN_BAD_SHAPE;
+    if (packed_blocks(d) > kMostBlocks) return COSMOS_ATTN_UNSUPPORTED;
     if (!d->B && out && !d->cu) return COSMOS_ATTN_BAD_ARG;
     for (int i = 0; st == COSMOS_ATTN_OK && i < 2; ++i) {
         const void* const at = i ? d->v_rows : d->k_rows;
@@ -740,10 +745,6 @@ int check_packed(const cosmos_attn_cache_desc* d, bool out) {
         st = out ? check_out(at, stride, d->rows, d->Hkv, d->D) : check_rows(at, stride);
     }
     return st;
-}
-int64_t packed_blocks(const cosmos_attn_cache_desc* d) {
-    const int64_t per = (int64_t)(kThreads / (d->D / each_of(d->kind)));
-    return 2 * ((d->rows * d->Hkv + per - 1) / per);
 }
 
 int check_attention(const cosmos_attn_cache_desc* d) {
@@ -754,7 +755,7 @@ int check_attention(const cosmos_attn_cache_desc* d) {
     if (!d->B) return COSMOS_ATTN_OK;
     if (!d->lens) return COSMOS_ATTN_BAD_ARG;
     // (tiles of all sequences are counted in 32 bits)
-    if ((int64_t)d->B * (((int64_t)d->width * d->page_size + kTile - 1) / kTile) > kMost / 2) return COSMOS_ATTN_UNSUPPORTED;
+    if ((int64_t)d->B * (((int64_t)d->width * d->page_size + kTile - 1) / kTile) > kMost / 2 || (int64_t)d->B * d->Hq > kMostBlocks / 2) return COSMOS_ATTN_UNSUPPORTED;
     st = check_rows(d->q, d->q_stride);
     return st != COSMOS_ATTN_OK ? st : check_out(d->o, d->o_stride, d->B, d->Hq, d->D);
 }

@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kJoinThreads) ragged_join_kernel(const RaggedP
 }
 
 // ---- C ABI
-constexpr int64_t kMost = 0x7FFFFFFF;
+constexpr int64_t kMost = 0x7FFFFFFF, kMostBlocks = 0xFFFFFFFF / kThreads;
 // rows of a step and a token's heads are addressed with 32 bits
 constexpr int64_t kMostRowBytes = (int64_t)1 << 23;
 
@@ -835,9 +835,9 @@ int check(const cosmos_attn_ragged_desc* d, bool backward) {
     if (d->Hq % d->Hkv) return COSMOS_ATTN_BAD_SHAPE;
     if (d->D != 64 && d->D != 128) return COSMOS_ATTN_UNSUPPORTED;
     const int64_t group = d->Hq / d->Hkv;
-    // (tile counts and rows are 32-bit numbers)
-    if (d->Tq * group > kMost / 2 || d->Tk > kMost / 2) return COSMOS_ATTN_UNSUPPORTED;
-    if (((d->Tq * group + d->Tk) / kRows + d->n_seq + 1) * d->Hkv > kMost / 32) return COSMOS_ATTN_UNSUPPORTED;
+    // (rows are 32-bit numbers, and so are the threads of a launch)
+    if (d->Tq > kMost || d->Tq * group > kMost / 2 || d->Tk > kMost / 2) return COSMOS_ATTN_UNSUPPORTED;
+    if (((d->Tq * group + d->Tk) / kRows + d->n_seq + 1) * d->Hkv > kMostBlocks) return COSMOS_ATTN_UNSUPPORTED;
     if (!d->cu_q || !d->cu_k) return COSMOS_ATTN_BAD_ARG;
     if ((reinterpret_cast<uintptr_t>(d->cu_q) | reinterpret_cast<uintptr_t>(d->cu_k)) & 3) return COSMOS_ATTN_BAD_STRIDE;
     int st = COSMOS_ATTN_OK;

@@ -28,7 +28,8 @@ def test_ragged_desc_layout_and_status_codes(pkg):
     cases = [
         (dict(abi_version=1), L.ST_BAD_ARG), (dict(n_seq=-1), L.ST_BAD_ARG), (dict(Hkv=0), L.ST_BAD_ARG), (dict(q=None), L.ST_BAD_ARG), (dict(cu_k=None), L.ST_BAD_ARG),
         (dict(sm_scale=float("nan")), L.ST_BAD_ARG), (dict(sm_scale=float("inf")), L.ST_BAD_ARG), (dict(Tq=-1), L.ST_BAD_ARG),
-        (dict(dtype=7), L.ST_UNSUPPORTED), (dict(D=96), L.ST_UNSUPPORTED), (dict(Tq=1 << 30), L.ST_UNSUPPORTED), (dict(Tk=1 << 31), L.ST_UNSUPPORTED),
+        (dict(dtype=7), L.ST_UNSUPPORTED), (dict(D=96), L.ST_UNSUPPORTED), (dict(Tq=1 << 30), L.ST_UNSUPPORTED), (dict(Tk=1 << 31), L.ST_UNSUPPORTED), (dict(Tq=1 << 62), L.ST_UNSUPPORTED),
+        (dict(n_seq=1 << 24), L.ST_UNSUPPORTED), (dict(Tk=1 << 30, Hkv=8), L.ST_UNSUPPORTED),
         (dict(Hkv=3), L.ST_BAD_SHAPE),
         (dict(k=P + 8), L.ST_BAD_STRIDE), (dict(cu_q=P + 2), L.ST_BAD_STRIDE), (dict(q_stride=(1020, 128)), L.ST_BAD_STRIDE), (dict(k_stride=(64, 128)), L.ST_BAD_STRIDE),
         (dict(v_stride=(256, -128)), L.ST_BAD_STRIDE), (dict(k_stride=((1 << 22) + 8, 128)), L.ST_BAD_STRIDE), (dict(q_stride=(1024, 1 << 27)), L.ST_BAD_STRIDE),
@@ -85,6 +86,9 @@ def test_cache_desc_layout_and_status_codes(pkg):
             D = cache_desc(pkg, cu=P, **over)
             assert call(D) == want, over
         assert lib.cosmos_attn_cache_attention_workspace_bytes(ctypes.byref(cache_desc(pkg, **over))) == 0
+    for call in (write, read):
+        assert call(cache_desc(pkg, cu=P, rows=1 << 30, Hkv=8)) == L.ST_UNSUPPORTED      # (more workgroups than a launch takes)
+    assert attend(cache_desc(pkg, B=1 << 21, width=1, Hq=8)) == L.ST_UNSUPPORTED
     for over, want in [(dict(rows=5), L.ST_BAD_SHAPE), (dict(lens=None), L.ST_BAD_ARG), (dict(k_rows=None), L.ST_BAD_ARG), (dict(v_rows_stride=(128, 60)), L.ST_BAD_STRIDE), (dict(rows=-1), L.ST_BAD_ARG)]:
         assert write(cache_desc(pkg, **over)) == want, over
     for over, want in [(dict(cu=None), L.ST_BAD_ARG), (dict(cu=P, k_rows_stride=(64, 64)), L.ST_BAD_STRIDE), (dict(cu=P, v_rows_stride=(128, 0)), L.ST_BAD_STRIDE)]:
