@@ -653,6 +653,7 @@ __global__ void __launch_bounds__(kThreads) cache_join_kernel(const CacheParams 
 
 // ---- C ABI
 constexpr int64_t kMost = 0x7FFFFFFF, kMostBlocks = 0xFFFFFFFF / kThreads;      // (the threads of a launch are a 32-bit number)
+constexpr int64_t kMostKeys = (int64_t)1 << 30;       // of a sequence: positions some steps behind its last are 32-bit numbers too
 constexpr int64_t kMostRowBytes = (int64_t)1 << 23;
 
 int check_half(const void* at, const int64_t* stride, int bytes, int D) {
@@ -685,7 +686,7 @@ int check(const cosmos_attn_cache_desc* d) {
     if (d->D != 64 && d->D != 128) return COSMOS_ATTN_UNSUPPORTED;
     if (d->Hkv < 1 || d->B < 0 || d->width < 0 || d->pages < 1 || d->pages > kMost) return COSMOS_ATTN_BAD_ARG;
     if (d->page_size < 16 || d->page_size > 1024 || (d->page_size & (d->page_size - 1))) return COSMOS_ATTN_BAD_SHAPE;
-    if ((int64_t)d->width * d->page_size > kMost) return COSMOS_ATTN_UNSUPPORTED;
+    if ((int64_t)d->width * d->page_size > kMostKeys) return COSMOS_ATTN_UNSUPPORTED;
     const int bytes = d->kind == COSMOS_ATTN_CACHE_SAME ? 2 : 1;
     int st = check_half(d->k, d->k_stride, bytes, d->D);
     if (st == COSMOS_ATTN_OK) st = check_half(d->v, d->v_stride, bytes, d->D);

@@ -32,9 +32,10 @@ _CALL_PART = struct.Struct("=2iQq2Qq2Q4q2ifi2Q4qQ")
 
 class KVCache:
     """Pages of keys and values, ``[pages, heads, page_size, head_dim]`` each: bf16, fp16, or 8 bits (float8_e4m3fn, int8) with an fp32 scale for each row of a head,
-    ``[pages, heads, page_size]``.  Takes the tensors as they are (any page, head and row strides of 16-byte steps) and writes into them."""
+    ``[pages, heads, page_size]``.  Takes the tensors as they are (any page, head and row strides of 16-byte steps) and writes into them:
+    ``k``, ``v``, ``k_scale``, ``v_scale`` are theirs, and stay so (a tensor's memory must not be exchanged below the cache, by ``set_`` or ``resize_``)."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page_size", "head_dim", "dtype", "device", "kind", "_parts", "_index")
+    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "pages", "heads", "page_size", "head_dim", "dtype", "device", "kind", "_parts", "_index")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
         assert k.dim() == 4 and v.shape == k.shape, "k and v must be [pages, heads, page_size, head_dim]"
@@ -58,7 +59,7 @@ class KVCache:
             for x in scales:
                 assert x is not None and x.shape == k.shape[:3] and x.dtype == torch.float32 and x.device == k.device, "8 bits need fp32 scales [pages, heads, page_size]"
                 assert x.stride(2) == 1 and x.stride(0) % 4 == 0 and x.stride(1) % 4 == 0 and x.data_ptr() % 16 == 0, "scales of a head's page lie side by side"
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
         self._index = k.get_device()
         at = lambda x: 0 if x is None else x.data_ptr()
         steps = lambda x, n: (0,) * n if x is None else x.stride()[:n]
@@ -66,6 +67,13 @@ class KVCache:
             dtype: _CACHE_PART.pack(_lib.ABI_VERSION, code, self.kind, self.heads, self.head_dim, self.page_size, self.pages, at(k), at(v), *steps(k, 3), *steps(v, 3),
                                     at(k_scale), at(v_scale), *steps(k_scale, 2), *steps(v_scale, 2))
             for dtype, code in _DTYPES.items()}
+
+    k, v = property(lambda self: self._k), property(lambda self: self._v)
+    k_scale, v_scale = property(lambda self: self._k_scale), property(lambda self: self._v_scale)
+
+    def __reduce__(self):
+        """A copy, or what is loaded, is a cache of its own tensors."""
+        return type(self), (self._k, self._v, self._k_scale, self._v_scale)
 
     @classmethod
     def empty(cls, pages: int, heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.bfloat16, device="cuda") -> "KVCache":
@@ -115,8 +123,8 @@ def cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, table: torch.T
     """Packed rows ``k``, ``v`` ``[rows, heads, D]`` into the cache: sequence i's are ``cu[i] .. cu[i + 1] - 1`` (``cu`` None: one for each sequence), its last positions; ``lens[i]`` counts them.
 
     8 bits: ``scale = max |x| * fp32(1 / 448)`` (e4m3) or ``* fp32(1 / 127)`` (int8), ``code = round(x / scale)``, all in fp32; a row with a value that is not finite reads back as NaN.
-    Rows of no sequence, sequences whose ``lens`` is below their rows or more than the table holds, and pages outside of the cache: nothing is written.  No two rows of a call may have
-    one place."""
+    Rows of no sequence, sequences whose ``lens`` is below their rows, positions that the table does not hold and pages outside of the cache: nothing is written.  No two rows of a call
+    may have one place."""
     k = _check_rows(k, "k", cache)
     v = _check_rows(v, "v", cache, k)
     assert k.shape == v.shape and k.shape[1] == cache.heads, "k and v must be [rows, heads, D] of the cache"

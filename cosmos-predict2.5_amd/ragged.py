@@ -12,6 +12,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -207,8 +208,9 @@ class _RaggedFn(torch.autograd.Function):
 
 
 def attention_ragged(q, k, v, cu_q, cu_k=None, softmax_scale=None, causal=False):
-    """Differentiable attention over packed sequences: o of :func:`ragged_fwd`, gradients by :func:`ragged_bwd`.  The offsets must not change between the two."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    """Differentiable attention over packed sequences: o of :func:`ragged_fwd`, gradients by :func:`ragged_bwd`.  The offsets must not change between the two.  No tangents: forward-mode
+    differentiation is refused."""
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or forward_ad._current_level >= 0:
         cu_q = int32_on(cu_q, q.device)
         return _RaggedFn.apply(q, k, v, cu_q, cu_q if cu_k is None else int32_on(cu_k, q.device), causal, softmax_scale)
     return ragged_fwd(q, k, v, cu_q, cu_k, causal=causal, sm_scale=softmax_scale, need_lse=False)[0]

@@ -442,8 +442,8 @@ COSMOS_ATTN_API int cosmos_attn_ragged_bwd(const cosmos_attn_ragged_desc *desc, 
  * element strides, of the 16-bit type `dtype` or of 8 bits with an fp32 scale for each row, [pages, Hkv, page_size] through (page, head) strides:
  *     scale = max |x| * fp32(1 / 448) (e4m3) or * fp32(1 / 127) (int8), code = round(x / scale), all in fp32;  a row with a value that is not finite has the scale NaN
  * Position j of sequence i lies in page table[i][j / page_size], place j % page_size.  Tables and lengths stay on the device and may change between replays of a captured call; entries
- * behind a sequence's last page are not looked at.  They are not trusted: a page outside of the cache or a length that the table does not hold writes nothing, reads back as NaN and
- * makes the sequence's attention NaN.  What pages hold behind a sequence's end may be anything.
+ * behind a sequence's last page are not looked at.  They are not trusted: positions that the table does not hold, or whose page is not in the cache, are not written and read back as NaN;
+ * the attention of a sequence with one, or with a length below 0, is NaN.  What pages hold behind a sequence's end may be anything.
  *
  * cosmos_attn_cache_write: packed rows k_rows, v_rows [rows, Hkv, D]; sequence i's are cu[i] .. cu[i + 1] - 1 (cu NULL: one for each sequence), its last positions: lens[i], which counts
  *     them, is where they end.  Rows of no sequence, and sequences with lens[i] below their rows, write nothing.  Two rows of a call must not have one place (two sequences sharing a page).
@@ -462,7 +462,7 @@ typedef struct cosmos_attn_cache_desc {
     int64_t k_stride[3], v_stride[3];  /* multiples of 16 bytes */
     float *k_scale, *v_scale;          /* 8 bits alone */
     int64_t k_scale_stride[2], v_scale_stride[2];   /* multiples of 4 */
-    int32_t B, width;                  /* sequences; entries of a row of the table: width * page_size below 2^31 */
+    int32_t B, width;                  /* sequences; entries of a row of the table: width * page_size at most 2^30 */
     const int32_t *table;              /* [B, width], rows table_stride elements apart */
     int64_t table_stride;
     const int32_t *lens;               /* [B]; not read by cosmos_attn_cache_read */

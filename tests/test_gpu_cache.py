@@ -1,4 +1,5 @@
 """The paged key-value cache: writing, reading back and attention of one token, against the definitions; and a prompt that goes through all of it in pieces."""
+import copy
 import math
 
 import pytest
@@ -145,6 +146,20 @@ def test_places_that_are_not_there(pkg, gpu):
     before = cache.k.clone()
     pkg.cache_write(cache, k[:8], k[:8], table, offsets([1, 0, -3, 1 << 30], gpu), offsets([0, 2, 4, 6, 8], gpu))
     assert torch.equal(cache.k, before)
+
+
+def test_copies_have_pages_of_their_own(pkg, gpu):
+    cache, table = empty(pkg, 2, 2, 16, 64, torch.int8, gpu), torch.tensor([[1]], dtype=torch.int32, device=gpu)
+    for x in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        x.zero_()
+    other, same = copy.deepcopy(cache), copy.copy(cache)
+    k = rows(3, 2, 64, BF16, gpu, 0)
+    pkg.cache_write(other, k, k, table, offsets([3], gpu), offsets([0, 3], gpu))
+    assert (other.k_scale[1, :, :3] > 0).all() and (cache.k == 0).all() and (cache.k_scale == 0).all()
+    pkg.cache_write(same, k, k, table, offsets([3], gpu), offsets([0, 3], gpu))
+    assert torch.equal(cache.k, other.k) and torch.equal(cache.v_scale, other.v_scale)
+    with pytest.raises(AttributeError):
+        cache.k = other.k
 
 
 def test_rows_of_no_sequence_are_neither_written_nor_read(pkg, gpu):

@@ -234,6 +234,19 @@ def test_gradients_of_shared_and_of_frozen_tensors(pkg, gpu):
     assert ((k2.grad.double() - dk.double()).abs() <= 2.0 ** -8 * (1 + 2.0 ** -7) * (two.abs().sum(1, keepdim=True) + k2.grad.double().abs() + dk.double().abs()) + 1e-5).all()
 
 
+def test_tangents_are_refused(pkg, gpu):
+    q, at = rows(4, 2, 64, torch.bfloat16, gpu, 0), offsets([0, 4], gpu)
+    with torch.autograd.forward_ad.dual_level():
+        for i in range(3):
+            x = [torch.autograd.forward_ad.make_dual(q, q) if i == j else q for j in range(3)]
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                pkg.attention_ragged(*x, at)
+        plain = pkg.attention_ragged(q, q, q, at)
+    assert torch.equal(plain, pkg.attention_ragged(q, q, q, at))
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda x: pkg.attention_ragged(x, q, q, at), (q,), (q,))
+
+
 def test_same_results_every_time(pkg, gpu):
     q, k, v, g = (rows(1000, h, 128, BF16, gpu, i) for i, h in enumerate((8, 2, 2, 8)))
     on = offsets([0, 300, 301, 1000], gpu)

@@ -77,7 +77,7 @@ def test_cache_desc_layout_and_status_codes(pkg):
     attend = lambda D: lib.cosmos_attn_cache_attention(ctypes.byref(D), P, 1 << 40, None)
     for over, want in [
         (dict(abi_version=1), L.ST_BAD_ARG), (dict(pages=0), L.ST_BAD_ARG), (dict(k=None), L.ST_BAD_ARG), (dict(v_scale=None), L.ST_BAD_ARG), (dict(table=None), L.ST_BAD_ARG), (dict(B=-1), L.ST_BAD_ARG),
-        (dict(dtype=5), L.ST_UNSUPPORTED), (dict(kind=3), L.ST_UNSUPPORTED), (dict(D=32), L.ST_UNSUPPORTED), (dict(width=1 << 26), L.ST_UNSUPPORTED),
+        (dict(dtype=5), L.ST_UNSUPPORTED), (dict(kind=3), L.ST_UNSUPPORTED), (dict(D=32), L.ST_UNSUPPORTED), (dict(width=1 << 26), L.ST_UNSUPPORTED), (dict(width=(1 << 25) + 1), L.ST_UNSUPPORTED),
         (dict(page_size=8), L.ST_BAD_SHAPE), (dict(page_size=48), L.ST_BAD_SHAPE), (dict(page_size=2048), L.ST_BAD_SHAPE),
         (dict(k=P + 8), L.ST_BAD_STRIDE), (dict(k_stride=(4096, 2048, 72)), L.ST_BAD_STRIDE), (dict(v_stride=(4096, 2048, 48)), L.ST_BAD_STRIDE),
         (dict(k_scale_stride=(64, 30)), L.ST_BAD_STRIDE), (dict(table=P + 1), L.ST_BAD_STRIDE), (dict(table_stride=-10), L.ST_BAD_STRIDE),
