@@ -112,6 +112,37 @@ def _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse):
     return o, lse
 
 
+def _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale):
+    """:func:`ragged_bwd`, as :func:`_fwd_as_it_is` (forward and gradients of 48 positions through autograd: 131 us, 138 with the checks one by one)."""
+    if not (q.dim() == 3 == k.dim() and q.is_cuda and o.is_contiguous() and lse.is_contiguous()):
+        return None
+    shape, dtype, device, kv = q.shape, q.dtype, q.get_device(), k.shape
+    (Tq, Hq, D), (Tk, Hkv, _), code = shape, kv, _DTYPES.get(dtype)
+    if cu_k is None:
+        cu_k = cu_q
+    if (code is None or D not in HEAD_DIMS or kv[2] != D or v.shape != kv or o.shape != shape or dout.shape != shape or lse.shape != (Hq, Tq) or lse.dtype is not torch.float32
+            or any(x.dtype is not dtype or x.get_device() != device for x in (k, v, o, dout)) or lse.get_device() != device
+            or Hq < 1 or Hkv < 1 or Hq % Hkv or not plain_int32(cu_q, 1, device) or not (cu_k is cu_q or plain_int32(cu_k, 1, device)) or cu_q.shape != cu_k.shape):
+        return None
+    (q0, q1, q2), (k0, k1, k2), (v0, v1, v2), (g0, g1, g2) = q.stride(), k.stride(), v.stride(), dout.stride()
+    pq, pk, pv, po, pg = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr()
+    if (not q2 == k2 == v2 == g2 == 1 or (pq | pk | pv | po | pg) & 15 or (q0 | q1 | k0 | k1 | v0 | v1 | g0 | g1) & 7 or min(q0, k0, v0, g0) < D or max(q0, k0, v0, g0, Hq * D) > _MOST_ROW_BYTES // 2
+            or max(q1 * Hq, k1 * Hkv, v1 * Hkv, g1 * Hq) > 1 << 29):
+        return None
+    dq, dk, dv = (torch.empty(x, device=q.device, dtype=dtype) for x in (shape, kv, kv))
+    desc = _RAGGED_DESC.pack(_lib.ABI_VERSION, code, cu_q.shape[0] - 1, Hq, Hkv, D, 1 if causal else 0, 1, Tq, Tk, D ** -0.5 if sm_scale is None else sm_scale, 0, pq, pk, pv, cu_q.data_ptr(),
+                             cu_k.data_ptr(), po, lse.data_ptr(), pg, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), q0, q1, k0, k1, v0, v1, Hq * D, D, g0, g1, Hq * D, D, Hkv * D, D, Hkv * D, D)
+    _launch_bwd(device, desc, q)
+    return dq, dk, dv
+
+
+def _launch_bwd(device, desc, like):
+    lib = _lib.load_library()
+    ws_bytes = lib.cosmos_attn_ragged_bwd_workspace_bytes(desc)
+    workspace = like.new_empty(ws_bytes, dtype=torch.uint8)
+    on_device(device, lib.cosmos_attn_ragged_bwd, desc, workspace.data_ptr(), ws_bytes)
+
+
 def _strides(*tensors):
     return [s for x in tensors for s in ((0, 0) if x is None else x.stride()[:2])]
 
@@ -178,6 +209,9 @@ def ragged_bwd(
     sm_scale: Optional[float] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(dq, dk, dv)`` of :func:`ragged_fwd` for the gradient ``dout`` of o, from its o and lse.  Rows of no sequence get zeros.  The same results every time (no atomics)."""
+    made = _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale)
+    if made is not None:
+        return made
     cu_q, cu_k = _check(q, k, v, cu_q, cu_k)
     for x, name in ((o, "o"), (dout, "dout")):
         assert x.shape == q.shape and x.dtype == q.dtype and x.device == q.device, f"{name} must have q's shape, type and device"
@@ -185,10 +219,7 @@ def ragged_bwd(
     q, k, v, o, dout, lse = packed(q), packed(k), packed(v), packed(o), packed(dout), lse.contiguous()
     dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
     desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, True, dout, dq, dk, dv)
-    lib = _lib.load_library()
-    ws_bytes = lib.cosmos_attn_ragged_bwd_workspace_bytes(desc)
-    workspace = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8)
-    on_device(q.get_device(), lib.cosmos_attn_ragged_bwd, desc, workspace.data_ptr(), ws_bytes)
+    _launch_bwd(q.get_device(), desc, q)
     return dq, dk, dv
 
 
