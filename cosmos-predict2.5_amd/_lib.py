@@ -260,6 +260,7 @@ class RaggedDesc(ctypes.Structure):
         ("dout", ctypes.c_void_p), ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p),
         ("q_stride", ctypes.c_int64 * 2), ("k_stride", ctypes.c_int64 * 2), ("v_stride", ctypes.c_int64 * 2), ("o_stride", ctypes.c_int64 * 2),
         ("dout_stride", ctypes.c_int64 * 2), ("dq_stride", ctypes.c_int64 * 2), ("dk_stride", ctypes.c_int64 * 2), ("dv_stride", ctypes.c_int64 * 2),
+        ("rest", ctypes.c_void_p),
     ]
 
 

@@ -37,6 +37,7 @@ struct RaggedParams {
     const char *q, *k, *v, *o_in, *dout;
     char *o, *dq, *dk, *dv;
     float* lse;                    // [Hq, Tq]; written by the forward (may be null), read by the backward
+    char* rest;                    // [Tq, Hq, D]: what rounding o left off, 16 bits again (may be null)
     float* delta;                  // [Hq, Tq]: of the backward's first kernel for its second
     const int *cu_q, *cu_k;
     // bytes between rows and between heads
@@ -103,6 +104,20 @@ template <typename T> __device__ __forceinline__ unsigned round2(float a, float 
     typedef T V2 __attribute__((ext_vector_type(2)));
     const V2 two = {(T)a, (T)b};
     return __builtin_bit_cast(unsigned, two);
+}
+// four elements of o, and what their rounding leaves off.  The backward's delta = dout . o is taken off every dP of a row, next to which it is large where a row's weight lies on few keys:
+// with o's 8 bits alone dq and dk of sharp softmaxes (scores of a deviation of 4, 1000 positions, bf16) are 3.6e-3 off, with 16 bits 2.5e-3; their own rounding is 1.7e-3.
+template <typename T> __device__ __forceinline__ float element(unsigned w, int i) {
+    typedef T V2 __attribute__((ext_vector_type(2)));
+    return (float)__builtin_bit_cast(V2, w)[i];
+}
+template <typename T> __device__ __forceinline__ void store_rounded(char* to, char* rest, float a, float b, float c, float d) {
+    u32x2 w = {round2<T>(a, b), round2<T>(c, d)};
+    *reinterpret_cast<u32x2*>(to) = w;
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm("" : "+v"(w));      // (what is stored: left to itself the compiler rounds a second time, a product of fp16 then in one step with the multiplication, which next to a tie goes elsewhere)
+#endif
+    if (rest) *reinterpret_cast<u32x2*>(rest) = u32x2{round2<T>(a - element<T>(w[0], 0), b - element<T>(w[0], 1)), round2<T>(c - element<T>(w[1], 0), d - element<T>(w[1], 1))};
 }
 // The order of a block's LDS reads and matrix products, READS to PRODUCTS: AHEAD reads first, then each product with its share of the others.  (Left alone the compiler reads the operands of two
 // products and waits for them: 2 % of the forward, and of the dK/dV kernel, where no more registers are free for it.)
@@ -401,11 +416,12 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
     float lse = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * 0.693147180559945309f : l == 0.f ? -INFINITY : l;
     if (rk.length < 0) by = lse = NAN;
     char* const at = p.o + (rq.start + token) * p.o_row + hq * p.o_head + 8 * half;
+    char* const rest = p.rest ? p.rest + ((int64_t)(rq.start + token) * p.group * p.Hkv + hq) * (2 * D) + 8 * half : nullptr;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<u32x2*>(at + 64 * b + 16 * i) = u32x2{round2<T>(acc[b][4 * i] * by, acc[b][4 * i + 1] * by), round2<T>(acc[b][4 * i + 2] * by, acc[b][4 * i + 3] * by)};
+            store_rounded<T>(at + 64 * b + 16 * i, rest ? rest + 64 * b + 16 * i : nullptr, acc[b][4 * i] * by, acc[b][4 * i + 1] * by, acc[b][4 * i + 2] * by, acc[b][4 * i + 3] * by);
     if (p.lse && half == 0) p.lse[(int64_t)hq * p.Tq + rq.start + token] = lse;
 #endif
 }
@@ -465,20 +481,22 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
         const char* const qa = p.q + (rq.start + token) * p.q_row + hq * p.q_head + 16 * half;
         const char* const ga = p.dout + (rq.start + token) * p.do_row + hq * p.do_head + 16 * half;
         const char* const oa = p.o_in + (rq.start + token) * p.o_row + hq * p.o_head + 16 * half;
+        const char* const ra = p.rest + ((int64_t)(rq.start + token) * p.group * p.Hkv + hq) * (2 * D) + 16 * half;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            u32x4 a = {0, 0, 0, 0}, b = a, o = a;
+            u32x4 a = {0, 0, 0, 0}, b = a, o = a, r = a;
             if (live) {
                 a = *reinterpret_cast<const u32x4*>(qa + 32 * c);
                 b = *reinterpret_cast<const u32x4*>(ga + 32 * c);
                 o = *reinterpret_cast<const u32x4*>(oa + 32 * c);
+                if (p.rest) r = *reinterpret_cast<const u32x4*>(ra + 32 * c);
             }
             a ^= p.flip;
             qf[c] = __builtin_bit_cast(V8, a);
             gf[c] = __builtin_bit_cast(V8, b);
-            const V8 of = __builtin_bit_cast(V8, o);
+            const V8 of = __builtin_bit_cast(V8, o), rf = __builtin_bit_cast(V8, r);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)gf[c][i], (float)of[i], delta);
+            for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)gf[c][i], (float)of[i] + (float)rf[i], delta);
         }
         delta = over_halves_sum(delta);
     }
@@ -786,7 +804,9 @@ __global__ void __launch_bounds__(kJoinThreads) ragged_join_kernel(const RaggedP
             sum += by * f32x4{lo[0], lo[1], hi[0], hi[1]};
         }
         const float by = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-        store(p.o + (r.start + token) * p.o_row + h * p.o_head, sum * by);
+        sum *= by;
+        char* const rest = p.rest ? p.rest + ((int64_t)(r.start + token) * p.group * p.Hkv + h) * (2 * D) + 2 * c : nullptr;
+        store_rounded<T>(p.o + (r.start + token) * p.o_row + h * p.o_head + 2 * c, rest, sum[0], sum[1], sum[2], sum[3]);
         if (p.lse && c == 0) p.lse[(int64_t)h * p.Tq + r.start + token] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * 0.693147180559945309f : l == 0.f ? -INFINITY : l;
     } else {
         f32x4 sum[WHICH];
@@ -846,6 +866,7 @@ int check(const cosmos_attn_ragged_desc* d, bool backward) {
     in(d->q, d->q_stride, d->Tq, d->Hq);
     in(d->k, d->k_stride, d->Tk, d->Hkv);
     in(d->v, d->v_stride, d->Tk, d->Hkv);
+    if (d->rest && !aligned16(d->rest)) return COSMOS_ATTN_BAD_STRIDE;
     if (!backward) {
         out(d->o, d->o_stride, d->Tq, d->Hq);
     } else {
@@ -865,6 +886,7 @@ RaggedParams params_of(const cosmos_attn_ragged_desc* d) {
     p.o = (char*)d->o; p.o_in = (const char*)d->o; p.dout = (const char*)d->dout;
     p.dq = (char*)d->dq; p.dk = (char*)d->dk; p.dv = (char*)d->dv;
     p.lse = d->lse;
+    p.rest = (char*)d->rest;
     p.cu_q = d->cu_q; p.cu_k = d->cu_k;
     p.q_row = 2 * d->q_stride[0]; p.q_head = 2 * d->q_stride[1];
     p.k_row = 2 * d->k_stride[0]; p.k_head = 2 * d->k_stride[1];

@@ -22,7 +22,7 @@ HEAD_DIMS = (64, 128)
 _MOST_ROW_BYTES = 1 << 23
 
 # struct cosmos_attn_ragged_desc in one go
-_RAGGED_DESC = struct.Struct("@8i2qfi11Q16q")
+_RAGGED_DESC = struct.Struct("@8i2qfi11Q16qQ")
 
 
 def packed_ready(x: torch.Tensor) -> bool:
@@ -85,7 +85,7 @@ def on_device(device: int, launch, desc: bytes, *rest) -> None:
         _lib.raise_for_status(status)
 
 
-def _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse):
+def _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse, rest):
     """:func:`ragged_fwd` of tensors that can be taken as they are, all of it looked at once: None where something is to be converted, copied or refused.  A small call is as long as what the
     host does for it: one short prompt 11 us, 17 with the checks one by one."""
     if not (q.dim() == 3 == k.dim() and q.is_cuda):
@@ -104,7 +104,7 @@ def _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse):
     o = torch.empty_like(q) if q.is_contiguous() else torch.empty((Tq, Hq, D), device=q.device, dtype=dtype)
     lse = q.new_empty((Hq, Tq), dtype=torch.float32) if need_lse else None
     desc = _RAGGED_DESC.pack(_lib.ABI_VERSION, code, cu_q.shape[0] - 1, Hq, Hkv, D, 1 if causal else 0, 1, Tq, Tk, D ** -0.5 if sm_scale is None else sm_scale, 0, pq, pk, pv, cu_q.data_ptr(),
-                             cu_k.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, q0, q1, k0, k1, v0, v1, Hq * D, D, 0, 0, 0, 0, 0, 0, 0, 0)
+                             cu_k.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, q0, q1, k0, k1, v0, v1, Hq * D, D, 0, 0, 0, 0, 0, 0, 0, 0, 0 if rest is None else rest.data_ptr())
     lib = _lib.load_library()
     ws_bytes = lib.cosmos_attn_ragged_workspace_bytes(desc)
     workspace = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
@@ -112,7 +112,7 @@ def _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse):
     return o, lse
 
 
-def _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale):
+def _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale, rest):
     """:func:`ragged_bwd`, as :func:`_fwd_as_it_is` (forward and gradients of 48 positions through autograd: 131 us, 138 with the checks one by one)."""
     if not (q.dim() == 3 == k.dim() and q.is_cuda and o.is_contiguous() and lse.is_contiguous()):
         return None
@@ -131,7 +131,7 @@ def _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale):
         return None
     dq, dk, dv = (torch.empty(x, device=q.device, dtype=dtype) for x in (shape, kv, kv))
     desc = _RAGGED_DESC.pack(_lib.ABI_VERSION, code, cu_q.shape[0] - 1, Hq, Hkv, D, 1 if causal else 0, 1, Tq, Tk, D ** -0.5 if sm_scale is None else sm_scale, 0, pq, pk, pv, cu_q.data_ptr(),
-                             cu_k.data_ptr(), po, lse.data_ptr(), pg, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), q0, q1, k0, k1, v0, v1, Hq * D, D, g0, g1, Hq * D, D, Hkv * D, D, Hkv * D, D)
+                             cu_k.data_ptr(), po, lse.data_ptr(), pg, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), q0, q1, k0, k1, v0, v1, Hq * D, D, g0, g1, Hq * D, D, Hkv * D, D, Hkv * D, D, 0 if rest is None else rest.data_ptr())
     _launch_bwd(device, desc, q)
     return dq, dk, dv
 
@@ -143,6 +143,10 @@ def _launch_bwd(device, desc, like):
     on_device(device, lib.cosmos_attn_ragged_bwd, desc, workspace.data_ptr(), ws_bytes)
 
 
+def _check_rest(rest, q):
+    assert rest.shape == q.shape and rest.dtype == q.dtype and rest.device == q.device and rest.is_contiguous() and rest.data_ptr() % 16 == 0, "rest must be a contiguous tensor like q"
+
+
 def _strides(*tensors):
     return [s for x in tensors for s in ((0, 0) if x is None else x.stride()[:2])]
 
@@ -151,10 +155,10 @@ def _pointers(*tensors):
     return [0 if x is None else x.data_ptr() for x in tensors]
 
 
-def _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, fill, dout=None, dq=None, dk=None, dv=None) -> bytes:
+def _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, fill, rest, dout=None, dq=None, dk=None, dv=None) -> bytes:
     return _RAGGED_DESC.pack(
         _lib.ABI_VERSION, _DTYPES[q.dtype], cu_q.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2], 1 if causal else 0, 1 if fill else 0, q.shape[0], k.shape[0],
-        q.shape[2] ** -0.5 if sm_scale is None else sm_scale, 0, *_pointers(q, k, v, cu_q, cu_k, o, lse, dout, dq, dk, dv), *_strides(q, k, v, o, dout, dq, dk, dv))
+        q.shape[2] ** -0.5 if sm_scale is None else sm_scale, 0, *_pointers(q, k, v, cu_q, cu_k, o, lse, dout, dq, dk, dv), *_strides(q, k, v, o, dout, dq, dk, dv), *_pointers(rest))
 
 
 def ragged_fwd(
@@ -167,15 +171,19 @@ def ragged_fwd(
     sm_scale: Optional[float] = None,
     need_lse: bool = True,
     out: Optional[torch.Tensor] = None,
+    rest: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``(o, lse)``: ``q [Tq, Hq, D]``, ``k``, ``v`` ``[Tk, Hkv, D]``; sequence i has the rows ``cu_q[i] .. cu_q[i + 1] - 1`` of q and ``cu_k[i] ..`` of k and v
     (``cu_k`` None: the same).  ``causal``: query t of Lq sees the keys up to ``t + Lk - Lq``.  ``lse``: fp32 ``[Hq, Tq]``.
 
     A row that sees no key: o = 0, lse = -inf.  Rows of no sequence (before ``cu_q[0]``, from the last offset on) become zeros, and -inf; in ``out``, a tensor that is given for o, they are
-    left as they are.  Offsets that do not ascend within the tensors: such ``cu_q`` leaves the sequence's rows unwritten, such ``cu_k`` makes them NaN.  ``out`` must not overlap the inputs.  No gradients:
+    left as they are.  Offsets that do not ascend within the tensors: such ``cu_q`` leaves the sequence's rows unwritten, such ``cu_k`` makes them NaN.  ``out`` must not overlap the inputs.
+    ``rest``, a contiguous tensor like q, takes what rounding o left off, for :func:`ragged_bwd` (rows of no sequence: left as they are).  No gradients:
     :func:`attention_ragged` has them."""
+    if rest is not None:
+        _check_rest(rest, q)
     if out is None:
-        made = _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse)
+        made = _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse, rest)
         if made is not None:
             return made
     cu_q, cu_k = _check(q, k, v, cu_q, cu_k)
@@ -188,7 +196,7 @@ def ragged_fwd(
             raise ValueError("out: rows of 16-byte steps are written in place, this view cannot be")
         o = out
     lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32) if need_lse else None
-    desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, out is None)
+    desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, out is None, rest)
     lib = _lib.load_library()
     ws_bytes = lib.cosmos_attn_ragged_workspace_bytes(desc)
     workspace = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
@@ -207,9 +215,13 @@ def ragged_bwd(
     cu_k: Optional[torch.Tensor] = None,
     causal: bool = False,
     sm_scale: Optional[float] = None,
+    rest: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """``(dq, dk, dv)`` of :func:`ragged_fwd` for the gradient ``dout`` of o, from its o and lse.  Rows of no sequence get zeros.  The same results every time (no atomics)."""
-    made = _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale)
+    """``(dq, dk, dv)`` of :func:`ragged_fwd` for the gradient ``dout`` of o, from its o and lse, and its ``rest``: without it dq and dk of sharp softmaxes, and of rows that see
+    few keys, have o's rounding in them.  Rows of no sequence get zeros.  The same results every time (no atomics)."""
+    if rest is not None:
+        _check_rest(rest, q)
+    made = _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale, rest)
     if made is not None:
         return made
     cu_q, cu_k = _check(q, k, v, cu_q, cu_k)
@@ -218,7 +230,7 @@ def ragged_bwd(
     assert lse.shape == (q.shape[1], q.shape[0]) and lse.dtype == torch.float32 and lse.device == q.device, "lse is the forward's, fp32 [Hq, Tq]"
     q, k, v, o, dout, lse = packed(q), packed(k), packed(v), packed(o), packed(dout), lse.contiguous()
     dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
-    desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, True, dout, dq, dk, dv)
+    desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, True, rest, dout, dq, dk, dv)
     _launch_bwd(q.get_device(), desc, q)
     return dq, dk, dv
 
@@ -226,16 +238,17 @@ def ragged_bwd(
 class _RaggedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, causal, softmax_scale):
-        o, lse = ragged_fwd(q, k, v, cu_q, cu_k, causal=causal, sm_scale=softmax_scale)
-        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k)
+        rest = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        o, lse = ragged_fwd(q, k, v, cu_q, cu_k, causal=causal, sm_scale=softmax_scale, rest=rest)
+        ctx.save_for_backward(q, k, v, o, lse, rest, cu_q, cu_k)
         ctx.causal, ctx.softmax_scale = causal, softmax_scale
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, o, lse, cu_q, cu_k = ctx.saved_tensors
-        return (*ragged_bwd(q, k, v, o, lse, dout, cu_q, cu_k, causal=ctx.causal, sm_scale=ctx.softmax_scale), None, None, None, None)
+        q, k, v, o, lse, rest, cu_q, cu_k = ctx.saved_tensors
+        return (*ragged_bwd(q, k, v, o, lse, dout, cu_q, cu_k, causal=ctx.causal, sm_scale=ctx.softmax_scale, rest=rest), None, None, None, None)
 
 
 def attention_ragged(q, k, v, cu_q, cu_k=None, softmax_scale=None, causal=False):

@@ -411,7 +411,8 @@ COSMOS_ATTN_API int cosmos_attn_gemm_preferred(const cosmos_attn_gemm_desc *desc
  * Offsets that do not ascend within the tensors: a sequence of such cu_q has no rows, one of such cu_k rows of NaN; neither reads or writes outside of the tensors.
  * What a row does not see has no influence on it as long as it is finite within the row's own sequence; what lies outside of the sequences may be anything.
  *
- * cosmos_attn_ragged_bwd: dq, dk, dv for the gradient dout of o, from the forward's o and lse; rows of no sequence become zeros.  No atomics: the same results every time.
+ * cosmos_attn_ragged_bwd: dq, dk, dv for the gradient dout of o, from the forward's o and lse (and, where softmaxes are sharp or rows see few keys, better with its `rest`); rows of no
+ * sequence become zeros.  No atomics: the same results every time.
  * The workspaces hold a number per row and head (backward) and the parts of tiles that are cut where there are few; the bytes follow from the sizes alone, and may be 0.  Outputs must not
  * overlap inputs or each other.
  */
@@ -430,6 +431,7 @@ typedef struct cosmos_attn_ragged_desc {
     void *dq, *dk, *dv;
     int64_t q_stride[2], k_stride[2], v_stride[2], o_stride[2];   /* (row, head) element strides, multiples of 8; a row at most 2^22 elements */
     int64_t dout_stride[2], dq_stride[2], dk_stride[2], dv_stride[2];
+    void *rest;                        /* [Tq, Hq, D] with nothing between, or NULL: the forward writes what rounding o left off, the backward adds it to o */
 } cosmos_attn_ragged_desc;
 
 COSMOS_ATTN_API size_t cosmos_attn_ragged_workspace_bytes(const cosmos_attn_ragged_desc *desc);

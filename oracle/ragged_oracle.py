@@ -36,8 +36,8 @@ def attend(q, k, v, mask, scale):
     return P @ v, lse, P, s, off
 
 
-def ragged_fwd(q, k, v, cu_q, cu_k, causal, scale, dtype):
-    """(o, lse, bound of o, bound of lse); rows of no sequence: zeros, -inf."""
+def ragged_fwd(q, k, v, cu_q, cu_k, causal, scale, dtype, rest=False):
+    """(o, lse, bound of o, bound of lse); rows of no sequence: zeros, -inf.  `rest`: o as the sum of its rounding and what that left off, rounded too."""
     q, k, v = (x.double().cpu() for x in (q, k, v))
     Tq, Hq, D = q.shape
     group = Hq // k.shape[1]
@@ -50,19 +50,19 @@ def ragged_fwd(q, k, v, cu_q, cu_k, causal, scale, dtype):
             K, V = k[c:d, h // group], v[c:d, h // group]
             o[a:b, h], lse[h, a:b], P, _, off = attend(q[a:b, h], K, V, mask, scale)
             size = P @ V.abs()
-            o_tol[a:b, h] = (u + off) * size + u * o[a:b, h].abs() + tiny * (V.abs().sum(0) + 2)
+            o_tol[a:b, h] = (u + off) * size + (u * u if rest else u) * o[a:b, h].abs() + tiny * (V.abs().sum(0) + 2)
             lse_tol[h, a:b] = off[:, 0] + 8 * F32 * lse[h, a:b].abs().nan_to_num(posinf=0)
     return o, lse, o_tol, lse_tol
 
 
-def ragged_bwd(q, k, v, dout, cu_q, cu_k, causal, scale, dtype):
-    """((dq, dk, dv), (their bounds)) of the forward's o, whose 16-bit rounding the row sums do . o have."""
+def ragged_bwd(q, k, v, dout, cu_q, cu_k, causal, scale, dtype, rest=False):
+    """((dq, dk, dv), (their bounds)) of the forward's o, whose 16-bit rounding the row sums do . o have (`rest`: that of its rounding and the rest)."""
     q, k, v, g = (x.double().cpu() for x in (q, k, v, dout))
     Hq, D = q.shape[1:]
     group = Hq // k.shape[1]
     grads, tols = [torch.zeros_like(x) for x in (q, k, v)], [torch.zeros_like(x) for x in (q, k, v)]
     u, tiny = _u(dtype)
-    o_tol = ragged_fwd(q, k, v, cu_q, cu_k, causal, scale, dtype)[2]
+    o_tol = ragged_fwd(q, k, v, cu_q, cu_k, causal, scale, dtype, rest)[2]
     for a, b, c, d in zip(cu_q[:-1], cu_q[1:], cu_k[:-1], cu_k[1:]):
         mask = visible(b - a, d - c, causal)
         for h in range(Hq):

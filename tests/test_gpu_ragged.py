@@ -219,18 +219,41 @@ def test_gradients_through_autograd(pkg, ragged_oracle, gpu):
         torch.autograd.grad(a.sum(), leaves[1])
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("ql, kl, causal, size", [([5, 3, 20, 1, 130], [5, 3, 20, 1, 130], True, 1.0), ([300, 7], [300, 70], True, 4.0), ([40, 3], [4000, 2], False, 2.0)])
+def test_what_rounding_left_off_o(pkg, ragged_oracle, gpu, ql, kl, causal, size, D, dtype):
+    """o and the rest together are o in twice the bits, and gradients from both have that much of it; the last case's tiles are cut."""
+    q, k, v, g = (rows(sum(n), h, D, dtype, gpu, i, s) for i, (n, h, s) in enumerate(((ql, 4, size), (kl, 2, 1.0), (kl, 2, 1.0), (ql, 4, 1.0))))
+    at = (cu(ql), cu(kl))
+    on, rest = [offsets(x, gpu) for x in at], torch.full_like(q, math.nan)
+    o, lse = pkg.ragged_fwd(q, k, v, *on, causal=causal, rest=rest)
+    same, _ = pkg.ragged_fwd(q, k, v, *on, causal=causal)
+    assert torch.equal(o, same)
+    O, _, tol, _ = ragged_oracle.ragged_fwd(q, k, v, *at, causal, D ** -0.5, dtype, rest=True)
+    near(o.double() + rest.double(), O, tol, "o and the rest")
+    got = pkg.ragged_bwd(q, k, v, o, lse, g, *on, causal=causal, rest=rest)
+    want, tols = ragged_oracle.ragged_bwd(q, k, v, g, *at, causal, D ** -0.5, dtype, rest=True)
+    for name, a, b, t in zip(("dq", "dk", "dv"), got, want, tols):
+        near(a, b, t, name)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    pkg.attention_ragged(*leaves, *on, causal=causal).backward(g)
+    assert all(torch.equal(x.grad, a) for x, a in zip(leaves, got))
+
+
 def test_gradients_of_shared_and_of_frozen_tensors(pkg, gpu):
     """One tensor as key and value gets both gradients; heads shared by expansion their sum; a frozen one none."""
     q, k = rows(90, 4, 64, BF16, gpu, 0), rows(90, 1, 64, BF16, gpu, 1).requires_grad_()
     on, g = offsets([0, 90], gpu), rows(90, 4, 64, BF16, gpu, 2)
     pkg.attention_ragged(q, k, k, on, causal=True).backward(g)
-    o, lse = pkg.ragged_fwd(q, k.detach(), k.detach(), on, causal=True)
-    _, dk, dv = pkg.ragged_bwd(q, k.detach(), k.detach(), o, lse, g, on, causal=True)
+    rest = torch.empty_like(q)
+    o, lse = pkg.ragged_fwd(q, k.detach(), k.detach(), on, causal=True, rest=rest)
+    _, dk, dv = pkg.ragged_bwd(q, k.detach(), k.detach(), o, lse, g, on, causal=True, rest=rest)
     assert torch.equal(k.grad, dk + dv) and q.grad is None
     k2 = k.detach().clone().requires_grad_()
     pkg.attention_ragged(q, k2.expand(-1, 2, -1), k.detach().expand(-1, 2, -1), on, causal=True).backward(g)
     # Two key heads of two query heads each: their gradients are rounded (half a step, 2^-8, of each: they may be far larger than their sum), their sum is, and the shared head's is.
-    two = pkg.ragged_bwd(q, k.detach().expand(-1, 2, -1), k.detach().expand(-1, 2, -1), o, lse, g, on, causal=True)[1].double()
+    two = pkg.ragged_bwd(q, k.detach().expand(-1, 2, -1), k.detach().expand(-1, 2, -1), o, lse, g, on, causal=True, rest=rest)[1].double()
     assert ((k2.grad.double() - dk.double()).abs() <= 2.0 ** -8 * (1 + 2.0 ** -7) * (two.abs().sum(1, keepdim=True) + k2.grad.double().abs() + dk.double().abs()) + 1e-5).all()
 
 

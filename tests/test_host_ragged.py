@@ -23,7 +23,7 @@ def ragged_desc(pkg, **over):
 
 def test_ragged_desc_layout_and_status_codes(pkg):
     L, lib = pkg._lib, pkg._lib.load_library()
-    assert ctypes.sizeof(L.RaggedDesc) == 8 * 4 + 2 * 8 + 8 + 11 * 8 + 16 * 8
+    assert ctypes.sizeof(L.RaggedDesc) == 8 * 4 + 2 * 8 + 8 + 11 * 8 + 16 * 8 + 8
     assert L.RaggedDesc.Tq.offset == 32 and L.RaggedDesc.q.offset == 56 and L.RaggedDesc.q_stride.offset == 144
     cases = [
         (dict(abi_version=1), L.ST_BAD_ARG), (dict(n_seq=-1), L.ST_BAD_ARG), (dict(Hkv=0), L.ST_BAD_ARG), (dict(q=None), L.ST_BAD_ARG), (dict(cu_k=None), L.ST_BAD_ARG),
@@ -32,7 +32,7 @@ def test_ragged_desc_layout_and_status_codes(pkg):
         (dict(n_seq=1 << 24), L.ST_UNSUPPORTED), (dict(Tk=1 << 30, Hkv=8), L.ST_UNSUPPORTED),
         (dict(Hkv=3), L.ST_BAD_SHAPE),
         (dict(k=P + 8), L.ST_BAD_STRIDE), (dict(cu_q=P + 2), L.ST_BAD_STRIDE), (dict(q_stride=(1020, 128)), L.ST_BAD_STRIDE), (dict(k_stride=(64, 128)), L.ST_BAD_STRIDE),
-        (dict(v_stride=(256, -128)), L.ST_BAD_STRIDE), (dict(k_stride=((1 << 22) + 8, 128)), L.ST_BAD_STRIDE), (dict(q_stride=(1024, 1 << 27)), L.ST_BAD_STRIDE),
+        (dict(v_stride=(256, -128)), L.ST_BAD_STRIDE), (dict(rest=P + 8), L.ST_BAD_STRIDE), (dict(k_stride=((1 << 22) + 8, 128)), L.ST_BAD_STRIDE), (dict(q_stride=(1024, 1 << 27)), L.ST_BAD_STRIDE),
         (dict(o_stride=(128, 64)), L.ST_BAD_STRIDE),
     ]
     for over, want in cases:
