@@ -276,6 +276,8 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const CacheParams 
 // A workgroup's share is an equal part of all sequences' keys, in tiles of kTile.  A sequence of more is cut into parts, of which each has a workgroup for each key head; one in one part
 // has its rows written at once, the others' parts leave sums, which cache_join_kernel adds up.  (Equal runs of one list of all sequences' tiles: a workgroup then waits for the first keys of each
 // of many short sequences in turn, 32 sequences of 1 to 2817 keys in int8 25 us instead of 19, though 48 of 1 to 7817 97 instead of 100.)
+// Memory: the live pages are read once, at the rate of a large copy where there are enough of them (131072 + 70001 + 99 keys of 8 heads in e4m3, 425 MB, 77 us, 5.5 TB/s; 48 sequences in bf16,
+// 504 MB, 95 us, 5.3 TB/s); 57 MB 16.6 us, 3.4 TB/s, of which the first loads, behind the lengths, the table and the pages, are some 5.
 constexpr int kTile = 128;           // keys: 32 of each wavefront
 constexpr float kLowest = -3.0e38f;
 
@@ -603,6 +605,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
 }
 
 // ---- the sequences that several workgroups have parts of: a workgroup for each sequence and query head, D / 4 lanes to a part, kThreads / (D / 4) parts at a time
+// (4 to 6 us, a launch and two trips to memory)
 template <typename T, int D, int NR>
 __global__ void __launch_bounds__(kThreads) cache_join_kernel(const CacheParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)

@@ -266,7 +266,9 @@ template <int D> __device__ __forceinline__ void clear_rows(char* out, int64_t r
 constexpr float kLowest = -3.0e38f;      // a max that no score has moved yet: exponentials of masked scores stay 0 and those of the sums so far too
 
 // ---- forward.  A workgroup: kRows rows of one sequence and key head; a wavefront 32 of them, one a lane and its other half: S^T = K Q^T has the keys in registers, so that the softmax
-// needs one exchange between the halves, and P^T, rounded, is the next product's operand where it lies.
+// needs one exchange between the halves, and P^T, rounded, is the next product's operand where it lies.  Two workgroups a compute unit (head dim 64: four), so that one's products and another's
+// exponentials go on beside each other.  16384 causal positions, 16 heads of 128 on 4: 980 us, 1.12 PFLOP/s; the matrix unit is busy 63 % of the time at 1.8 GHz,
+// the softmax's issue slots take the rest.  Short calls end with their longest tiles: 12 causal prompts of 1 to 2048 positions, 32 heads on 8, 123 us, 0.78 PFLOP/s, 84 % of the units busy.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -426,7 +428,8 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
 #endif
 }
 
-// ---- backward, first kernel: delta and dq.  The forward's rows and tiles, with P from lse, dP^T = V dO^T beside S^T, and dQ^T = K^T dS^T.
+// ---- backward, first kernel: delta and dq.  The forward's rows and tiles, with P from lse, dP^T = V dO^T beside S^T, and dQ^T = K^T dS^T.  Matrix unit busy 65 % at 1.7 GHz (8192 positions, 32
+// heads of 128 on 8): three products to an exponential, under the power limit.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -583,7 +586,8 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
 // ---- backward, second kernel: dk and dv.  A workgroup: 128 keys of one sequence and key head, a wavefront 32 of them, one a lane; the sequence's rows (of all heads of the group) go by in
 // steps of STEP.  S = Q K^T has the rows in registers: P and dS, rounded, are operands of dV^T += dO^T P and dK^T += Q^T dS where they lie.  K stays in registers, V too at head dim 64 and in
 // LDS at 128: with both in registers there are too many for two wavefronts on a SIMD, whose matrix products and other arithmetic go on beside each other (head dim 64, 1560 + 880 + 390 positions,
-// 16 heads, us, dq with it, V in LDS / in registers: 95 / 87).
+// 16 heads, us, dq with it, V in LDS / in registers: 95 / 87).  Matrix unit busy 51 % at 1.8 GHz (8192 positions, 32 heads of 128 on 8); what it waits for are reads from LDS, four to a product
+// of K's and V's side, for which no more registers are free to be ahead (two wavefronts a SIMD have 256 each, all taken).  With dq 1.12 PFLOP/s of seven products.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -769,7 +773,8 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
 #endif
 }
 
-// ---- the tiles that were cut: their parts added up, D / 4 lanes to a row.  WHICH: 0 o and lse, 1 dq, 2 dk and dv
+// ---- the tiles that were cut: their parts added up, D / 4 lanes to a row.  WHICH: 0 o and lse, 1 dq, 2 dk and dv.  Memory and a launch: 512 + 77
+// + 1 queries of 16 heads, the long ones in some four parts each, 10 us; dk and dv of four causal documents, 7678 keys of 8 heads, 29 us.
 constexpr int kJoinThreads = 1024;
 template <int D> constexpr int kJoinBlocks = kRows * (D / 4) / kJoinThreads;      // of a tile
 template <typename T, int D, int WHICH>
