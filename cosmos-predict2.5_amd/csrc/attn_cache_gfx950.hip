@@ -53,6 +53,7 @@ struct CacheParams {
     float scale_log2;
     unsigned flip;
     float* parts;
+    int* share;                                   // behind the parts: a share, and the most that a part has
 };
 
 // ---- 16-bit pairs
@@ -281,8 +282,8 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const CacheParams 
 constexpr int kTile = 128;           // keys: 32 of each wavefront
 constexpr float kLowest = -3.0e38f;
 
-__device__ __forceinline__ int tiles_of(const CacheParams& p, int i) {
-    const int n = p.lens[i];
+// tiles of a length
+__device__ __forceinline__ int tiles_of(const CacheParams& p, int n) {
     return n > 0 && n <= (int64_t)p.width << p.page_shift ? (n + kTile - 1) / kTile : 0;
 }
 // sums over the wavefront's lanes up to each one (data-parallel-primitive moves: within rows of 16, then the rows' ends)
@@ -303,31 +304,94 @@ struct Share {
     __device__ __forceinline__ int parts(int tiles) const { return tiles > per ? (tiles + most - 1) / most : 1; }
     __device__ __forceinline__ bool is_long(int tiles) const { return 2 * tiles > per; }
 };
-__device__ __forceinline__ Share share_of(const CacheParams& p) {
-    const int lane = threadIdx.x & 63;
-    int mine = 0;
-    for (int base = 0; base < p.B; base += 64) mine += base + lane < p.B ? tiles_of(p, base + lane) : 0;
-    int per = (sum_of(mine) + p.slots - 1) / p.slots;
+__device__ __forceinline__ Share share_of(const CacheParams& p, int tiles) {
+    int per = (tiles + p.slots - 1) / p.slots;
     per = per > 1 ? per : 1;
     return {per, per >= 8 && 4 * (int64_t)p.B > p.slots ? (3 * per + 3) / 4 : per};
 }
+// Every workgroup looks through all sequences: up to 64 each wavefront for itself, more of them kOwn in order to a thread, so that the lengths of kBatch are one wait (1000 sequences of 1 to 1500
+// keys, 32 heads of 128 on 8, int8, 277 us, each wavefront 64 at a time 400; but 32 sequences 20.2 instead of 19.4).
+constexpr int kOwn = 4, kBatch = kOwn * kThreads, kWaves = kThreads / 64;
+struct Batch {
+    int tiles[kOwn];
+    __device__ __forceinline__ Batch(const CacheParams& p, int base) {
+        int n[kOwn];
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) { const int i = base + kOwn * threadIdx.x + c; n[c] = p.lens[i < p.B ? i : 0]; }
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) tiles[c] = base + kOwn * (int)threadIdx.x + c < p.B ? tiles_of(p, n[c]) : 0;
+    }
+};
 // The part `slot`: first come the parts of sequences of more than half a share, in order, then the shorter ones, which end the call on what those leave (without keys: one part too).
 // seq < 0: behind the last.
 struct Part { int seq, part, parts, tiles; };
 __device__ __forceinline__ Part part_of(const CacheParams& p, int slot) {
-    const int lane = threadIdx.x & 63;
-    const Share share = share_of(p);
-    int before = 0;
-    for (int shorter = 0; shorter < 2; ++shorter)
-        for (int base = 0; base < p.B; base += 64) {
-            const int tiles = base + lane < p.B ? tiles_of(p, base + lane) : 0;
-            const int parts = base + lane < p.B && share.is_long(tiles) != (bool)shorter ? share.parts(tiles) : 0, sum = sums_up_to(parts);
+    if (p.B <= 64) {
+        const int lane = threadIdx.x & 63, n = p.lens[lane < p.B ? lane : 0], tiles = lane < p.B ? tiles_of(p, n) : 0;
+        const Share share = share_of(p, sum_of(tiles));
+        if (blockIdx.x == 0 && threadIdx.x == 0) { p.share[0] = share.per; p.share[1] = share.most; }
+        int before = 0;
+#pragma unroll
+        for (int shorter = 0; shorter < 2; ++shorter) {
+            const int parts = lane < p.B && share.is_long(tiles) != (bool)shorter ? share.parts(tiles) : 0, sum = sums_up_to(parts);
             const unsigned long long past = __ballot(before + sum > slot);
             if (past) {
                 const int at = __builtin_ctzll(past), of = __builtin_amdgcn_readlane(parts, at);
-                return {base + at, slot - (before + __builtin_amdgcn_readlane(sum, at) - of), of, __builtin_amdgcn_readlane(tiles, at)};
+                return {at, slot - (before + __builtin_amdgcn_readlane(sum, at) - of), of, __builtin_amdgcn_readlane(tiles, at)};
             }
             before += __builtin_amdgcn_readlane(sum, 63);
+        }
+        return {-1, 0, 0, 0};
+    }
+    __shared__ int totals[kWaves], sums[2][kWaves];
+    __shared__ Part found;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Batch first(p, 0);
+    int mine = 0;
+    for (int base = 0; base < p.B; base += kBatch) {
+        const Batch b = base ? Batch(p, base) : first;
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) mine += b.tiles[c];
+    }
+    mine = sum_of(mine);
+    if (lane == 0) totals[wave] = mine;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all += totals[w];
+    const Share share = share_of(p, all);
+    if (blockIdx.x == 0 && threadIdx.x == 0) { p.share[0] = share.per; p.share[1] = share.most; }
+    int before = 0, turn = 0;
+    for (int shorter = 0; shorter < 2; ++shorter)
+        for (int base = 0; base < p.B; base += kBatch, turn ^= 1) {
+            const Batch b = base ? Batch(p, base) : first;
+            int parts[kOwn], own = 0;
+#pragma unroll
+            for (int c = 0; c < kOwn; ++c) {
+                parts[c] = base + kOwn * (int)threadIdx.x + c < p.B && share.is_long(b.tiles[c]) != (bool)shorter ? share.parts(b.tiles[c]) : 0;
+                own += parts[c];
+            }
+            const int sum = sums_up_to(own);
+            if (lane == 63) sums[turn][wave] = sum;
+            __syncthreads();
+            int at = before + sum - own, past = before;       // parts before this thread's, up to the batch's end
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                at += w < wave ? sums[turn][w] : 0;
+                past += sums[turn][w];
+            }
+            if (slot < past) {
+                if (slot >= at && slot < at + own) {
+#pragma unroll
+                    for (int c = 0; c < kOwn; ++c) {
+                        if (slot >= at && slot < at + parts[c]) found = {base + kOwn * (int)threadIdx.x + c, slot - at, parts[c], b.tiles[c]};
+                        at += parts[c];
+                    }
+                }
+                __syncthreads();
+                return {__builtin_amdgcn_readfirstlane(found.seq), __builtin_amdgcn_readfirstlane(found.part), __builtin_amdgcn_readfirstlane(found.parts), __builtin_amdgcn_readfirstlane(found.tiles)};
+            }
+            before = past;
         }
     return {-1, 0, 0, 0};
 }
@@ -364,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
         }
     };
     Part mine = {slot, 0, 1, 0};
-    if (p.whole) mine.tiles = __builtin_amdgcn_readfirstlane(tiles_of(p, slot));
+    if (p.whole) mine.tiles = __builtin_amdgcn_readfirstlane(tiles_of(p, p.lens[slot]));
     else mine = part_of(p, slot);
     if (mine.seq < 0) return;
     const int seq = mine.seq;
@@ -613,15 +677,22 @@ __global__ void __launch_bounds__(kThreads) cache_join_kernel(const CacheParams 
     __shared__ __attribute__((aligned(16))) float smem[AT_ONCE][D + 4];
     const int heads = p.group * p.Hkv, seq = blockIdx.x / heads, hq = blockIdx.x - seq * heads, head = hq / p.group, row = hq - head * p.group, block = row / (16 * NR), r = row % (16 * NR);
     const int lane = threadIdx.x & 63;
-    const Share share = share_of(p);
-    const int parts = share.parts(__builtin_amdgcn_readfirstlane(tiles_of(p, seq)));
+    const Share share = {p.share[0], p.share[1]};
+    const int parts = share.parts(__builtin_amdgcn_readfirstlane(tiles_of(p, p.lens[seq])));
     if (parts == 1) return;
+    __shared__ int sums[kWaves];
     int before = 0;
-    for (int base = 0; base < seq; base += 64) {
-        const int n = base + lane < seq ? tiles_of(p, base + lane) : 0;
+    for (int i = threadIdx.x; i < seq; i += kThreads) {
+        const int n = tiles_of(p, p.lens[i]);
         before += share.is_long(n) ? share.parts(n) : 0;
     }
-    const int w0 = sum_of(before), w1 = w0 + parts - 1;
+    before = sum_of(before);
+    if (lane == 0) sums[threadIdx.x >> 6] = before;
+    __syncthreads();
+    int w0 = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) w0 += sums[w];
+    const int w1 = w0 + parts - 1;
     const int c = 4 * (threadIdx.x % LANES), slice = threadIdx.x / LANES;
     float top = kLowest, sum = 0.f;
     f32x4 f = {0.f, 0.f, 0.f, 0.f};
@@ -763,19 +834,22 @@ int check_attention(const cosmos_attn_cache_desc* d) {
     st = check_rows(d->q, d->q_stride);
     return st != COSMOS_ATTN_OK ? st : check_out(d->o, d->o_stride, d->B, d->Hq, d->D);
 }
-// Tables of few tiles: a workgroup for each sequence, and nothing to join, which a second launch would be for (333 keys of 4 heads: 6.3 us, as parts 5.8 and 3.8 for the join).
-constexpr int kWholeTiles = 4;
+// Tables of few tiles: a workgroup for each sequence and head, and nothing to join, which a second launch would be for (333 keys of 4 heads: 6.3 us, as parts 5.8 and 3.8 for the join).  Of
+// some more tiles too where there are many workgroups (us, whole / as parts: 32 sequences of 1000 keys, 64 heads of 64 on 8, 13.9 / 20.2; 300 of them in int8 78 / 90; 128 of 2000 keys, 32 heads of 128 on
+// 8, 101 / 106; but 40 of them 70 / 68), up to lengths at which the longest alone takes some 20 us.
+constexpr int kWholeTiles = 4, kWholeManyTiles = 16, kMany = 32;       // kMany: workgroups to a tile of the table's
 struct Shape { int row_blocks, rows16, slots; bool whole; };
 Shape shape_of(const cosmos_attn_cache_desc* d) {
     const int group = d->Hq / d->Hkv, rows16 = group <= 16 ? 1 : 2, row_blocks = (group + 16 * rows16 - 1) / (16 * rows16);
     const int64_t capacity = ((int64_t)d->width * d->page_size + kTile - 1) / kTile, most = (int64_t)d->B * capacity;
-    if (capacity <= kWholeTiles) return {row_blocks, rows16, 1, true};
+    if (capacity <= kWholeTiles || (capacity <= kWholeManyTiles && (int64_t)d->B * d->Hkv * row_blocks >= kMany * capacity)) return {row_blocks, rows16, 1, true};
     // two workgroups a compute unit, if the tables hold that many tiles
     int64_t slots = 2 * kNumCUs / ((int64_t)d->Hkv * row_blocks);
     slots = slots < 1 ? 1 : slots;
     return {row_blocks, rows16, (int)(slots > most ? most : slots), false};
 }
 
+constexpr size_t kShareBytes = 16;
 // parts of all sequences, for a head: each rounds up once (parts are three quarters of a share, rounded up, at least)
 int64_t most_parts(int64_t B, int64_t slots) { return 4 * slots / 3 + 1 + B; }
 
@@ -806,7 +880,7 @@ int cosmos_attn_cache_read(const cosmos_attn_cache_desc* desc, void* stream) {
 size_t cosmos_attn_cache_attention_workspace_bytes(const cosmos_attn_cache_desc* desc) {
     if (check_attention(desc) != COSMOS_ATTN_OK || !desc->B) return 0;
     const Shape s = shape_of(desc);
-    return s.whole ? 0 : (size_t)most_parts(desc->B, s.slots) * s.row_blocks * desc->Hkv * 16 * s.rows16 * (desc->D + 2) * sizeof(float);
+    return s.whole ? 0 : (size_t)most_parts(desc->B, s.slots) * s.row_blocks * desc->Hkv * 16 * s.rows16 * (desc->D + 2) * sizeof(float) + kShareBytes;
 }
 
 int cosmos_attn_cache_attention(const cosmos_attn_cache_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
@@ -824,6 +898,7 @@ int cosmos_attn_cache_attention(const cosmos_attn_cache_desc* desc, void* worksp
     p.scale_log2 = fmaxf(fabsf(desc->sm_scale) * 1.44269504088896341f, 1e-37f);
     p.flip = signbit(desc->sm_scale) ? 0x80008000u : 0u;
     p.parts = (float*)workspace;
+    p.share = wanted ? (int*)((char*)workspace + wanted - kShareBytes) : nullptr;
     return with_type(desc, [&](auto* t, auto dim, auto kind) {
         typedef std::remove_pointer_t<decltype(t)> T;
         constexpr int D = decltype(dim)::value, K = decltype(kind)::value;

@@ -588,6 +588,8 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
 // LDS at 128: with both in registers there are too many for two wavefronts on a SIMD, whose matrix products and other arithmetic go on beside each other (head dim 64, 1560 + 880 + 390 positions,
 // 16 heads, us, dq with it, V in LDS / in registers: 95 / 87).  Matrix unit busy 51 % at 1.8 GHz (8192 positions, 32 heads of 128 on 8); what it waits for are reads from LDS, four to a product
 // of K's and V's side, for which no more registers are free to be ahead (two wavefronts a SIMD have 256 each, all taken).  With dq 1.12 PFLOP/s of seven products.
+// (64 keys and half of a step's rows to a wavefront, one on a SIMD with all 512 registers, so that every fragment of Q and dO feeds two products: as fast on 8192 positions, 10 to 20 % slower on 512 to
+// 4096 and on prompts of mixed lengths, where a tile's start and end then have no other workgroup beside them.)
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)

@@ -216,6 +216,15 @@ def test_long_and_short_ones_together(pkg, ragged_oracle, gpu):
     check_decode(pkg, ragged_oracle, gpu, lens, 16, 4, 2, 64, BF16, INT8)
 
 
+@pytest.mark.parametrize("B, longest, of", [(100, 1500, 99), (65, 700, 0), (300, 900, 150), (1100, 2176, 1050), (1024, 2200, 1023)])
+def test_many_sequences(pkg, ragged_oracle, gpu, B, longest, of):
+    """More sequences than one look at their lengths takes, cut and whole, the longest anywhere, empty ones between."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 40, (B,), generator=g).tolist()
+    lens[of], lens[B // 3], lens[2 * B // 3] = longest, longest // 2, 300
+    check_decode(pkg, ragged_oracle, gpu, lens, 16, 2, 1, 64, BF16, INT8)
+
+
 def test_small_values_in_fp16(pkg, ragged_oracle, gpu):
     """Scales far below the range of fp16: weights are held relative to the largest."""
     lens = [400]
