@@ -200,33 +200,72 @@ struct Found { int seq, tile, parts; Lengths n; };     // seq < 0: behind the la
 // Tile `index` of all sequences', in the sequences' order and the longest of each first, and how many parts it is cut into.
 // (The longest of all first, by counts of the tiles longer than some length, for which the length is searched: 5 % slower on 12 prompts and on four documents.  Short tiles, which are mostly
 // waiting, then run beside each other at the end instead of beside long ones.)
-template <typename Kind> __device__ __forceinline__ Found find(const RaggedParams& p, int index) {
+// Few sequences each wavefront looks through for itself, 64 at a time; more of them the workgroup's THREADS together (1000 prompts of 30 positions, 32 heads of 128 on 8, us, forward / gradients,
+// together 238 / 565, each wavefront for itself 315 / 650; but 100 of them 24 / 101, and 24 / 93).
+constexpr int kFew = 128;
+template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Found find(const RaggedParams& p, int index) {
     constexpr bool KEYS = Kind::OF_KEYS;
     const Kind T{p};
     const int lane = threadIdx.x & 63;
     Found f = {-1, 0, 1, {0, 0}};
-    // (a sequence's: all of its tiles times the mean of the longest and the shortest; no more than 64 of them add up to in 32 bits)
-    auto share_of = [&](Lengths n, int tiles) {
+    // (a sequence's: all of its tiles times the mean of the longest and the shortest; as many of them as are added up in 32 bits are no more than those hold)
+    auto share_of = [&](Lengths n, int tiles, int most) {
         const int64_t sum = tiles ? (int64_t)tiles * (T.steps(n, T.at(0, tiles)) + T.steps(n, T.at(tiles - 1, tiles))) / 2 : 0;
-        return (int)(sum < (1 << 25) ? sum : (1 << 25) - 1);
+        return (int)(sum < most ? sum : most);
     };
     int before = 0;
     int64_t all = 0;                 // steps
-    for (int base = 0; base < p.n_seq; base += 64) {
-        Lengths n = {-1, -1};
-        int tiles = 0;
-        if (base + lane < p.n_seq) { n = T.lengths(base + lane); tiles = T.count(n); }
-        const int sum = sums_up_to(tiles);
-        const unsigned long long past = __ballot(before + sum > index);
-        if (past && f.seq < 0) {
-            const int at = __builtin_ctzll(past), of = __builtin_amdgcn_readlane(tiles, at);
-            f.seq = base + at;
-            f.n = {__builtin_amdgcn_readlane(n.lq, at), __builtin_amdgcn_readlane(n.lk, at)};
-            f.tile = T.at(index - (before + __builtin_amdgcn_readlane(sum, at) - of), of);
-            if (p.most_parts <= 1) return f;
+    if (p.n_seq <= kFew) {
+        for (int base = 0; base < p.n_seq; base += 64) {
+            const Lengths n = base + lane < p.n_seq ? T.lengths(base + lane) : Lengths{-1, -1};
+            const int tiles = T.count(n), sum = sums_up_to(tiles);
+            const unsigned long long past = __ballot(before + sum > index);
+            if (past && f.seq < 0) {
+                const int at = __builtin_ctzll(past), of = __builtin_amdgcn_readlane(tiles, at);
+                f.seq = base + at;
+                f.n = {__builtin_amdgcn_readlane(n.lq, at), __builtin_amdgcn_readlane(n.lk, at)};
+                f.tile = T.at(index - (before + __builtin_amdgcn_readlane(sum, at) - of), of);
+                if (p.most_parts <= 1) return f;
+            }
+            before += __builtin_amdgcn_readlane(sum, 63);
+            if (p.most_parts > 1) all += sum_of(share_of(n, tiles, (1 << 25) - 1));
         }
-        before += __builtin_amdgcn_readlane(sum, 63);
-        if (p.most_parts > 1) all += sum_of(share_of(n, tiles));
+    } else {
+        constexpr int WAVES = THREADS / 64;
+        __shared__ int sums[2][WAVES];
+        __shared__ int64_t shares[WAVES];
+        __shared__ Found found;
+        const int wave = threadIdx.x >> 6;
+        for (int base = 0, turn = 0; base < p.n_seq; base += THREADS, turn ^= 1) {
+            const int mine = base + threadIdx.x;
+            const Lengths n = mine < p.n_seq ? T.lengths(mine) : Lengths{-1, -1};
+            // (sequences that overlap may have any number of tiles: what is far behind the last index is as good as any other number there)
+            const int tiles = T.count(n), sum = sums_up_to(tiles);
+            if (lane == 63) sums[turn][wave] = sum < 1 << 26 ? sum : 1 << 26;
+            if (p.most_parts > 1) all += sum_of(share_of(n, tiles, (1 << 25) - 1));
+            __syncthreads();
+            int at = before + sum - tiles, past = before;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                at += w < wave ? sums[turn][w] : 0;
+                past += sums[turn][w];
+            }
+            if (f.seq < 0 && index < past) {
+                if (index >= at && index < at + tiles) found = {mine, T.at(index - at, tiles), 1, n};
+                f.seq = 0;           // (it is in `found`)
+                if (p.most_parts <= 1) break;
+            }
+            before = past < 1 << 26 ? past : 1 << 26;
+        }
+        if (lane == 0) shares[wave] = all;
+        __syncthreads();
+        if (f.seq >= 0) {
+            f = {__builtin_amdgcn_readfirstlane(found.seq), __builtin_amdgcn_readfirstlane(found.tile), 1, {__builtin_amdgcn_readfirstlane(found.n.lq), __builtin_amdgcn_readfirstlane(found.n.lk)}};
+            if (p.most_parts <= 1) return f;
+            all = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) all += shares[w];
+        }
     }
     if (f.seq < 0) { f.tile = index - before; return f; }
     const int64_t share = (all * p.Hkv + kAtOnce - 1) / kAtOnce;
@@ -785,7 +824,7 @@ __global__ void __launch_bounds__(kJoinThreads) ragged_join_kernel(const RaggedP
     constexpr bool KEYS = WHICH == 2;
     constexpr int LANES = D / 4, AT_ONCE = kJoinThreads / LANES;
     const int head = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv % p.tiles;
-    const Found f = find<std::conditional_t<KEYS, KeyTiles<D>, RowTiles>>(p, index);
+    const Found f = find<std::conditional_t<KEYS, KeyTiles<D>, RowTiles>, kJoinThreads>(p, index);
     if (f.seq < 0 || f.parts <= 1) return;
     const int c = 4 * (threadIdx.x % LANES);
     const Range r = range_of(KEYS ? p.cu_k : p.cu_q, f.seq, KEYS ? p.Tk : p.Tq);

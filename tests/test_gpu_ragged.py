@@ -74,6 +74,16 @@ def test_many_sequences(pkg, ragged_oracle, gpu):
     both(pkg, ragged_oracle, gpu, lens, lens, 2, 1, 64, FP16, True)
 
 
+@pytest.mark.parametrize("n, D, longest", [(65, 128, (40, 3500)), (100, 64, (900, 5000)), (300, 128, (1500, 1500)), (1100, 64, (300, 300)), (1030, 128, (1, 2500))])
+def test_many_sequences_and_a_long_one(pkg, ragged_oracle, gpu, n, D, longest):
+    """More sequences than a wavefront, or the workgroup's first look, takes; the long one's tiles are cut where they are few."""
+    g = torch.Generator().manual_seed(n)
+    ql = torch.randint(0, 12, (n,), generator=g).tolist()
+    kl = [x + i % 3 for i, x in enumerate(ql)]
+    ql[n - 2], kl[n - 2] = longest
+    both(pkg, ragged_oracle, gpu, ql, kl, 2, 1, D, BF16, n % 2 == 0)
+
+
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("ql, kl", [([1], [9000]), ([3, 1, 0, 40], [700, 5000, 300, 1100]), ([1500], [1500]), ([900, 1300, 17], [900, 1300, 17]), ([600] + [1] * 70, [2000] + [3] * 70), ([1200, 64], [500, 1100])])
 def test_few_tiles_that_are_cut(pkg, ragged_oracle, gpu, ql, kl, causal):
@@ -184,6 +194,18 @@ def test_offsets_that_do_not_ascend_within_the_tensors(pkg, gpu):
     assert o.isnan().all()
     grads = pkg.ragged_bwd(q, k, k, good, lse, q, offsets([0, 30, 100], gpu), offsets([-5, 30, 20], gpu))
     assert (grads[0] == 0).all()
+
+
+@pytest.mark.parametrize("n", [40, 200, 1200])
+def test_offsets_that_go_back(pkg, gpu, n):
+    """0, 300, 0, 300, ...: every second sequence is the same one, the others are none; there are more tiles than the rows allow for."""
+    q, k, g = rows(300, 4, 64, BF16, gpu, 0), rows(300, 2, 64, BF16, gpu, 1), rows(300, 4, 64, BF16, gpu, 2)
+    on, once = offsets([300 * (i % 2) for i in range(n)], gpu), offsets([0, 300], gpu)
+    o, lse = pkg.ragged_fwd(q, k, k, on)
+    O, L = pkg.ragged_fwd(q, k, k, once)
+    assert (o.float() - O.float()).abs().max() <= 2.0 ** -7 * O.float().abs().max() and (lse - L).abs().max() <= 1e-4      # (tiles cut in other parts: sums in another order)
+    for x in pkg.ragged_bwd(q, k, k, O, L, g, on):
+        assert x.isfinite().all()
 
 
 def test_values_that_are_not_finite_stay_in_their_rows(pkg, gpu):
