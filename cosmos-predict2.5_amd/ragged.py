@@ -8,6 +8,7 @@ The reference has no counterpart: its attention takes one length for the batch (
 """
 from __future__ import annotations
 
+import functools
 import struct
 from typing import Optional, Tuple
 
@@ -77,12 +78,21 @@ def plain_int32(x: torch.Tensor, dims: int, device: int) -> bool:
 
 def on_device(device: int, launch, desc: bytes, *rest) -> None:
     """``launch(desc, *rest, stream)`` with the device current, on its current stream."""
-    if torch.cuda.current_device() == device:
+    if torch._C._cuda_getDevice() == device:      # (there is a tensor on a GPU: nothing is left to be initialised)
         status = launch(desc, *rest, torch._C._cuda_getCurrentRawStream(device))
     else:
         status = _on_device(torch.device("cuda", device), lambda stream: launch(desc, *rest, stream))
     if status:
         _lib.raise_for_status(status)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(backward: bool, n_seq: int, Hq: int, Hkv: int, D: int, Tq: int, Tk: int) -> int:
+    """What the library asks for, which follows from sizes alone (addresses are never dereferenced)."""
+    desc = _RAGGED_DESC.pack(_lib.ABI_VERSION, _lib.DTYPE_BF16, n_seq, Hq, Hkv, D, 0, 0, Tq, Tk, 1.0, 0, *(16,) * 11, *(Hq * D, D, Hkv * D, D, Hkv * D, D, Hq * D, D), Hq * D, D, Hq * D, D,
+                             Hkv * D, D, Hkv * D, D, 0)
+    lib = _lib.load_library()
+    return (lib.cosmos_attn_ragged_bwd_workspace_bytes if backward else lib.cosmos_attn_ragged_workspace_bytes)(desc)
 
 
 def _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse, rest):
@@ -105,10 +115,9 @@ def _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse, rest):
     lse = q.new_empty((Hq, Tq), dtype=torch.float32) if need_lse else None
     desc = _RAGGED_DESC.pack(_lib.ABI_VERSION, code, cu_q.shape[0] - 1, Hq, Hkv, D, 1 if causal else 0, 1, Tq, Tk, D ** -0.5 if sm_scale is None else sm_scale, 0, pq, pk, pv, cu_q.data_ptr(),
                              cu_k.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, q0, q1, k0, k1, v0, v1, Hq * D, D, 0, 0, 0, 0, 0, 0, 0, 0, 0 if rest is None else rest.data_ptr())
-    lib = _lib.load_library()
-    ws_bytes = lib.cosmos_attn_ragged_workspace_bytes(desc)
+    ws_bytes = _workspace_bytes(False, cu_q.shape[0] - 1, Hq, Hkv, D, Tq, Tk)
     workspace = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
-    on_device(device, lib.cosmos_attn_ragged, desc, 0 if workspace is None else workspace.data_ptr(), ws_bytes)
+    on_device(device, _lib.load_library().cosmos_attn_ragged, desc, 0 if workspace is None else workspace.data_ptr(), ws_bytes)
     return o, lse
 
 
@@ -132,15 +141,10 @@ def _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale, rest):
     dq, dk, dv = (torch.empty(x, device=q.device, dtype=dtype) for x in (shape, kv, kv))
     desc = _RAGGED_DESC.pack(_lib.ABI_VERSION, code, cu_q.shape[0] - 1, Hq, Hkv, D, 1 if causal else 0, 1, Tq, Tk, D ** -0.5 if sm_scale is None else sm_scale, 0, pq, pk, pv, cu_q.data_ptr(),
                              cu_k.data_ptr(), po, lse.data_ptr(), pg, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), q0, q1, k0, k1, v0, v1, Hq * D, D, g0, g1, Hq * D, D, Hkv * D, D, Hkv * D, D, 0 if rest is None else rest.data_ptr())
-    _launch_bwd(device, desc, q)
+    ws_bytes = _workspace_bytes(True, cu_q.shape[0] - 1, Hq, Hkv, D, Tq, Tk)
+    workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
+    on_device(device, _lib.load_library().cosmos_attn_ragged_bwd, desc, workspace.data_ptr(), ws_bytes)
     return dq, dk, dv
-
-
-def _launch_bwd(device, desc, like):
-    lib = _lib.load_library()
-    ws_bytes = lib.cosmos_attn_ragged_bwd_workspace_bytes(desc)
-    workspace = like.new_empty(ws_bytes, dtype=torch.uint8)
-    on_device(device, lib.cosmos_attn_ragged_bwd, desc, workspace.data_ptr(), ws_bytes)
 
 
 def _check_rest(rest, q):
@@ -231,7 +235,10 @@ def ragged_bwd(
     q, k, v, o, dout, lse = packed(q), packed(k), packed(v), packed(o), packed(dout), lse.contiguous()
     dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
     desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, True, rest, dout, dq, dk, dv)
-    _launch_bwd(q.get_device(), desc, q)
+    lib = _lib.load_library()
+    ws_bytes = lib.cosmos_attn_ragged_bwd_workspace_bytes(desc)
+    workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
+    on_device(q.get_device(), lib.cosmos_attn_ragged_bwd, desc, workspace.data_ptr(), ws_bytes)
     return dq, dk, dv
 
 
