@@ -241,6 +241,18 @@ def test_gradients_through_autograd(pkg, ragged_oracle, gpu):
         torch.autograd.grad(a.sum(), leaves[1])
 
 
+def test_gradients_of_a_sum_and_of_views(pkg, gpu):
+    """A gradient without memory of its own (expanded from one element), and one that lies heads first."""
+    on, x = offsets([0, 37, 90], gpu), [rows(90, h, 128, BF16, gpu, i) for i, h in enumerate((4, 2, 2))]
+    grads = []
+    for make in (lambda o: o.sum(), lambda o: (o * torch.ones_like(o)).sum(), lambda o: (o.transpose(0, 1) * torch.ones_like(o.transpose(0, 1).contiguous())).sum()):
+        leaves = [t.clone().requires_grad_() for t in x]
+        make(pkg.attention_ragged(*leaves, on, causal=True)).backward()
+        grads.append([t.grad for t in leaves])
+    assert all(torch.equal(a, b) for other in grads[1:] for a, b in zip(grads[0], other))
+    assert all(t.abs().max() > 0 for t in grads[0][2:])
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("ql, kl, causal, size", [([5, 3, 20, 1, 130], [5, 3, 20, 1, 130], True, 1.0), ([300, 7], [300, 70], True, 4.0), ([40, 3], [4000, 2], False, 2.0)])
