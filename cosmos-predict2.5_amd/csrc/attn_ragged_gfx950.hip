@@ -13,7 +13,8 @@
 // list, no copy to the host, nothing to prepare, and a captured call follows its offsets.  Where a call has few tiles, those with more than an equal share of all steps are cut along
 // their keys (rows), and a second kernel adds the parts up, in their order.
 //
-// Offsets are not trusted: a sequence whose offsets do not ascend within the tensors has no rows; one whose keys' offsets do not has rows of NaN (no gradients: zeros).
+// Offsets are not trusted: a sequence whose offsets do not ascend within the tensors, or that begins before the end of an earlier one, has no rows; one whose keys' offsets are such has rows of
+// NaN (no gradients: zeros).  No two sequences then have a row or a key in common, whatever the offsets hold: each row is one workgroup's to write, and there are never more tiles than workgroups.
 #include <hip/hip_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -142,6 +143,21 @@ __device__ __forceinline__ Range range_of(const int* cu, int i, int total) {
     const int a = cu[i], b = cu[i + 1];
     return a >= 0 && a <= b && b <= total ? Range{a, b - a} : Range{0, -1};
 }
+// the rows of sequence i, of which find() says how many there are
+__device__ __forceinline__ Range rows_of_sequence(const int* cu, int i, int length) { return {length < 0 ? 0 : cu[i], length}; }
+// Where some sequence of all up to here has offsets that do not ascend, others behind it may begin before `end`, the last end so far: of the 64 from `base` on, a lane's length, -1 where it has
+// none of its own.  (One after the other, as each depends on those before; empty ones hold nothing and are passed over, so that zeros behind the last offset cost little.)
+__device__ __forceinline__ int apart(const int* cu, int base, int n_seq, int total, int& end) {
+    const int lane = threadIdx.x & 63;
+    const Range r = base + lane < n_seq ? range_of(cu, base + lane, total) : Range{0, -1};
+    unsigned long long none = 0;
+    for (unsigned long long left = __ballot(r.length > 0); left; left &= left - 1) {
+        const int at = __builtin_ctzll(left), a = __builtin_amdgcn_readlane(r.start, at);
+        if (a < end) none |= 1ull << at;
+        else end = a + __builtin_amdgcn_readlane(r.length, at);
+    }
+    return none >> lane & 1 ? -1 : r.length;
+}
 // sums over the wavefront's lanes up to each one (data-parallel-primitive moves: within rows of 16, then the rows' ends)
 template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
 __device__ __forceinline__ int sums_up_to(int v) {
@@ -196,7 +212,7 @@ typedef Tiles<false, kRows, kStep> RowTiles;
 // of dk and dv
 constexpr int row_step(int D) { return D == 128 ? 32 : 64; }
 template <int D> using KeyTiles = Tiles<true, kRows, row_step(D)>;
-struct Found { int seq, tile, parts; Lengths n; };     // seq < 0: behind the last tile, `tile` of them
+struct Found { int seq, tile, parts; Lengths n; bool odd; };     // seq < 0: behind the last tile, `tile` of them; odd: offsets that do not ascend were among those looked at
 // Tile `index` of all sequences', in the sequences' order and the longest of each first, and how many parts it is cut into.
 // (The longest of all first, by counts of the tiles longer than some length, for which the length is searched: 5 % slower on 12 prompts and on four documents.  Short tiles, which are mostly
 // waiting, then run beside each other at the end instead of beside long ones.)
@@ -207,7 +223,7 @@ template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Foun
     constexpr bool KEYS = Kind::OF_KEYS;
     const Kind T{p};
     const int lane = threadIdx.x & 63;
-    Found f = {-1, 0, 1, {0, 0}};
+    Found f = {-1, 0, 1, {0, 0}, false};
     // (a sequence's: all of its tiles times the mean of the longest and the shortest; as many of them as are added up in 32 bits are no more than those hold)
     auto share_of = [&](Lengths n, int tiles, int most) {
         const int64_t sum = tiles ? (int64_t)tiles * (T.steps(n, T.at(0, tiles)) + T.steps(n, T.at(tiles - 1, tiles))) / 2 : 0;
@@ -215,33 +231,41 @@ template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Foun
     };
     int before = 0;
     int64_t all = 0;                 // steps
+    auto lengths = [&](int i) { return i < p.n_seq ? T.lengths(i) : Lengths{-1, -1}; };
+    auto is_odd = [&](int i, Lengths n) { return i < p.n_seq && (n.lq < 0 || n.lk < 0); };
+    // 64 sequences from `base` on; is that all there is to know?
+    auto look = [&](int base, Lengths n) __attribute__((always_inline)) {
+        const int tiles = T.count(n), sum = sums_up_to(tiles);
+        const unsigned long long past = __ballot(before + sum > index);
+        if (past && f.seq < 0) {
+            const int at = __builtin_ctzll(past), of = __builtin_amdgcn_readlane(tiles, at);
+            f.seq = base + at;
+            f.n = {__builtin_amdgcn_readlane(n.lq, at), __builtin_amdgcn_readlane(n.lk, at)};
+            f.tile = T.at(index - (before + __builtin_amdgcn_readlane(sum, at) - of), of);
+            if (p.most_parts <= 1) return true;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+        if (p.most_parts > 1) all += sum_of(share_of(n, tiles, (1 << 25) - 1));
+        return false;
+    };
     if (p.n_seq <= kFew) {
         for (int base = 0; base < p.n_seq; base += 64) {
-            const Lengths n = base + lane < p.n_seq ? T.lengths(base + lane) : Lengths{-1, -1};
-            const int tiles = T.count(n), sum = sums_up_to(tiles);
-            const unsigned long long past = __ballot(before + sum > index);
-            if (past && f.seq < 0) {
-                const int at = __builtin_ctzll(past), of = __builtin_amdgcn_readlane(tiles, at);
-                f.seq = base + at;
-                f.n = {__builtin_amdgcn_readlane(n.lq, at), __builtin_amdgcn_readlane(n.lk, at)};
-                f.tile = T.at(index - (before + __builtin_amdgcn_readlane(sum, at) - of), of);
-                if (p.most_parts <= 1) return f;
-            }
-            before += __builtin_amdgcn_readlane(sum, 63);
-            if (p.most_parts > 1) all += sum_of(share_of(n, tiles, (1 << 25) - 1));
+            const Lengths n = lengths(base + lane);
+            if (__any(is_odd(base + lane, n))) { f.odd = true; break; }
+            if (look(base, n)) return f;
         }
     } else {
-        constexpr int WAVES = THREADS / 64;
+        constexpr int WAVES = THREADS / 64, ODD = 1 << 26;      // (more than there are tiles)
         __shared__ int sums[2][WAVES];
         __shared__ int64_t shares[WAVES];
         __shared__ Found found;
         const int wave = threadIdx.x >> 6;
         for (int base = 0, turn = 0; base < p.n_seq; base += THREADS, turn ^= 1) {
             const int mine = base + threadIdx.x;
-            const Lengths n = mine < p.n_seq ? T.lengths(mine) : Lengths{-1, -1};
-            // (sequences that overlap may have any number of tiles: what is far behind the last index is as good as any other number there)
+            const Lengths n = lengths(mine);
             const int tiles = T.count(n), sum = sums_up_to(tiles);
-            if (lane == 63) sums[turn][wave] = sum < 1 << 26 ? sum : 1 << 26;
+            const bool odd = __any(is_odd(mine, n));
+            if (lane == 63) sums[turn][wave] = odd ? ODD : sum;
             if (p.most_parts > 1) all += sum_of(share_of(n, tiles, (1 << 25) - 1));
             __syncthreads();
             int at = before + sum - tiles, past = before;
@@ -250,22 +274,33 @@ template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Foun
                 at += w < wave ? sums[turn][w] : 0;
                 past += sums[turn][w];
             }
+            if (__builtin_amdgcn_readfirstlane(past) >= ODD) { f.odd = true; break; }
             if (f.seq < 0 && index < past) {
-                if (index >= at && index < at + tiles) found = {mine, T.at(index - at, tiles), 1, n};
+                if (index >= at && index < at + tiles) found = {mine, T.at(index - at, tiles), 1, n, false};
                 f.seq = 0;           // (it is in `found`)
                 if (p.most_parts <= 1) break;
             }
-            before = past < 1 << 26 ? past : 1 << 26;
+            before = past;
         }
-        if (lane == 0) shares[wave] = all;
-        __syncthreads();
-        if (f.seq >= 0) {
-            f = {__builtin_amdgcn_readfirstlane(found.seq), __builtin_amdgcn_readfirstlane(found.tile), 1, {__builtin_amdgcn_readfirstlane(found.n.lq), __builtin_amdgcn_readfirstlane(found.n.lk)}};
-            if (p.most_parts <= 1) return f;
-            all = 0;
+        if (!f.odd) {
+            if (lane == 0) shares[wave] = all;
+            __syncthreads();
+            if (f.seq >= 0) {
+                f = {__builtin_amdgcn_readfirstlane(found.seq), __builtin_amdgcn_readfirstlane(found.tile), 1, {__builtin_amdgcn_readfirstlane(found.n.lq), __builtin_amdgcn_readfirstlane(found.n.lk)}, false};
+                if (p.most_parts <= 1) return f;
+                all = 0;
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) all += shares[w];
+                for (int w = 0; w < WAVES; ++w) all += shares[w];
+            }
         }
+    }
+    if (f.odd) {                     // once more from the start, each wavefront for itself
+        int end_q = 0, end_k = 0;
+        f.seq = -1;
+        before = 0;
+        all = 0;
+        for (int base = 0; base < p.n_seq; base += 64)
+            if (look(base, {apart(p.cu_q, base, p.n_seq, p.Tq, end_q), apart(p.cu_k, base, p.n_seq, p.Tk, end_k)})) return f;
     }
     if (f.seq < 0) { f.tile = index - before; return f; }
     const int64_t share = (all * p.Hkv + kAtOnce - 1) / kAtOnce;
@@ -285,8 +320,17 @@ __device__ __forceinline__ Block block_of(const RaggedParams& p, int b) {
 }
 
 // ---- rows of no sequence: zeros, lse = -inf
-template <int D> __device__ __forceinline__ void clear_rows(char* out, int64_t row, int64_t head, const int* cu, int n, int total, int heads, int first_head, int rows, int tile, float* lse) {
+template <int D> __device__ __forceinline__ void clear_rows(char* out, int64_t row, int64_t head, const int* cu, int n, int total, int heads, int first_head, int rows, Found f, float* lse) {
+    const int tile = f.tile;
     int lead = cu[0], from = cu[n];
+    if (f.odd) {                     // (the last offset need not be the last sequence's end)
+        lead = -1;
+        from = 0;
+        for (int base = 0; base < n; base += 64) {
+            const unsigned long long some = __ballot(apart(cu, base, n, total, from) > 0);
+            if (lead < 0 && some) lead = cu[base + __builtin_ctzll(some)];
+        }
+    }
     lead = lead < 0 ? 0 : lead > total ? total : lead;
     from = from < lead ? lead : from > total ? total : from;
     const int64_t count = (int64_t)(lead + total - from) * heads;
@@ -320,12 +364,12 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
     const int head = block.head;
     const Found f = find<RowTiles>(p, block.index);
     if (f.seq < 0) {
-        if (p.fill && block.part == 0) clear_rows<D>(p.o, p.o_row, p.o_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f.tile, p.lse);
+        if (p.fill && block.part == 0) clear_rows<D>(p.o, p.o_row, p.o_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f, p.lse);
         return;
     }
     if (block.part >= f.parts) return;
     const int tile = f.tile;
-    const Range rq = range_of(p.cu_q, f.seq, p.Tq), rk = range_of(p.cu_k, f.seq, p.Tk);
+    const Range rq = rows_of_sequence(p.cu_q, f.seq, f.n.lq), rk = rows_of_sequence(p.cu_k, f.seq, f.n.lk);
     const int rows = rq.length * p.group, lk = rk.length > 0 ? rk.length : 0, shift = lk - rq.length;
     const int row = tile * kRows + 32 * wave + (lane & 31);
     const bool live = row < rows;
@@ -481,12 +525,12 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
     const int head = block.head;
     const Found f = find<RowTiles>(p, block.index);
     if (f.seq < 0) {
-        if (block.part == 0) clear_rows<D>(p.dq, p.dq_row, p.dq_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f.tile, nullptr);
+        if (block.part == 0) clear_rows<D>(p.dq, p.dq_row, p.dq_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f, nullptr);
         return;
     }
     if (block.part >= f.parts) return;
     const int tile = f.tile;
-    const Range rq = range_of(p.cu_q, f.seq, p.Tq), rk = range_of(p.cu_k, f.seq, p.Tk);
+    const Range rq = rows_of_sequence(p.cu_q, f.seq, f.n.lq), rk = rows_of_sequence(p.cu_k, f.seq, f.n.lk);
     const int rows = rq.length * p.group, lk = rk.length > 0 ? rk.length : 0, shift = lk - rq.length;
     const int row = tile * kRows + 32 * wave + (lane & 31);
     const bool live = row < rows;
@@ -646,12 +690,12 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     const Found f = find<KeyTiles<D>>(p, block.index);
     if (f.seq < 0) {
         if (block.part) return;
-        clear_rows<D>(p.dk, p.dk_row, p.dk_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f.tile, nullptr);
-        clear_rows<D>(p.dv, p.dv_row, p.dv_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f.tile, nullptr);
+        clear_rows<D>(p.dk, p.dk_row, p.dk_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f, nullptr);
+        clear_rows<D>(p.dv, p.dv_row, p.dv_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f, nullptr);
         return;
     }
     if (block.part >= f.parts) return;
-    const Range rq = range_of(p.cu_q, f.seq, p.Tq), rk = range_of(p.cu_k, f.seq, p.Tk);
+    const Range rq = rows_of_sequence(p.cu_q, f.seq, f.n.lq), rk = rows_of_sequence(p.cu_k, f.seq, f.n.lk);
     const int lq = rq.length > 0 ? rq.length : 0;
     const int key0 = f.tile * kRows, key = key0 + 32 * wave + (lane & 31);
     const bool live = key < rk.length;
@@ -677,39 +721,36 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
             if constexpr (!V_IN_LDS) vf[c] = __builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(va + 32 * c));
         }
     }
-    // this lane's row of each load: the token and the head; both go on by STEP rows a step
-    const int step_tokens = STEP / p.group, step_heads = STEP - step_tokens * p.group;
-    int token[L::LOADS], hd[L::LOADS], byte[L::LOADS];
+    // this lane's row of the first load: the token and the head; they go on by ROWS_PER_LOAD rows a load (no registers are left for each load's own) and by STEP rows a step
+    const int step_tokens = STEP / p.group, step_heads = STEP - step_tokens * p.group, load_tokens = L::ROWS_PER_LOAD / p.group, load_heads = L::ROWS_PER_LOAD - load_tokens * p.group;
+    int token = (t0 * STEP + L::load_row(lane, wave, 0)) / p.group, hd = t0 * STEP + L::load_row(lane, wave, 0) - token * p.group, byte[L::LOADS];
 #pragma unroll
-    for (int i = 0; i < L::LOADS; ++i) {
-        const int r = t0 * STEP + L::load_row(lane, wave, i);
-        token[i] = r / p.group;
-        hd[i] = r - token[i] * p.group;
-        byte[i] = L::load_byte(lane, wave, i);
-    }
+    for (int i = 0; i < L::LOADS; ++i) byte[i] = L::load_byte(lane, wave, i);
     const int stat_row = threadIdx.x & (STEP - 1);
     int stat_token = (t0 * STEP + stat_row) / p.group, stat_head = t0 * STEP + stat_row - stat_token * p.group;
     float stat = 0.f;
     const char* const qp = p.q + rq.start * p.q_row + (int64_t)head * p.group * p.q_head;
     const char* const gp = p.dout + rq.start * p.do_row + (int64_t)head * p.group * p.do_head;
-    auto next = [&](int& t, int& h) { t += step_tokens; h += step_heads; const bool over = h >= p.group; t += over; h -= over ? p.group : 0; };
+    auto next = [&](int& t, int& h, int tokens, int heads) { t += tokens; h += heads; const bool over = h >= p.group; t += over; h -= over ? p.group : 0; };
     auto fill = [&](int t, char* qt, char* gt) __attribute__((always_inline)) {
         const int base = t * STEP / p.group;      // (uniform) token that offsets are counted from
         const auto qr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(qp + base * p.q_row), 0, 0x7FFFFFFF, 0x00020000);
         const auto gr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(gp + base * p.do_row), 0, 0x7FFFFFFF, 0x00020000);
+        int at = token, h = hd;
 #pragma unroll
         for (int i = 0; i < L::LOADS; ++i) {
-            const bool in = token[i] < lq;
-            load_to_lds(qr, qt + L::load_to(wave, i), in ? (token[i] - base) * (int)p.q_row + hd[i] * (int)p.q_head + byte[i] : (int)0x80000000);
-            load_to_lds(gr, gt + L::load_to(wave, i), in ? (token[i] - base) * (int)p.do_row + hd[i] * (int)p.do_head + byte[i] : (int)0x80000000);
-            next(token[i], hd[i]);
+            const bool in = at < lq;
+            load_to_lds(qr, qt + L::load_to(wave, i), in ? (at - base) * (int)p.q_row + h * (int)p.q_head + byte[i] : (int)0x80000000);
+            load_to_lds(gr, gt + L::load_to(wave, i), in ? (at - base) * (int)p.do_row + h * (int)p.do_head + byte[i] : (int)0x80000000);
+            next(at, h, load_tokens, load_heads);
         }
+        next(token, hd, step_tokens, step_heads);
         if (threadIdx.x < 2 * STEP) {             // lse (threads 0 ..) and delta (threads STEP ..) of the step's rows
             const bool in = stat_token < lq;
             const float* const of = threadIdx.x < STEP ? p.lse : p.delta;
             stat = threadIdx.x < STEP ? -INFINITY : 0.f;
             if (in) stat = of[(int64_t)(head * p.group + stat_head) * p.Tq + rq.start + stat_token];
-            next(stat_token, stat_head);
+            next(stat_token, stat_head, step_tokens, step_heads);
         }
     };
     int q_at[NC], q_tr[NB][2];
@@ -815,11 +856,12 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
 }
 
 // ---- the tiles that were cut: their parts added up, D / 4 lanes to a row.  WHICH: 0 o and lse, 1 dq, 2 dk and dv.  Memory and a launch: 512 + 77
-// + 1 queries of 16 heads, the long ones in some four parts each, 10 us; dk and dv of four causal documents, 7678 keys of 8 heads, 29 us.
+// + 1 queries of 16 heads, the long ones in some four parts each, 10 us; dk and dv of four causal documents, 7678 keys of 8 heads, 30 us.  (80 scalar registers: with 83 a unit holds one workgroup
+// of 16 wavefronts instead of two, 37 us.)
 constexpr int kJoinThreads = 1024;
 template <int D> constexpr int kJoinBlocks = kRows * (D / 4) / kJoinThreads;      // of a tile
 template <typename T, int D, int WHICH>
-__global__ void __launch_bounds__(kJoinThreads) ragged_join_kernel(const RaggedParams p) {
+__global__ void __launch_bounds__(kJoinThreads) __attribute__((amdgpu_num_sgpr(80))) ragged_join_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr bool KEYS = WHICH == 2;
     constexpr int LANES = D / 4, AT_ONCE = kJoinThreads / LANES;
@@ -827,7 +869,7 @@ __global__ void __launch_bounds__(kJoinThreads) ragged_join_kernel(const RaggedP
     const Found f = find<std::conditional_t<KEYS, KeyTiles<D>, RowTiles>, kJoinThreads>(p, index);
     if (f.seq < 0 || f.parts <= 1) return;
     const int c = 4 * (threadIdx.x % LANES);
-    const Range r = range_of(KEYS ? p.cu_k : p.cu_q, f.seq, KEYS ? p.Tk : p.Tq);
+    const Range r = rows_of_sequence(KEYS ? p.cu_k : p.cu_q, f.seq, KEYS ? f.n.lk : f.n.lq);
     const int rows = KEYS ? r.length : r.length * p.group;
     const float* const from = p.parts + ((int64_t)index * p.Hkv + head) * p.most_parts * (WHICH == 0 ? kPartFloats<D> : WHICH * kRows * D);
     auto store = [&](char* to, f32x4 x) { *reinterpret_cast<u32x2*>(to + 2 * c) = u32x2{round2<T>(x[0], x[1]), round2<T>(x[2], x[3])}; };

@@ -369,3 +369,66 @@ def test_rows_behind_32_bits(pkg, ragged_oracle, gpu):
     a = pkg.ragged_bwd(*views, out, got[1], g, on, causal=True)
     b = pkg.ragged_bwd(*(x.contiguous() for x in views), want[0], want[1], g, on, causal=True)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def sequences(cu_q, cu_k, Tq, Tk):
+    """What offsets of any kind stand for: (rows, keys) of each sequence that has rows, keys None where its offsets say none."""
+    def apart(at, total):
+        end, kept = 0, []
+        for a, b in zip(at[:-1], at[1:]):
+            good = 0 <= a <= b <= total and (a == b or a >= end)
+            end = b if good and a < b else end
+            kept.append((a, b) if good else None)
+        return kept
+    return [(r, c) for r, c in zip(apart(cu_q, Tq), apart(cu_k, Tk)) if r and r[0] < r[1]], apart(cu_k, Tk)
+
+
+ODD_OFFSETS = [
+    ([0, 100, 300, 0, 0], None), ([0, 30, 20], None), ([200, 30, 100], None), ([0, 100, 300, 50, 120, 300], None), ([-5, 30, 20, 40, 100], None), ([5] * 70 + [3, 60, 10, 90, 300], None),
+    ([0, 300, 0, 300, 250, 290], None), ([0, 1 << 30, 50, 90, -(1 << 31), 200, 300], None), ([0, 100, 200, 300], [0, 250, 200, 300]), ([0, 100, 60, 200, 300], [0, 80, 80, 230, 300]),
+    ([0, 10, 10, 20], [0, 300, 100, 300]), ([0, 299, 0, 1], [300, 0, 300, 0]),
+]
+
+
+@pytest.mark.parametrize("behind", [0, 150, 1200])
+@pytest.mark.parametrize("cu_q, cu_k", ODD_OFFSETS)
+def test_sequences_before_and_beside_odd_offsets(pkg, ragged_oracle, gpu, cu_q, cu_k, behind):
+    """Whatever the other offsets are, no two sequences share a row or a key, and those that are apart have their values; `behind` more offsets of zero."""
+    cu_q = cu_q + [0] * behind
+    cu_k = cu_q if cu_k is None else cu_k + [0] * behind
+    q, k, v, g = (rows(300, h, 64, BF16, gpu, i) for i, h in enumerate((4, 2, 2, 4)))
+    held, keys = sequences(cu_q, cu_k, 300, 300)
+    on = (offsets(cu_q, gpu), offsets(cu_k, gpu))
+    o, lse = pkg.ragged_fwd(q, k, v, *on, causal=True)
+    grads = pkg.ragged_bwd(q, k, v, o, lse, g, *on, causal=True)
+    for _ in range(3):
+        again = pkg.ragged_fwd(q, k, v, *on, causal=True)
+        more = pkg.ragged_bwd(q, k, v, o, lse, g, *on, causal=True)
+        for (a, b), c in held:
+            assert torch.equal(again[0][a:b].nan_to_num(7), o[a:b].nan_to_num(7)) and torch.equal(again[1][:, a:b].nan_to_num(7), lse[:, a:b].nan_to_num(7)) and torch.equal(more[0][a:b], grads[0][a:b])
+        for c in keys:
+            if c:
+                assert all(torch.equal(x[slice(*c)], y[slice(*c)]) for x, y in zip(more[1:], grads[1:]))
+    for (a, b), c in held:
+        if c is None:
+            assert o[a:b].isnan().all() and lse[:, a:b].isnan().all() and (grads[0][a:b] == 0).all()
+            continue
+        part = (q[a:b], k[slice(*c)], v[slice(*c)])
+        at = ([0, b - a], [0, c[1] - c[0]])
+        O, L, o_tol, l_tol = ragged_oracle.ragged_fwd(*part, *at, True, 0.125, BF16)
+        near(o[a:b], O, o_tol, f"o of {a} .. {b}")
+        near(lse[:, a:b], L, l_tol, f"lse of {a} .. {b}")
+        want, tols = ragged_oracle.ragged_bwd(*part, g[a:b], *at, True, 0.125, BF16)
+        for x, (i, j), w, t in zip(grads, ((a, b), c, c), want, tols):
+            near(x[i:j], w, t, f"a gradient of {i} .. {j}")
+
+
+@pytest.mark.parametrize("n", [40, 200, 1200])
+def test_gradients_of_offsets_that_go_back(pkg, ragged_oracle, gpu, n):
+    """0, 300, 0, 300, ...: the sequence's gradients are those it has by itself."""
+    q, k, g = rows(300, 4, 64, BF16, gpu, 0), rows(300, 2, 64, BF16, gpu, 1), rows(300, 4, 64, BF16, gpu, 2)
+    o, lse = pkg.ragged_fwd(q, k, k, offsets([0, 300], gpu))
+    got = pkg.ragged_bwd(q, k, k, o, lse, g, offsets([300 * (i % 2) for i in range(n)], gpu))
+    want, tols = ragged_oracle.ragged_bwd(q, k, k, g, [0, 300], [0, 300], False, 0.125, BF16)
+    for name, x, w, t in zip(("dq", "dk", "dv"), got, want, tols):
+        near(x, w, t, name)
