@@ -14,7 +14,7 @@
 // their keys (rows), and a second kernel adds the parts up, in their order.
 //
 // Offsets are not trusted: a sequence whose offsets do not ascend within the tensors, or that begins before the end of an earlier one, has no rows; one whose keys' offsets are such has rows of
-// NaN (no gradients: zeros).  No two sequences then have a row or a key in common, whatever the offsets hold: each row is one workgroup's to write, and there are never more tiles than workgroups.
+// NaN (no gradients: zeros).  Rows that no sequence is left for are those of no sequence.  No two sequences then have a row or a key in common, whatever the offsets hold: each row is one workgroup's to write, and there are never more tiles than workgroups.
 #include <hip/hip_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -319,31 +319,39 @@ __device__ __forceinline__ Block block_of(const RaggedParams& p, int b) {
     return {b - rest * p.Hkv, rest - before * p.tiles, p.most_parts - 1 - before};
 }
 
-// ---- rows of no sequence: zeros, lse = -inf
+// ---- rows of no sequence: zeros, lse = -inf.  They are counted through, whatever lies between them, and a workgroup behind the last tile has `rows` of them.
 template <int D> __device__ __forceinline__ void clear_rows(char* out, int64_t row, int64_t head, const int* cu, int n, int total, int heads, int first_head, int rows, Found f, float* lse) {
-    const int tile = f.tile;
-    int lead = cu[0], from = cu[n];
-    if (f.odd) {                     // (the last offset need not be the last sequence's end)
-        lead = -1;
-        from = 0;
-        for (int base = 0; base < n; base += 64) {
-            const unsigned long long some = __ballot(apart(cu, base, n, total, from) > 0);
-            if (lead < 0 && some) lead = cu[base + __builtin_ctzll(some)];
+    constexpr int CHUNKS = D / 8;
+    int64_t first = (int64_t)f.tile * rows;      // the workgroup's first one, counted from the next row to be cleared
+    auto clear = [&](int from, int to) {         // the tensor's rows from .. to - 1
+        const int64_t count = (int64_t)(to - from) * heads, lo = first < 0 ? 0 : first, hi = first + rows < count ? first + rows : count;
+        for (int i = threadIdx.x; i < (hi - lo) * CHUNKS; i += kThreads) {
+            const int64_t r = lo + i / CHUNKS;
+            const int t = from + (int)(r / heads), h = first_head + (int)(r % heads);
+            *reinterpret_cast<u32x4*>(out + t * row + h * head + 16 * (i % CHUNKS)) = u32x4{0, 0, 0, 0};
+            if (lse && i % CHUNKS == 0) lse[(int64_t)h * total + t] = -INFINITY;
+        }
+        first -= count;
+    };
+    if (!f.odd) {
+        int lead = cu[0], from = cu[n];
+        lead = lead < 0 ? 0 : lead > total ? total : lead;
+        from = from < lead ? lead : from > total ? total : from;
+        clear(0, lead);
+        clear(from, total);
+        return;
+    }
+    // (between the sequences that there are as well)
+    int end = 0, done = 0;
+    for (int base = 0; base < n; base += 64) {
+        const int i = base + (threadIdx.x & 63), start = cu[i < n ? i : n], length = apart(cu, base, n, total, end);
+        for (unsigned long long left = __ballot(length > 0); left; left &= left - 1) {
+            const int at = __builtin_ctzll(left), a = __builtin_amdgcn_readlane(start, at);
+            clear(done, a);
+            done = a + __builtin_amdgcn_readlane(length, at);
         }
     }
-    lead = lead < 0 ? 0 : lead > total ? total : lead;
-    from = from < lead ? lead : from > total ? total : from;
-    const int64_t count = (int64_t)(lead + total - from) * heads;
-    constexpr int CHUNKS = D / 8;
-    for (int i = threadIdx.x; i < rows * CHUNKS; i += kThreads) {
-        const int64_t r = (int64_t)tile * rows + i / CHUNKS;
-        if (r >= count) continue;
-        int t = (int)(r / heads);
-        const int h = first_head + (int)(r % heads);
-        t = t < lead ? t : from + (t - lead);
-        *reinterpret_cast<u32x4*>(out + t * row + h * head + 16 * (i % CHUNKS)) = u32x4{0, 0, 0, 0};
-        if (lse && i % CHUNKS == 0) lse[(int64_t)h * total + t] = -INFINITY;
-    }
+    clear(done, total);
 }
 
 constexpr float kLowest = -3.0e38f;      // a max that no score has moved yet: exponentials of masked scores stay 0 and those of the sums so far too

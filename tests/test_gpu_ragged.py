@@ -432,3 +432,40 @@ def test_gradients_of_offsets_that_go_back(pkg, ragged_oracle, gpu, n):
     want, tols = ragged_oracle.ragged_bwd(q, k, k, g, [0, 300], [0, 300], False, 0.125, BF16)
     for name, x, w, t in zip(("dq", "dk", "dv"), got, want, tols):
         near(x, w, t, name)
+
+
+def fill_free_memory(*like):
+    """The memory that the next tensors of these sizes get holds NaN."""
+    torch.cuda.synchronize()
+    kept = [torch.full_like(x, math.nan) for x in like for _ in range(4)]
+    torch.cuda.synchronize()
+    del kept
+
+
+@pytest.mark.parametrize("behind", [0, 150])
+@pytest.mark.parametrize("cu_q, cu_k", ODD_OFFSETS + [([0, 30, 100], [-5, 30, 20]), ([7, 40, 1000, 60, 61], [0, 0, 1, -1, 5])])
+@pytest.mark.parametrize("group", [1, 3])
+def test_rows_that_no_sequence_is_left_for(pkg, gpu, cu_q, cu_k, behind, group):
+    """Between the sequences that there are, too: zeros, lse -inf, and gradients of zero, never what the memory held."""
+    cu_q = cu_q + [0] * behind
+    cu_k = cu_q if cu_k is None else cu_k + [0] * behind
+    q, k, v, g = (rows(300, h, 128, BF16, gpu, i) for i, h in enumerate((2 * group, 2, 2, 2 * group)))
+    held, keys = sequences(cu_q, cu_k, 300, 300)
+    on = (offsets(cu_q, gpu), offsets(cu_k, gpu))
+    none_q, none_k = torch.ones(300, dtype=torch.bool, device=gpu), torch.ones(300, dtype=torch.bool, device=gpu)
+    for (a, b), _ in held:
+        none_q[a:b] = False
+    for c in keys:
+        if c:
+            none_k[slice(*c)] = False
+    lse_like = torch.empty(2 * group, 300, device=gpu)
+    fill_free_memory(q, lse_like)
+    o, lse = pkg.ragged_fwd(q, k, v, *on)
+    assert (o[none_q] == 0).all() and (lse[:, none_q] == -math.inf).all()
+    fill_free_memory(q, k, v, lse_like)
+    dq, dk, dv = pkg.ragged_bwd(q, k, v, o, lse, g, *on)
+    assert (dq[none_q] == 0).all() and (dk[none_k] == 0).all() and (dv[none_k] == 0).all()
+    assert all(x.isfinite().all() for x in (dq, dk, dv))
+    out = torch.full_like(q, 3.0)
+    pkg.ragged_fwd(q, k, v, *on, out=out)
+    assert (out[none_q] == 3).all() and torch.equal(out[~none_q].nan_to_num(7), o[~none_q].nan_to_num(7))
