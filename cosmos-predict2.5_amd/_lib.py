@@ -288,6 +288,7 @@ class CacheDesc(ctypes.Structure):
     ]
 
 
+FILL_ALL, FILL_LSE = 1, 2
 CACHE_SAME, CACHE_E4M3, CACHE_INT8 = 0, 1, 2
 GEMM_XWT, GEMM_XW, GEMM_XTX = 0, 1, 2
 GEMM_SUM = 1

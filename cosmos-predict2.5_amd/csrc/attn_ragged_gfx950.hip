@@ -328,7 +328,7 @@ template <int D> __device__ __forceinline__ void clear_rows(char* out, int64_t r
         for (int i = threadIdx.x; i < (hi - lo) * CHUNKS; i += kThreads) {
             const int64_t r = lo + i / CHUNKS;
             const int t = from + (int)(r / heads), h = first_head + (int)(r % heads);
-            *reinterpret_cast<u32x4*>(out + t * row + h * head + 16 * (i % CHUNKS)) = u32x4{0, 0, 0, 0};
+            if (out) *reinterpret_cast<u32x4*>(out + t * row + h * head + 16 * (i % CHUNKS)) = u32x4{0, 0, 0, 0};
             if (lse && i % CHUNKS == 0) lse[(int64_t)h * total + t] = -INFINITY;
         }
         first -= count;
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
     const int head = block.head;
     const Found f = find<RowTiles>(p, block.index);
     if (f.seq < 0) {
-        if (p.fill && block.part == 0) clear_rows<D>(p.o, p.o_row, p.o_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f, p.lse);
+        if (p.fill && block.part == 0) clear_rows<D>(p.fill == COSMOS_ATTN_FILL_LSE ? nullptr : p.o, p.o_row, p.o_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f, p.lse);
         return;
     }
     if (block.part >= f.parts) return;
@@ -993,7 +993,7 @@ RaggedParams params_of(const cosmos_attn_ragged_desc* d) {
     p.dk_row = 2 * d->dk_stride[0]; p.dk_head = 2 * d->dk_stride[1];
     p.dv_row = 2 * d->dv_stride[0]; p.dv_head = 2 * d->dv_stride[1];
     p.n_seq = d->n_seq; p.Tq = (int)d->Tq; p.Tk = (int)d->Tk; p.Hkv = d->Hkv; p.group = d->Hq / d->Hkv;
-    p.causal = d->causal != 0; p.fill = d->fill != 0;
+    p.causal = d->causal != 0; p.fill = d->fill == COSMOS_ATTN_FILL_LSE && !d->lse ? 0 : d->fill;
     p.scale = d->sm_scale;
     p.scale_log2 = fmaxf(fabsf(d->sm_scale) * 1.44269504088896341f, 1e-37f);      // (a masked score of -inf stays that)
     p.flip = signbit(d->sm_scale) ? 0x80008000u : 0u;

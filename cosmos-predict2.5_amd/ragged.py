@@ -161,7 +161,7 @@ def _pointers(*tensors):
 
 def _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, fill, rest, dout=None, dq=None, dk=None, dv=None) -> bytes:
     return _RAGGED_DESC.pack(
-        _lib.ABI_VERSION, _DTYPES[q.dtype], cu_q.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2], 1 if causal else 0, 1 if fill else 0, q.shape[0], k.shape[0],
+        _lib.ABI_VERSION, _DTYPES[q.dtype], cu_q.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2], 1 if causal else 0, fill, q.shape[0], k.shape[0],
         q.shape[2] ** -0.5 if sm_scale is None else sm_scale, 0, *_pointers(q, k, v, cu_q, cu_k, o, lse, dout, dq, dk, dv), *_strides(q, k, v, o, dout, dq, dk, dv), *_pointers(rest))
 
 
@@ -181,7 +181,7 @@ def ragged_fwd(
     (``cu_k`` None: the same).  ``causal``: query t of Lq sees the keys up to ``t + Lk - Lq``.  ``lse``: fp32 ``[Hq, Tq]``.
 
     A row that sees no key: o = 0, lse = -inf.  Rows of no sequence (before ``cu_q[0]``, from the last offset on) become zeros, and -inf; in ``out``, a tensor that is given for o, they are
-    left as they are.  Offsets that do not ascend within the tensors, or a sequence that begins before an earlier one's end: a sequence of such ``cu_q`` is none (its rows are of no
+    left as they are (lse is -inf there too).  Offsets that do not ascend within the tensors, or a sequence that begins before an earlier one's end: a sequence of such ``cu_q`` is none (its rows are of no
     sequence, unless another one has them), one of such ``cu_k`` has rows of NaN; the sequences before are as ever (zeros behind the last offset, say, are sequences without rows).  ``out``
     must not overlap the inputs.
     ``rest``, a contiguous tensor like q, takes what rounding o left off, for :func:`ragged_bwd` (rows of no sequence: left as they are).  No gradients:
@@ -202,7 +202,7 @@ def ragged_fwd(
             raise ValueError("out: rows of 16-byte steps are written in place, this view cannot be")
         o = out
     lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32) if need_lse else None
-    desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, out is None, rest)
+    desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, _lib.FILL_ALL if out is None else _lib.FILL_LSE, rest)
     lib = _lib.load_library()
     ws_bytes = lib.cosmos_attn_ragged_workspace_bytes(desc)
     workspace = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
@@ -236,7 +236,7 @@ def ragged_bwd(
     assert lse.shape == (q.shape[1], q.shape[0]) and lse.dtype == torch.float32 and lse.device == q.device, "lse is the forward's, fp32 [Hq, Tq]"
     q, k, v, o, dout, lse = packed(q), packed(k), packed(v), packed(o), packed(dout), lse.contiguous()
     dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
-    desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, True, rest, dout, dq, dk, dv)
+    desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, _lib.FILL_ALL, rest, dout, dq, dk, dv)
     lib = _lib.load_library()
     ws_bytes = lib.cosmos_attn_ragged_bwd_workspace_bytes(desc)
     workspace = q.new_empty(ws_bytes, dtype=torch.uint8)

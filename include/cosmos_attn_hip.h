@@ -407,7 +407,8 @@ COSMOS_ATTN_API int cosmos_attn_gemm_preferred(const cosmos_attn_gemm_desc *desc
  * offsets stay on the device and may change between replays of a captured call.  With t and j counted from the sequence's start and Lq, Lk its lengths:
  *     o_t = sum_j softmax_j(sm_scale q_t k_j) v_j over the visible keys: all, or (causal) j <= t + Lk - Lq: the last query sees all keys
  *     lse_t = log sum_j exp(sm_scale q_t k_j)
- * A row that sees no key: o = 0, lse = -inf, and no gradient.  Rows of no sequence (before cu_q[0], from cu_q[n_seq] on) are left as they are, or with `fill` become zeros (lse -inf).
+ * A row that sees no key: o = 0, lse = -inf, and no gradient.  Rows of no sequence (before cu_q[0], from cu_q[n_seq] on) are left as they are, or with `fill` become zeros (lse -inf;
+ * COSMOS_ATTN_FILL_LSE: lse's alone, where o is the caller's and lse is new).
  * Offsets that do not ascend within the tensors: a sequence of such cu_q has no rows (what only such ones would have are rows of no sequence), one of such cu_k rows of NaN (and gradients of zero); neither reads or writes outside of the tensors.  A
  * sequence that begins before the end of an earlier one has such offsets too, so that no two share a row or a key; those before it are as ever.
  * What a row does not see has no influence on it as long as it is finite within the row's own sequence; what lies outside of the sequences may be anything.
@@ -417,6 +418,7 @@ COSMOS_ATTN_API int cosmos_attn_gemm_preferred(const cosmos_attn_gemm_desc *desc
  * The workspaces hold a number per row and head (backward) and the parts of tiles that are cut where there are few; the bytes follow from the sizes alone, and may be 0.  Outputs must not
  * overlap inputs or each other.
  */
+enum cosmos_attn_ragged_fill { COSMOS_ATTN_FILL_NONE = 0, COSMOS_ATTN_FILL_ALL = 1, COSMOS_ATTN_FILL_LSE = 2 };   /* (any other value: as ALL) */
 typedef struct cosmos_attn_ragged_desc {
     int32_t abi_version, dtype;
     int32_t n_seq, Hq, Hkv, D;         /* Hq % Hkv == 0; D 64 or 128 */

@@ -469,3 +469,20 @@ def test_rows_that_no_sequence_is_left_for(pkg, gpu, cu_q, cu_k, behind, group):
     out = torch.full_like(q, 3.0)
     pkg.ragged_fwd(q, k, v, *on, out=out)
     assert (out[none_q] == 3).all() and torch.equal(out[~none_q].nan_to_num(7), o[~none_q].nan_to_num(7))
+
+
+@pytest.mark.parametrize("at", [[7, 47, 147], [0, 147, 100, 140], [0], [0, 156]])
+def test_lse_beside_a_given_output(pkg, gpu, at):
+    """lse is a new tensor, also where o is the caller's: -inf where there is no sequence."""
+    q, k, v = (rows(156, h, 64, BF16, gpu, i) for i, h in enumerate((4, 2, 2)))
+    on = offsets(at, gpu)
+    want_o, want = pkg.ragged_fwd(q, k, v, on, causal=True)
+    out = torch.full_like(q, 3.0)
+    fill_free_memory(want)
+    o, lse = pkg.ragged_fwd(q, k, v, on, causal=True, out=out)
+    none = torch.ones(156, dtype=torch.bool, device=gpu)
+    for (a, b), _ in sequences(at, at, 156, 156)[0]:
+        none[a:b] = False
+    assert o is out and torch.equal(lse, want) and (lse[:, none] == -math.inf).all()
+    assert (out[none] == 3).all() and torch.equal(out[~none], want_o[~none])
+    assert pkg.ragged_fwd(q, k, v, on, causal=True, out=out, need_lse=False)[1] is None and (out[none] == 3).all()
