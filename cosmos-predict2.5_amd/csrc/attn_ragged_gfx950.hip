@@ -120,6 +120,22 @@ template <typename T> __device__ __forceinline__ void store_rounded(char* to, ch
 #endif
     if (rest) *reinterpret_cast<u32x2*>(rest) = u32x2{round2<T>(a - element<T>(w[0], 0), b - element<T>(w[0], 1)), round2<T>(c - element<T>(w[1], 0), d - element<T>(w[1], 1))};
 }
+// dS in fp16.  P is about one over the number of keys and dP as large as dout, so that dS = P (dP - delta) leaves fp16's range downwards (2^-14) where dq and dk are well within it (4096 keys,
+// dout 1e-3: they would be 5e-3 off), and upwards (65504) where dout is scaled up and weights lie on few keys.  It is held as 2^up dS: from 2^kUp on down, whenever one is above kMostDs, to as
+// many bits as the largest so far leaves above 2^8, and what is summed up is scaled with it.  A row (dq) or a key (dk) has its own `up`.  bf16 has the range of fp32.
+// (Gradients in fp16 take 3 % longer at head dim 128, 5 at 64: four documents of 7678 positions, 32 heads on 8, us, without / with 789 / 814; 8192 positions, 16 heads of 64, 570 / 598.)
+template <typename T> constexpr bool kNarrow = __is_same(T, _Float16);
+constexpr int kUp = 48;
+constexpr float kMostDs = 16384.f;
+__device__ __forceinline__ float largest(f32x16 s) {
+    float top = fabsf(s[0]);
+#pragma unroll
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, fabsf(s[e]));
+    return top;
+}
+// how far down, in powers of two, for a largest one of `top`
+__device__ __forceinline__ int too_many(float top) { return top > kMostDs && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 9 : 0; }
+__device__ __forceinline__ float power_of_two(int n) { return __builtin_amdgcn_ldexpf(1.f, n); }
 // The order of a block's LDS reads and matrix products, READS to PRODUCTS: AHEAD reads first, then each product with its share of the others.  (Left alone the compiler reads the operands of two
 // products and waits for them: 2 % of the forward, and of the dK/dV kernel, where no more registers are free for it.)
 template <int READS, int PRODUCTS, int AHEAD> __device__ __forceinline__ void reads_ahead() {
@@ -601,6 +617,8 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
         lse2 = x == -INFINITY ? INFINITY : x * 1.44269504088896341f;
         if (half == 0 && block.part == 0) p.delta[stat] = delta;
     }
+    const float lse0 = lse2;
+    if constexpr (kNarrow<T>) lse2 -= kUp;      // (P is not needed but for dS: 2^up is part of its exponent)
     int k_at[NC], k_tr[NB][2];
 #pragma unroll
     for (int c = 0; c < NC; ++c) k_at[c] = L::at(lane, c);
@@ -632,6 +650,16 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
             if (masked)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = 32 * h + 8 * (e >> 2) + (e & 3) < left ? s[e] : 0.f;
+            if constexpr (kNarrow<T>) {
+                const float top = largest(s);
+                if (__any(top > kMostDs)) {
+                    const int down = too_many(over_halves_max(top));
+                    lse2 += down;
+                    s *= power_of_two(-down);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) acc[b] *= power_of_two(-down);
+                }
+            }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 u32x4 w;
@@ -656,6 +684,11 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
         step(t + 1, tile2, tile3);
     }
     if (!live) return;
+    if constexpr (kNarrow<T>) {
+        const float back = lse0 < INFINITY ? power_of_two((int)rintf(lse2 - lse0)) : 1.f;      // (a whole number but for its rounding)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[b] *= back;
+    }
     if (f.parts > 1) {
         float* const part = p.parts + (((int64_t)block.index * p.Hkv + head) * p.most_parts + block.part) * (kRows * D) + (32 * wave + (lane & 31)) * D;
 #pragma unroll
@@ -770,6 +803,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     f32x16 dk[NB], dv[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) dk[b] = dv[b] = f32x16{};
+    float up = power_of_two(kUp);
 
     auto step = [&](int t, const char* qt, const char* gt, const float* st) __attribute__((always_inline)) {
         const int row0 = t * STEP;
@@ -800,6 +834,18 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
                 for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) >= left ? s[e] : 0.f;
             }
             V8 pf[2], df[2];
+            g *= s;
+            if constexpr (kNarrow<T>) {
+                g *= up;
+                const float top = largest(g);
+                if (__any(top > kMostDs)) {
+                    const float by = power_of_two(-too_many(over_halves_max(top)));
+                    up *= by;
+                    g *= by;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) dk[b] *= by;
+                }
+            }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 u32x4 w, x;
@@ -807,7 +853,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
                 for (int i = 0; i < 4; ++i) {
                     const int e = 8 * c + 2 * i;
                     w[i] = round2<T>(s[e], s[e + 1]);
-                    x[i] = round2<T>(s[e] * g[e], s[e + 1] * g[e + 1]);
+                    x[i] = round2<T>(g[e], g[e + 1]);
                 }
                 pf[c] = __builtin_bit_cast(V8, w);
                 df[c] = __builtin_bit_cast(V8, x);
@@ -839,6 +885,11 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
         step(t + 1, tile2, tile3, stats1);
     }
     if (!live) return;
+    if constexpr (kNarrow<T>) {
+        const float back = power_of_two(1 - __builtin_amdgcn_frexp_expf(up));      // (of a power of two: the exponent and one)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) dk[b] *= back;
+    }
     if (f.parts > 1) {
         float* const part = p.parts + (((int64_t)block.index * p.Hkv + head) * p.most_parts + block.part) * (2 * kRows * D) + (32 * wave + (lane & 31)) * D;
 #pragma unroll

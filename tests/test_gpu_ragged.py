@@ -486,3 +486,82 @@ def test_lse_beside_a_given_output(pkg, gpu, at):
     assert o is out and torch.equal(lse, want) and (lse[:, none] == -math.inf).all()
     assert (out[none] == 3).all() and torch.equal(out[~none], want_o[~none])
     assert pkg.ragged_fwd(q, k, v, on, causal=True, out=out, need_lse=False)[1] is None and (out[none] == 3).all()
+
+
+@pytest.mark.parametrize("ql, kl, Hq, Hkv, D, causal", [([5, 3, 20, 1, 130], [5, 3, 20, 1, 130], 4, 2, 64, True), ([700, 90], [700, 300], 2, 1, 128, True), ([40, 9], [5000, 12], 4, 1, 64, False),
+                                                         ([3000], [3000], 1, 1, 128, True), ([200], [4096], 2, 2, 128, False)])
+@pytest.mark.parametrize("power", [-12, -8, 10])
+def test_gradients_scale_with_dout_in_fp16(pkg, gpu, ql, kl, Hq, Hkv, D, causal, power):
+    """2^power times dout has 2^power times the gradients, to their own rounding (u = 2^-11, half of fp16's smallest step 2^-25) on both sides: dS has the range it needs wherever dout lies.
+    Products and sums in fp32 scale exactly; an element of dS far below the largest of its row or key is rounded to 2^-33 of that one at most.  For dq the power of two is part of P's exponent,
+    c s - lse + up in fp32, whose rounding goes by its size: dS moves by some 2^-20 of itself, so that where it lies next to a tie of fp16 the two sides round to neighbours, 2 u apart."""
+    q, k, v = rows(sum(ql), Hq, D, FP16, gpu, 0), rows(sum(kl), Hkv, D, FP16, gpu, 1), rows(sum(kl), Hkv, D, FP16, gpu, 2)
+    r = torch.Generator().manual_seed(3)
+    g = ((1 + torch.randint(0, 4, q.shape, generator=r) / 4) * 2.0 ** torch.randint(-1, 1, q.shape, generator=r) * (2 * torch.randint(0, 2, q.shape, generator=r) - 1)).to(FP16).to(gpu)
+    on, rest = [offsets(cu(x), gpu) for x in (ql, kl)], torch.empty_like(q)
+    o, lse = pkg.ragged_fwd(q, k, v, *on, causal=causal, rest=rest)
+    one = pkg.ragged_bwd(q, k, v, o, lse, g, *on, causal=causal, rest=rest)
+    scaled = g * 2.0 ** power
+    assert torch.equal(scaled.double(), g.double() * 2.0 ** power)
+    other = pkg.ragged_bwd(q, k, v, o, lse, scaled, *on, causal=causal, rest=rest)
+    flips = torch.zeros(q.shape, dtype=torch.float64, device=gpu)         # sum of |c dS K|
+    for (a, b), (x, y) in zip(zip(cu(ql), cu(ql)[1:]), zip(cu(kl), cu(kl)[1:])):
+        mask = torch.arange(y - x, device=gpu) <= torch.arange(b - a, device=gpu)[:, None] + (y - x - b + a) if causal else torch.ones(b - a, y - x, dtype=torch.bool, device=gpu)
+        for h in range(Hq):
+            Q, G, K, V = q[a:b, h].double(), g[a:b, h].double(), k[x:y, h * Hkv // Hq].double(), v[x:y, h * Hkv // Hq].double()
+            P = torch.exp(D ** -0.5 * Q @ K.t().contiguous() - lse[h, a:b, None]) * mask
+            flips[a:b, h] = D ** -0.5 * (P * (G @ V.t().contiguous() - (G * (P @ V)).sum(-1, keepdim=True))).abs() @ K.abs()
+    most = 2 * float(g.double().norm(dim=2).max() * v.double().norm(dim=2).max()) * D ** -0.5      # of c dS
+    for name, x, y, by, n in zip(("dq", "dk", "dv"), one, other, (k, q, g), (max(kl), max(ql) * Hq // Hkv, 0)):
+        x, y = x.double(), y.double() * 2.0 ** -power
+        assert y.isfinite().all(), name
+        size = torch.maximum(x.abs(), y.abs()) * (1 + 2.0 ** -10)
+        tol = 2 * 2.0 ** -11 * (size + (flips if name == "dq" else 0)) * (1 + 2.0 ** -8) + 2.0 ** -25 * (1 + 2.0 ** -power) + n * 2.0 ** -33 * most * float(by.abs().max())
+        near(y, x.cpu(), tol.cpu(), name)
+
+
+def gradients_and_their_roundings(q, k, v, g, c):
+    """dq, dk, dv of one key head's sequence in 64 bits (rows of all its query heads together), and how far from them roundings of fp16 are: P and dS once each as operands of the last products
+    and the result once, each by u = 2^-11 at most (the result by 2^-25 besides), independent of each other, so that their squares add up."""
+    u = 2.0 ** -11
+    s = c * q @ k.t()
+    P = torch.exp(s - torch.logsumexp(s, -1, keepdim=True))
+    dS = c * P * (g @ v.t() - (g * (P @ v)).sum(-1, keepdim=True))
+    grads = dS @ k, dS.t() @ q, P.t() @ g
+    far = (u * dS) ** 2 @ k ** 2, ((u * dS) ** 2).t() @ q ** 2, ((u * P) ** 2).t() @ g ** 2
+    return grads, [f + (u * x) ** 2 + 2.0 ** -50 for f, x in zip(far, grads)]
+
+
+def check_norms(pkg, gpu, Lq, Lk, D, size):
+    """The errors' norm is their roundings', whose expectation is below that of `far`; three hundredths more than 1 are what sums in fp32 and the spread of a norm of thousands are."""
+    q, k, v, g = rows(Lq, 2, D, FP16, gpu, 0), rows(Lk, 1, D, FP16, gpu, 1), rows(Lk, 1, D, FP16, gpu, 2), rows(Lq, 2, D, FP16, gpu, 3, size)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    pkg.attention_ragged(*leaves, offsets([0, Lq], gpu), offsets([0, Lk], gpu)).backward(g)
+    one = lambda x: x.transpose(0, 1).reshape(-1, D).double()
+    grads, far = gradients_and_their_roundings(one(q), one(k), one(v), one(g), D ** -0.5)
+    for name, x, w, f in zip(("dq", "dk", "dv"), leaves, grads, far):
+        off = float((one(x.grad) - w).norm())
+        assert off <= 1.03 * float(f.sum().sqrt()), f"{name}: {off / float(w.norm())} of it, roundings {float(f.sum().sqrt()) / float(w.norm())}"
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [2.0 ** 8, 1.0, 2.0 ** -10, 2.0 ** -13])
+def test_fp16_gradients_over_many_keys(pkg, gpu, D, size):
+    """P is about 2^-12, dout of any size."""
+    check_norms(pkg, gpu, 300, 4096, D, size)
+
+
+def test_fp16_gradients_of_weights_on_few_keys(pkg, gpu):
+    """dS of more than fp16 holds, of which dq and dk are well within it: weights of about one half and dout of some thousands."""
+    q, k, v = rows(6, 1, 64, FP16, gpu, 0), rows(2, 1, 64, FP16, gpu, 1, 2.0 ** -6), rows(2, 1, 64, FP16, gpu, 2, 8.0)
+    q *= 2.0 ** -6
+    g = rows(6, 1, 64, FP16, gpu, 3, 2.0 ** 12)
+    on = [offsets([0, 6], gpu), offsets([0, 2], gpu)]
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    pkg.attention_ragged(*leaves, *on).backward(g)
+    one = lambda x: x[:, 0].double()
+    grads, far = gradients_and_their_roundings(one(q), one(k), one(v), one(g), 0.125)
+    c = (one(g) @ one(v).t()).abs().max()
+    assert c > 65504 and grads[0].abs().max() < 65504
+    for name, x, w, f in zip(("dq", "dk", "dv"), leaves, grads, far):
+        assert x.grad.isfinite().all() and (one(x.grad) - w).norm() <= 2 * f.sum().sqrt(), name
