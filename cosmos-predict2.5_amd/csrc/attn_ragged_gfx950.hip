@@ -126,6 +126,8 @@ template <typename T> __device__ __forceinline__ void store_rounded(char* to, ch
 // (Gradients in fp16 take 3 % longer at head dim 128, 5 at 64: four documents of 7678 positions, 32 heads on 8, us, without / with 789 / 814; 8192 positions, 16 heads of 64, 570 / 598.)
 template <typename T> constexpr bool kNarrow = __is_same(T, _Float16);
 constexpr int kUp = 48;
+// P as dv's operand, which is 1 at most and below 2^-14 from some 16 000 keys on, is 2^kUpP P throughout.
+constexpr int kUpP = 14;
 constexpr float kMostDs = 16384.f;
 __device__ __forceinline__ float largest(f32x16 s) {
     float top = fabsf(s[0]);
@@ -803,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     f32x16 dk[NB], dv[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) dk[b] = dv[b] = f32x16{};
-    float up = power_of_two(kUp);
+    float up = power_of_two(kUp - kUpP);        // (of what is P here)
 
     auto step = [&](int t, const char* qt, const char* gt, const float* st) __attribute__((always_inline)) {
         const int row0 = t * STEP;
@@ -870,7 +872,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     };
     // (P = 0 where there is no row, or nothing that it sees)
     auto keep = [&](float* st) __attribute__((always_inline)) {
-        if (threadIdx.x < 2 * STEP) st[threadIdx.x] = threadIdx.x >= STEP ? stat : stat == -INFINITY ? INFINITY : stat * 1.44269504088896341f;
+        if (threadIdx.x < 2 * STEP) st[threadIdx.x] = threadIdx.x >= STEP ? stat : stat == -INFINITY ? INFINITY : stat * 1.44269504088896341f - (kNarrow<T> ? kUpP : 0);
     };
     if (t0 < n) fill(t0, tile0, tile1);
     for (int t = t0; t < n; t += 2) {
@@ -886,9 +888,12 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     }
     if (!live) return;
     if constexpr (kNarrow<T>) {
-        const float back = power_of_two(1 - __builtin_amdgcn_frexp_expf(up));      // (of a power of two: the exponent and one)
+        const float back = power_of_two(1 - kUpP - __builtin_amdgcn_frexp_expf(up));      // (of a power of two: the exponent and one)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) dk[b] *= back;
+        for (int b = 0; b < NB; ++b) {
+            dk[b] *= back;
+            dv[b] *= power_of_two(-kUpP);
+        }
     }
     if (f.parts > 1) {
         float* const part = p.parts + (((int64_t)block.index * p.Hkv + head) * p.most_parts + block.part) * (2 * kRows * D) + (32 * wave + (lane & 31)) * D;

@@ -565,3 +565,10 @@ def test_fp16_gradients_of_weights_on_few_keys(pkg, gpu):
     assert c > 65504 and grads[0].abs().max() < 65504
     for name, x, w, f in zip(("dq", "dk", "dv"), leaves, grads, far):
         assert x.grad.isfinite().all() and (one(x.grad) - w).norm() <= 2 * f.sum().sqrt(), name
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("keys", [30000, 262144])
+def test_fp16_gradients_over_very_many_keys(pkg, gpu, keys, D):
+    """P itself is below fp16's normal numbers."""
+    check_norms(pkg, gpu, 32, keys, D, 2.0 ** 8)
