@@ -591,6 +591,14 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
             for (int i = 0; i < 4; ++i) w[i] = round2<T>(x[2 * i], x[2 * i + 1]);
             pf[r] = __builtin_bit_cast(V8, w);
         }
+        // Past the end lie the last rows once more, whose infinite values with a weight of 0 would be NaN.  (The last step alone reaches there; a code's scale is what is infinite, or NaN, and is
+        // not taken there.)
+        if constexpr (!CODES && !decltype(more)::value) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < VWORDS; ++j) vw[i][j] = i < left ? vw[i][j] : 0u;
+        }
         // output rows NB n + b, n = 0 .. 15: what lane n16 holds of V, transposed in its registers
         unsigned vx[8][NB / 2];
 #pragma unroll

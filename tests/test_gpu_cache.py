@@ -408,3 +408,30 @@ def test_two_streams_at_once(pkg, ragged_oracle, gpu):
                 got[i].append(pkg.cache_attention(q[i], cache, table, on)[0])
     torch.cuda.synchronize()
     assert all(torch.equal(x, w) for g, w in zip(got, want) for x in g)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens, page", [([1, 5, 8, 13, 0, 33, 100], 16), ([129, 700, 6], 64), ([2500, 3, 1030], 16)])
+def test_infinite_values(pkg, ragged_oracle, gpu, lens, page, D, dtype):
+    """In the last row, and in any of a sequence: infinite in their channels, and nothing elsewhere."""
+    table, pages = tables(lens, page, gpu)
+    cache = empty(pkg, pages, 2, page, D, dtype, gpu)
+    k, v, q = rows(sum(lens), 2, D, dtype, gpu, 0), rows(sum(lens), 2, D, dtype, gpu, 1), rows(len(lens), 4, D, dtype, gpu, 2, 0.5)
+    on = cu(lens)
+    plain = v.clone()
+    want = {}
+    for i, (a, b) in enumerate(zip(on[:-1], on[1:])):
+        for channel, row, sign in ((3, b - 1, 1), (D - 1, max(a, b - 6), -1), (20, a + (b - a) // 2, 1)):
+            if a < b:
+                v[row, :, channel], plain[a:b, :, channel] = sign * math.inf, 0
+                want[i, channel] = sign * math.inf
+    pkg.cache_write(cache, k, v, table, offsets(lens, gpu), offsets(on, gpu))
+    o, lse = pkg.cache_attention(q, cache, table, offsets(lens, gpu), need_lse=True)
+    for (i, channel), w in want.items():
+        assert (o[i, :, channel] == w).all(), (i, channel)
+        o[i, :, channel] = 0
+    c = lambda x: [x[a:b].double().cpu() for a, b in zip(on[:-1], on[1:])]
+    O, L, tol, l_tol = ragged_oracle.decode(q, c(k), c(plain), D ** -0.5, dtype)
+    near(o, O, tol, "o")
+    near(lse, L, l_tol, "lse")
