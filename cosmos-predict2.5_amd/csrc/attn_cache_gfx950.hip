@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
 #pragma unroll
                 for (int i = 1; i < 8; ++i) top = fmaxf(top, by[i]);
                 if (__any(top > 64.f * R)) {
-                    top = fmaxf(R, over_quarters_max(top));
+                    top = fmaxf(fmaxf(R, over_quarters_max(top)), 0x1p-100f);      // (far below what fp16 holds, and its reciprocal is a number)
                     const float f = R / top;
 #pragma unroll
                     for (int r = 0; r < NR; ++r)

@@ -435,3 +435,24 @@ def test_infinite_values(pkg, ragged_oracle, gpu, lens, page, D, dtype):
     O, L, tol, l_tol = ragged_oracle.decode(q, c(k), c(plain), D ** -0.5, dtype)
     near(o, O, tol, "o")
     near(lse, L, l_tol, "lse")
+
+
+@pytest.mark.parametrize("kind", [E4M3, INT8])
+@pytest.mark.parametrize("power", [-132, -126, -120, -60])
+def test_values_that_fp16_does_not_reach(pkg, ragged_oracle, gpu, kind, power):
+    """Written as bf16 with scales below fp32's normal numbers, attended to in fp16: zeros, and beside larger values nothing.  (2^132 is infinite in fp32: the third sequence has rows that are
+    not finite then, and NaN by definition.)"""
+    lens = [200, 40, 300]
+    table, pages = tables(lens, 16, gpu)
+    cache = empty(pkg, pages, 2, 16, 64, kind, gpu)
+    k, v = rows(540, 2, 64, BF16, gpu, 0), rows(540, 2, 64, BF16, gpu, 1) * 2.0 ** power
+    v[500:] *= 2.0 ** -power
+    on = cu(lens)
+    pkg.cache_write(cache, k, v, table, offsets(lens, gpu), offsets(on, gpu))
+    q = rows(3, 4, 64, FP16, gpu, 2)
+    o, lse = pkg.cache_attention(q, cache, table, offsets(lens, gpu), need_lse=True)
+    K, V = ([stands_for(ragged_oracle, x[a:b], kind) for a, b in zip(on[:-1], on[1:])] for x in (k, v))
+    O, L, tol, l_tol = ragged_oracle.decode(q, K, V, 0.125, FP16)
+    near(o, O, tol.nan_to_num(0), "o")
+    near(lse, L, l_tol, "lse")
+    assert (o[:2] == 0).all() and (o[2].isnan().all() if power == -132 else o[2].abs().max() > 0.01)
