@@ -33,9 +33,9 @@ _CALL_PART = struct.Struct("=2iQq2Qq2Q4q2ifi2Q4qQ")
 class KVCache:
     """Pages of keys and values, ``[pages, heads, page_size, head_dim]`` each: bf16, fp16, or 8 bits (float8_e4m3fn, int8) with an fp32 scale for each row of a head,
     ``[pages, heads, page_size]``.  Takes the tensors as they are (any page, head and row strides of 16-byte steps) and writes into them:
-    ``k``, ``v``, ``k_scale``, ``v_scale`` are theirs, and stay so (a tensor's memory must not be exchanged below the cache, by ``set_`` or ``resize_``)."""
+    ``k``, ``v``, ``k_scale``, ``v_scale`` are theirs, and stay so: once a tensor's memory is exchanged (``.data``, ``set_``, ``resize_``) its cache is refused."""
 
-    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "pages", "heads", "page_size", "head_dim", "dtype", "device", "kind", "_parts", "_index")
+    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "pages", "heads", "page_size", "head_dim", "dtype", "device", "kind", "_parts", "_index", "_at")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
         assert k.dim() == 4 and v.shape == k.shape, "k and v must be [pages, heads, page_size, head_dim]"
@@ -62,6 +62,7 @@ class KVCache:
         self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
         self._index = k.get_device()
         at = lambda x: 0 if x is None else x.data_ptr()
+        self._at = tuple((x, x.data_ptr()) for x in (k, v, k_scale, v_scale) if x is not None)
         steps = lambda x, n: (0,) * n if x is None else x.stride()[:n]
         self._parts = {
             dtype: _CACHE_PART.pack(_lib.ABI_VERSION, code, self.kind, self.heads, self.head_dim, self.page_size, self.pages, at(k), at(v), *steps(k, 3), *steps(v, 3),
@@ -85,6 +86,9 @@ class KVCache:
         return cls(new(), new(), scale(), scale())
 
     def _part(self, dtype: torch.dtype) -> bytes:
+        for x, at in self._at:          # (the addresses in `_parts` are what a call writes to)
+            if x.data_ptr() != at:
+                raise RuntimeError("the memory of this cache's tensors was exchanged: make another KVCache of them")
         if self.kind == _lib.CACHE_SAME:
             assert dtype == self.dtype, f"a cache of {self.dtype} holds rows of that type, not {dtype}"
         return self._parts[dtype]

@@ -187,3 +187,32 @@ def test_refusals_before_a_launch(pkg, monkeypatch):
     ]:
         with pytest.raises(error):
             call()
+
+
+@pytest.mark.parametrize("which", ["k", "v", "k_scale", "v_scale"])
+@pytest.mark.parametrize("how", ["data", "set_", "resize_"])
+def test_a_cache_whose_memory_was_exchanged_is_refused(pkg, monkeypatch, which, how):
+    """Its descriptor holds addresses: what lies there may be another tensor's by now."""
+    launched = []
+    monkeypatch.setattr(pkg.kv_cache, "on_device", lambda *a: launched.append(a))
+    monkeypatch.setattr(pkg.kv_cache, "plain_int32", lambda *a: True)
+    make = lambda: (on(torch.zeros(5, 2, 16, 64, dtype=torch.int8)), on(torch.zeros(5, 2, 16, dtype=torch.float32)))
+    (k, k_scale), (v, v_scale) = make(), make()
+    cache = pkg.KVCache(k, v, k_scale, v_scale)
+    cache._index = -1                 # (where a host tensor says it is)
+    table, lens, one = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), on(torch.zeros(3, 2, 64, dtype=torch.bfloat16))
+    calls = [lambda: pkg.cache_write(cache, one, one, table, lens), lambda: pkg.cache_read(cache, table, torch.zeros(4, dtype=torch.int32), 3), lambda: pkg.cache_attention(one, cache, table, lens)]
+    for call in calls:
+        call()
+    assert len(launched) == 3
+    x = getattr(cache, which)
+    if how == "data":
+        x.data = torch.zeros_like(x).as_subclass(torch.Tensor).clone()
+    elif how == "set_":
+        x.set_(torch.zeros_like(x).as_subclass(torch.Tensor).clone())
+    else:
+        x.resize_(500, *x.shape[1:])
+    for call in calls:
+        with pytest.raises(RuntimeError, match="exchanged"):
+            call()
+    assert len(launched) == 3
