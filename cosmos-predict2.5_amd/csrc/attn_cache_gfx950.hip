@@ -761,6 +761,29 @@ int check_scale(const float* at, const int64_t* stride) {
     if (!at) return COSMOS_ATTN_BAD_ARG;
     return aligned16(at) && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[0] >= 0 && stride[1] >= 0 ? COSMOS_ATTN_OK : COSMOS_ATTN_BAD_STRIDE;
 }
+// pages to be written: of three dims of `size` elements each holds those of smaller strides, down to runs of `run` elements
+bool apart(const int64_t (&stride)[3], const int64_t (&size)[3], int64_t run) {
+    int order[3] = {0, 1, 2};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (stride[order[j]] < stride[order[i]]) std::swap(order[i], order[j]);
+    __int128 extent = run;
+    for (int i : order) {
+        if (size[i] <= 1) continue;
+        if (stride[i] < extent) return false;
+        extent += (__int128)(size[i] - 1) * stride[i];
+    }
+    return true;
+}
+int check_written(const cosmos_attn_cache_desc* d) {
+    const int64_t size[3] = {d->pages, d->Hkv, d->page_size}, ks[3] = {d->k_stride[0], d->k_stride[1], d->k_stride[2]}, vs[3] = {d->v_stride[0], d->v_stride[1], d->v_stride[2]};
+    if (d->k == d->v) return COSMOS_ATTN_BAD_ARG;
+    if (!apart(ks, size, d->D) || !apart(vs, size, d->D)) return COSMOS_ATTN_BAD_STRIDE;
+    if (d->kind == COSMOS_ATTN_CACHE_SAME) return COSMOS_ATTN_OK;
+    const int64_t kss[3] = {d->k_scale_stride[0], d->k_scale_stride[1], 1}, vss[3] = {d->v_scale_stride[0], d->v_scale_stride[1], 1};
+    if (d->k_scale == d->v_scale) return COSMOS_ATTN_BAD_ARG;
+    return apart(kss, size, 1) && apart(vss, size, 1) ? COSMOS_ATTN_OK : COSMOS_ATTN_BAD_STRIDE;
+}
 int check(const cosmos_attn_cache_desc* d) {
     if (!d || d->abi_version != COSMOS_ATTN_ABI_VERSION) return COSMOS_ATTN_BAD_ARG;
     if (d->dtype != COSMOS_ATTN_BF16 && d->dtype != COSMOS_ATTN_FP16) return COSMOS_ATTN_UNSUPPORTED;
@@ -821,6 +844,8 @@ int check_packed(const cosmos_attn_cache_desc* d, bool out) {
     if (d->B && !(out ? (const void*)d->cu : (const void*)d->lens)) return COSMOS_ATTN_BAD_ARG;
     if (!out && !d->cu && d->rows != d->B) return COSMOS_ATTN_BAD_SHAPE;
     if (packed_blocks(d) > kMostBlocks) return COSMOS_ATTN_UNSUPPORTED;
+    if (!out) st = check_written(d);
+    if (st != COSMOS_ATTN_OK) return st;
     if (!d->B && out && !d->cu) return COSMOS_ATTN_BAD_ARG;
     for (int i = 0; st == COSMOS_ATTN_OK && i < 2; ++i) {
         const void* const at = i ? d->v_rows : d->k_rows;

@@ -33,7 +33,8 @@ _CALL_PART = struct.Struct("=2iQq2Qq2Q4q2ifi2Q4qQ")
 class KVCache:
     """Pages of keys and values, ``[pages, heads, page_size, head_dim]`` each: bf16, fp16, or 8 bits (float8_e4m3fn, int8) with an fp32 scale for each row of a head,
     ``[pages, heads, page_size]``.  Takes the tensors as they are (any page, head and row strides of 16-byte steps) and writes into them:
-    ``k``, ``v``, ``k_scale``, ``v_scale`` are theirs, and stay so: once a tensor's memory is exchanged (``.data``, ``set_``, ``resize_``) its cache is refused."""
+    ``k``, ``v``, ``k_scale``, ``v_scale`` are theirs, and stay so: once a tensor's memory is exchanged (``.data``, ``set_``, ``resize_``) its cache is refused.
+    Pages or heads that share memory (``expand``) can be read and attended to; writing them is refused."""
 
     __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "pages", "heads", "page_size", "head_dim", "dtype", "device", "kind", "_parts", "_index", "_at")
 

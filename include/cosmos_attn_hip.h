@@ -452,6 +452,7 @@ COSMOS_ATTN_API int cosmos_attn_ragged_bwd(const cosmos_attn_ragged_desc *desc, 
  *
  * cosmos_attn_cache_write: packed rows k_rows, v_rows [rows, Hkv, D]; sequence i's are cu[i] .. cu[i + 1] - 1 (cu NULL: one for each sequence), its last positions: lens[i], which counts
  *     them, is where they end.  Rows of no sequence, and sequences with lens[i] below their rows, write nothing.  Two rows of a call must not have one place (two sequences sharing a page).
+ *     Pages, heads or rows that lie over each other, or k where v is, are refused here (they can be read).
  * cosmos_attn_cache_read: the first cu[i + 1] - cu[i] positions of sequence i to the rows cu[i] .. of k_rows and v_rows, code * scale rounded to `dtype`; rows of no sequence are left as
  *     they are, or with `fill` become zeros.
  * cosmos_attn_cache_attention: o[i] = softmax(sm_scale q[i] K^T) V over the first lens[i] positions, q, o [B, Hq, D], query head h on key head h / (Hq / Hkv); lse [B, Hq] fp32 or NULL.

@@ -216,3 +216,22 @@ def test_a_cache_whose_memory_was_exchanged_is_refused(pkg, monkeypatch, which, 
         with pytest.raises(RuntimeError, match="exchanged"):
             call()
     assert len(launched) == 3
+
+
+def test_pages_that_share_memory_are_not_written(pkg):
+    """Pages, heads or rows that lie over each other (`expand`), and one memory as keys and values: to be read, but no two workgroups may write one place."""
+    L, lib = pkg._lib, pkg._lib.load_library()
+    write = lambda D: lib.cosmos_attn_cache_write(ctypes.byref(D), None)
+    read = lambda D: lib.cosmos_attn_cache_read(ctypes.byref(D), None)
+    good = [dict(), dict(k_stride=(64, 50 * 32 * 64, 50 * 64)), dict(v_stride=(2 * 2 * 32 * 64, 64, 128)), dict(pages=1, k_stride=(0, 2048, 64)), dict(Hkv=1, rows=4, v_stride=(2048, 0, 64)),
+            dict(k_scale_stride=(32, 1600)), dict(k_stride=(1 << 40, 1 << 50, 64))]
+    for over in good:
+        for call in (write, read):
+            assert call(cache_desc(pkg, cu=P, **over)) not in (L.ST_BAD_STRIDE, L.ST_BAD_ARG), over
+    for over in [dict(k_stride=(0, 2048, 64)), dict(v_stride=(4096, 0, 64)), dict(k_stride=(2048, 2048, 64)), dict(v_stride=(4096, 2032, 64)), dict(k_stride=(4096, 64, 64)), dict(k_stride=(4080, 2048, 64)),
+                 dict(k_scale_stride=(0, 32)), dict(v_scale_stride=(64, 28)), dict(k_scale_stride=(32, 32))]:
+        assert write(cache_desc(pkg, cu=P, **over)) == L.ST_BAD_STRIDE, over
+        assert read(cache_desc(pkg, cu=P, **over)) != L.ST_BAD_STRIDE, over
+    for over in [dict(v=P), dict(v_scale=P + 2 * 4096)]:
+        assert write(cache_desc(pkg, cu=P, **over)) == L.ST_BAD_ARG, over
+        assert read(cache_desc(pkg, cu=P, **over)) != L.ST_BAD_ARG, over
