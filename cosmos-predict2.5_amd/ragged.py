@@ -55,6 +55,8 @@ def int32_on(x: torch.Tensor, device: torch.device) -> torch.Tensor:
     """Offsets, lengths and tables as the kernels take them: int32 on the device, elements of the last dim side by side."""
     assert not x.is_floating_point() and not x.is_complex() and x.dtype != torch.bool, "offsets, lengths and tables are whole numbers"
     if x.dtype != torch.int32 or x.device != device:
+        if x.dtype in (torch.int64, torch.uint64):      # (2^32 + 5 is not 5)
+            x = x.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1)
         x = x.to(device=device, dtype=torch.int32)
     return x if x.dim() == 0 or x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
 

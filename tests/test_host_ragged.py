@@ -235,3 +235,14 @@ def test_pages_that_share_memory_are_not_written(pkg):
     for over in [dict(v=P), dict(v_scale=P + 2 * 4096)]:
         assert write(cache_desc(pkg, cu=P, **over)) == L.ST_BAD_ARG, over
         assert read(cache_desc(pkg, cu=P, **over)) != L.ST_BAD_ARG, over
+
+
+def test_numbers_past_32_bits_stay_out_of_range(pkg):
+    """Offsets, lengths and tables of 64 bits: what 32 do not hold is not taken for a number that they do."""
+    far = torch.tensor([0, (1 << 32) + 5, 1 << 31, -(1 << 40) + 3, (1 << 31) - 1, -7])
+    got = pkg.ragged.int32_on(far, far.device)
+    assert got.dtype == torch.int32 and got.tolist() == [0, (1 << 31) - 1, (1 << 31) - 1, -(1 << 31), (1 << 31) - 1, -7]
+    assert pkg.ragged.int32_on(torch.tensor([3, 1 << 62], dtype=torch.uint64), far.device).tolist() == [3, (1 << 31) - 1]
+    for dtype in (torch.uint8, torch.int8, torch.int16, torch.int32):
+        assert pkg.ragged.int32_on(torch.tensor([[3, 100], [0, 9]], dtype=dtype), far.device).tolist() == [[3, 100], [0, 9]]
+    assert pkg.ragged.int32_on(far[::2], far.device).tolist() == [0, (1 << 31) - 1, (1 << 31) - 1]
