@@ -57,11 +57,6 @@ struct CacheParams {
 };
 
 // ---- 16-bit pairs
-template <typename T> __device__ __forceinline__ unsigned round2(float a, float b) {
-    typedef T V2 __attribute__((ext_vector_type(2)));
-    const V2 two = {(T)a, (T)b};
-    return __builtin_bit_cast(unsigned, two);
-}
 template <typename T> __device__ __forceinline__ float low(unsigned w) {
     if constexpr (__is_same(T, __bf16)) return __builtin_bit_cast(float, w << 16);
     else return (float)__builtin_bit_cast(_Float16, (uint16_t)w);
@@ -286,17 +281,6 @@ constexpr float kLowest = -3.0e38f;
 __device__ __forceinline__ int tiles_of(const CacheParams& p, int n) {
     return n > 0 && n <= (int64_t)p.width << p.page_shift ? (n + kTile - 1) / kTile : 0;
 }
-// sums over the wavefront's lanes up to each one (data-parallel-primitive moves: within rows of 16, then the rows' ends)
-template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
-__device__ __forceinline__ int sums_up_to(int v) {
-    v = dpp_add<0x111, 0xF>(v);      // row_shr 1, 2, 4, 8
-    v = dpp_add<0x112, 0xF>(v);
-    v = dpp_add<0x114, 0xF>(v);
-    v = dpp_add<0x118, 0xF>(v);
-    v = dpp_add<0x142, 0xA>(v);      // row_bcast 15 to rows 1 and 3
-    return dpp_add<0x143, 0xC>(v);   // row_bcast 31 to rows 2 and 3
-}
-__device__ __forceinline__ int sum_of(int v) { return __builtin_amdgcn_readlane(sums_up_to(v), 63); }
 // A sequence's parts have a share at most; three quarters of one where shares are large and most sequences have only a few parts, which rounding up leaves far from equal (48 sequences of 1 to
 // 7817 keys, us, a share / three quarters: 106 / 100; but 131072 + 70001 + 99 keys in e4m3 84 / 88, 32 of 1 to 2817 in int8 18.9 / 20.5).
 struct Share {

@@ -39,6 +39,25 @@ __device__ __forceinline__ void both_halves(float x, float& lo, float& hi) {
     hi = __builtin_bit_cast(float, b);
 }
 
+// two values rounded, side by side
+template <typename T> __device__ __forceinline__ unsigned round2(float a, float b) {
+    typedef T V2 __attribute__((ext_vector_type(2)));
+    const V2 two = {(T)a, (T)b};
+    return __builtin_bit_cast(unsigned, two);
+}
+
+// sums over the wavefront's lanes up to each one (data-parallel-primitive moves: within rows of 16, then the rows' ends)
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+__device__ __forceinline__ int sums_up_to(int v) {
+    v = dpp_add<0x111, 0xF>(v);      // row_shr 1, 2, 4, 8
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);      // row_bcast 15 to rows 1 and 3
+    return dpp_add<0x143, 0xC>(v);   // row_bcast 31 to rows 2 and 3
+}
+__device__ __forceinline__ int sum_of(int v) { return __builtin_amdgcn_readlane(sums_up_to(v), 63); }
+
 constexpr int kFragBytes = 1024;   // one MFMA A-operand fragment: 64 lanes x 16 B
 // The running row max that the softmax exponentials refer to is allowed to lag the true one.  In the kernels with a score role
 // (attn_fwd_jvp_kernel, attn_qstream_kernel) it moves (and everything

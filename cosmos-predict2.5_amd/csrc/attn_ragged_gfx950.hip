@@ -101,11 +101,6 @@ template <int D, int N = kStep> __device__ __forceinline__ __amdgpu_buffer_rsrc_
     const int rows = rows_left < N ? rows_left : N;
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, rows > 0 ? (int)((rows - 1) * row_bytes) + 2 * D : 0, 0x00020000);
 }
-template <typename T> __device__ __forceinline__ unsigned round2(float a, float b) {
-    typedef T V2 __attribute__((ext_vector_type(2)));
-    const V2 two = {(T)a, (T)b};
-    return __builtin_bit_cast(unsigned, two);
-}
 // four elements of o, and what their rounding leaves off.  The backward's delta = dout . o is taken off every dP of a row, next to which it is large where a row's weight lies on few keys:
 // with o's 8 bits alone dq and dk of sharp softmaxes (scores of a deviation of 4, 1000 positions, bf16) are 3.6e-3 off, with 16 bits 2.5e-3; their own rounding is 1.7e-3.
 template <typename T> __device__ __forceinline__ float element(unsigned w, int i) {
@@ -176,17 +171,6 @@ __device__ __forceinline__ int apart(const int* cu, int base, int n_seq, int tot
     }
     return none >> lane & 1 ? -1 : r.length;
 }
-// sums over the wavefront's lanes up to each one (data-parallel-primitive moves: within rows of 16, then the rows' ends)
-template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
-__device__ __forceinline__ int sums_up_to(int v) {
-    v = dpp_add<0x111, 0xF>(v);      // row_shr 1, 2, 4, 8
-    v = dpp_add<0x112, 0xF>(v);
-    v = dpp_add<0x114, 0xF>(v);
-    v = dpp_add<0x118, 0xF>(v);
-    v = dpp_add<0x142, 0xA>(v);      // row_bcast 15 to rows 1 and 3
-    return dpp_add<0x143, 0xC>(v);   // row_bcast 31 to rows 2 and 3
-}
-__device__ __forceinline__ int sum_of(int v) { return __builtin_amdgcn_readlane(sums_up_to(v), 63); }
 
 // The tiles of a kernel: ROWS rows (or keys) of a sequence each, with `steps` of STEP keys (rows) that go by.  Rank 0 of a sequence's tiles is the longest one; the last rows
 // see the most keys, the first keys are seen by the most rows.
