@@ -206,7 +206,8 @@ template <bool KEYS, int ROWS, int STEP> struct Tiles {
 // Parts are written and read in fp32 and joined by a launch of its own, so they have `least` steps at least.  dk and dv, and where shares are large: parts of three fifths of a workgroup's
 // share of all steps, as 512 causal tiles are dealt out evenly only if the long ones are in pieces that short ones fit beside (gradients of 16384 positions, 16 heads on 4, us, parts of a
 // share / of 3/5 / of 2/5: 4558 / 3973 / 3890).  Else five quarters, which are all on the chip at once: a few more than fit take a second round (512 queries, 8 heads each, on 8192 keys: 704
-// parts 72, 520 75, 455 63).
+// parts 72, 520 75, 455 63).  On other sizes, us, this rule / five quarters throughout, forward and gradients: 3000 + 1700 + 1040 positions, 16 heads on 4, 109 / 95 and 311 / 285; 4096 108 / 105 and
+// 323 / 309; 1024 queries on 8192 keys, 16 heads on 2, 94 / 91 and 306 / 297; 512 on 32768, 8 heads on 1, 84 / 89 and 302 / 298; 8192, 8 heads on 2, 178 / 177 and 548 / 548.
 constexpr int kAtOnce = 2 * kNumCUs;      // workgroups
 constexpr int least_steps(int D) { return D == 128 ? 12 : 24; }
 constexpr int least_rows(int D) { return D == 128 ? 512 : 2048; }       // (of dk and dv, in rows)
@@ -360,8 +361,9 @@ constexpr float kLowest = -3.0e38f;      // a max that no score has moved yet: e
 
 // ---- forward.  A workgroup: kRows rows of one sequence and key head; a wavefront 32 of them, one a lane and its other half: S^T = K Q^T has the keys in registers, so that the softmax
 // needs one exchange between the halves, and P^T, rounded, is the next product's operand where it lies.  Two workgroups a compute unit (head dim 64: four), so that one's products and another's
-// exponentials go on beside each other.  16384 causal positions, 16 heads of 128 on 4: 980 us, 1.12 PFLOP/s; the matrix unit is busy 63 % of the time at 1.8 GHz,
-// the softmax's issue slots take the rest.  Short calls end with their longest tiles: 12 causal prompts of 1 to 2048 positions, 32 heads on 8, 123 us, 0.78 PFLOP/s, 84 % of the units busy.
+// exponentials go on beside each other.  16384 causal positions, 16 heads of 128 on 4: 950 to 1000 us, 1.1 to 1.15 PFLOP/s, the matrix unit busy 63 % of the time at 1.8 GHz: every product of
+// 32 x 32 x 16 has a fragment from LDS to itself, which a stream of such products alone runs at 1.09 to 1.15 PFLOP/s with.  Head dim 64: 8192 positions, 16 heads, 297 us, 0.92 PFLOP/s (causal 187,
+// 0.73).  Short calls end with their longest tiles: 12 causal prompts of 1 to 2048 positions, 32 heads on 8, 125 us, 0.77 PFLOP/s, 84 % of the units busy.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)

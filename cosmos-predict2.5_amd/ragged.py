@@ -226,7 +226,8 @@ def ragged_bwd(
     rest: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(dq, dk, dv)`` of :func:`ragged_fwd` for the gradient ``dout`` of o, from its o and lse, and its ``rest``: without it dq and dk of sharp softmaxes, and of rows that see
-    few keys, have o's rounding in them.  Rows of no sequence get zeros.  The same results every time (no atomics)."""
+    few keys, have o's rounding in them.  Rows of no sequence get zeros.  The same results every time (no atomics).  A call takes up to 400 MB of workspace from torch's allocator while it runs
+    (the forward up to 200), where tiles are few enough to be cut."""
     if rest is not None:
         _check_rest(rest, q)
     made = _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale, rest)

@@ -415,8 +415,9 @@ COSMOS_ATTN_API int cosmos_attn_gemm_preferred(const cosmos_attn_gemm_desc *desc
  *
  * cosmos_attn_ragged_bwd: dq, dk, dv for the gradient dout of o, from the forward's o and lse (and, where softmaxes are sharp or rows see few keys, better with its `rest`); rows of no
  * sequence become zeros.  No atomics: the same results every time.
- * The workspaces hold a number per row and head (backward) and the parts of tiles that are cut where there are few; the bytes follow from the sizes alone, and may be 0.  Outputs must not
- * overlap inputs or each other.
+ * The workspaces hold a number per row and head (backward) and the parts of tiles that are cut where there are few; the bytes follow from the sizes alone, and may be 0.  Parts have room for
+ * as many as sizes allow, of which a call writes those that its offsets make: up to 200 MB forward and 400 MB backward (D 128; half at 64), most where a call has somewhat fewer than 1536 tiles
+ * of 128 rows (tokens times group) or keys over all key heads, and none from there on.  Outputs must not overlap inputs or each other.
  */
 enum cosmos_attn_ragged_fill { COSMOS_ATTN_FILL_NONE = 0, COSMOS_ATTN_FILL_ALL = 1, COSMOS_ATTN_FILL_LSE = 2 };   /* (any other value: as ALL) */
 typedef struct cosmos_attn_ragged_desc {
