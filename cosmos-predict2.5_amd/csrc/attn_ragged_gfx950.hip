@@ -1027,8 +1027,9 @@ RaggedParams params_of(const cosmos_attn_ragged_desc* d) {
     p.rest = (char*)d->rest;
     p.cu_q = d->cu_q; p.cu_k = d->cu_k;
     p.q_row = 2 * d->q_stride[0]; p.q_head = 2 * d->q_stride[1];
-    p.k_row = 2 * d->k_stride[0]; p.k_head = 2 * d->k_stride[1];
-    p.v_row = 2 * d->v_stride[0]; p.v_head = 2 * d->v_stride[1];
+    // (one row may have any stride; those behind it, which are read as zeros, lie past its end)
+    p.k_row = 2 * (d->Tk > 1 ? d->k_stride[0] : d->D); p.k_head = 2 * d->k_stride[1];
+    p.v_row = 2 * (d->Tk > 1 ? d->v_stride[0] : d->D); p.v_head = 2 * d->v_stride[1];
     p.o_row = 2 * d->o_stride[0]; p.o_head = 2 * d->o_stride[1];
     p.do_row = 2 * d->dout_stride[0]; p.do_head = 2 * d->dout_stride[1];
     p.dq_row = 2 * d->dq_stride[0]; p.dq_head = 2 * d->dq_stride[1];

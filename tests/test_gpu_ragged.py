@@ -572,3 +572,19 @@ def test_fp16_gradients_of_weights_on_few_keys(pkg, gpu):
 def test_fp16_gradients_over_very_many_keys(pkg, gpu, keys, D):
     """P itself is below fp16's normal numbers."""
     check_norms(pkg, gpu, 32, keys, D, 2.0 ** 8)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_one_key_of_an_expanded_tensor(pkg, gpu, dtype, D):
+    """A row without a stride of its own, whose infinite values are infinite: the rows of a step behind it are zeros, not the same row again."""
+    q = rows(5, 4, D, dtype, gpu, 0)
+    v = torch.ones(1, 2, D, dtype=dtype, device=gpu)
+    v[:, :, 3] = math.inf
+    one = lambda x: x[0].as_strided((1, 2, D), (0, D, 1))
+    assert pkg.ragged.packed_ready(one(v)) and one(v).stride(0) == 0
+    k = rows(1, 2, D, dtype, gpu, 1)
+    on = (offsets([0, 5], gpu), offsets([0, 1], gpu))
+    o, _ = pkg.ragged_fwd(q, one(k), one(v), *on)
+    want, _ = pkg.ragged_fwd(q, k, v, *on)
+    assert torch.equal(o, want) and (o[:, :, 3] == math.inf).all() and (o[:, :, 4:] == 1).all()
