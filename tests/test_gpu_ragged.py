@@ -588,3 +588,39 @@ def test_one_key_of_an_expanded_tensor(pkg, gpu, dtype, D):
     o, _ = pkg.ragged_fwd(q, one(k), one(v), *on)
     want, _ = pkg.ragged_fwd(q, k, v, *on)
     assert torch.equal(o, want) and (o[:, :, 3] == math.inf).all() and (o[:, :, 4:] == 1).all()
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_offsets_at_random(pkg, ragged_oracle, gpu, seed):
+    """Any numbers as offsets, ascending for a while or not at all."""
+    r = torch.Generator().manual_seed(seed)
+    number = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=r))
+    n = (3, 9, 70, 140, 300)[seed % 5]
+
+    def some():
+        at, x = [], number(-3, 20)
+        for _ in range(n + 1):
+            x = number(-20, 330) if number(0, 8) == 0 else x + number(0, 400 // n + 2)
+            at.append(x)
+        return at
+    cu_q, cu_k = some(), some()
+    q, k, v, g = (rows(300, h, 64, BF16, gpu, i) for i, h in enumerate((4, 2, 2, 4)))
+    on = (offsets(cu_q, gpu), offsets(cu_k, gpu))
+    fill_free_memory(q, k, torch.empty(4, 300, device=gpu))
+    o, lse = pkg.ragged_fwd(q, k, v, *on, causal=True)
+    grads = pkg.ragged_bwd(q, k, v, o, lse, g, *on, causal=True)
+    O, O_tol, L, L_tol = torch.zeros(300, 4, 64, dtype=torch.float64), torch.zeros(300, 4, 64, dtype=torch.float64), torch.full((4, 300), -math.inf, dtype=torch.float64), torch.zeros(4, 300, dtype=torch.float64)
+    want, tols = [[torch.zeros(x.shape, dtype=torch.float64) for x in (q, k, v)] for _ in range(2)]
+    for (a, b), c in sequences(cu_q, cu_k, 300, 300)[0]:
+        if c is None:
+            O[a:b], L[:, a:b] = math.nan, math.nan
+            continue
+        part, at = (q[a:b], k[slice(*c)], v[slice(*c)]), ([0, b - a], [0, c[1] - c[0]])
+        O[a:b], L[:, a:b], O_tol[a:b], L_tol[:, a:b] = ragged_oracle.ragged_fwd(*part, *at, True, 0.125, BF16)
+        for i, (w, t) in enumerate(zip(*ragged_oracle.ragged_bwd(*part, g[a:b], *at, True, 0.125, BF16))):
+            x = slice(*((a, b) if i == 0 else c))
+            want[i][x], tols[i][x] = w, t
+    near(o, O, O_tol, "o")
+    near(lse, L, L_tol, "lse")
+    for name, x, w, t in zip(("dq", "dk", "dv"), grads, want, tols):
+        near(x, w, t, name)
