@@ -116,8 +116,9 @@ template <typename T> __device__ __forceinline__ void store_rounded(char* to, ch
     if (rest) *reinterpret_cast<u32x2*>(rest) = u32x2{round2<T>(a - element<T>(w[0], 0), b - element<T>(w[0], 1)), round2<T>(c - element<T>(w[1], 0), d - element<T>(w[1], 1))};
 }
 // dS in fp16.  P is about one over the number of keys and dP as large as dout, so that dS = P (dP - delta) leaves fp16's range downwards (2^-14) where dq and dk are well within it (4096 keys,
-// dout 1e-3: they would be 5e-3 off), and upwards (65504) where dout is scaled up and weights lie on few keys.  It is held as 2^up dS: from 2^kUp on down, whenever one is above kMostDs, to as
-// many bits as the largest so far leaves above 2^8, and what is summed up is scaled with it.  A row (dq) or a key (dk) has its own `up`.  bf16 has the range of fp32.
+// dout 1e-3: they would be 5e-3 off), and upwards (65504) where dout is scaled up and weights lie on few keys.  It is held as 2^up dS: `up` begins at kUp and
+// goes down whenever one is above kMostDs, so that the largest so far lies between 2^8 and 2^9; what is summed up is scaled with it.  A row (dq) or a key (dk) has its own.  bf16 has the range
+// of fp32.
 // (Gradients in fp16 take 3 % longer at head dim 128, 5 at 64: four documents of 7678 positions, 32 heads on 8, us, without / with 789 / 814; 8192 positions, 16 heads of 64, 570 / 598.)
 template <typename T> constexpr bool kNarrow = __is_same(T, _Float16);
 constexpr int kUp = 48;
@@ -158,18 +159,37 @@ __device__ __forceinline__ Range range_of(const int* cu, int i, int total) {
 }
 // the rows of sequence i, of which find() says how many there are
 __device__ __forceinline__ Range rows_of_sequence(const int* cu, int i, int length) { return {length < 0 ? 0 : cu[i], length}; }
-// Where some sequence of all up to here has offsets that do not ascend, others behind it may begin before `end`, the last end so far: of the 64 from `base` on, a lane's length, -1 where it has
-// none of its own.  (One after the other, as each depends on those before; empty ones hold nothing and are passed over, so that zeros behind the last offset cost little.)
-__device__ __forceinline__ int apart(const int* cu, int base, int n_seq, int total, int& end) {
+// Where offsets do not ascend throughout, a sequence may begin before the end of an earlier one.  Of the 64 from `base` on, in a lane each: the length, -1 where it has none of its own, and the
+// end of the last one in front of it; `end`: of the last one so far.  Empty ones hold nothing and are passed over.  If no start lies before an end in front of it, all of them are sequences
+// (500 prompts of 30 positions and 500 offsets of zero behind them, 32 heads of 128 on 8, forward and gradients 345 and 749 us, one
+// after the other 3085 and 6096; the last offset again instead of zeros, which ascends, 134 and 347); if not, one after the other, as each depends on those in front.
+struct Own { int start, length, before; };
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_most(int v) {
+    const int moved = __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);      // (0 where no lane is)
+    return v > moved ? v : moved;
+}
+__device__ __forceinline__ Own apart(const int* cu, int base, int n_seq, int total, int& end) {
     const int lane = threadIdx.x & 63;
     const Range r = base + lane < n_seq ? range_of(cu, base + lane, total) : Range{0, -1};
-    unsigned long long none = 0;
+    int most = r.length > 0 ? r.start + r.length : 0;      // of the ends up to this lane
+    most = dpp_most<0x111, 0xF>(most);
+    most = dpp_most<0x112, 0xF>(most);
+    most = dpp_most<0x114, 0xF>(most);
+    most = dpp_most<0x118, 0xF>(most);
+    most = dpp_most<0x142, 0xA>(most);
+    most = dpp_most<0x143, 0xC>(most);
+    const int front = __shfl_up(most, 1), last = __builtin_amdgcn_readlane(most, 63);
+    Own own = {r.start, r.length, lane && front > end ? front : end};
+    if (!__any(r.length > 0 && r.start < own.before)) {
+        end = last > end ? last : end;
+        return own;
+    }
     for (unsigned long long left = __ballot(r.length > 0); left; left &= left - 1) {
         const int at = __builtin_ctzll(left), a = __builtin_amdgcn_readlane(r.start, at);
-        if (a < end) none |= 1ull << at;
-        else end = a + __builtin_amdgcn_readlane(r.length, at);
+        if (lane == at) own = {a, a < end ? -1 : r.length, end};
+        if (a >= end) end = a + __builtin_amdgcn_readlane(r.length, at);
     }
-    return none >> lane & 1 ? -1 : r.length;
+    return own;
 }
 
 // The tiles of a kernel: ROWS rows (or keys) of a sequence each, with `steps` of STEP keys (rows) that go by.  Rank 0 of a sequence's tiles is the longest one; the last rows
@@ -303,7 +323,7 @@ template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Foun
         before = 0;
         all = 0;
         for (int base = 0; base < p.n_seq; base += 64)
-            if (look(base, {apart(p.cu_q, base, p.n_seq, p.Tq, end_q), apart(p.cu_k, base, p.n_seq, p.Tk, end_k)})) return f;
+            if (look(base, {apart(p.cu_q, base, p.n_seq, p.Tq, end_q).length, apart(p.cu_k, base, p.n_seq, p.Tk, end_k).length})) return f;
     }
     if (f.seq < 0) { f.tile = index - before; return f; }
     const int64_t share = (all * p.Hkv + kAtOnce - 1) / kAtOnce;
@@ -345,16 +365,15 @@ template <int D> __device__ __forceinline__ void clear_rows(char* out, int64_t r
         return;
     }
     // (between the sequences that there are as well)
-    int end = 0, done = 0;
-    for (int base = 0; base < n; base += 64) {
-        const int i = base + (threadIdx.x & 63), start = cu[i < n ? i : n], length = apart(cu, base, n, total, end);
-        for (unsigned long long left = __ballot(length > 0); left; left &= left - 1) {
-            const int at = __builtin_ctzll(left), a = __builtin_amdgcn_readlane(start, at);
-            clear(done, a);
-            done = a + __builtin_amdgcn_readlane(length, at);
+    int end = 0;
+    for (int base = 0; base < n && first > -rows; base += 64) {
+        const Own own = apart(cu, base, n, total, end);
+        for (unsigned long long left = __ballot(own.length > 0 && own.start > own.before); left; left &= left - 1) {
+            const int at = __builtin_ctzll(left);
+            clear(__builtin_amdgcn_readlane(own.before, at), __builtin_amdgcn_readlane(own.start, at));
         }
     }
-    clear(done, total);
+    if (first > -rows) clear(end, total);
 }
 
 constexpr float kLowest = -3.0e38f;      // a max that no score has moved yet: exponentials of masked scores stay 0 and those of the sums so far too

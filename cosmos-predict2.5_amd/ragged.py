@@ -184,7 +184,8 @@ def ragged_fwd(
 
     A row that sees no key: o = 0, lse = -inf.  Rows of no sequence (before ``cu_q[0]``, from the last offset on) become zeros, and -inf; in ``out``, a tensor that is given for o, they are
     left as they are (lse is -inf there too).  Offsets that do not ascend within the tensors, or a sequence that begins before an earlier one's end: a sequence of such ``cu_q`` is none (its rows are of no
-    sequence, unless another one has them), one of such ``cu_k`` has rows of NaN; the sequences before are as ever (zeros behind the last offset, say, are sequences without rows).  ``out``
+    sequence, unless another one has them), one of such ``cu_k`` has rows of NaN; the sequences before are as ever (zeros behind the last offset, say, are sequences without rows; the last offset
+    again is less to look through).  ``out``
     must not overlap the inputs.
     ``rest``, a contiguous tensor like q, takes what rounding o left off, for :func:`ragged_bwd` (rows of no sequence: left as they are).  No gradients:
     :func:`attention_ragged` has them."""
