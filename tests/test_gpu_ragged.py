@@ -624,3 +624,37 @@ def test_offsets_at_random(pkg, ragged_oracle, gpu, seed):
     near(lse, L, L_tol, "lse")
     for name, x, w, t in zip(("dq", "dk", "dv"), grads, want, tols):
         near(x, w, t, name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_a_captured_training_step(pkg, gpu, dtype):
+    """Forward and gradients through autograd in a graph: inputs, gradients and offsets change between replays."""
+    leaves = [rows(400, h, 64, dtype, gpu, i).requires_grad_() for i, h in enumerate((4, 2, 2))]
+    g, on = rows(400, 4, 64, dtype, gpu, 9), offsets([0, 100, 400], gpu)
+
+    def step():
+        o = pkg.attention_ragged(*leaves, on, causal=True)
+        return (o.detach(), *torch.autograd.grad(o, leaves, g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        made = step()
+    for i, at in enumerate(([0, 100, 400], [0, 399, 400], [0, 250, 0], [5, 100, 390])):
+        on.copy_(offsets(at, gpu))
+        g.copy_(rows(400, 4, 64, dtype, gpu, 20 + i, 2.0 ** (-4 * i)))
+        with torch.no_grad():
+            for x, h in zip(leaves, (4, 2, 2)):
+                x.copy_(rows(400, h, 64, dtype, gpu, 30 + 3 * i + h))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in made]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del want
