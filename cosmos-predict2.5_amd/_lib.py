@@ -329,6 +329,10 @@ EXPORTS = {
     "cosmos_attn_ragged": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "cosmos_attn_ragged_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p]),
     "cosmos_attn_ragged_bwd": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "cosmos_attn_ragged_window_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64]),
+    "cosmos_attn_ragged_window": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "cosmos_attn_ragged_window_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64]),
+    "cosmos_attn_ragged_window_bwd": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "cosmos_attn_cache_write": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "cosmos_attn_cache_read": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "cosmos_attn_cache_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p]),

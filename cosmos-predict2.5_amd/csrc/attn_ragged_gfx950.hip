@@ -30,360 +30,14 @@ namespace {
 
 #include "attn_common_gfx950.h"
 
-constexpr int kThreads = 256;      // four wavefronts of 32 rows (or keys) each
-constexpr int kRows = 128;         // of a workgroup
-constexpr int kStep = 64;          // keys (or rows) that are in LDS at a time, twice
-
-struct RaggedParams {
-    const char *q, *k, *v, *o_in, *dout;
-    char *o, *dq, *dk, *dv;
-    float* lse;                    // [Hq, Tq]; written by the forward (may be null), read by the backward
-    char* rest;                    // [Tq, Hq, D]: what rounding o left off, 16 bits again (may be null)
-    float* delta;                  // [Hq, Tq]: of the backward's first kernel for its second
-    const int *cu_q, *cu_k;
-    // bytes between rows and between heads
-    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
-    int n_seq, Tq, Tk, Hkv, group, causal, fill;
-    int tiles, most_parts, least;  // tiles that there may be, parts that one may be cut into, steps of a part
-    float* parts;                  // what they leave: of part s of tile i and key head h, at (i Hkv + h) most_parts + s
-    float scale, scale_log2;       // scale_log2 >= 0: `flip` says that q's signs are turned instead
-    unsigned flip;
-};
-
-// ---- a tile in LDS: N rows of D 16-bit elements, as chunks of 16 bytes.  Chunk c of row r lies at c XOR mix(r): what a wavefront reads at once, 16 bytes of each of 32 rows (a fragment
-// with lane = row) or, transposing, 64 bytes of each of 8 rows, then lies in different banks, and a load to LDS still takes whole rows.
-template <int D, int N = kStep> struct Tile {
-    static constexpr int ROW = 2 * D, BYTES = N * ROW, CHUNKS = D / 8, ROWS_PER_LOAD = 1024 / ROW, LOADS = N / 4 / ROWS_PER_LOAD;
-    static __device__ __forceinline__ int mix(int r) { return D == 128 ? 4 * (r & 3) | ((r >> 2) & 3) : 4 * ((r >> 1) & 1) | ((r >> 2) & 3); }
-    // where lane reads chunk 2 c + lane / 32 of row lane % 32
-    static __device__ __forceinline__ int at(int lane, int c) { return (lane & 31) * ROW + ((((2 * c) | (lane >> 5)) ^ mix(lane & 31)) << 4); }
-    // where lane passes the address for channels 32 db .. + 31, rows 4 (lane / 32) .. + 3 + 8 s, transposing
-    static __device__ __forceinline__ int at_transposed(int lane, int db, int s) {
-        const int row = 8 * s + 4 * (lane >> 5) + ((lane & 15) >> 2), chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-        return row * ROW + ((chunk ^ mix(row)) << 4) + 8 * (lane & 1);
-    }
-    // the row (of the tile) and the byte in that row that this lane loads with load i of wavefront `wave`
-    static __device__ __forceinline__ int load_row(int lane, int wave, int i) { return N / 4 * wave + i * ROWS_PER_LOAD + lane / CHUNKS; }
-    static __device__ __forceinline__ int load_byte(int lane, int wave, int i) { return ((lane % CHUNKS) ^ mix(load_row(lane, wave, i))) << 4; }
-    static __device__ __forceinline__ int load_to(int wave, int i) { return (N / 4 * wave + i * ROWS_PER_LOAD) * ROW; }
-};
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-// of a tile's part: its rows' max, sum of exponentials and D sums
-template <int D> constexpr int kPartFloats = kRows * (D + 2);
-
-__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, char* dst, int offset) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)dst, 16, offset, 0, 0, 0);
-}
-template <typename V8> __device__ __forceinline__ V8 read_rows(const char* part, int at) { return *reinterpret_cast<const V8*>(part + at); }
-// the 16 rows 16 c .. + 15 of 32 channels as an operand with lane = channel: slot s of a lane is row 16 c + 8 (s / 4) + 4 (lane / 32) + s % 4, the order of a product's result registers
-template <typename V8> __device__ __forceinline__ V8 read_channels(const char* part, int at0, int at1) {
-    typedef __attribute__((address_space(3))) s16x4* P;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(part + at0)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(part + at1));
-    return __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-// Two pairs of tiles, the one read while the other is loaded.  Arrays of their own: the compiler waits for loads to LDS in front of a read that may be of the same array.
-#define LDS_TILES(L) __shared__ __attribute__((aligned(1024))) char tile0[L::BYTES], tile1[L::BYTES], tile2[L::BYTES], tile3[L::BYTES]
-// all loads to LDS have landed and all reads have returned; then the workgroup meets.  (Through the builtin, which the compiler counts with: it then waits for nothing else in front of reads.)
-constexpr int kNothingUnderWay = 0x0070;      // vmcnt 0, lgkmcnt 0
-__device__ __forceinline__ void meet() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(kNothingUnderWay);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-// `rows_left` rows from `at` on (at most N are read), what lies behind them reads as zeros
-template <int D, int N = kStep> __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const char* at, int64_t row_bytes, int rows_left) {
-    const int rows = rows_left < N ? rows_left : N;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, rows > 0 ? (int)((rows - 1) * row_bytes) + 2 * D : 0, 0x00020000);
-}
-// four elements of o, and what their rounding leaves off.  The backward's delta = dout . o is taken off every dP of a row, next to which it is large where a row's weight lies on few keys:
-// with o's 8 bits alone dq and dk of sharp softmaxes (scores of a deviation of 4, 1000 positions, bf16) are 3.6e-3 off, with 16 bits 2.5e-3; their own rounding is 1.7e-3.
-template <typename T> __device__ __forceinline__ float element(unsigned w, int i) {
-    typedef T V2 __attribute__((ext_vector_type(2)));
-    return (float)__builtin_bit_cast(V2, w)[i];
-}
-template <typename T> __device__ __forceinline__ void store_rounded(char* to, char* rest, float a, float b, float c, float d) {
-    u32x2 w = {round2<T>(a, b), round2<T>(c, d)};
-    *reinterpret_cast<u32x2*>(to) = w;
-#if defined(__HIP_DEVICE_COMPILE__)
-    asm("" : "+v"(w));      // (what is stored: left to itself the compiler rounds a second time, a product of fp16 then in one step with the multiplication, which next to a tie goes elsewhere)
-#endif
-    if (rest) *reinterpret_cast<u32x2*>(rest) = u32x2{round2<T>(a - element<T>(w[0], 0), b - element<T>(w[0], 1)), round2<T>(c - element<T>(w[1], 0), d - element<T>(w[1], 1))};
-}
-// dS in fp16.  P is about one over the number of keys and dP as large as dout, so that dS = P (dP - delta) leaves fp16's range downwards (2^-14) where dq and dk are well within it (4096 keys,
-// dout 1e-3: they would be 5e-3 off), and upwards (65504) where dout is scaled up and weights lie on few keys.  It is held as 2^up dS: `up` begins at kUp and
-// goes down whenever one is above kMostDs, so that the largest so far lies between 2^8 and 2^9; what is summed up is scaled with it.  A row (dq) or a key (dk) has its own.  bf16 has the range
-// of fp32.
-// (Gradients in fp16 take 3 % longer at head dim 128, 5 at 64: four documents of 7678 positions, 32 heads on 8, us, without / with 789 / 814; 8192 positions, 16 heads of 64, 570 / 598.)
-template <typename T> constexpr bool kNarrow = __is_same(T, _Float16);
-constexpr int kUp = 48;
-// P as dv's operand, which is 1 at most and below 2^-14 from some 16 000 keys on, is 2^kUpP P throughout.
-constexpr int kUpP = 14;
-constexpr float kMostDs = 16384.f;
-__device__ __forceinline__ float largest(f32x16 s) {
-    float top = fabsf(s[0]);
-#pragma unroll
-    for (int e = 1; e < 16; ++e) top = fmaxf(top, fabsf(s[e]));
-    return top;
-}
-// how far down, in powers of two, for a largest one of `top`
-__device__ __forceinline__ int too_many(float top) { return top > kMostDs && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 9 : 0; }
-__device__ __forceinline__ float power_of_two(int n) { return __builtin_amdgcn_ldexpf(1.f, n); }
-// The order of a block's LDS reads and matrix products, READS to PRODUCTS: AHEAD reads first, then each product with its share of the others.  (Left alone the compiler reads the operands of two
-// products and waits for them: 2 % of the forward, and of the dK/dV kernel, where no more registers are free for it.)
-template <int READS, int PRODUCTS, int AHEAD> __device__ __forceinline__ void reads_ahead() {
-#if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int FIRST = AHEAD < READS ? AHEAD : READS, PER = READS / PRODUCTS, WITH = (READS - FIRST) / PER;
-    __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
-#pragma unroll
-    for (int i = 0; i < WITH; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - WITH, 0);
-#endif
-}
-__device__ __forceinline__ float over_halves_sum(float x) { float lo, hi; both_halves(x, lo, hi); return lo + hi; }
-__device__ __forceinline__ float over_halves_max(float x) { float lo, hi; both_halves(x, lo, hi); return fmaxf(lo, hi); }
-
-// ---- which sequence
-struct Range { int start, length; };
-__device__ __forceinline__ Range range_of(const int* cu, int i, int total) {
-    const int a = cu[i], b = cu[i + 1];
-    return a >= 0 && a <= b && b <= total ? Range{a, b - a} : Range{0, -1};
-}
-// the rows of sequence i, of which find() says how many there are
-__device__ __forceinline__ Range rows_of_sequence(const int* cu, int i, int length) { return {length < 0 ? 0 : cu[i], length}; }
-// Where offsets do not ascend throughout, a sequence may begin before the end of an earlier one.  Of the 64 from `base` on, in a lane each: the length, -1 where it has none of its own, and the
-// end of the last one in front of it; `end`: of the last one so far.  Empty ones hold nothing and are passed over.  If no start lies before an end in front of it, all of them are sequences
-// (500 prompts of 30 positions and 500 offsets of zero behind them, 32 heads of 128 on 8, forward and gradients 345 and 749 us, one
-// after the other 3085 and 6096; the last offset again instead of zeros, which ascends, 134 and 347); if not, one after the other, as each depends on those in front.
-struct Own { int start, length, before; };
-template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_most(int v) {
-    const int moved = __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);      // (0 where no lane is)
-    return v > moved ? v : moved;
-}
-__device__ __forceinline__ Own apart(const int* cu, int base, int n_seq, int total, int& end) {
-    const int lane = threadIdx.x & 63;
-    const Range r = base + lane < n_seq ? range_of(cu, base + lane, total) : Range{0, -1};
-    int most = r.length > 0 ? r.start + r.length : 0;      // of the ends up to this lane
-    most = dpp_most<0x111, 0xF>(most);
-    most = dpp_most<0x112, 0xF>(most);
-    most = dpp_most<0x114, 0xF>(most);
-    most = dpp_most<0x118, 0xF>(most);
-    most = dpp_most<0x142, 0xA>(most);
-    most = dpp_most<0x143, 0xC>(most);
-    const int front = __shfl_up(most, 1), last = __builtin_amdgcn_readlane(most, 63);
-    Own own = {r.start, r.length, lane && front > end ? front : end};
-    if (!__any(r.length > 0 && r.start < own.before)) {
-        end = last > end ? last : end;
-        return own;
-    }
-    for (unsigned long long left = __ballot(r.length > 0); left; left &= left - 1) {
-        const int at = __builtin_ctzll(left), a = __builtin_amdgcn_readlane(r.start, at);
-        if (lane == at) own = {a, a < end ? -1 : r.length, end};
-        if (a >= end) end = a + __builtin_amdgcn_readlane(r.length, at);
-    }
-    return own;
-}
-
-// The tiles of a kernel: ROWS rows (or keys) of a sequence each, with `steps` of STEP keys (rows) that go by.  Rank 0 of a sequence's tiles is the longest one; the last rows
-// see the most keys, the first keys are seen by the most rows.
-struct Lengths { int lq, lk; };      // lq < 0 or lk < 0: bad offsets
-template <bool KEYS, int ROWS, int STEP> struct Tiles {
-    const RaggedParams& p;
-    __device__ __forceinline__ Lengths lengths(int i) const { return {range_of(p.cu_q, i, p.Tq).length, range_of(p.cu_k, i, p.Tk).length}; }
-    __device__ __forceinline__ int count(Lengths n) const {
-        const int64_t rows = KEYS ? n.lk : (int64_t)n.lq * p.group;
-        return rows > 0 ? (int)((rows + ROWS - 1) / ROWS) : 0;
-    }
-    static __device__ __forceinline__ int at(int rank, int tiles) { return KEYS ? rank : tiles - 1 - rank; }
-    // first row that sees key j, in rows; (rounded up to steps where none does)
-    __device__ __forceinline__ int first_row(Lengths n, int j) const {
-        const int lq = n.lq > 0 ? n.lq : 0, t = j - (n.lk - lq);
-        return !p.causal || t <= 0 ? 0 : t >= lq ? (lq * p.group + STEP - 1) / STEP * STEP : t * p.group;
-    }
-    // keys that row r's token sees
-    __device__ __forceinline__ int keys(Lengths n, int r) const {
-        const int lk = n.lk > 0 ? n.lk : 0, e = r / p.group + lk - n.lq + 1;
-        return !p.causal || e > lk ? lk : e < 0 ? 0 : e;
-    }
-    __device__ __forceinline__ int first_step(Lengths n, int tile) const { return KEYS ? first_row(n, tile * ROWS) / STEP : 0; }
-    __device__ __forceinline__ int end_step(Lengths n, int tile) const {
-        if (KEYS) return n.lq > 0 ? (n.lq * p.group + STEP - 1) / STEP : 0;
-        const int rows = n.lq * p.group, last = tile * ROWS + ROWS - 1;
-        return (keys(n, last < rows ? last : rows - 1) + STEP - 1) / STEP;
-    }
-    __device__ __forceinline__ int steps(Lengths n, int tile) const { return end_step(n, tile) - first_step(n, tile); }
-    static constexpr bool OF_KEYS = KEYS;
-};
-
-// Parts are written and read in fp32 and joined by a launch of its own, so they have `least` steps at least.  dk and dv, and where shares are large: parts of three fifths of a workgroup's
-// share of all steps, as 512 causal tiles are dealt out evenly only if the long ones are in pieces that short ones fit beside (gradients of 16384 positions, 16 heads on 4, us, parts of a
-// share / of 3/5 / of 2/5: 4558 / 3973 / 3890).  Else five quarters, which are all on the chip at once: a few more than fit take a second round (512 queries, 8 heads each, on 8192 keys: 704
-// parts 72, 520 75, 455 63).  On other sizes, us, this rule / five quarters throughout, forward and gradients: 3000 + 1700 + 1040 positions, 16 heads on 4, 109 / 95 and 311 / 285; 4096 108 / 105 and
-// 323 / 309; 1024 queries on 8192 keys, 16 heads on 2, 94 / 91 and 306 / 297; 512 on 32768, 8 heads on 1, 84 / 89 and 302 / 298; 8192, 8 heads on 2, 178 / 177 and 548 / 548.
-constexpr int kAtOnce = 2 * kNumCUs;      // workgroups
-constexpr int least_steps(int D) { return D == 128 ? 12 : 24; }
-constexpr int least_rows(int D) { return D == 128 ? 512 : 2048; }       // (of dk and dv, in rows)
-typedef Tiles<false, kRows, kStep> RowTiles;
-// of dk and dv
-constexpr int row_step(int D) { return D == 128 ? 32 : 64; }
-template <int D> using KeyTiles = Tiles<true, kRows, row_step(D)>;
-struct Found { int seq, tile, parts; Lengths n; bool odd; };     // seq < 0: behind the last tile, `tile` of them; odd: offsets that do not ascend were among those looked at
-// Tile `index` of all sequences', in the sequences' order and the longest of each first, and how many parts it is cut into.
-// (The longest of all first, by counts of the tiles longer than some length, for which the length is searched: 5 % slower on 12 prompts and on four documents.  Short tiles, which are mostly
-// waiting, then run beside each other at the end instead of beside long ones.)
-// Few sequences each wavefront looks through for itself, 64 at a time; more of them the workgroup's THREADS together (1000 prompts of 30 positions, 32 heads of 128 on 8, us, forward / gradients,
-// together 238 / 565, each wavefront for itself 315 / 650; but 100 of them 24 / 101, and 24 / 93).
-constexpr int kFew = 128;
-template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Found find(const RaggedParams& p, int index) {
-    constexpr bool KEYS = Kind::OF_KEYS;
-    const Kind T{p};
-    const int lane = threadIdx.x & 63;
-    Found f = {-1, 0, 1, {0, 0}, false};
-    // (a sequence's: all of its tiles times the mean of the longest and the shortest; as many of them as are added up in 32 bits are no more than those hold)
-    auto share_of = [&](Lengths n, int tiles, int most) {
-        const int64_t sum = tiles ? (int64_t)tiles * (T.steps(n, T.at(0, tiles)) + T.steps(n, T.at(tiles - 1, tiles))) / 2 : 0;
-        return (int)(sum < most ? sum : most);
-    };
-    int before = 0;
-    int64_t all = 0;                 // steps
-    auto lengths = [&](int i) { return i < p.n_seq ? T.lengths(i) : Lengths{-1, -1}; };
-    auto is_odd = [&](int i, Lengths n) { return i < p.n_seq && (n.lq < 0 || n.lk < 0); };
-    // 64 sequences from `base` on; is that all there is to know?
-    auto look = [&](int base, Lengths n) __attribute__((always_inline)) {
-        const int tiles = T.count(n), sum = sums_up_to(tiles);
-        const unsigned long long past = __ballot(before + sum > index);
-        if (past && f.seq < 0) {
-            const int at = __builtin_ctzll(past), of = __builtin_amdgcn_readlane(tiles, at);
-            f.seq = base + at;
-            f.n = {__builtin_amdgcn_readlane(n.lq, at), __builtin_amdgcn_readlane(n.lk, at)};
-            f.tile = T.at(index - (before + __builtin_amdgcn_readlane(sum, at) - of), of);
-            if (p.most_parts <= 1) return true;
-        }
-        before += __builtin_amdgcn_readlane(sum, 63);
-        if (p.most_parts > 1) all += sum_of(share_of(n, tiles, (1 << 25) - 1));
-        return false;
-    };
-    if (p.n_seq <= kFew) {
-        for (int base = 0; base < p.n_seq; base += 64) {
-            const Lengths n = lengths(base + lane);
-            if (__any(is_odd(base + lane, n))) { f.odd = true; break; }
-            if (look(base, n)) return f;
-        }
-    } else {
-        constexpr int WAVES = THREADS / 64, ODD = 1 << 26;      // (more than there are tiles)
-        __shared__ int sums[2][WAVES];
-        __shared__ int64_t shares[WAVES];
-        __shared__ Found found;
-        const int wave = threadIdx.x >> 6;
-        for (int base = 0, turn = 0; base < p.n_seq; base += THREADS, turn ^= 1) {
-            const int mine = base + threadIdx.x;
-            const Lengths n = lengths(mine);
-            const int tiles = T.count(n), sum = sums_up_to(tiles);
-            const bool odd = __any(is_odd(mine, n));
-            if (lane == 63) sums[turn][wave] = odd ? ODD : sum;
-            if (p.most_parts > 1) all += sum_of(share_of(n, tiles, (1 << 25) - 1));
-            __syncthreads();
-            int at = before + sum - tiles, past = before;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                at += w < wave ? sums[turn][w] : 0;
-                past += sums[turn][w];
-            }
-            if (__builtin_amdgcn_readfirstlane(past) >= ODD) { f.odd = true; break; }
-            if (f.seq < 0 && index < past) {
-                if (index >= at && index < at + tiles) found = {mine, T.at(index - at, tiles), 1, n, false};
-                f.seq = 0;           // (it is in `found`)
-                if (p.most_parts <= 1) break;
-            }
-            before = past;
-        }
-        if (!f.odd) {
-            if (lane == 0) shares[wave] = all;
-            __syncthreads();
-            if (f.seq >= 0) {
-                f = {__builtin_amdgcn_readfirstlane(found.seq), __builtin_amdgcn_readfirstlane(found.tile), 1, {__builtin_amdgcn_readfirstlane(found.n.lq), __builtin_amdgcn_readfirstlane(found.n.lk)}, false};
-                if (p.most_parts <= 1) return f;
-                all = 0;
-#pragma unroll
-                for (int w = 0; w < WAVES; ++w) all += shares[w];
-            }
-        }
-    }
-    if (f.odd) {                     // once more from the start, each wavefront for itself
-        int end_q = 0, end_k = 0;
-        f.seq = -1;
-        before = 0;
-        all = 0;
-        for (int base = 0; base < p.n_seq; base += 64)
-            if (look(base, {apart(p.cu_q, base, p.n_seq, p.Tq, end_q).length, apart(p.cu_k, base, p.n_seq, p.Tk, end_k).length})) return f;
-    }
-    if (f.seq < 0) { f.tile = index - before; return f; }
-    const int64_t share = (all * p.Hkv + kAtOnce - 1) / kAtOnce;
-    const int steps = T.steps(f.n, f.tile);
-    const int64_t wish = KEYS || share >= 2 * p.least ? 3 * share / 5 : 5 * share / 4;
-    const int per = wish > p.least ? (int)wish : p.least, parts = (steps + per - 1) / per;
-    f.parts = __builtin_amdgcn_readfirstlane(parts < 1 ? 1 : parts < p.most_parts ? parts : p.most_parts);
-    return f;
-}
-// Of block `b`: the key head, the tile's place among all, the part.  Last parts first, which only long tiles have, and all tiles' first parts at the end, so that short tiles end the call.
-// Parts of one number lie together: a die hands workgroups to its four shader engines in turn, and parts that are
-// not there (their workgroups end at once) among the others leave some engines with nothing else: 37 us became 54 on 368 tiles of 25 steps.
-struct Block { int head, index, part; };
-__device__ __forceinline__ Block block_of(const RaggedParams& p, int b) {
-    const int rest = b / p.Hkv, before = p.most_parts > 1 ? rest / p.tiles : 0;
-    return {b - rest * p.Hkv, rest - before * p.tiles, p.most_parts - 1 - before};
-}
-
-// ---- rows of no sequence: zeros, lse = -inf.  They are counted through, whatever lies between them, and a workgroup behind the last tile has `rows` of them.
-template <int D> __device__ __forceinline__ void clear_rows(char* out, int64_t row, int64_t head, const int* cu, int n, int total, int heads, int first_head, int rows, Found f, float* lse) {
-    constexpr int CHUNKS = D / 8;
-    int64_t first = (int64_t)f.tile * rows;      // the workgroup's first one, counted from the next row to be cleared
-    auto clear = [&](int from, int to) {         // the tensor's rows from .. to - 1
-        const int64_t count = (int64_t)(to - from) * heads, lo = first < 0 ? 0 : first, hi = first + rows < count ? first + rows : count;
-        for (int i = threadIdx.x; i < (hi - lo) * CHUNKS; i += kThreads) {
-            const int64_t r = lo + i / CHUNKS;
-            const int t = from + (int)(r / heads), h = first_head + (int)(r % heads);
-            if (out) *reinterpret_cast<u32x4*>(out + t * row + h * head + 16 * (i % CHUNKS)) = u32x4{0, 0, 0, 0};
-            if (lse && i % CHUNKS == 0) lse[(int64_t)h * total + t] = -INFINITY;
-        }
-        first -= count;
-    };
-    if (!f.odd) {
-        int lead = cu[0], from = cu[n];
-        lead = lead < 0 ? 0 : lead > total ? total : lead;
-        from = from < lead ? lead : from > total ? total : from;
-        clear(0, lead);
-        clear(from, total);
-        return;
-    }
-    // (between the sequences that there are as well)
-    int end = 0;
-    for (int base = 0; base < n && first > -rows; base += 64) {
-        const Own own = apart(cu, base, n, total, end);
-        for (unsigned long long left = __ballot(own.length > 0 && own.start > own.before); left; left &= left - 1) {
-            const int at = __builtin_ctzll(left);
-            clear(__builtin_amdgcn_readlane(own.before, at), __builtin_amdgcn_readlane(own.start, at));
-        }
-    }
-    if (first > -rows) clear(end, total);
-}
-
-constexpr float kLowest = -3.0e38f;      // a max that no score has moved yet: exponentials of masked scores stay 0 and those of the sums so far too
+#include "attn_ragged_gfx950.h"
 
 // ---- forward.  A workgroup: kRows rows of one sequence and key head; a wavefront 32 of them, one a lane and its other half: S^T = K Q^T has the keys in registers, so that the softmax
 // needs one exchange between the halves, and P^T, rounded, is the next product's operand where it lies.  Two workgroups a compute unit (head dim 64: four), so that one's products and another's
 // exponentials go on beside each other.  16384 causal positions, 16 heads of 128 on 4: 950 to 1000 us, 1.1 to 1.15 PFLOP/s, the matrix unit busy 63 % of the time at 1.8 GHz: every product of
 // 32 x 32 x 16 has a fragment from LDS to itself, which a stream of such products alone runs at 1.09 to 1.15 PFLOP/s with.  Head dim 64: 8192 positions, 16 heads, 297 us, 0.92 PFLOP/s (causal 187,
 // 0.73).  Short calls end with their longest tiles: 12 causal prompts of 1 to 2048 positions, 32 heads on 8, 125 us, 0.77 PFLOP/s, 84 % of the units busy.
-template <typename T, int D>
+template <typename T, int D, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef typename VecOf<T>::v8 V8;
@@ -393,9 +47,10 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Block block = block_of(p, blockIdx.x);
     const int head = block.head;
-    const Found f = find<RowTiles>(p, block.index);
+    typedef RowTilesOf<WINDOW> Rows;
+    const Found f = find<Rows>(p, block.index);
     if (f.seq < 0) {
-        if (p.fill && block.part == 0) clear_rows<D>(p.fill == COSMOS_ATTN_FILL_LSE ? nullptr : p.o, p.o_row, p.o_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f, p.lse);
+        if (p.fill && block.part == 0) clear_rows<D>(p.fill == COSMOS_ATTN_FILL_LSE ? nullptr : p.o, p.o_row, p.o_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f, p.lse, p.lse_row, p.lse_head);
         return;
     }
     if (block.part >= f.parts) return;
@@ -406,13 +61,17 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
     const bool live = row < rows;
     const int token = row / p.group, hq = head * p.group + (row - token * p.group);
     // keys that this lane's row sees, the most of this wavefront's and of the workgroup's rows, the fewest of this wavefront's
-    auto keys_of = [&](int t) { const int e = t + shift + 1; return !p.causal || e > lk ? lk : e < 0 ? 0 : e; };
+    auto keys_of = [&](int t) { const int e = t + shift + 1; return (!WINDOW && !p.causal) || e > lk ? lk : e < 0 ? 0 : e; };
     const int end = live ? keys_of(token) : 0;
     const int first = tile * kRows + 32 * wave;
     auto token_at = [&](int r) { return __builtin_amdgcn_readfirstlane((r < rows ? r : rows - 1) / p.group); };
     const int wave_end = first < rows ? keys_of(token_at(first + 31)) : 0, wave_all = keys_of(token_at(first));
-    // steps of this part
-    const int steps = RowTiles{p}.end_step(f.n, tile);
+    // (WINDOW: the first key that this lane's row looks back on, the last and the first of those of this wavefront's)
+    const int from = WINDOW ? Rows{p}.first_key(f.n, row) : 0, wave_from = WINDOW ? __builtin_amdgcn_readfirstlane(Rows{p}.first_key(f.n, first + 31)) : 0,
+              wave_first = WINDOW ? __builtin_amdgcn_readfirstlane(Rows{p}.first_key(f.n, first)) : 0;
+    // steps of this part; of step u, where its keys begin
+    const int steps = Rows{p}.end_step(f.n, tile), sink_steps = Rows{p}.sink_steps(), gap = Rows{p}.gap(f.n, tile);
+    auto at_step = [&](int u) { return WINDOW && u >= sink_steps ? u + gap : u; };
     const int t0 = (int)((int64_t)block.part * steps / f.parts), n = (int)((int64_t)(block.part + 1) * steps / f.parts);
 
     const char* const kp = p.k + rk.start * p.k_row + head * p.k_head;
@@ -423,7 +82,8 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
         k_off[i] = L::load_row(lane, wave, i) * (int)p.k_row + L::load_byte(lane, wave, i);
         v_off[i] = L::load_row(lane, wave, i) * (int)p.v_row + L::load_byte(lane, wave, i);
     }
-    auto fill = [&](int t, char* kt, char* vt) __attribute__((always_inline)) {
+    auto fill = [&](int u, char* kt, char* vt) __attribute__((always_inline)) {
+        const int t = at_step(u);
         const auto kr = rows_of<D>(kp + (int64_t)t * kStep * p.k_row, p.k_row, lk - t * kStep), vr = rows_of<D>(vp + (int64_t)t * kStep * p.v_row, p.v_row, lk - t * kStep);
 #pragma unroll
         for (int i = 0; i < L::LOADS; ++i) load_to_lds(kr, kt + L::load_to(wave, i), k_off[i]);
@@ -455,9 +115,11 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
     float m = kLowest, l = 0.f;       // (l: of this lane's half of the keys)
 
-    auto step = [&](int t, const char* kt, const char* vt) __attribute__((always_inline)) {
-        const int key0 = t * kStep;
+    auto step = [&](int u, const char* kt, const char* vt) __attribute__((always_inline)) {
+        const int key0 = at_step(u) * kStep;
         if (key0 >= wave_end) return;
+        if (WINDOW && key0 >= p.sinks && key0 + kStep <= wave_first) return;
+        const bool behind = WINDOW && key0 < wave_from && key0 + kStep > p.sinks;      // (some row of the wavefront does not look back on all of these keys)
         f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
         for (int c = 0; c < NC; ++c)
@@ -470,6 +132,13 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[h][e] = 32 * h + 8 * (e >> 2) + (e & 3) < left ? s[h][e] : -INFINITY;
+        }
+        if (behind) {
+            const int out = from - key0 - 4 * half, in = p.sinks - key0 - 4 * half;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) { const int j = 32 * h + 8 * (e >> 2) + (e & 3); s[h][e] = j >= out || j < in ? s[h][e] : -INFINITY; }
         }
         float top = s[0][0];
 #pragma unroll
@@ -544,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
 
 // ---- backward, first kernel: delta and dq.  The forward's rows and tiles, with P from lse, dP^T = V dO^T beside S^T, and dQ^T = K^T dS^T.  Matrix unit busy 65 % at 1.7 GHz (8192 positions, 32
 // heads of 128 on 8): three products to an exponential, under the power limit.
-template <typename T, int D>
+template <typename T, int D, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef typename VecOf<T>::v8 V8;
@@ -554,7 +223,8 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Block block = block_of(p, blockIdx.x);
     const int head = block.head;
-    const Found f = find<RowTiles>(p, block.index);
+    typedef RowTilesOf<WINDOW> Rows;
+    const Found f = find<Rows>(p, block.index);
     if (f.seq < 0) {
         if (block.part == 0) clear_rows<D>(p.dq, p.dq_row, p.dq_head, p.cu_q, p.n_seq, p.Tq, p.group, head * p.group, kRows, f, nullptr);
         return;
@@ -566,13 +236,17 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
     const int row = tile * kRows + 32 * wave + (lane & 31);
     const bool live = row < rows;
     const int token = row / p.group, hq = head * p.group + (row - token * p.group);
-    auto keys_of = [&](int t) { const int e = t + shift + 1; return !p.causal || e > lk ? lk : e < 0 ? 0 : e; };
+    auto keys_of = [&](int t) { const int e = t + shift + 1; return (!WINDOW && !p.causal) || e > lk ? lk : e < 0 ? 0 : e; };
     const int end = live ? keys_of(token) : 0;
     const int first = tile * kRows + 32 * wave;
     auto token_at = [&](int r) { return __builtin_amdgcn_readfirstlane((r < rows ? r : rows - 1) / p.group); };
     const int wave_end = first < rows ? keys_of(token_at(first + 31)) : 0, wave_all = keys_of(token_at(first));
-    // steps of this part
-    const int steps = RowTiles{p}.end_step(f.n, tile);
+    // (WINDOW: the first key that this lane's row looks back on, the last and the first of those of this wavefront's)
+    const int from = WINDOW ? Rows{p}.first_key(f.n, row) : 0, wave_from = WINDOW ? __builtin_amdgcn_readfirstlane(Rows{p}.first_key(f.n, first + 31)) : 0,
+              wave_first = WINDOW ? __builtin_amdgcn_readfirstlane(Rows{p}.first_key(f.n, first)) : 0;
+    // steps of this part; of step u, where its keys begin
+    const int steps = Rows{p}.end_step(f.n, tile), sink_steps = Rows{p}.sink_steps(), gap = Rows{p}.gap(f.n, tile);
+    auto at_step = [&](int u) { return WINDOW && u >= sink_steps ? u + gap : u; };
     const int t0 = (int)((int64_t)block.part * steps / f.parts), n = (int)((int64_t)(block.part + 1) * steps / f.parts);
 
     const char* const kp = p.k + rk.start * p.k_row + head * p.k_head;
@@ -583,7 +257,8 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
         k_off[i] = L::load_row(lane, wave, i) * (int)p.k_row + L::load_byte(lane, wave, i);
         v_off[i] = L::load_row(lane, wave, i) * (int)p.v_row + L::load_byte(lane, wave, i);
     }
-    auto fill = [&](int t, char* kt, char* vt) __attribute__((always_inline)) {
+    auto fill = [&](int u, char* kt, char* vt) __attribute__((always_inline)) {
+        const int t = at_step(u);
         const auto kr = rows_of<D>(kp + (int64_t)t * kStep * p.k_row, p.k_row, lk - t * kStep), vr = rows_of<D>(vp + (int64_t)t * kStep * p.v_row, p.v_row, lk - t * kStep);
 #pragma unroll
         for (int i = 0; i < L::LOADS; ++i) load_to_lds(kr, kt + L::load_to(wave, i), k_off[i]);
@@ -635,9 +310,11 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
 
-    auto step = [&](int t, const char* kt, const char* vt) __attribute__((always_inline)) {
-        const int key0 = t * kStep;
+    auto step = [&](int u, const char* kt, const char* vt) __attribute__((always_inline)) {
+        const int key0 = at_step(u) * kStep;
         if (key0 >= wave_end) return;
+        if (WINDOW && key0 >= p.sinks && key0 + kStep <= wave_first) return;
+        const bool behind = WINDOW && key0 < wave_from && key0 + kStep > p.sinks;      // (some row of the wavefront does not look back on all of these keys)
         const bool masked = key0 + kStep > wave_all;
         const int left = end - key0 - 4 * half;
 #pragma unroll
@@ -657,6 +334,11 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
             if (masked)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = 32 * h + 8 * (e >> 2) + (e & 3) < left ? s[e] : 0.f;
+            if (behind) {
+                const int out = from - key0 - 4 * half, in = p.sinks - key0 - 4 * half;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) { const int j = 32 * h + 8 * (e >> 2) + (e & 3); s[e] = j >= out || j < in ? s[e] : 0.f; }
+            }
             if constexpr (kNarrow<T>) {
                 const float top = largest(s);
                 if (__any(top > kMostDs)) {
@@ -721,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
 // of K's and V's side, for which no more registers are free to be ahead (two wavefronts a SIMD have 256 each, all taken).  With dq 1.12 PFLOP/s of seven products.
 // (64 keys and half of a step's rows to a wavefront, one on a SIMD with all 512 registers, so that every fragment of Q and dO feeds two products: as fast on 8192 positions, 10 to 20 % slower on 512 to
 // 4096 and on prompts of mixed lengths, where a tile's start and end then have no other workgroup beside them.)
-template <typename T, int D>
+template <typename T, int D, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef typename VecOf<T>::v8 V8;
@@ -735,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Block block = block_of(p, blockIdx.x);
     const int head = block.head;
-    const Found f = find<KeyTiles<D>>(p, block.index);
+    const Found f = find<KeyTiles<D, WINDOW>>(p, block.index);
     if (f.seq < 0) {
         if (block.part) return;
         clear_rows<D>(p.dk, p.dk_row, p.dk_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f, nullptr);
@@ -747,8 +429,12 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     const int lq = rq.length > 0 ? rq.length : 0;
     const int key0 = f.tile * kRows, key = key0 + 32 * wave + (lane & 31);
     const bool live = key < rk.length;
-    const KeyTiles<D> tiles{p};
+    const KeyTiles<D, WINDOW> tiles{p};
     const int from = tiles.first_row(f.n, key);
+    // (WINDOW: one behind the last row that sees this lane's key; the most and the fewest of the wavefront's)
+    const int wave_key = key0 + 32 * wave, until = WINDOW ? tiles.end_row(f.n, key) : 0;
+    const int wave_until = WINDOW ? __builtin_amdgcn_readfirstlane(tiles.end_row(f.n, wave_key < p.sinks ? 0 : wave_key + 31)) : 0,
+              wave_least = WINDOW ? __builtin_amdgcn_readfirstlane(tiles.end_row(f.n, wave_key < p.sinks && p.sinks < wave_key + 32 ? p.sinks : wave_key)) : 0;
     const int wave_first = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave)), wave_all = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave + 31));
     // steps of this part
     const int begin = tiles.first_step(f.n, f.tile), steps = tiles.end_step(f.n, f.tile) - begin;
@@ -814,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
 
     auto step = [&](int t, const char* qt, const char* gt, const float* st) __attribute__((always_inline)) {
         const int row0 = t * STEP;
-        if (row0 + STEP <= wave_first) return;
+        if (row0 + STEP <= wave_first || (WINDOW && row0 >= wave_until)) return;
 #pragma unroll
         for (int h = 0; h < STEP / 32; ++h) {
             if constexpr (D == 128) SCHED_FENCE();      // (both halves at once need more registers than there are)
@@ -839,6 +525,11 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
                 const int left = from - row0 - 32 * h - 4 * half;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) >= left ? s[e] : 0.f;
+            }
+            if (WINDOW && row0 + STEP > wave_least) {
+                const int left = until - row0 - 32 * h - 4 * half;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) < left ? s[e] : 0.f;
             }
             V8 pf[2], df[2];
             g *= s;
@@ -924,65 +615,6 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
 #endif
 }
 
-// ---- the tiles that were cut: their parts added up, D / 4 lanes to a row.  WHICH: 0 o and lse, 1 dq, 2 dk and dv.  Memory and a launch: 512 + 77
-// + 1 queries of 16 heads, the long ones in some four parts each, 10 us; dk and dv of four causal documents, 7678 keys of 8 heads, 30 us.  (80 scalar registers: with 83 a unit holds one workgroup
-// of 16 wavefronts instead of two, 37 us.)
-constexpr int kJoinThreads = 1024;
-template <int D> constexpr int kJoinBlocks = kRows * (D / 4) / kJoinThreads;      // of a tile
-template <typename T, int D, int WHICH>
-__global__ void __launch_bounds__(kJoinThreads) __attribute__((amdgpu_num_sgpr(80))) ragged_join_kernel(const RaggedParams p) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    constexpr bool KEYS = WHICH == 2;
-    constexpr int LANES = D / 4, AT_ONCE = kJoinThreads / LANES;
-    const int head = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv % p.tiles;
-    const Found f = find<std::conditional_t<KEYS, KeyTiles<D>, RowTiles>, kJoinThreads>(p, index);
-    if (f.seq < 0 || f.parts <= 1) return;
-    const int c = 4 * (threadIdx.x % LANES);
-    const Range r = rows_of_sequence(KEYS ? p.cu_k : p.cu_q, f.seq, KEYS ? f.n.lk : f.n.lq);
-    const int rows = KEYS ? r.length : r.length * p.group;
-    const float* const from = p.parts + ((int64_t)index * p.Hkv + head) * p.most_parts * (WHICH == 0 ? kPartFloats<D> : WHICH * kRows * D);
-    auto store = [&](char* to, f32x4 x) { *reinterpret_cast<u32x2*>(to + 2 * c) = u32x2{round2<T>(x[0], x[1]), round2<T>(x[2], x[3])}; };
-    const int i = blockIdx.x / (p.Hkv * p.tiles) * AT_ONCE + threadIdx.x / LANES;
-    const int row = f.tile * kRows + i;
-    if (row >= rows) return;
-    const int token = KEYS ? row : row / p.group, h = KEYS ? head : head * p.group + (row - token * p.group);
-    if constexpr (WHICH == 0) {
-        const float* const at = from + i * (D + 2);
-        float m = kLowest, l = 0.f;
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int s = 0; s < f.parts; ++s) m = fmaxf(m, at[s * kPartFloats<D>]);
-#pragma unroll 4
-        for (int s = 0; s < f.parts; ++s) {
-            const float* const a = at + s * kPartFloats<D>;
-            const float by = __builtin_amdgcn_exp2f(a[0] - m);
-            const f32x2 lo = *reinterpret_cast<const f32x2*>(a + 2 + c), hi = *reinterpret_cast<const f32x2*>(a + 4 + c);
-            l += by * a[1];
-            sum += by * f32x4{lo[0], lo[1], hi[0], hi[1]};
-        }
-        const float by = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-        sum *= by;
-        char* const rest = p.rest ? p.rest + ((int64_t)(r.start + token) * p.group * p.Hkv + h) * (2 * D) + 2 * c : nullptr;
-        store_rounded<T>(p.o + (r.start + token) * p.o_row + h * p.o_head + 2 * c, rest, sum[0], sum[1], sum[2], sum[3]);
-        if (p.lse && c == 0) p.lse[(int64_t)h * p.Tq + r.start + token] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * 0.693147180559945309f : l == 0.f ? -INFINITY : l;
-    } else {
-        f32x4 sum[WHICH];
-#pragma unroll
-        for (int w = 0; w < WHICH; ++w) {
-            sum[w] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-            for (int s = 0; s < f.parts; ++s) sum[w] += *reinterpret_cast<const f32x4*>(from + (WHICH * s + w) * (kRows * D) + i * D + c);
-        }
-        if constexpr (WHICH == 1) {
-            store(p.dq + (r.start + token) * p.dq_row + h * p.dq_head, sum[0] * p.scale);
-        } else {
-            store(p.dk + (r.start + token) * p.dk_row + h * p.dk_head, sum[0] * p.scale);
-            store(p.dv + (r.start + token) * p.dv_row + h * p.dv_head, sum[1]);
-        }
-    }
-#endif
-}
-
 // ---- C ABI
 constexpr int64_t kMost = 0x7FFFFFFF, kMostBlocks = 0xFFFFFFFF / kThreads;
 // rows of a step and a token's heads are addressed with 32 bits
@@ -1054,6 +686,7 @@ RaggedParams params_of(const cosmos_attn_ragged_desc* d) {
     p.dq_row = 2 * d->dq_stride[0]; p.dq_head = 2 * d->dq_stride[1];
     p.dk_row = 2 * d->dk_stride[0]; p.dk_head = 2 * d->dk_stride[1];
     p.dv_row = 2 * d->dv_stride[0]; p.dv_head = 2 * d->dv_stride[1];
+    p.lse_row = 1; p.lse_head = d->Tq;
     p.n_seq = d->n_seq; p.Tq = (int)d->Tq; p.Tk = (int)d->Tk; p.Hkv = d->Hkv; p.group = d->Hq / d->Hkv;
     p.causal = d->causal != 0; p.fill = d->fill == COSMOS_ATTN_FILL_LSE && !d->lse ? 0 : d->fill;
     p.scale = d->sm_scale;
@@ -1084,69 +717,111 @@ int most_parts(int64_t tiles, int64_t longest, int least) {
     return parts > 1 ? (int)parts : 1;
 }
 struct Cut { int64_t tiles; int parts, least; size_t bytes; };
-Cut cut_of(const cosmos_attn_ragged_desc* d, int which) {
+// The window of a call, 0 keys where it hides none (sizes say so: a row's position is below Tk).
+struct Window { int window = 0, sinks = 0; };
+int check_window(const cosmos_attn_ragged_desc* d, int64_t window, int64_t sinks) {
+    if (window < 0 || sinks < 0) return COSMOS_ATTN_BAD_ARG;
+    return window && !d->causal ? COSMOS_ATTN_UNSUPPORTED : COSMOS_ATTN_OK;
+}
+Window window_of(const cosmos_attn_ragged_desc* d, int64_t window, int64_t sinks) {
+    return window && window < d->Tk && sinks < d->Tk ? Window{(int)window, (int)sinks} : Window{};
+}
+Cut cut_of(const cosmos_attn_ragged_desc* d, int which, Window w) {
     const int step = row_step(d->D);
     const int64_t group = d->Hq / d->Hkv, rows = d->Tq * group, tiles = which == 2 ? most_tiles(d->Tk, d->n_seq) : most_tiles(rows, d->n_seq);
-    const int64_t longest = which == 2 ? (rows + step - 1) / step : (d->Tk + kStep - 1) / kStep;
+    int64_t longest = which == 2 ? (rows + step - 1) / step : (d->Tk + kStep - 1) / kStep;
+    if (w.window && !(which == 2 && w.sinks)) {       // (the first keys' tiles are as long as ever)
+        const int64_t seen = which == 2 ? ((int64_t)w.window + kRows) * group / step + 2 : ((int64_t)w.window + kRows / group + 1) / kStep + 2 + (w.sinks + kStep - 1) / kStep;
+        longest = seen < longest ? seen : longest;
+    }
     const int least = which == 2 ? least_rows(d->D) / step : least_steps(d->D), parts = most_parts(tiles * d->Hkv, longest, least);
     return {tiles, parts, least, parts > 1 ? (size_t)tiles * d->Hkv * parts * kRows * (which == 0 ? d->D + 2 : which * d->D) * sizeof(float) : 0};
 }
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
-}  // namespace
-
-extern "C" {
-
-size_t cosmos_attn_ragged_workspace_bytes(const cosmos_attn_ragged_desc* desc) { return check(desc, false) == COSMOS_ATTN_OK ? cut_of(desc, 0).bytes : 0; }
-
-int cosmos_attn_ragged(const cosmos_attn_ragged_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
-    const int st = check(desc, false);
+size_t forward_bytes(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks) {
+    return check(desc, false) == COSMOS_ATTN_OK && check_window(desc, window, sinks) == COSMOS_ATTN_OK ? cut_of(desc, 0, window_of(desc, window, sinks)).bytes : 0;
+}
+int forward(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
+    int st = check(desc, false);
+    if (st == COSMOS_ATTN_OK) st = check_window(desc, window, sinks);
     if (st != COSMOS_ATTN_OK) return st;
     if (!desc->Tq) return COSMOS_ATTN_OK;
-    const Cut cut = cut_of(desc, 0);
+    const Window w = window_of(desc, window, sinks);
+    const Cut cut = cut_of(desc, 0, w);
     if (workspace_bytes < cut.bytes || (cut.bytes && !workspace)) return COSMOS_ATTN_WORKSPACE_TOO_SMALL;
     if (cut.bytes && !aligned16(workspace)) return COSMOS_ATTN_BAD_STRIDE;
     if (!device_is_whole_mi355x()) return COSMOS_ATTN_WRONG_DEVICE;
     RaggedParams p = params_of(desc);
     p.tiles = (int)cut.tiles; p.most_parts = cut.parts; p.least = cut.least;
+    p.window = w.window; p.sinks = w.sinks;
     p.parts = (float*)workspace;
     return with_type(desc->dtype, desc->D, [&](auto* t, auto d) {
         constexpr int D = decltype(d)::value;
         typedef std::remove_pointer_t<decltype(t)> T;
-        const int done = launch(ragged_fwd_kernel<T, D>, cut.tiles * p.Hkv * cut.parts, p, stream);
-        return done != COSMOS_ATTN_OK || cut.parts == 1 ? done : launch(ragged_join_kernel<T, D, 0>, cut.tiles * p.Hkv * kJoinBlocks<D>, p, stream, kJoinThreads);
+        auto run = [&](auto windowed) {
+            constexpr bool WINDOW = decltype(windowed)::value;
+            const int done = launch(ragged_fwd_kernel<T, D, WINDOW>, cut.tiles * p.Hkv * cut.parts, p, stream);
+            return done != COSMOS_ATTN_OK || cut.parts == 1 ? done : launch(ragged_join_kernel<T, D, 0, WINDOW>, cut.tiles * p.Hkv * kJoinBlocks<D>, p, stream, kJoinThreads);
+        };
+        return w.window ? run(Int<1>{}) : run(Int<0>{});
     });
 }
 
-size_t cosmos_attn_ragged_bwd_workspace_bytes(const cosmos_attn_ragged_desc* desc) {
-    if (check(desc, true) != COSMOS_ATTN_OK) return 0;
-    const size_t a = cut_of(desc, 1).bytes, b = cut_of(desc, 2).bytes;
+size_t backward_bytes(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks) {
+    if (check(desc, true) != COSMOS_ATTN_OK || check_window(desc, window, sinks) != COSMOS_ATTN_OK) return 0;
+    const Window w = window_of(desc, window, sinks);
+    const size_t a = cut_of(desc, 1, w).bytes, b = cut_of(desc, 2, w).bytes;
     return up((size_t)desc->Tq * desc->Hq * sizeof(float)) + (a > b ? a : b);
 }
-
-int cosmos_attn_ragged_bwd(const cosmos_attn_ragged_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
-    const int st = check(desc, true);
+int backward(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
+    int st = check(desc, true);
+    if (st == COSMOS_ATTN_OK) st = check_window(desc, window, sinks);
     if (st != COSMOS_ATTN_OK) return st;
-    const size_t wanted = cosmos_attn_ragged_bwd_workspace_bytes(desc);
+    const size_t wanted = backward_bytes(desc, window, sinks);
     if (workspace_bytes < wanted || (wanted && !workspace)) return COSMOS_ATTN_WORKSPACE_TOO_SMALL;
     if (wanted && !aligned16(workspace)) return COSMOS_ATTN_BAD_STRIDE;
     if (!device_is_whole_mi355x()) return COSMOS_ATTN_WRONG_DEVICE;
+    const Window w = window_of(desc, window, sinks);
     RaggedParams p = params_of(desc);
+    p.window = w.window; p.sinks = w.sinks;
     p.delta = (float*)workspace;
     p.parts = (float*)((char*)workspace + up((size_t)desc->Tq * desc->Hq * sizeof(float)));      // (of dq, then of dk and dv)
     return with_type(desc->dtype, desc->D, [&](auto* t, auto d) {
         constexpr int D = decltype(d)::value;
         typedef std::remove_pointer_t<decltype(t)> T;
         int done = COSMOS_ATTN_OK;
-        auto run = [&](const Cut& cut, auto kernel, auto join) {
+        auto one = [&](const Cut& cut, auto kernel, auto join) {
             p.tiles = (int)cut.tiles; p.most_parts = cut.parts; p.least = cut.least;
             if (done == COSMOS_ATTN_OK) done = launch(kernel, cut.tiles * p.Hkv * cut.parts, p, stream);
             if (done == COSMOS_ATTN_OK && cut.parts > 1) done = launch(join, cut.tiles * p.Hkv * kJoinBlocks<D>, p, stream, kJoinThreads);
         };
-        if (desc->Tq) run(cut_of(desc, 1), ragged_dq_kernel<T, D>, ragged_join_kernel<T, D, 1>);
-        if (desc->Tk) run(cut_of(desc, 2), ragged_dkdv_kernel<T, D>, ragged_join_kernel<T, D, 2>);
-        return done;
+        auto run = [&](auto windowed) {
+            constexpr bool WINDOW = decltype(windowed)::value;
+            if (desc->Tq) one(cut_of(desc, 1, w), ragged_dq_kernel<T, D, WINDOW>, ragged_join_kernel<T, D, 1, WINDOW>);
+            if (desc->Tk) one(cut_of(desc, 2, w), ragged_dkdv_kernel<T, D, WINDOW>, ragged_join_kernel<T, D, 2, WINDOW>);
+            return done;
+        };
+        return w.window ? run(Int<1>{}) : run(Int<0>{});
     });
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t cosmos_attn_ragged_workspace_bytes(const cosmos_attn_ragged_desc* desc) { return forward_bytes(desc, 0, 0); }
+int cosmos_attn_ragged(const cosmos_attn_ragged_desc* desc, void* workspace, size_t workspace_bytes, void* stream) { return forward(desc, 0, 0, workspace, workspace_bytes, stream); }
+size_t cosmos_attn_ragged_bwd_workspace_bytes(const cosmos_attn_ragged_desc* desc) { return backward_bytes(desc, 0, 0); }
+int cosmos_attn_ragged_bwd(const cosmos_attn_ragged_desc* desc, void* workspace, size_t workspace_bytes, void* stream) { return backward(desc, 0, 0, workspace, workspace_bytes, stream); }
+
+size_t cosmos_attn_ragged_window_workspace_bytes(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks) { return forward_bytes(desc, window, sinks); }
+int cosmos_attn_ragged_window(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
+    return forward(desc, window, sinks, workspace, workspace_bytes, stream);
+}
+size_t cosmos_attn_ragged_window_bwd_workspace_bytes(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks) { return backward_bytes(desc, window, sinks); }
+int cosmos_attn_ragged_window_bwd(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
+    return backward(desc, window, sinks, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

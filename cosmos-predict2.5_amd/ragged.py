@@ -2,13 +2,15 @@
 
 All sequences of a batch lie one behind the other, ``[rows, heads, D]``, and int32 offsets on the device say where each begins: no padding, no copy of the lengths to the host, and a captured
 call follows offsets that change between replays.  Each ``Hq / Hkv`` query heads in a row share a key head.  With ``causal`` the masks are aligned at the sequences' ends: the last query sees
-every key, so queries may be the last few of a prompt whose first keys come from elsewhere (``kv_cache.cache_read``).
+every key, so queries may be the last few of a prompt whose first keys come from elsewhere (``kv_cache.cache_read``).  With ``window`` a query looks back on that many keys, its own among them, and
+on the first ``sinks`` of its sequence; time goes by what is seen.
 
 The reference has no counterpart: its attention takes one length for the batch (cosmos_predict2/_src/predict2/networks/attention.py:90-181 ignores ``q_lens`` / ``k_lens``).
 """
 from __future__ import annotations
 
 import functools
+import operator
 import struct
 from typing import Optional, Tuple
 
@@ -73,6 +75,20 @@ def _check(q, k, v, cu_q, cu_k):
     return cu_q, cu_k
 
 
+def checked_window(window: Optional[int], sinks: int, causal: bool = True) -> Tuple[int, int]:
+    """``(window, sinks)`` as the library takes them, ``(0, 0)`` where none is asked for."""
+    sinks = operator.index(sinks)
+    assert sinks >= 0, "sinks counts first keys"
+    if window is None:
+        assert not sinks, "first keys that stay visible need a window that passes them"
+        return 0, 0
+    window = operator.index(window)
+    assert window >= 1, "window counts keys, a query's own among them (None: all)"
+    if not causal:
+        raise NotImplementedError("a window needs causal=True")
+    return min(window, 1 << 31), min(sinks, 1 << 31)
+
+
 def plain_int32(x: torch.Tensor, dims: int, device: int) -> bool:
     """Is it as :func:`int32_on` would give it?"""
     return x.dtype is torch.int32 and x.dim() == dims and x.get_device() == device and x.stride()[-1] == 1
@@ -89,15 +105,15 @@ def on_device(device: int, launch, desc: bytes, *rest) -> None:
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(backward: bool, n_seq: int, Hq: int, Hkv: int, D: int, Tq: int, Tk: int) -> int:
+def _workspace_bytes(backward: bool, n_seq: int, Hq: int, Hkv: int, D: int, Tq: int, Tk: int, window: int = 0, sinks: int = 0) -> int:
     """What the library asks for, which follows from sizes alone (addresses are never dereferenced)."""
-    desc = _RAGGED_DESC.pack(_lib.ABI_VERSION, _lib.DTYPE_BF16, n_seq, Hq, Hkv, D, 0, 0, Tq, Tk, 1.0, 0, *(16,) * 11, *(Hq * D, D, Hkv * D, D, Hkv * D, D, Hq * D, D), Hq * D, D, Hq * D, D,
+    desc = _RAGGED_DESC.pack(_lib.ABI_VERSION, _lib.DTYPE_BF16, n_seq, Hq, Hkv, D, 1, 0, Tq, Tk, 1.0, 0, *(16,) * 11, *(Hq * D, D, Hkv * D, D, Hkv * D, D, Hq * D, D), Hq * D, D, Hq * D, D,
                              Hkv * D, D, Hkv * D, D, 0)
     lib = _lib.load_library()
-    return (lib.cosmos_attn_ragged_bwd_workspace_bytes if backward else lib.cosmos_attn_ragged_workspace_bytes)(desc)
+    return (lib.cosmos_attn_ragged_window_bwd_workspace_bytes if backward else lib.cosmos_attn_ragged_window_workspace_bytes)(desc, window, sinks)
 
 
-def _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse, rest):
+def _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse, rest, window, sinks):
     """:func:`ragged_fwd` of tensors that can be taken as they are, all of it looked at once: None where something is to be converted, copied or refused.  A small call is as long as what the
     host does for it: one short prompt 11 us, 17 with the checks one by one."""
     if not (q.dim() == 3 == k.dim() and q.is_cuda):
@@ -117,13 +133,13 @@ def _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse, rest):
     lse = q.new_empty((Hq, Tq), dtype=torch.float32) if need_lse else None
     desc = _RAGGED_DESC.pack(_lib.ABI_VERSION, code, cu_q.shape[0] - 1, Hq, Hkv, D, 1 if causal else 0, 1, Tq, Tk, D ** -0.5 if sm_scale is None else sm_scale, 0, pq, pk, pv, cu_q.data_ptr(),
                              cu_k.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, q0, q1, k0, k1, v0, v1, Hq * D, D, 0, 0, 0, 0, 0, 0, 0, 0, 0 if rest is None else rest.data_ptr())
-    ws_bytes = _workspace_bytes(False, cu_q.shape[0] - 1, Hq, Hkv, D, Tq, Tk)
+    ws_bytes = _workspace_bytes(False, cu_q.shape[0] - 1, Hq, Hkv, D, Tq, Tk, window, sinks)
     workspace = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
-    on_device(device, _lib.load_library().cosmos_attn_ragged, desc, 0 if workspace is None else workspace.data_ptr(), ws_bytes)
+    on_device(device, _lib.load_library().cosmos_attn_ragged_window, desc, window, sinks, 0 if workspace is None else workspace.data_ptr(), ws_bytes)
     return o, lse
 
 
-def _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale, rest):
+def _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale, rest, window, sinks):
     """:func:`ragged_bwd`, as :func:`_fwd_as_it_is` (forward and gradients of 48 positions through autograd: 131 us, 138 with the checks one by one)."""
     if not (q.dim() == 3 == k.dim() and q.is_cuda and o.is_contiguous() and lse.is_contiguous()):
         return None
@@ -143,9 +159,9 @@ def _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale, rest):
     dq, dk, dv = (torch.empty(x, device=q.device, dtype=dtype) for x in (shape, kv, kv))
     desc = _RAGGED_DESC.pack(_lib.ABI_VERSION, code, cu_q.shape[0] - 1, Hq, Hkv, D, 1 if causal else 0, 1, Tq, Tk, D ** -0.5 if sm_scale is None else sm_scale, 0, pq, pk, pv, cu_q.data_ptr(),
                              cu_k.data_ptr(), po, lse.data_ptr(), pg, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), q0, q1, k0, k1, v0, v1, Hq * D, D, g0, g1, Hq * D, D, Hkv * D, D, Hkv * D, D, 0 if rest is None else rest.data_ptr())
-    ws_bytes = _workspace_bytes(True, cu_q.shape[0] - 1, Hq, Hkv, D, Tq, Tk)
+    ws_bytes = _workspace_bytes(True, cu_q.shape[0] - 1, Hq, Hkv, D, Tq, Tk, window, sinks)
     workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
-    on_device(device, _lib.load_library().cosmos_attn_ragged_bwd, desc, workspace.data_ptr(), ws_bytes)
+    on_device(device, _lib.load_library().cosmos_attn_ragged_window_bwd, desc, window, sinks, workspace.data_ptr(), ws_bytes)
     return dq, dk, dv
 
 
@@ -178,9 +194,12 @@ def ragged_fwd(
     need_lse: bool = True,
     out: Optional[torch.Tensor] = None,
     rest: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``(o, lse)``: ``q [Tq, Hq, D]``, ``k``, ``v`` ``[Tk, Hkv, D]``; sequence i has the rows ``cu_q[i] .. cu_q[i + 1] - 1`` of q and ``cu_k[i] ..`` of k and v
-    (``cu_k`` None: the same).  ``causal``: query t of Lq sees the keys up to ``t + Lk - Lq``.  ``lse``: fp32 ``[Hq, Tq]``.
+    (``cu_k`` None: the same).  ``causal``: query t of Lq sees the keys up to ``t + Lk - Lq``, with ``window`` (causal alone) the last ``window`` of these and those below ``sinks``.
+    ``lse``: fp32 ``[Hq, Tq]``.
 
     A row that sees no key: o = 0, lse = -inf.  Rows of no sequence (before ``cu_q[0]``, from the last offset on) become zeros, and -inf; in ``out``, a tensor that is given for o, they are
     left as they are (lse is -inf there too).  Offsets that do not ascend within the tensors, or a sequence that begins before an earlier one's end: a sequence of such ``cu_q`` is none (its rows are of no
@@ -189,10 +208,11 @@ def ragged_fwd(
     must not overlap the inputs.
     ``rest``, a contiguous tensor like q, takes what rounding o left off, for :func:`ragged_bwd` (rows of no sequence: left as they are).  No gradients:
     :func:`attention_ragged` has them."""
+    window, sinks = checked_window(window, sinks, causal)
     if rest is not None:
         _check_rest(rest, q)
     if out is None:
-        made = _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse, rest)
+        made = _fwd_as_it_is(q, k, v, cu_q, cu_k, causal, sm_scale, need_lse, rest, window, sinks)
         if made is not None:
             return made
     cu_q, cu_k = _check(q, k, v, cu_q, cu_k)
@@ -207,9 +227,9 @@ def ragged_fwd(
     lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32) if need_lse else None
     desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, _lib.FILL_ALL if out is None else _lib.FILL_LSE, rest)
     lib = _lib.load_library()
-    ws_bytes = lib.cosmos_attn_ragged_workspace_bytes(desc)
+    ws_bytes = lib.cosmos_attn_ragged_window_workspace_bytes(desc, window, sinks)
     workspace = torch.empty(ws_bytes, device=q.device, dtype=torch.uint8) if ws_bytes else None
-    on_device(q.get_device(), lib.cosmos_attn_ragged, desc, 0 if workspace is None else workspace.data_ptr(), ws_bytes)
+    on_device(q.get_device(), lib.cosmos_attn_ragged_window, desc, window, sinks, 0 if workspace is None else workspace.data_ptr(), ws_bytes)
     return o, lse
 
 
@@ -225,13 +245,16 @@ def ragged_bwd(
     causal: bool = False,
     sm_scale: Optional[float] = None,
     rest: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """``(dq, dk, dv)`` of :func:`ragged_fwd` for the gradient ``dout`` of o, from its o and lse, and its ``rest``: without it dq and dk of sharp softmaxes, and of rows that see
+    """``(dq, dk, dv)`` of :func:`ragged_fwd` (of the same ``causal``, ``sm_scale``, ``window`` and ``sinks``) for the gradient ``dout`` of o, from its o and lse, and its ``rest``: without it dq and dk of sharp softmaxes, and of rows that see
     few keys, have o's rounding in them.  Rows of no sequence get zeros.  The same results every time (no atomics).  A call takes up to 400 MB of workspace from torch's allocator while it runs
     (the forward up to 200), where tiles are few enough to be cut."""
+    window, sinks = checked_window(window, sinks, causal)
     if rest is not None:
         _check_rest(rest, q)
-    made = _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale, rest)
+    made = _bwd_as_it_is(q, k, v, o, lse, dout, cu_q, cu_k, causal, sm_scale, rest, window, sinks)
     if made is not None:
         return made
     cu_q, cu_k = _check(q, k, v, cu_q, cu_k)
@@ -242,32 +265,33 @@ def ragged_bwd(
     dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
     desc = _desc(q, k, v, o, lse, cu_q, cu_k, causal, sm_scale, _lib.FILL_ALL, rest, dout, dq, dk, dv)
     lib = _lib.load_library()
-    ws_bytes = lib.cosmos_attn_ragged_bwd_workspace_bytes(desc)
+    ws_bytes = lib.cosmos_attn_ragged_window_bwd_workspace_bytes(desc, window, sinks)
     workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
-    on_device(q.get_device(), lib.cosmos_attn_ragged_bwd, desc, workspace.data_ptr(), ws_bytes)
+    on_device(q.get_device(), lib.cosmos_attn_ragged_window_bwd, desc, window, sinks, workspace.data_ptr(), ws_bytes)
     return dq, dk, dv
 
 
 class _RaggedFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, cu_q, cu_k, causal, softmax_scale):
+    def forward(ctx, q, k, v, cu_q, cu_k, causal, softmax_scale, window, sinks):
         rest = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        o, lse = ragged_fwd(q, k, v, cu_q, cu_k, causal=causal, sm_scale=softmax_scale, rest=rest)
+        o, lse = ragged_fwd(q, k, v, cu_q, cu_k, causal=causal, sm_scale=softmax_scale, rest=rest, window=window, sinks=sinks)
         ctx.save_for_backward(q, k, v, o, lse, rest, cu_q, cu_k)
-        ctx.causal, ctx.softmax_scale = causal, softmax_scale
+        ctx.causal, ctx.softmax_scale, ctx.window, ctx.sinks = causal, softmax_scale, window, sinks
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, o, lse, rest, cu_q, cu_k = ctx.saved_tensors
-        return (*ragged_bwd(q, k, v, o, lse, dout, cu_q, cu_k, causal=ctx.causal, sm_scale=ctx.softmax_scale, rest=rest), None, None, None, None)
+        grads = ragged_bwd(q, k, v, o, lse, dout, cu_q, cu_k, causal=ctx.causal, sm_scale=ctx.softmax_scale, rest=rest, window=ctx.window, sinks=ctx.sinks)
+        return (*grads, None, None, None, None, None, None)
 
 
-def attention_ragged(q, k, v, cu_q, cu_k=None, softmax_scale=None, causal=False):
+def attention_ragged(q, k, v, cu_q, cu_k=None, softmax_scale=None, causal=False, window=None, sinks=0):
     """Differentiable attention over packed sequences: o of :func:`ragged_fwd`, gradients by :func:`ragged_bwd`.  The offsets must not change between the two.  No tangents: forward-mode
     differentiation is refused."""
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or forward_ad._current_level >= 0:
         cu_q = int32_on(cu_q, q.device)
-        return _RaggedFn.apply(q, k, v, cu_q, cu_q if cu_k is None else int32_on(cu_k, q.device), causal, softmax_scale)
-    return ragged_fwd(q, k, v, cu_q, cu_k, causal=causal, sm_scale=softmax_scale, need_lse=False)[0]
+        return _RaggedFn.apply(q, k, v, cu_q, cu_q if cu_k is None else int32_on(cu_k, q.device), causal, softmax_scale, window, sinks)
+    return ragged_fwd(q, k, v, cu_q, cu_k, causal=causal, sm_scale=softmax_scale, need_lse=False, window=window, sinks=sinks)[0]

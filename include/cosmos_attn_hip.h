@@ -444,6 +444,15 @@ COSMOS_ATTN_API size_t cosmos_attn_ragged_bwd_workspace_bytes(const cosmos_attn_
 COSMOS_ATTN_API int cosmos_attn_ragged_bwd(const cosmos_attn_ragged_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
+ * The same where a query looks back on a window of keys and on the first ones: the row at position p = t + Lk - Lq of its sequence's keys sees key j if j <= p and (j > p - window or j < sinks).
+ * window 0: all keys (sinks says nothing then).  A window needs `causal`.  Time and workspace go by what is seen; the backward takes the window of its forward.
+ */
+COSMOS_ATTN_API size_t cosmos_attn_ragged_window_workspace_bytes(const cosmos_attn_ragged_desc *desc, int64_t window, int64_t sinks);
+COSMOS_ATTN_API int cosmos_attn_ragged_window(const cosmos_attn_ragged_desc *desc, int64_t window, int64_t sinks, void *workspace, size_t workspace_bytes, void *stream);
+COSMOS_ATTN_API size_t cosmos_attn_ragged_window_bwd_workspace_bytes(const cosmos_attn_ragged_desc *desc, int64_t window, int64_t sinks);
+COSMOS_ATTN_API int cosmos_attn_ragged_window_bwd(const cosmos_attn_ragged_desc *desc, int64_t window, int64_t sinks, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * A paged key-value cache (no counterpart in the reference).  k and v: pages of page_size rows of D elements for each of Hkv heads, [pages, Hkv, page_size, D] through (page, head, row)
  * element strides, of the 16-bit type `dtype` or of 8 bits with an fp32 scale for each row, [pages, Hkv, page_size] through (page, head) strides:
  *     scale = max |x| * fp32(1 / 448) (e4m3) or * fp32(1 / 127) (int8), code = round(x / scale), all in fp32;  a row with a value that is not finite has the scale NaN

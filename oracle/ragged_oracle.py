@@ -19,8 +19,10 @@ def _u(dtype):
     return torch.finfo(dtype).eps / 2, (2.0 ** -25 if dtype == torch.float16 else 0.0)
 
 
-def visible(lq, lk, causal):
+def visible(lq, lk, causal, window=None, sinks=0):
     t, j = torch.arange(lq)[:, None], torch.arange(lk)[None]
+    if window is not None:
+        return (j <= t + lk - lq) & ((j > t + lk - lq - window) | (j < sinks))
     return (j <= t + lk - lq) if causal else torch.ones(lq, lk, dtype=torch.bool)
 
 
@@ -36,7 +38,7 @@ def attend(q, k, v, mask, scale):
     return P @ v, lse, P, s, off
 
 
-def ragged_fwd(q, k, v, cu_q, cu_k, causal, scale, dtype, rest=False):
+def ragged_fwd(q, k, v, cu_q, cu_k, causal, scale, dtype, rest=False, window=None, sinks=0):
     """(o, lse, bound of o, bound of lse); rows of no sequence: zeros, -inf.  `rest`: o as the sum of its rounding and what that left off, rounded too."""
     q, k, v = (x.double().cpu() for x in (q, k, v))
     Tq, Hq, D = q.shape
@@ -45,7 +47,7 @@ def ragged_fwd(q, k, v, cu_q, cu_k, causal, scale, dtype, rest=False):
     o_tol, lse_tol = torch.zeros_like(q), torch.zeros_like(lse)
     u, tiny = _u(dtype)
     for a, b, c, d in zip(cu_q[:-1], cu_q[1:], cu_k[:-1], cu_k[1:]):
-        mask = visible(b - a, d - c, causal)
+        mask = visible(b - a, d - c, causal, window, sinks)
         for h in range(Hq):
             K, V = k[c:d, h // group], v[c:d, h // group]
             o[a:b, h], lse[h, a:b], P, _, off = attend(q[a:b, h], K, V, mask, scale)
@@ -55,16 +57,16 @@ def ragged_fwd(q, k, v, cu_q, cu_k, causal, scale, dtype, rest=False):
     return o, lse, o_tol, lse_tol
 
 
-def ragged_bwd(q, k, v, dout, cu_q, cu_k, causal, scale, dtype, rest=False):
+def ragged_bwd(q, k, v, dout, cu_q, cu_k, causal, scale, dtype, rest=False, window=None, sinks=0):
     """((dq, dk, dv), (their bounds)) of the forward's o, whose 16-bit rounding the row sums do . o have (`rest`: that of its rounding and the rest)."""
     q, k, v, g = (x.double().cpu() for x in (q, k, v, dout))
     Hq, D = q.shape[1:]
     group = Hq // k.shape[1]
     grads, tols = [torch.zeros_like(x) for x in (q, k, v)], [torch.zeros_like(x) for x in (q, k, v)]
     u, tiny = _u(dtype)
-    o_tol = ragged_fwd(q, k, v, cu_q, cu_k, causal, scale, dtype, rest)[2]
+    o_tol = ragged_fwd(q, k, v, cu_q, cu_k, causal, scale, dtype, rest, window, sinks)[2]
     for a, b, c, d in zip(cu_q[:-1], cu_q[1:], cu_k[:-1], cu_k[1:]):
-        mask = visible(b - a, d - c, causal)
+        mask = visible(b - a, d - c, causal, window, sinks)
         for h in range(Hq):
             Q, G, K, V = q[a:b, h], g[a:b, h], k[c:d, h // group], v[c:d, h // group]
             o, lse, P, s, off = attend(Q, K, V, mask, scale)
