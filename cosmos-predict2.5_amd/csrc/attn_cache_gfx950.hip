@@ -1,13 +1,5 @@
 // A paged key-value cache for gfx950: writing it, reading it back, and attention of one new token of each sequence over it: kernels and C ABI (cosmos_attn_cache_write,
 // cosmos_attn_cache_read, cosmos_attn_cache_attention).
-//
-// Position j of sequence i lies in page table[i][j / page_size], place j % page_size.  Pages hold, for each head, page_size rows of D elements of the 16-bit type, or of 8 bits with one fp32
-// scale for each row of a head:
-//     scale = max |x| r,  r = fp32(1 / 448) (e4m3) or fp32(1 / 127) (int8),   code = round(x / scale) (nearest, ties to even),   x' = code scale
-// in fp32, the quotient an IEEE division: values of 8 bits of mantissa often lie on a border between two codes, and these are then the same ones everywhere.  A row with a value that
-// is not finite has the scale NaN.
-//
-// What the host's tables say is not trusted: a page outside of the cache or a length that the table does not hold makes the sequence's output NaN (attention, reading back) or writes nothing.
 #include <hip/hip_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -23,94 +15,8 @@ namespace {
 
 #include "attn_common_gfx950.h"
 
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-
 constexpr int kThreads = 256;
-enum Kind { SAME16 = COSMOS_ATTN_CACHE_SAME, E4M3 = COSMOS_ATTN_CACHE_E4M3, INT8 = COSMOS_ATTN_CACHE_INT8 };
-
-// keys, or values
-struct Side {
-    char* pages;                                  // bytes between pages, heads and rows
-    int64_t page, head, row;
-    float* scales;                                // elements between pages and heads
-    int64_t scale_page, scale_head;
-    char* packed;                                 // rows outside of the cache: bytes between rows and heads
-    int64_t packed_row, packed_head;
-};
-struct CacheParams {
-    Side side[2];                                 // keys, values
-    const int *table, *lens, *cu;
-    int64_t table_row;
-    int width, B, pages, page_shift, Hkv, fill;
-    int64_t rows;                                 // packed rows
-    // attention
-    const char* q;
-    char* o;
-    float* lse;
-    int64_t q_row, q_head, o_row, o_head;
-    int group, row_blocks, slots, whole;          // slots: workgroups for the shares, per head and block of rows; whole: a workgroup has all of a sequence
-    float scale_log2;
-    unsigned flip;
-    float* parts;
-    int* share;                                   // behind the parts: a share, and the most that a part has
-};
-
-// ---- 16-bit pairs
-template <typename T> __device__ __forceinline__ float low(unsigned w) {
-    if constexpr (__is_same(T, __bf16)) return __builtin_bit_cast(float, w << 16);
-    else return (float)__builtin_bit_cast(_Float16, (uint16_t)w);
-}
-template <typename T> __device__ __forceinline__ float high(unsigned w) {
-    if constexpr (__is_same(T, __bf16)) return __builtin_bit_cast(float, w & 0xFFFF0000u);
-    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16));
-}
-// elements 2 H and 2 H + 1 of four 8-bit codes as a pair of T (both types hold every code exactly)
-template <typename T, int KIND, bool H> __device__ __forceinline__ unsigned code_pair(unsigned w) {
-    if constexpr (KIND == E4M3) {
-        if constexpr (__is_same(T, __bf16)) return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, H));
-        else return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, H));
-    } else {
-        const int a = (int)(w << (H ? 8 : 24)) >> 24, b = (int)(w << (H ? 0 : 16)) >> 24;
-        return round2<T>((float)a, (float)b);
-    }
-}
-
-// max over the LANES (4 or 8) neighbouring lanes of a row
-template <int CTRL> __device__ __forceinline__ unsigned dpp_max(unsigned v) {
-    const unsigned moved = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
-    return v > moved ? v : moved;
-}
-template <int LANES> __device__ __forceinline__ unsigned row_max(unsigned v) {
-    v = dpp_max<0xB1>(v);       // quad_perm [1, 0, 3, 2]
-    v = dpp_max<0x4E>(v);       // quad_perm [2, 3, 0, 1]
-    return LANES == 8 ? dpp_max<0x141>(v) : v;      // row_half_mirror
-}
-
-// ---- packed rows: which sequence a row is of, and its place there
-// the last offset of lo .. hi at or below the row (or lo)
-__device__ __forceinline__ int last_below(const int* cu, int lo, int hi, int64_t row) {
-    while (lo < hi) {
-        const int mid = (int)(((unsigned)lo + (unsigned)hi + 1) >> 1);
-        if (cu[mid] <= row) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
-struct Place {
-    int seq, start, end, len;     // its offsets; keys in the cache (writing)
-    __device__ __forceinline__ Place(const CacheParams& p, int at, bool lens) : seq(at), start(0), end(0), len(0) {
-        if (!p.cu) {              // one row to a sequence
-            start = at;
-            end = at + 1;
-        } else {
-            start = p.cu[at];
-            end = at < p.B ? p.cu[at + 1] : start;
-        }
-        if (lens && at < p.B) len = p.lens[at];
-    }
-    __device__ __forceinline__ bool has(const CacheParams& p, int row) const { return seq < p.B && start >= 0 && row >= start && row < end && end <= p.rows; }
-};
+#include "attn_cache_gfx950.h"
 
 // Both kernels: a lane has EACH elements of a row of a head, 8 where pages hold 16 bits and 16 where they hold codes: 16 bytes of the narrower side.  A workgroup has kThreads EACH / D rows,
 // in the packed rows' order, of the keys or of the values (even and odd workgroups), so that their addresses are the scalar unit's to form, and so is the place of the first row's sequence,
@@ -142,23 +48,6 @@ template <int D, int EACH> struct Rows {
     __device__ __forceinline__ char* packed() const { return side.packed + row0 * side.packed_row + row * side.packed_row + head * side.packed_head + 2 * EACH * (threadIdx.x % LANES); }
     __device__ __forceinline__ char* cached(int page, int key) const { return side.pages + page * side.page + head * side.head + key * side.row + 16 * (threadIdx.x % LANES); }
     __device__ __forceinline__ float* scale(int page, int key) const { return side.scales + page * side.scale_page + head * side.scale_head + key; }
-};
-
-// x / s as IEEE division rounds it, for |x / s| up to some hundreds: x r corrected by the remainder, which fma gives exactly (Markstein's division), with r = 1 / s good to an ulp.  (That one
-// correction is enough has been seen for all there is: a 16-bit x has 2^7 or 2^10 significands and s, which follows from another one, as many.)  Rows whose scale would leave the range
-// in which all of that is exact are multiplied with a power of two first, as their scale is.
-struct Divide {
-    float s, r, by;
-    __device__ __forceinline__ explicit Divide(float scale) {
-        by = scale < 0x1p-60f ? 0x1p64f : 1.f;
-        s = scale * by;
-        r = __builtin_amdgcn_rcpf(s);
-        r = __builtin_fmaf(__builtin_fmaf(-s, r, 1.f), r, r);
-    }
-    __device__ __forceinline__ float operator()(float x) const {
-        const float q = x * r;
-        return __builtin_fmaf(__builtin_fmaf(-s, q, x), r, q);
-    }
 };
 
 // ---- writing
@@ -204,24 +93,8 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const CacheParams
 #pragma unroll
         for (int j = 0; j < 16; ++j) f[j] = over(f[j]);
         u32x4 codes = {0, 0, 0, 0};
-        if constexpr (KIND == E4M3) {
-            // (scale's own rounding may leave a quotient just above 448; the conversion's largest code takes those below 464)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j], f[4 * j + 1], 0, false);
-                codes[j] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j + 2], f[4 * j + 3], w, true);
-            }
-        } else {
-            // 2^23 + 2^22 + f: f rounded to a whole number, ties to even, in the low bits
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                unsigned w[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) w[k] = __builtin_bit_cast(unsigned, f[4 * j + k] + 12582912.f);
-                const unsigned lo = __builtin_amdgcn_perm(w[1], w[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(w[3], w[2], 0x04000C0Cu);
-                codes[j] = lo | hi;
-            }
-        }
+        for (int j = 0; j < 4; ++j) codes[j] = code_word<KIND>(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
         if (in) {
             *reinterpret_cast<u32x4*>(rows.cached(page, key)) = codes;
             if (threadIdx.x % R::LANES == 0) *rows.scale(page, key) = scale;
@@ -277,9 +150,21 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const CacheParams 
 constexpr int kTile = 128;           // keys: 32 of each wavefront
 constexpr float kLowest = -3.0e38f;
 
+// WINDOW: the token at the end of n keys sees those from n - window on and the first ones.  Its tiles are those of the first keys and, behind the `gap` that it does not look at, those of the
+// window: tile u is tile u, or from `first` on u + gap.  Keys between are not read, nor are their pages looked up: what they hold, and what the table says of them, may be anything.
+struct Gap {
+    int from, first, gap;       // the first key that is looked back on
+    __device__ __forceinline__ Gap(const CacheParams& p, int n) {
+        from = n > p.window ? n - p.window : 0;
+        first = ((p.sinks < from ? p.sinks : from) + kTile - 1) / kTile;
+        gap = from / kTile - first;
+        gap = gap > 0 ? gap : 0;
+    }
+};
 // tiles of a length
-__device__ __forceinline__ int tiles_of(const CacheParams& p, int n) {
-    return n > 0 && n <= (int64_t)p.width << p.page_shift ? (n + kTile - 1) / kTile : 0;
+template <bool WINDOW> __device__ __forceinline__ int tiles_of(const CacheParams& p, int n) {
+    const int tiles = n > 0 && n <= (int64_t)p.width << p.page_shift ? (n + kTile - 1) / kTile : 0;
+    return WINDOW && tiles ? tiles - Gap(p, n).gap : tiles;
 }
 // A sequence's parts have a share at most; three quarters of one where shares are large and most sequences have only a few parts, which rounding up leaves far from equal (48 sequences of 1 to
 // 7817 keys, us, a share / three quarters: 106 / 100; but 131072 + 70001 + 99 keys in e4m3 84 / 88, 32 of 1 to 2817 in int8 18.9 / 20.5).  On eleven other sizes, 8 to 100 sequences of up to 3000 to 60000 keys, the rule is within 2 % of the better one
@@ -298,22 +183,22 @@ __device__ __forceinline__ Share share_of(const CacheParams& p, int tiles) {
 // Every workgroup looks through all sequences: up to 64 each wavefront for itself, more of them kOwn in order to a thread, so that the lengths of kBatch are one wait (1000 sequences of 1 to 1500
 // keys in tables of 4096, which are not taken whole, 32 heads of 128 on 8, int8, 306 us, 5.2 TB/s, each wavefront 64 at a time 443; but 32 sequences 20.2 instead of 19.4).
 constexpr int kOwn = 4, kBatch = kOwn * kThreads, kWaves = kThreads / 64;
-struct Batch {
+template <bool WINDOW> struct Batch {
     int tiles[kOwn];
     __device__ __forceinline__ Batch(const CacheParams& p, int base) {
         int n[kOwn];
 #pragma unroll
         for (int c = 0; c < kOwn; ++c) { const int i = base + kOwn * threadIdx.x + c; n[c] = p.lens[i < p.B ? i : 0]; }
 #pragma unroll
-        for (int c = 0; c < kOwn; ++c) tiles[c] = base + kOwn * (int)threadIdx.x + c < p.B ? tiles_of(p, n[c]) : 0;
+        for (int c = 0; c < kOwn; ++c) tiles[c] = base + kOwn * (int)threadIdx.x + c < p.B ? tiles_of<WINDOW>(p, n[c]) : 0;
     }
 };
 // The part `slot`: first come the parts of sequences of more than half a share, in order, then the shorter ones, which end the call on what those leave (without keys: one part too).
 // seq < 0: behind the last.
 struct Part { int seq, part, parts, tiles; };
-__device__ __forceinline__ Part part_of(const CacheParams& p, int slot) {
+template <bool WINDOW> __device__ __forceinline__ Part part_of(const CacheParams& p, int slot) {
     if (p.B <= 64) {
-        const int lane = threadIdx.x & 63, n = p.lens[lane < p.B ? lane : 0], tiles = lane < p.B ? tiles_of(p, n) : 0;
+        const int lane = threadIdx.x & 63, n = p.lens[lane < p.B ? lane : 0], tiles = lane < p.B ? tiles_of<WINDOW>(p, n) : 0;
         const Share share = share_of(p, sum_of(tiles));
         if (blockIdx.x == 0 && threadIdx.x == 0) { p.share[0] = share.per; p.share[1] = share.most; }
         int before = 0;
@@ -332,10 +217,10 @@ __device__ __forceinline__ Part part_of(const CacheParams& p, int slot) {
     __shared__ int totals[kWaves], sums[2][kWaves];
     __shared__ Part found;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Batch first(p, 0);
+    const Batch<WINDOW> first(p, 0);
     int mine = 0;
     for (int base = 0; base < p.B; base += kBatch) {
-        const Batch b = base ? Batch(p, base) : first;
+        const Batch<WINDOW> b = base ? Batch<WINDOW>(p, base) : first;
 #pragma unroll
         for (int c = 0; c < kOwn; ++c) mine += b.tiles[c];
     }
@@ -350,7 +235,7 @@ __device__ __forceinline__ Part part_of(const CacheParams& p, int slot) {
     int before = 0, turn = 0;
     for (int shorter = 0; shorter < 2; ++shorter)
         for (int base = 0; base < p.B; base += kBatch, turn ^= 1) {
-            const Batch b = base ? Batch(p, base) : first;
+            const Batch<WINDOW> b = base ? Batch<WINDOW>(p, base) : first;
             int parts[kOwn], own = 0;
 #pragma unroll
             for (int c = 0; c < kOwn; ++c) {
@@ -391,7 +276,7 @@ __device__ __forceinline__ float over_quarters_max(float x) {
     return fmaxf(x, __shfl_xor(x, 16));
 }
 
-template <typename T, int KIND, int D, int NR>
+template <typename T, int KIND, int D, int NR, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const CacheParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef typename VecOf<T>::v8 V8;
@@ -414,8 +299,8 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
         }
     };
     Part mine = {slot, 0, 1, 0};
-    if (p.whole) mine.tiles = __builtin_amdgcn_readfirstlane(tiles_of(p, p.lens[slot]));
-    else mine = part_of(p, slot);
+    if (p.whole) mine.tiles = __builtin_amdgcn_readfirstlane(tiles_of<WINDOW>(p, p.lens[slot]));
+    else mine = part_of<WINDOW>(p, slot);
     if (mine.seq < 0) return;
     const int seq = mine.seq;
     if (!mine.tiles) {
@@ -455,15 +340,19 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
     // addresses, and little for what they point at.  Keys past the end are the last one's, with weights of 0: whatever else the page holds is not looked at.
     constexpr int KLOADS = CODES ? NC / 2 : NC, VWORDS = NB * BYTES / 4;
     const int most = len - 1, first_key = 32 * wave;
-    int end = (len - first_key + kTile - 1) / kTile;                  // this wavefront's steps
+    const Gap between(p, len);
+    auto base_of = [&](int u) { return (WINDOW && u >= between.first ? u + between.gap : u) * kTile + first_key; };      // this wavefront's first key of step u
+    auto is_seen = [&](int key) { return !WINDOW || key >= between.from || key < p.sinks; };
+    int end = (len - first_key + kTile - 1) / kTile - (WINDOW ? between.gap : 0);      // this wavefront's steps
     end = to < end ? to : end;
     u32x4 kw[2][KLOADS];
     unsigned vw[8][VWORDS];
     float ks[8], vs[8];
     // K: row n16 of key half u is key 8 (n16 / 4) + 4 u + n16 % 4, so that a lane's results of the two halves are those of 8 keys in order, 8 g .. 8 g + 7
-    auto k_key = [&](int t, int u) { const int key = t * kTile + first_key + 8 * (n16 >> 2) + 4 * u + (n16 & 3); return key < most ? key : most; };
+    // (WINDOW: instead of a key that is not seen the first one that is looked back on)
+    auto k_key = [&](int t, int u) { const int key = base_of(t) + 8 * (n16 >> 2) + 4 * u + (n16 & 3); return key >= most ? most : is_seen(key) ? key : between.from; };
     // V: keys 8 g .. 8 g + 7, channels NB n16 .. NB n16 + NB - 1; 8 keys in order share a page
-    auto v_key = [&](int t) { const int key = t * kTile + first_key + 8 * g; return key < (most & ~7) ? key : (most & ~7); };
+    auto v_key = [&](int t) { const int key = base_of(t) + 8 * g; return key >= (most & ~7) ? most & ~7 : is_seen(key) || is_seen(key + 7) ? key : between.from & ~7; };
     int kp[2], vp;
     auto look_up = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
@@ -523,11 +412,12 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
             vnext = checked(vp);
             look_up(t + 2);
         }
-        const int left = len - t * kTile - first_key - 8 * g;
+        const int left = len - base_of(t) - 8 * g, out = WINDOW ? between.from - base_of(t) - 8 * g : 0, in = WINDOW ? p.sinks - base_of(t) - 8 * g : 0;
+        auto counts = [&](int i) { return i < left && (!WINDOW || i >= out || i < in); };
         float by[8];                            // what V's weights are multiplied with
         if constexpr (CODES) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) by[i] = i < left ? vs[i] : 0.f;
+            for (int i = 0; i < 8; ++i) by[i] = counts(i) ? vs[i] : 0.f;
             if constexpr (__is_same(T, _Float16)) {
                 // Weights p scale in fp16 would leave its range where values are small.  They are held relative to the largest scale so far, but for a factor of up to 64.
                 float top = by[0];
@@ -555,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
             for (int i = 0; i < 8; ++i) {
                 x[i] = s[r][i / 4][i % 4] * p.scale_log2;
                 if constexpr (CODES) x[i] *= ks[i];
-                x[i] = i < left ? x[i] : -INFINITY;
+                x[i] = counts(i) ? x[i] : -INFINITY;
                 top = fmaxf(top, x[i]);
             }
             if (__any(top > m[r] + kMaxSlack)) {
@@ -578,12 +468,12 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
             pf[r] = __builtin_bit_cast(V8, w);
         }
         // Past the end lie the last rows once more, whose infinite values with a weight of 0 would be NaN.  (The last step alone reaches there; a code's scale is what is infinite, or NaN, and is
-        // not taken there.)
-        if constexpr (!CODES && !decltype(more)::value) {
+        // not taken there.  WINDOW: rows that are not seen beside others that are may hold anything, codes of NaN as well.)
+        if constexpr (WINDOW || (!CODES && !decltype(more)::value)) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int j = 0; j < VWORDS; ++j) vw[i][j] = i < left ? vw[i][j] : 0u;
+                for (int j = 0; j < VWORDS; ++j) vw[i][j] = counts(i) ? vw[i][j] : 0u;
         }
         // output rows NB n + b, n = 0 .. 15: what lane n16 holds of V, transposed in its registers
         unsigned vx[8][NB / 2];
@@ -664,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
 
 // ---- the sequences that several workgroups have parts of: a workgroup for each sequence and query head, D / 4 lanes to a part, kThreads / (D / 4) parts at a time
 // (4 to 6 us, a launch and two trips to memory)
-template <typename T, int D, int NR>
+template <typename T, int D, int NR, bool WINDOW>
 __global__ void __launch_bounds__(kThreads) cache_join_kernel(const CacheParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int LANES = D / 4, AT_ONCE = kThreads / LANES;
@@ -672,12 +562,12 @@ __global__ void __launch_bounds__(kThreads) cache_join_kernel(const CacheParams 
     const int heads = p.group * p.Hkv, seq = blockIdx.x / heads, hq = blockIdx.x - seq * heads, head = hq / p.group, row = hq - head * p.group, block = row / (16 * NR), r = row % (16 * NR);
     const int lane = threadIdx.x & 63;
     const Share share = {p.share[0], p.share[1]};
-    const int parts = share.parts(__builtin_amdgcn_readfirstlane(tiles_of(p, p.lens[seq])));
+    const int parts = share.parts(__builtin_amdgcn_readfirstlane(tiles_of<WINDOW>(p, p.lens[seq])));
     if (parts == 1) return;
     __shared__ int sums[kWaves];
     int before = 0;
     for (int i = threadIdx.x; i < seq; i += kThreads) {
-        const int n = tiles_of(p, p.lens[i]);
+        const int n = tiles_of<WINDOW>(p, p.lens[i]);
         before += share.is_long(n) ? share.parts(n) : 0;
     }
     before = sum_of(before);
@@ -720,104 +610,6 @@ __global__ void __launch_bounds__(kThreads) cache_join_kernel(const CacheParams 
 }
 
 // ---- C ABI
-constexpr int64_t kMost = 0x7FFFFFFF, kMostBlocks = 0xFFFFFFFF / kThreads;      // (the threads of a launch are a 32-bit number)
-constexpr int64_t kMostKeys = (int64_t)1 << 30;       // of a sequence: positions some steps behind its last are 32-bit numbers too
-constexpr int64_t kMostRowBytes = (int64_t)1 << 23;
-
-int check_half(const void* at, const int64_t* stride, int bytes, int D) {
-    if (!at) return COSMOS_ATTN_BAD_ARG;
-    const int64_t unit = 16 / bytes;
-    if (!aligned16(at) || stride[0] % unit || stride[1] % unit || stride[2] % unit) return COSMOS_ATTN_BAD_STRIDE;
-    if (stride[0] < 0 || stride[1] < 0 || stride[2] < D || stride[2] * bytes > kMostRowBytes) return COSMOS_ATTN_BAD_STRIDE;
-    return COSMOS_ATTN_OK;
-}
-int check_rows(const void* at, const int64_t* stride) {
-    if (!at) return COSMOS_ATTN_BAD_ARG;
-    return aligned16(at) && stride[0] % 8 == 0 && stride[1] % 8 == 0 && stride[0] >= 0 && stride[1] >= 0 ? COSMOS_ATTN_OK : COSMOS_ATTN_BAD_STRIDE;
-}
-// outputs: rows and heads that do not share memory
-int check_out(const void* at, const int64_t* stride, int64_t rows, int heads, int D) {
-    const int st = check_rows(at, stride);
-    if (st != COSMOS_ATTN_OK) return st;
-    if ((rows > 1 && stride[0] < D) || (heads > 1 && stride[1] < D)) return COSMOS_ATTN_BAD_STRIDE;
-    const bool by_row = rows <= 1 || stride[0] >= (heads - 1) * stride[1] + D, by_head = heads <= 1 || stride[1] >= (rows - 1) * stride[0] + D;
-    return by_row || by_head ? COSMOS_ATTN_OK : COSMOS_ATTN_BAD_STRIDE;
-}
-int check_scale(const float* at, const int64_t* stride) {
-    if (!at) return COSMOS_ATTN_BAD_ARG;
-    return aligned16(at) && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[0] >= 0 && stride[1] >= 0 ? COSMOS_ATTN_OK : COSMOS_ATTN_BAD_STRIDE;
-}
-// pages to be written: of three dims of `size` elements each holds those of smaller strides, down to runs of `run` elements
-bool apart(const int64_t (&stride)[3], const int64_t (&size)[3], int64_t run) {
-    int order[3] = {0, 1, 2};
-    for (int i = 0; i < 3; ++i)
-        for (int j = i + 1; j < 3; ++j)
-            if (stride[order[j]] < stride[order[i]]) std::swap(order[i], order[j]);
-    __int128 extent = run;
-    for (int i : order) {
-        if (size[i] <= 1) continue;
-        if (stride[i] < extent) return false;
-        extent += (__int128)(size[i] - 1) * stride[i];
-    }
-    return true;
-}
-int check_written(const cosmos_attn_cache_desc* d) {
-    const int64_t size[3] = {d->pages, d->Hkv, d->page_size}, ks[3] = {d->k_stride[0], d->k_stride[1], d->k_stride[2]}, vs[3] = {d->v_stride[0], d->v_stride[1], d->v_stride[2]};
-    if (d->k == d->v) return COSMOS_ATTN_BAD_ARG;
-    if (!apart(ks, size, d->D) || !apart(vs, size, d->D)) return COSMOS_ATTN_BAD_STRIDE;
-    if (d->kind == COSMOS_ATTN_CACHE_SAME) return COSMOS_ATTN_OK;
-    const int64_t kss[3] = {d->k_scale_stride[0], d->k_scale_stride[1], 1}, vss[3] = {d->v_scale_stride[0], d->v_scale_stride[1], 1};
-    if (d->k_scale == d->v_scale) return COSMOS_ATTN_BAD_ARG;
-    return apart(kss, size, 1) && apart(vss, size, 1) ? COSMOS_ATTN_OK : COSMOS_ATTN_BAD_STRIDE;
-}
-int check(const cosmos_attn_cache_desc* d) {
-    if (!d || d->abi_version != COSMOS_ATTN_ABI_VERSION) return COSMOS_ATTN_BAD_ARG;
-    if (d->dtype != COSMOS_ATTN_BF16 && d->dtype != COSMOS_ATTN_FP16) return COSMOS_ATTN_UNSUPPORTED;
-    if (d->kind < COSMOS_ATTN_CACHE_SAME || d->kind > COSMOS_ATTN_CACHE_INT8) return COSMOS_ATTN_UNSUPPORTED;
-    if (d->D != 64 && d->D != 128) return COSMOS_ATTN_UNSUPPORTED;
-    if (d->Hkv < 1 || d->B < 0 || d->width < 0 || d->pages < 1 || d->pages > kMost) return COSMOS_ATTN_BAD_ARG;
-    if (d->page_size < 16 || d->page_size > 1024 || (d->page_size & (d->page_size - 1))) return COSMOS_ATTN_BAD_SHAPE;
-    if ((int64_t)d->width * d->page_size > kMostKeys) return COSMOS_ATTN_UNSUPPORTED;
-    const int bytes = d->kind == COSMOS_ATTN_CACHE_SAME ? 2 : 1;
-    int st = check_half(d->k, d->k_stride, bytes, d->D);
-    if (st == COSMOS_ATTN_OK) st = check_half(d->v, d->v_stride, bytes, d->D);
-    if (st == COSMOS_ATTN_OK && bytes == 1) st = check_scale(d->k_scale, d->k_scale_stride);
-    if (st == COSMOS_ATTN_OK && bytes == 1) st = check_scale(d->v_scale, d->v_scale_stride);
-    if (st != COSMOS_ATTN_OK || !d->B) return st;
-    if (!d->table && d->width) return COSMOS_ATTN_BAD_ARG;
-    if (d->table_stride < 0 || (reinterpret_cast<uintptr_t>(d->table) | reinterpret_cast<uintptr_t>(d->lens) | reinterpret_cast<uintptr_t>(d->cu)) & 3) return COSMOS_ATTN_BAD_STRIDE;
-    return COSMOS_ATTN_OK;
-}
-
-CacheParams params_of(const cosmos_attn_cache_desc* d) {
-    CacheParams p = {};
-    const int bytes = d->kind == COSMOS_ATTN_CACHE_SAME ? 2 : 1;
-    auto side = [&](void* pages, const int64_t* stride, float* scales, const int64_t* scale_stride, void* packed, const int64_t* packed_stride) {
-        return Side{(char*)pages, bytes * stride[0], bytes * stride[1], bytes * stride[2], scales, scale_stride[0], scale_stride[1], (char*)packed, 2 * packed_stride[0], 2 * packed_stride[1]};
-    };
-    p.side[0] = side(d->k, d->k_stride, d->k_scale, d->k_scale_stride, d->k_rows, d->k_rows_stride);
-    p.side[1] = side(d->v, d->v_stride, d->v_scale, d->v_scale_stride, d->v_rows, d->v_rows_stride);
-    p.table = d->table; p.lens = d->lens; p.cu = d->cu; p.table_row = d->table_stride;
-    p.width = d->width; p.B = d->B; p.pages = (int)d->pages; p.page_shift = __builtin_ctz(d->page_size); p.Hkv = d->Hkv; p.fill = d->fill != 0;
-    p.rows = d->rows;
-    return p;
-}
-
-template <typename F> int with_type(const cosmos_attn_cache_desc* d, F&& f) {
-    auto kind = [&](auto* t, auto dim) {
-        return d->kind == COSMOS_ATTN_CACHE_SAME ? f(t, dim, Int<SAME16>{}) : d->kind == COSMOS_ATTN_CACHE_E4M3 ? f(t, dim, Int<E4M3>{}) : f(t, dim, Int<INT8>{});
-    };
-    if (d->dtype == COSMOS_ATTN_BF16) return d->D == 128 ? kind((__bf16*)nullptr, Int<128>{}) : kind((__bf16*)nullptr, Int<64>{});
-    return d->D == 128 ? kind((_Float16*)nullptr, Int<128>{}) : kind((_Float16*)nullptr, Int<64>{});
-}
-int launch(void (*kernel)(CacheParams), int64_t blocks, size_t lds, const CacheParams& p, void* stream) {
-    if (blocks <= 0) return COSMOS_ATTN_OK;
-    if (blocks > kMostBlocks) return COSMOS_ATTN_UNSUPPORTED;
-    if (lds && !allow_lds((const void*)kernel, lds)) return COSMOS_ATTN_LAUNCH_FAILED;
-    kernel<<<dim3((unsigned)blocks), dim3(kThreads), lds, (hipStream_t)stream>>>(p);
-    return hipGetLastError() == hipSuccess ? COSMOS_ATTN_OK : COSMOS_ATTN_LAUNCH_FAILED;
-}
-
 int64_t packed_blocks(const cosmos_attn_cache_desc* d) {
     const int64_t per = kThreads / (d->D / each_of(d->kind));
     return 2 * ((d->rows * d->Hkv + per - 1) / per);
@@ -858,9 +650,14 @@ int check_attention(const cosmos_attn_cache_desc* d) {
 // 8, 101 / 106; but 40 of them 70 / 68), up to lengths at which the longest alone takes some 20 us.
 constexpr int kWholeTiles = 4, kWholeManyTiles = 16, kMany = 32;       // kMany: workgroups to a tile of the table's
 struct Shape { int row_blocks, rows16, slots; bool whole; };
-Shape shape_of(const cosmos_attn_cache_desc* d) {
+Shape shape_of(const cosmos_attn_cache_desc* d, Window w) {
     const int group = d->Hq / d->Hkv, rows16 = group <= 16 ? 1 : 2, row_blocks = (group + 16 * rows16 - 1) / (16 * rows16);
-    const int64_t capacity = ((int64_t)d->width * d->page_size + kTile - 1) / kTile, most = (int64_t)d->B * capacity;
+    int64_t capacity = ((int64_t)d->width * d->page_size + kTile - 1) / kTile;
+    if (w.window) {             // (a window may begin anywhere in its first tile)
+        const int64_t seen = ((int64_t)w.window + kTile - 2) / kTile + 1 + ((int64_t)w.sinks + kTile - 1) / kTile;
+        capacity = seen < capacity ? seen : capacity;
+    }
+    const int64_t most = (int64_t)d->B * capacity;
     if (capacity <= kWholeTiles || (capacity <= kWholeManyTiles && (int64_t)d->B * d->Hkv * row_blocks >= kMany * capacity)) return {row_blocks, rows16, 1, true};
     // two workgroups a compute unit, if the tables hold that many tiles
     int64_t slots = 2 * kNumCUs / ((int64_t)d->Hkv * row_blocks);
@@ -896,21 +693,29 @@ int cosmos_attn_cache_read(const cosmos_attn_cache_desc* desc, void* stream) {
     });
 }
 
-size_t cosmos_attn_cache_attention_workspace_bytes(const cosmos_attn_cache_desc* desc) {
-    if (check_attention(desc) != COSMOS_ATTN_OK || !desc->B) return 0;
-    const Shape s = shape_of(desc);
+size_t cosmos_attn_cache_attention_workspace_bytes(const cosmos_attn_cache_desc* desc) { return cosmos_attn_cache_window_workspace_bytes(desc, 0, 0); }
+int cosmos_attn_cache_attention(const cosmos_attn_cache_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
+    return cosmos_attn_cache_window(desc, 0, 0, workspace, workspace_bytes, stream);
+}
+
+size_t cosmos_attn_cache_window_workspace_bytes(const cosmos_attn_cache_desc* desc, int64_t window, int64_t sinks) {
+    if (check_attention(desc) != COSMOS_ATTN_OK || window < 0 || sinks < 0 || !desc->B) return 0;
+    const Shape s = shape_of(desc, window_of(desc, window, sinks));
     return s.whole ? 0 : (size_t)most_parts(desc->B, s.slots) * s.row_blocks * desc->Hkv * 16 * s.rows16 * (desc->D + 2) * sizeof(float) + kShareBytes;
 }
 
-int cosmos_attn_cache_attention(const cosmos_attn_cache_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
-    const int st = check_attention(desc);
+int cosmos_attn_cache_window(const cosmos_attn_cache_desc* desc, int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
+    int st = check_attention(desc);
+    if (st == COSMOS_ATTN_OK && (window < 0 || sinks < 0)) st = COSMOS_ATTN_BAD_ARG;
     if (st != COSMOS_ATTN_OK || !desc->B) return st;
-    const size_t wanted = cosmos_attn_cache_attention_workspace_bytes(desc);
+    const size_t wanted = cosmos_attn_cache_window_workspace_bytes(desc, window, sinks);
     if (workspace_bytes < wanted || (wanted && !workspace)) return COSMOS_ATTN_WORKSPACE_TOO_SMALL;
     if (wanted && !aligned16(workspace)) return COSMOS_ATTN_BAD_STRIDE;
     if (!device_is_whole_mi355x()) return COSMOS_ATTN_WRONG_DEVICE;
-    const Shape s = shape_of(desc);
+    const Window seen = window_of(desc, window, sinks);
+    const Shape s = shape_of(desc, seen);
     CacheParams p = params_of(desc);
+    p.window = seen.window; p.sinks = seen.sinks;
     p.q = (const char*)desc->q; p.o = (char*)desc->o; p.lse = desc->lse;
     p.q_row = 2 * desc->q_stride[0]; p.q_head = 2 * desc->q_stride[1]; p.o_row = 2 * desc->o_stride[0]; p.o_head = 2 * desc->o_stride[1];
     p.group = desc->Hq / desc->Hkv; p.row_blocks = s.row_blocks; p.slots = s.slots; p.whole = s.whole;
@@ -921,12 +726,14 @@ int cosmos_attn_cache_attention(const cosmos_attn_cache_desc* desc, void* worksp
     return with_type(desc, [&](auto* t, auto dim, auto kind) {
         typedef std::remove_pointer_t<decltype(t)> T;
         constexpr int D = decltype(dim)::value, K = decltype(kind)::value;
-        auto run = [&](auto blocks16) {
+        auto run = [&](auto blocks16, auto windowed) {
             constexpr int NR = decltype(blocks16)::value;
-            const int done = launch(cache_attention_kernel<T, K, D, NR>, (int64_t)p.Hkv * p.row_blocks * (s.whole ? p.B : most_parts(p.B, p.slots)), 4 * 16 * NR * (D + 2) * sizeof(float), p, stream);
-            return done != COSMOS_ATTN_OK || s.whole ? done : launch(cache_join_kernel<T, D, NR>, (int64_t)desc->Hq * p.B, 0, p, stream);
+            constexpr bool WINDOW = decltype(windowed)::value;
+            const int done = launch(cache_attention_kernel<T, K, D, NR, WINDOW>, (int64_t)p.Hkv * p.row_blocks * (s.whole ? p.B : most_parts(p.B, p.slots)), 4 * 16 * NR * (D + 2) * sizeof(float), p, stream);
+            return done != COSMOS_ATTN_OK || s.whole ? done : launch(cache_join_kernel<T, D, NR, WINDOW>, (int64_t)desc->Hq * p.B, 0, p, stream);
         };
-        return s.rows16 == 1 ? run(Int<1>{}) : run(Int<2>{});
+        if (seen.window) return s.rows16 == 1 ? run(Int<1>{}, Int<1>{}) : run(Int<2>{}, Int<1>{});
+        return s.rows16 == 1 ? run(Int<1>{}, Int<0>{}) : run(Int<2>{}, Int<0>{});
     });
 }
 

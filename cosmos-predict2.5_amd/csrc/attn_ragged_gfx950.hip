@@ -704,18 +704,6 @@ template <typename F> int with_type(int dtype, int D, F&& f) {
     if (dtype == COSMOS_ATTN_BF16) return D == 128 ? f((__bf16*)nullptr, Int<128>{}) : f((__bf16*)nullptr, Int<64>{});
     return D == 128 ? f((_Float16*)nullptr, Int<128>{}) : f((_Float16*)nullptr, Int<64>{});
 }
-// at most so many tiles are there: each sequence rounds up once, and so do the rows of none
-int64_t most_tiles(int64_t rows, int n_seq) { return rows / kRows + n_seq + 1; }
-// Parts that a tile may be cut into.  A call with fewer tiles than some rounds of workgroups ends with its longest tiles on a few compute units; one with more is dealt out evenly as it is.
-// (The workgroups of parts that a tile does not have end at once.)
-constexpr int64_t kFullGrid = 6 * kNumCUs;
-int most_parts(int64_t tiles, int64_t longest, int least) {
-    int64_t parts = (kFullGrid + tiles - 1) / tiles;
-    parts = parts < 16 ? parts : 16;
-    const int64_t of_length = longest / least;
-    parts = parts < of_length ? parts : of_length;
-    return parts > 1 ? (int)parts : 1;
-}
 struct Cut { int64_t tiles; int parts, least; size_t bytes; };
 // The window of a call, 0 keys where it hides none (sizes say so: a row's position is below Tk).
 struct Window { int window = 0, sinks = 0; };

@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from .ops import _DTYPES
-from .ragged import HEAD_DIMS, check_rows, int32_on, on_device, packed, packed_ready, plain_int32
+from .ragged import HEAD_DIMS, check_rows, checked_window, int32_on, on_device, packed, packed_ready, plain_int32
 
 KINDS = {torch.bfloat16: _lib.CACHE_SAME, torch.float16: _lib.CACHE_SAME, torch.float8_e4m3fn: _lib.CACHE_E4M3, torch.int8: _lib.CACHE_INT8}
 
@@ -163,11 +163,12 @@ def cache_read(cache: KVCache, table: torch.Tensor, cu: torch.Tensor, rows: int,
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(Hkv: int, D: int, page_size: int, B: int, width: int, Hq: int) -> int:
-    """What the library asks for, which follows from sizes alone (addresses are never dereferenced)."""
+def _workspace_bytes(Hkv: int, D: int, page_size: int, B: int, width: int, Hq: int, window: int = 0, sinks: int = 0, rows: int = -1) -> int:
+    """What the library asks for, which follows from sizes alone (addresses are never dereferenced).  `rows`: of a call with offsets."""
     part = _CACHE_PART.pack(_lib.ABI_VERSION, _lib.DTYPE_BF16, _lib.CACHE_SAME, Hkv, D, page_size, 1, 16, 16, *(page_size * Hkv * D, page_size * D, D) * 2, 0, 0, 0, 0, 0, 0)
-    call = _CALL_PART.pack(B, width, 16, width, 16, 0, 0, 0, 0, 0, 0, 0, 0, 0, Hq, 1.0, 0, 16, 16, Hq * D, D, Hq * D, D, 0)
-    return _lib.load_library().cosmos_attn_cache_attention_workspace_bytes(part + call)
+    call = _CALL_PART.pack(B, width, 16, width, 16, 16, max(rows, 0), 0, 0, 0, 0, 0, 0, 0, Hq, 1.0, 0, 16, 16, Hq * D, D, Hq * D, D, 0)
+    lib = _lib.load_library()
+    return (lib.cosmos_attn_cache_window_workspace_bytes if rows < 0 else lib.cosmos_attn_cache_chunk_workspace_bytes)(part + call, window, sinks)
 
 
 def cache_attention(
@@ -178,27 +179,41 @@ def cache_attention(
     sm_scale: Optional[float] = None,
     need_lse: bool = False,
     out: Optional[torch.Tensor] = None,
+    cu: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``(o, lse)``: attention of one token of each sequence, ``q [B, Hq, D]``, over the first ``lens[i]`` positions that its row of ``table`` holds; ``lse``: fp32 ``[B, Hq]``.
 
-    ``lens[i] == 0``: o = 0, lse = -inf.  A length that the table does not hold, or a page outside of the cache among a sequence's: NaN.  ``out``: a tensor for o."""
+    ``cu``: of the sequences' last tokens, packed, ``q [rows, Hq, D]``: sequence i's are the rows ``cu[i] .. cu[i + 1] - 1`` and its last positions of ``lens[i]``, whose keys and values are in the
+    cache already; each sees the positions up to its own.  ``lse``: ``[rows, Hq]``.  Offsets as in :func:`ragged_fwd`; rows of no sequence become zeros, and -inf (in ``out``: left as they are).
+    ``window``: a token sees that many last positions, its own among them, and those below ``sinks``; pages that no token of a sequence sees are not looked up, whatever the table says of them.
+
+    A token that sees nothing (``lens[i] == 0``, or below its rows): o = 0, lse = -inf.  A length that the table does not hold: NaN.  A page outside of the cache: NaN for the tokens that see it.
+    ``out``: a tensor for o."""
+    window, sinks = checked_window(window, sinks)
     q = _check_rows(q, "q", cache)
-    B, Hq, D = q.shape
-    assert Hq >= 1 and Hq % cache.heads == 0, "q must be [B, Hq, D], Hq a multiple of the cache's heads"
+    rows, Hq, D = q.shape
+    assert Hq >= 1 and Hq % cache.heads == 0, "q must be [rows, Hq, D], Hq a multiple of the cache's heads"
     part, table = cache._part(q.dtype), _check_table(cache, table)
-    assert table.shape[0] == B, "a row of the table for each sequence"
+    B = table.shape[0]
     lens = _check_numbers(lens, B, cache, "as many lengths as there are sequences: their")
+    if cu is None:
+        assert rows == B, "a row of the table for each sequence, or offsets"
+    else:
+        cu = _check_numbers(cu, B + 1, cache, "one offset more than the table has sequences: its")
     if out is None:
-        o = torch.empty_like(q) if q.is_contiguous() else torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+        o = torch.empty_like(q) if q.is_contiguous() else torch.empty((rows, Hq, D), dtype=q.dtype, device=q.device)
     else:
         assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out must have q's shape, type and device"
         if not packed_ready(out):
             raise ValueError("out: rows of 16-byte steps are written in place, this view cannot be")
         o = out
-    lse = q.new_empty((B, Hq), dtype=torch.float32) if need_lse else None
-    ws_bytes = _workspace_bytes(cache.heads, D, cache.page_size, B, table.shape[1], Hq)
+    lse = q.new_empty((rows, Hq), dtype=torch.float32) if need_lse else None
+    ws_bytes = _workspace_bytes(cache.heads, D, cache.page_size, B, table.shape[1], Hq, window, sinks, -1 if cu is None else rows)
     workspace = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
-    desc = part + _call(table, lens.data_ptr(), 0, 0, 0, 0, (0, 0), (0, 0), 0, Hq, D ** -0.5 if sm_scale is None else sm_scale, q.data_ptr(), o.data_ptr(), q.stride()[:2], o.stride()[:2],
-                        0 if lse is None else lse.data_ptr())
-    on_device(cache._index, _lib.load_library().cosmos_attn_cache_attention, desc, 0 if workspace is None else workspace.data_ptr(), ws_bytes)
+    desc = part + _call(table, lens.data_ptr(), 0 if cu is None else cu.data_ptr(), rows, 0, 0, (0, 0), (0, 0), _lib.FILL_ALL if out is None else _lib.FILL_LSE, Hq,
+                        D ** -0.5 if sm_scale is None else sm_scale, q.data_ptr(), o.data_ptr(), q.stride()[:2], o.stride()[:2], 0 if lse is None else lse.data_ptr())
+    lib = _lib.load_library()
+    on_device(cache._index, lib.cosmos_attn_cache_window if cu is None else lib.cosmos_attn_cache_chunk, desc, window, sinks, 0 if workspace is None else workspace.data_ptr(), ws_bytes)
     return o, lse

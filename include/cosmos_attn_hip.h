@@ -500,6 +500,20 @@ COSMOS_ATTN_API int cosmos_attn_cache_read(const cosmos_attn_cache_desc *desc, v
 COSMOS_ATTN_API size_t cosmos_attn_cache_attention_workspace_bytes(const cosmos_attn_cache_desc *desc);
 COSMOS_ATTN_API int cosmos_attn_cache_attention(const cosmos_attn_cache_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * cosmos_attn_cache_window: cosmos_attn_cache_attention where the token, at position lens[i] - 1, sees the last `window` positions, its own among them, and those below `sinks` (window 0: all).
+ *     Pages without a position that is seen are not looked up: their entries of the table may be anything.
+ * cosmos_attn_cache_chunk: attention of several tokens of each sequence, q, o [rows, Hq, D]; sequence i's are the rows cu[i] .. cu[i + 1] - 1, its last positions of lens[i], written before the call.
+ *     The token at position p sees the positions j <= p, with a window those with j > p - window or j < sinks; pages that none of a sequence's tokens sees are not looked up.  lse [rows, Hq]
+ *     fp32 or NULL.  A row that sees nothing (lens[i] below its rows): o = 0, lse = -inf.  A length below 0 or that the table does not hold: NaN; a page outside of the cache: NaN for the rows
+ *     that see it.  Rows of no sequence as `fill` says (enum cosmos_attn_ragged_fill); offsets as in cosmos_attn_ragged.  Values that a row does not see have to be finite where another row of its
+ *     sequence in the call sees them.
+ */
+COSMOS_ATTN_API size_t cosmos_attn_cache_window_workspace_bytes(const cosmos_attn_cache_desc *desc, int64_t window, int64_t sinks);
+COSMOS_ATTN_API int cosmos_attn_cache_window(const cosmos_attn_cache_desc *desc, int64_t window, int64_t sinks, void *workspace, size_t workspace_bytes, void *stream);
+COSMOS_ATTN_API size_t cosmos_attn_cache_chunk_workspace_bytes(const cosmos_attn_cache_desc *desc, int64_t window, int64_t sinks);
+COSMOS_ATTN_API int cosmos_attn_cache_chunk(const cosmos_attn_cache_desc *desc, int64_t window, int64_t sinks, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

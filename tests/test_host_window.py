@@ -45,3 +45,48 @@ def test_window_arguments(pkg, monkeypatch):
         for call in (lambda: pkg.ragged_fwd(q, k, k, cu, **over), lambda: pkg.ragged_bwd(q, k, k, q, lse, q, cu, **over), lambda: pkg.attention_ragged(q, k, k, cu, **over)):
             with pytest.raises(error, match="" if error is not AssertionError else "window|sinks|first keys"):
                 call()
+
+
+def test_cache_window_and_chunk_status_codes(pkg):
+    L, lib = pkg._lib, pkg._lib.load_library()
+    one = lambda D, w=0, s=0: lib.cosmos_attn_cache_window(ctypes.byref(D), w, s, P, 1 << 40, None)
+    more = lambda D, w=0, s=0: lib.cosmos_attn_cache_chunk(ctypes.byref(D), w, s, P, 1 << 40, None)
+    for call in (one, more):
+        assert call(cache_desc(pkg, cu=P), -1, 0) == call(cache_desc(pkg, cu=P), 5, -1) == L.ST_BAD_ARG
+        for over, status in [(dict(abi_version=1), L.ST_BAD_ARG), (dict(kind=3), L.ST_UNSUPPORTED), (dict(D=32), L.ST_UNSUPPORTED), (dict(page_size=8), L.ST_BAD_SHAPE), (dict(Hq=0), L.ST_BAD_ARG),
+                             (dict(Hq=7), L.ST_BAD_SHAPE), (dict(lens=None), L.ST_BAD_ARG), (dict(q=None), L.ST_BAD_ARG), (dict(o_stride=(512, 0)), L.ST_BAD_STRIDE), (dict(o_stride=(64, 64)), L.ST_BAD_STRIDE),
+                             (dict(q=P + 2), L.ST_BAD_STRIDE), (dict(sm_scale=float("inf")), L.ST_BAD_ARG), (dict(table=None), L.ST_BAD_ARG)]:
+            assert call(cache_desc(pkg, **{"cu": P, **over}), 5, 1) == status, over
+    for over, status in [(dict(cu=None), L.ST_BAD_ARG), (dict(rows=-1), L.ST_BAD_ARG), (dict(rows=1 << 29), L.ST_UNSUPPORTED), (dict(rows=1 << 32), L.ST_UNSUPPORTED), (dict(B=1 << 24, Hkv=8), L.ST_UNSUPPORTED),
+                         (dict(q_stride=((1 << 22) + 8, 64)), L.ST_BAD_STRIDE)]:
+        assert more(cache_desc(pkg, **{"cu": P, **over})) == status, over
+    assert more(cache_desc(pkg, cu=P, rows=0, q=None, o=None)) == L.ST_OK == one(cache_desc(pkg, B=0))
+    long = cache_desc(pkg, cu=P, width=100, table_stride=100)
+    assert lib.cosmos_attn_cache_chunk_workspace_bytes(ctypes.byref(long), 0, 0) > 0 == lib.cosmos_attn_cache_chunk_workspace_bytes(ctypes.byref(long), 64, 4)
+    assert lib.cosmos_attn_cache_chunk(ctypes.byref(long), 0, 0, None, 0, None) == L.ST_WORKSPACE
+    assert lib.cosmos_attn_cache_window_workspace_bytes(ctypes.byref(long), 0, 0) > 0 == lib.cosmos_attn_cache_window_workspace_bytes(ctypes.byref(long), 64, 4)
+
+
+def test_refusals_of_pieces(pkg, monkeypatch):
+    def no_launch(*a):
+        raise AssertionError("launched")
+
+    monkeypatch.setattr(pkg.kv_cache, "on_device", no_launch)
+    new = lambda *shape, dtype=torch.bfloat16: on(torch.zeros(*shape, dtype=dtype))
+    cache = pkg.KVCache(new(5, 2, 16, 64), new(5, 2, 16, 64))
+    table, lens, cu, q = new(3, 2, dtype=torch.int32), new(3, dtype=torch.int32), new(4, dtype=torch.int32), new(9, 4, 64)
+    for call, error in [
+        (lambda: pkg.cache_attention(q, cache, table, lens), AssertionError),                       # nine rows for three sequences, no offsets
+        (lambda: pkg.cache_attention(q, cache, table, lens, cu=lens), AssertionError),
+        (lambda: pkg.cache_attention(q, cache, table, cu, cu=cu), AssertionError),
+        (lambda: pkg.cache_attention(q, cache, table, lens, cu=new(4)), AssertionError),
+        (lambda: pkg.cache_attention(new(9, 5, 64), cache, table, lens, cu=cu), AssertionError),
+        (lambda: pkg.cache_attention(new(9, 4, 64, dtype=torch.float16), cache, table, lens, cu=cu), AssertionError),
+        (lambda: pkg.cache_attention(q, cache, table, lens, cu=cu, window=0), AssertionError),
+        (lambda: pkg.cache_attention(q, cache, table, lens, cu=cu, sinks=4), AssertionError),
+        (lambda: pkg.cache_attention(q, cache, table, lens, cu=cu, window=1.5), TypeError),
+        (lambda: pkg.cache_attention(q, cache, table, lens, cu=cu, out=new(8, 4, 64)), AssertionError),
+        (lambda: pkg.cache_attention(q, cache, table, lens, cu=cu, out=on(torch.zeros(9, 4, 128, dtype=torch.bfloat16)[:, :, ::2])), ValueError),
+    ]:
+        with pytest.raises(error):
+            call()
