@@ -288,6 +288,17 @@ class CacheDesc(ctypes.Structure):
     ]
 
 
+class CacheRope(ctypes.Structure):
+    """Mirror of ``struct cosmos_attn_cache_rope``."""
+
+    _fields_ = [
+        ("freqs", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("positions_stride", ctypes.c_int64),
+        ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+        ("pairs", ctypes.c_int32), ("axes", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("weight_16", ctypes.c_int32),
+        ("eps", ctypes.c_float), ("reserved", ctypes.c_int32),
+    ]
+
+
 FILL_ALL, FILL_LSE = 1, 2
 CACHE_SAME, CACHE_E4M3, CACHE_INT8 = 0, 1, 2
 GEMM_XWT, GEMM_XW, GEMM_XTX = 0, 1, 2
@@ -337,6 +348,7 @@ EXPORTS = {
     "cosmos_attn_cache_read": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "cosmos_attn_cache_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p]),
     "cosmos_attn_cache_attention": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "cosmos_attn_cache_append": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "cosmos_attn_cache_window_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64]),
     "cosmos_attn_cache_window": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "cosmos_attn_cache_chunk_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64]),

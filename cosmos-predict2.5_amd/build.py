@@ -15,7 +15,7 @@ REPO_ROOT = os.path.dirname(PKG_DIR)
 LIB_NAME = "libcosmos_attn_hip.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = [os.path.join(PKG_DIR, "csrc", name) for name in ("attn_fwd_jvp_gfx950.hip", "attn_bwd_gfx950.hip", "norm_rope_gfx950.hip", "block_elementwise_gfx950.hip", "gemm_gfx950.hip",
-                                                          "attn_ragged_gfx950.hip", "attn_cache_gfx950.hip", "attn_chunk_gfx950.hip")]
+                                                          "attn_ragged_gfx950.hip", "attn_cache_gfx950.hip", "attn_chunk_gfx950.hip", "attn_append_gfx950.hip")]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

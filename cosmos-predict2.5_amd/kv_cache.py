@@ -5,9 +5,10 @@ device; nothing is copied to the host, and a captured step follows what they hol
 
     cache = KVCache.empty(pages, heads, page_size, head_dim, dtype=torch.int8, device="cuda")
     cache_write(cache, k, v, table, lens, cu)                  # a prompt's keys and values, packed
-    keys, values = cache_read(cache, table, cu_known, rows)    # back, in 16 bits: for the next piece of a prompt with ``attention_ragged``
-    cache_write(cache, k1, v1, table, lens)                    # one new token of each sequence, ``lens`` with it
-    o, _ = cache_attention(q, cache, table, lens)              # its attention over all of them
+    o, _ = cache_attention(q, cache, table, lens, cu=cu)       # its attention over them and all before, causal
+    q1 = cache_append(cache, q1, k1, v1, table, lens, freqs=freqs)      # one new token of each sequence, ``lens`` with it: queries and keys turned by their positions, keys and values written
+    o, _ = cache_attention(q1, cache, table, lens)             # its attention over all of them
+    keys, values = cache_read(cache, table, cu_known, rows)    # back, in 16 bits
 
 The reference has no counterpart (its networks see all of a video at once).  No gradients.
 """
@@ -28,6 +29,8 @@ KINDS = {torch.bfloat16: _lib.CACHE_SAME, torch.float16: _lib.CACHE_SAME, torch.
 # struct cosmos_attn_cache_desc in two parts: what the cache says, and what the call does
 _CACHE_PART = struct.Struct("=6iq2Q6q2Q4q")
 _CALL_PART = struct.Struct("=2iQq2Qq2Q4q2ifi2Q4qQ")
+# struct cosmos_attn_cache_rope
+_ROPE = struct.Struct("=2Qq2Q4ifi")
 
 
 class KVCache:
@@ -142,6 +145,94 @@ def cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, table: torch.T
         cu = _check_numbers(cu, B + 1, cache, "one offset more than the table has sequences: its")
     desc = part + _call(table, lens.data_ptr(), 0 if cu is None else cu.data_ptr(), rows, k.data_ptr(), v.data_ptr(), k.stride()[:2], v.stride()[:2])
     on_device(cache._index, _lib.load_library().cosmos_attn_cache_write, desc)
+
+
+def _check_weight(weight: Optional[torch.Tensor], like: torch.Tensor, name: str) -> Optional[torch.Tensor]:
+    """A norm's weight as the kernels take it: fp32, or of the rows' type, at 16 bytes."""
+    if weight is None:
+        return None
+    assert weight.dim() == 1 and weight.shape[0] == like.shape[2] and weight.device == like.device, f"{name} must be [D], on the rows' device"
+    if weight.dtype != like.dtype and weight.dtype != torch.float32:
+        weight = weight.float()
+    return weight if weight.stride(0) == 1 and weight.data_ptr() % 16 == 0 else weight.clone(memory_format=torch.contiguous_format)
+
+
+def cache_append(
+    cache: KVCache,
+    q: Optional[torch.Tensor],
+    k: torch.Tensor,
+    v: torch.Tensor,
+    table: torch.Tensor,
+    lens: torch.Tensor,
+    cu: Optional[torch.Tensor] = None,
+    *,
+    freqs: Optional[torch.Tensor] = None,
+    positions: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    q_weight: Optional[torch.Tensor] = None,
+    k_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    out: Optional[torch.Tensor] = None,
+) -> Optional[torch.Tensor]:
+    """New tokens, packed as for :func:`cache_write`: keys are normalised and turned by their positions and written with their values; returns the queries, normalised and turned, ``[rows, Hq, D]``
+    (``q`` None: None; ``out``, which may be ``q``, takes them).
+
+    ``freqs``: fp32 ``[R]`` or ``[axes, R]``, radians a position, for R pairs of channels (a multiple of 8, ``2 R <= D``): ``(i, i + R)``, or with ``interleaved`` ``(2 i, 2 i + 1)``; the channels behind
+    are not turned (None: none are).  The angle of pair i is ``sum_a positions[row, a] * freqs[a, i]``, formed in 64 bits; ``positions``: whole numbers ``[rows]`` or ``[rows, axes]``, of images and
+    videos say; None: the token's place in its sequence.
+    ``q_weight``, ``k_weight``: ``[D]`` of the RMS norm (``eps``) of each head's row in front of that; None: no norm.  All of it in fp32, rounded once: to the rows' type, or to the cache's 8 bits.
+    Queries of no sequence, and of sequences whose ``lens`` is below their rows, become zeros (in ``out``: left as they are).  As in :func:`cache_write`, what has no place is not written."""
+    k = _check_rows(k, "k", cache)
+    v = _check_rows(v, "v", cache, k)
+    assert k.shape == v.shape and k.shape[1] == cache.heads, "k and v must be [rows, heads, D] of the cache"
+    part, table = cache._part(k.dtype), _check_table(cache, table)
+    B, rows, D = table.shape[0], k.shape[0], cache.head_dim
+    lens = _check_numbers(lens, B, cache, "as many lengths as the table has sequences: its")
+    if cu is None:
+        assert rows == B, "one row for each sequence, or offsets"
+    else:
+        cu = _check_numbers(cu, B + 1, cache, "one offset more than the table has sequences: its")
+    if q is None:
+        assert out is None and q_weight is None, "out and q_weight are the queries'"
+        o, Hq = None, 0
+    else:
+        q = _check_rows(q, "q", cache, k)
+        Hq = q.shape[1]
+        assert q.shape[0] == rows and Hq >= 1, "q must be [rows, Hq, D], a row for each of k's"
+        if out is None:
+            o = torch.empty_like(q) if q.is_contiguous() else torch.empty((rows, Hq, D), dtype=q.dtype, device=q.device)
+        else:
+            assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out must have q's shape, type and device"
+            if not packed_ready(out):
+                raise ValueError("out: rows of 16-byte steps are written in place, this view cannot be")
+            o = out
+    q_weight, k_weight = _check_weight(q_weight, k, "q_weight"), _check_weight(k_weight, k, "k_weight")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        q_weight, k_weight = q_weight.float(), k_weight.float()
+    weight_16 = any(w is not None and w.dtype != torch.float32 for w in (q_weight, k_weight))
+    axes, pairs = 1, 0
+    if freqs is None:
+        assert positions is None, "positions need freqs"
+    else:
+        assert freqs.dim() in (1, 2) and freqs.is_floating_point(), "freqs must be [pairs] or [axes, pairs]"
+        if freqs.dtype != torch.float32 or freqs.get_device() != cache._index or not freqs.is_contiguous() or freqs.data_ptr() % 16:
+            freqs = freqs.to(device=cache.device, dtype=torch.float32).clone(memory_format=torch.contiguous_format)
+        axes, pairs = freqs.shape if freqs.dim() == 2 else (1, freqs.shape[0])
+        assert pairs % 8 == 0 and 2 * pairs <= D and axes >= 1, "freqs hold a multiple of 8 pairs, of at most D channels"
+        assert positions is not None or axes == 1, "several axes need positions"
+    if positions is not None:
+        positions = int32_on(positions, cache.device)
+        if positions.dim() == 1:
+            positions = positions[:, None]
+        assert positions.dim() == 2 and positions.shape == (rows, axes), "positions must be [rows, axes]"
+        if (axes > 1 and positions.stride(1) != 1) or positions.stride(0) < 0:
+            positions = positions.contiguous()
+    at = lambda x: 0 if x is None else x.data_ptr()
+    desc = part + _call(table, lens.data_ptr(), at(cu), rows, k.data_ptr(), v.data_ptr(), k.stride()[:2], v.stride()[:2], 0 if out is not None else 1, Hq, 0.0, at(q), at(o),
+                        (0, 0) if q is None else q.stride()[:2], (0, 0) if q is None else o.stride()[:2])
+    rope = _ROPE.pack(at(freqs), at(positions), 0 if positions is None else positions.stride(0), at(q_weight), at(k_weight), pairs, axes, 1 if interleaved else 0, 1 if weight_16 else 0, eps, 0)
+    on_device(cache._index, _lib.load_library().cosmos_attn_cache_append, desc, rope)
+    return o
 
 
 def cache_read(cache: KVCache, table: torch.Tensor, cu: torch.Tensor, rows: int, dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:

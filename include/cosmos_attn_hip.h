@@ -514,6 +514,27 @@ COSMOS_ATTN_API int cosmos_attn_cache_window(const cosmos_attn_cache_desc *desc,
 COSMOS_ATTN_API size_t cosmos_attn_cache_chunk_workspace_bytes(const cosmos_attn_cache_desc *desc, int64_t window, int64_t sinks);
 COSMOS_ATTN_API int cosmos_attn_cache_chunk(const cosmos_attn_cache_desc *desc, int64_t window, int64_t sinks, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * cosmos_attn_cache_append: cosmos_attn_cache_write of keys that are normalised and turned by their positions first, and of their values, with the queries of the same tokens in the same pass.
+ * q, o [rows, Hq, D] (o may be q; q NULL: no queries), k_rows, v_rows [rows, Hkv, D]; lens, cu, table as in cosmos_attn_cache_write.  A row x of a head of q or k becomes
+ *     x rsqrt(mean(x^2) + eps) w                                   where there is a weight w
+ *     (u, v) -> (u cos a_i - v sin a_i, v cos a_i + u sin a_i)     for `pairs` pairs of channels, (i, i + pairs) or with `interleaved` (2 i, 2 i + 1);   a_i = sum over axes of position * freqs[axis][i]
+ * in fp32 (angles in 64 bits), rounded once, to `dtype` or to the cache's codes.  The position is the token's place in its sequence, or positions[row][axis].
+ * Rows of o of no sequence, and of sequences with lens[i] below their rows, are left as they are, or with `fill` become zeros; their keys and values, and those whose place is not there, are not written.
+ */
+typedef struct cosmos_attn_cache_rope {
+    const float *freqs;                /* [axes, pairs] */
+    const int32_t *positions;          /* [rows, axes], rows positions_stride elements apart, or NULL: places in the sequences (one axis) */
+    int64_t positions_stride;
+    const void *q_weight, *k_weight;   /* [D] fp32, or of `dtype` with weight_16; NULL: no norm */
+    int32_t pairs, axes;               /* pairs % 8 == 0, 2 pairs at most D; axes 1 .. 8 */
+    int32_t interleaved, weight_16;
+    float eps;
+    int32_t reserved;
+} cosmos_attn_cache_rope;
+
+COSMOS_ATTN_API int cosmos_attn_cache_append(const cosmos_attn_cache_desc *desc, const cosmos_attn_cache_rope *rope, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -102,6 +102,27 @@ def dequantise(codes, scale):
     return codes.float().double() * scale.double()[..., None]
 
 
+def turned(x, weight, eps, positions, freqs, interleaved):
+    """(y, bound): rows [n, heads, D] normalised (weight None: not) and turned, positions [n, axes] and freqs [axes, pairs], in 64 bits; how far arithmetic in fp32 may be from it.
+    The norm: D + 2 roundings of a sum under a root, its own two and the product's: (D + 2) / 2 + 4.  cos and sin: an angle in turns is rounded to fp32 below 1/2, 2^-26 of a turn, 2 pi 2^-26 < 2^-23;
+    the series and their last steps another 2^-23; formed in 64 bits it is off by 2^-52 of itself.  Two products and a sum: 3."""
+    x = x.double().cpu()
+    off = torch.zeros(x.shape[:2] + (1,), dtype=torch.float64)
+    if weight is not None:
+        x = x / ((x * x).mean(-1, keepdim=True) + eps).sqrt() * weight.double().cpu()
+        off = off + ((x.shape[2] + 2) / 2 + 4) * F32
+    y, far = x.clone(), off * x.abs()
+    if freqs is not None:
+        angle = positions.double().cpu() @ freqs.double().cpu()
+        turns = (positions.double().cpu().abs() @ freqs.double().cpu().abs())[:, None]
+        c, s, R = angle.cos()[:, None], angle.sin()[:, None], freqs.shape[1]
+        a, b = (slice(0, 2 * R, 2), slice(1, 2 * R, 2)) if interleaved else (slice(0, R), slice(R, 2 * R))
+        u, v = x[..., a], x[..., b]
+        y[..., a], y[..., b] = u * c - v * s, v * c + u * s
+        far[..., a] = far[..., b] = (off + 2.0 ** -22 + 3 * F32 + 2.0 ** -50 * turns) * (u.abs() + v.abs())
+    return y, far
+
+
 def decode(q, keys, values, scale, dtype):
     """One token of each sequence over its rows (lists of [n, Hkv, D] in 64 bits): (o, lse, their bounds)."""
     q = q.double().cpu()

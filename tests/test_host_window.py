@@ -90,3 +90,51 @@ def test_refusals_of_pieces(pkg, monkeypatch):
     ]:
         with pytest.raises(error):
             call()
+
+
+def rope(pkg, **over):
+    R = pkg._lib.CacheRope()
+    R.freqs, R.pairs, R.axes, R.eps = P, 32, 1, 1e-6
+    for k, v in over.items():
+        setattr(R, k, v)
+    return R
+
+
+def test_append_layout_and_status_codes(pkg):
+    L, lib = pkg._lib, pkg._lib.load_library()
+    assert ctypes.sizeof(L.CacheRope) == 64 == pkg.kv_cache._ROPE.size and L.CacheRope.pairs.offset == 40 and L.CacheRope.eps.offset == 56
+    append = lambda D, R: lib.cosmos_attn_cache_append(ctypes.byref(D), ctypes.byref(R), None)
+    for over, status in [(dict(abi_version=1), L.ST_BAD_ARG), (dict(kind=3), L.ST_UNSUPPORTED), (dict(D=32), L.ST_UNSUPPORTED), (dict(rows=5), L.ST_BAD_SHAPE), (dict(lens=None), L.ST_BAD_ARG),
+                         (dict(k_rows=None), L.ST_BAD_ARG), (dict(v_rows_stride=(128, 60)), L.ST_BAD_STRIDE), (dict(rows=-1), L.ST_BAD_ARG), (dict(Hq=0), L.ST_BAD_ARG), (dict(o=None), L.ST_BAD_ARG),
+                         (dict(q_stride=(512, 60)), L.ST_BAD_STRIDE), (dict(o_stride=(64, 64)), L.ST_BAD_STRIDE), (dict(v=P), L.ST_BAD_ARG), (dict(k_stride=(0, 2048, 64)), L.ST_BAD_STRIDE),
+                         (dict(cu=P, rows=1 << 30, Hq=64, Hkv=8, q_stride=(4096, 64), o_stride=(4096, 64), k_stride=(8 * 32 * 64, 32 * 64, 64), v_stride=(8 * 32 * 64, 32 * 64, 64), k_scale_stride=(256, 32),
+                               v_scale_stride=(256, 32)), L.ST_UNSUPPORTED)]:
+        assert append(cache_desc(pkg, **over), rope(pkg)) == status, over
+    for over, status in [(dict(pairs=12), L.ST_BAD_SHAPE), (dict(pairs=40), L.ST_BAD_SHAPE), (dict(pairs=-8), L.ST_BAD_ARG), (dict(axes=0), L.ST_BAD_ARG), (dict(axes=9, positions=P), L.ST_UNSUPPORTED),
+                         (dict(axes=2), L.ST_BAD_ARG), (dict(freqs=None), L.ST_BAD_ARG), (dict(freqs=P + 4), L.ST_BAD_STRIDE), (dict(q_weight=P + 8), L.ST_BAD_STRIDE), (dict(positions=P + 2), L.ST_BAD_STRIDE),
+                         (dict(positions=P, positions_stride=-1), L.ST_BAD_STRIDE), (dict(eps=float("nan")), L.ST_BAD_ARG), (dict(eps=-1.0), L.ST_BAD_ARG)]:
+        assert append(cache_desc(pkg), rope(pkg, **over)) == status, over
+    assert append(cache_desc(pkg, rows=0, cu=P, k_rows=None, q=None), rope(pkg)) == L.ST_OK
+    assert lib.cosmos_attn_cache_append(ctypes.byref(cache_desc(pkg)), None, None) == L.ST_BAD_ARG
+
+
+def test_refusals_of_append(pkg, monkeypatch):
+    def no_launch(*a):
+        raise AssertionError("launched")
+
+    monkeypatch.setattr(pkg.kv_cache, "on_device", no_launch)
+    new = lambda *shape, dtype=torch.bfloat16: on(torch.zeros(*shape, dtype=dtype))
+    f32 = torch.float32
+    cache = pkg.KVCache(new(5, 2, 16, 64), new(5, 2, 16, 64))
+    table, lens, q, k, freqs = new(3, 2, dtype=torch.int32), new(3, dtype=torch.int32), new(3, 4, 64), new(3, 2, 64), new(32, dtype=f32)
+    for args, over, error in [
+        ((q, k, new(4, 2, 64)), {}, AssertionError), ((q, new(4, 2, 64), new(4, 2, 64)), {}, AssertionError), ((new(4, 4, 64), k, k), {}, AssertionError), ((q, new(3, 1, 64), new(3, 1, 64)), {}, AssertionError),
+        ((new(3, 4, 64, dtype=torch.float16), k, k), {}, AssertionError), ((new(3, 4, 128), k, k), {}, AssertionError), ((q, k, k), dict(freqs=new(30, dtype=f32)), AssertionError),
+        ((q, k, k), dict(freqs=new(40, dtype=f32)), AssertionError), ((q, k, k), dict(freqs=new(2, 32, dtype=f32)), AssertionError), ((q, k, k), dict(freqs=new(32, dtype=torch.int32)), AssertionError),
+        ((q, k, k), dict(freqs=freqs, positions=new(4, dtype=torch.int32)), AssertionError), ((q, k, k), dict(freqs=freqs, positions=new(3, 2, dtype=torch.int32)), AssertionError),
+        ((q, k, k), dict(freqs=freqs, positions=new(3, dtype=f32)), AssertionError), ((q, k, k), dict(freqs=None, positions=new(3, dtype=torch.int32)), AssertionError),
+        ((q, k, k), dict(q_weight=new(32)), AssertionError), ((None, k, k), dict(q_weight=new(64)), AssertionError), ((None, k, k), dict(out=q), AssertionError), ((q, k, k), dict(out=new(3, 2, 64)), AssertionError),
+        ((q, k, k), dict(out=on(torch.zeros(3, 4, 128, dtype=torch.bfloat16)[:, :, ::2])), ValueError), ((q, k, k), dict(cu=lens), AssertionError),
+    ]:
+        with pytest.raises(error):
+            pkg.cache_append(cache, *args, table, lens, **{"freqs": freqs, **over})
