@@ -22,6 +22,8 @@ struct RaggedParams {
     const int* lens;               // keys in pages: a sequence's number of them, which `most_keys` is the most of
     int most_keys;
     int64_t lse_row, lse_head;     // elements
+    int piece, slots, sink_tiles;  // the first keys' tiles, dk and dv: steps of a piece, pieces that there may be, tiles of a sequence
+    float* pieces;                 // of slot s, tile j and key head h, at (s sink_tiles + j) Hkv + h
     float* parts;                  // what they leave: of part s of tile i and key head h, at (i Hkv + h) most_parts + s
     float scale, scale_log2;       // scale_log2 >= 0: `flip` says that q's signs are turned instead
     unsigned flip;
@@ -227,6 +229,12 @@ template <bool KEYS, int ROWS, int STEP, bool WINDOW = false, bool PAGED = false
         return (keys(n, last < rows ? last : rows - 1) + STEP - 1) / STEP - gap(n, tile);
     }
     __device__ __forceinline__ int steps(Lengths n, int tile) const { return end_step(n, tile) - first_step(n, tile); }
+    // pieces that a tile with some of the first keys is cut into, 0 or 2 and more
+    __device__ __forceinline__ int pieces(Lengths n, int tile) const {
+        if (!WINDOW || !KEYS || tile >= p.sink_tiles || n.lq <= 0) return 0;
+        const int count = (n.lq * p.group / STEP - first_step(n, tile)) / p.piece;
+        return count > 1 ? count : 0;
+    }
     // of all of its tiles: all of them times the mean of the longest and the shortest; of a window's, which are of one length but for the first rows' and the first keys', the middle one
     __device__ __forceinline__ int64_t all_steps(Lengths n, int tiles) const {
         if (WINDOW) return (int64_t)tiles * steps(n, tiles / 2) + (KEYS && tiles > 1 ? steps(n, 0) : 0);
@@ -359,6 +367,32 @@ __device__ __forceinline__ Block block_of(const RaggedParams& p, int b) {
     return {b - rest * p.Hkv, rest - before * p.tiles, p.most_parts - 1 - before};
 }
 
+// ---- WINDOW, dk and dv: the first keys are seen by all rows, so that their tiles have all of a sequence's steps where the others have a window's.  From two pieces of `piece` steps on such a tile is
+// cut into these (the last one has what is left over), in workgroups of their own, which go first.  How many there are follows from the rows, and which slot a piece has from its place
+// among all of them: pieces are `piece` STEP rows and more, disjoint, so that no two begin in one slot of as many rows.
+template <int STEP> __device__ __forceinline__ int slot_of(const RaggedParams& p, int row0, int step) { return (int)(((int64_t)row0 + (int64_t)step * STEP) / ((int64_t)p.piece * STEP)); }
+struct Piece { int seq, index, count; Lengths n; };      // seq < 0: no piece begins there
+template <typename Kind, int STEP> __device__ __forceinline__ Piece find_piece(const RaggedParams& p, int tile, int slot) {
+    const Kind T{p};
+    const int lane = threadIdx.x & 63;
+    const int64_t size = (int64_t)p.piece * STEP;
+    int end_q = 0, end_k = 0;
+    for (int base = 0; base < p.n_seq; base += 64) {
+        const Own q = apart(p.cu_q, base, p.n_seq, p.Tq, end_q), k = apart(p.cu_k, base, p.n_seq, p.Tk, end_k);
+        const Lengths n = {q.length, k.length};
+        const int count = tile < T.count(n) ? T.pieces(n, tile) : 0;
+        const int64_t first = (int64_t)q.start * p.group + (int64_t)T.first_step(n, tile) * STEP, past = slot * size - first;
+        const int64_t index = past <= 0 ? 0 : (past + size - 1) / size;
+        const bool mine = index < count && first + index * size < (slot + 1) * size;
+        const unsigned long long found = __ballot(mine);
+        if (found) {
+            const int at = __builtin_ctzll(found);
+            return {base + at, __builtin_amdgcn_readlane((int)index, at), __builtin_amdgcn_readlane(count, at), {__builtin_amdgcn_readlane(n.lq, at), __builtin_amdgcn_readlane(n.lk, at)}};
+        }
+    }
+    return {-1, 0, 0, {0, 0}};
+}
+
 // ---- rows of no sequence: zeros, lse = -inf.  They are counted through, whatever lies between them, and a workgroup behind the last tile has `rows` of them.
 template <int D> __device__ __forceinline__ void clear_rows(char* out, int64_t row, int64_t head, const int* cu, int n, int total, int heads, int first_head, int rows, Found f, float* lse, int64_t lse_row = 0, int64_t lse_head = 0) {
     constexpr int CHUNKS = D / 8;
@@ -408,6 +442,9 @@ __global__ void __launch_bounds__(kJoinThreads) __attribute__((amdgpu_num_sgpr(8
     const int head = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv % p.tiles;
     const Found f = find<std::conditional_t<KEYS, KeyTiles<D, WINDOW>, RowTilesOf<WINDOW, PAGED>>, kJoinThreads>(p, index);
     if (f.seq < 0 || f.parts <= 1) return;
+    if constexpr (KEYS && WINDOW) {
+        if (KeyTiles<D, WINDOW>{p}.pieces(f.n, f.tile)) return;
+    }
     const int c = 4 * (threadIdx.x % LANES);
     const Range r = rows_of_sequence(KEYS ? p.cu_k : p.cu_q, f.seq, KEYS ? f.n.lk : f.n.lq);
     const int rows = KEYS ? r.length : r.length * p.group;
@@ -451,6 +488,35 @@ __global__ void __launch_bounds__(kJoinThreads) __attribute__((amdgpu_num_sgpr(8
             store(p.dv + (r.start + token) * p.dv_row + h * p.dv_head, sum[1]);
         }
     }
+#endif
+}
+
+// WINDOW: the pieces of a tile with some of the first keys, at the workgroup whose slot is the first one's.  A key's sums are in the pieces with a row that sees it: a first key's in all.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) ragged_pieces_kernel(const RaggedParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int LANES = D / 4, AT_ONCE = kJoinThreads / LANES, STEP = row_step(D);
+    typedef KeyTiles<D, true> Tiles;
+    const int head = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv, tile = rest % p.sink_tiles, slot = rest / p.sink_tiles % p.slots;
+    const Piece f = find_piece<Tiles, STEP>(p, tile, slot);
+    if (f.seq < 0 || f.index) return;
+    const Range q = rows_of_sequence(p.cu_q, f.seq, f.n.lq), k = rows_of_sequence(p.cu_k, f.seq, f.n.lk);
+    const int c = 4 * (threadIdx.x % LANES), i = rest / p.sink_tiles / p.slots * AT_ONCE + threadIdx.x / LANES, key = tile * kRows + i;
+    if (key >= k.length) return;
+    const Tiles tiles{p};
+    const int begin = tiles.first_step(f.n, tile), until = tiles.end_row(f.n, key);
+    f32x4 dk = {0.f, 0.f, 0.f, 0.f}, dv = dk;
+#pragma unroll 4
+    for (int s = 0; s < f.count; ++s) {
+        const int step = begin + s * p.piece;
+        if (step * STEP >= until) break;
+        const float* const at = p.pieces + (((int64_t)slot_of<STEP>(p, q.start * p.group, step) * p.sink_tiles + tile) * p.Hkv + head) * (2 * kRows * D) + i * D + c;
+        dk += *reinterpret_cast<const f32x4*>(at);
+        dv += *reinterpret_cast<const f32x4*>(at + kRows * D);
+    }
+    dk *= p.scale;
+    *reinterpret_cast<u32x2*>(p.dk + (k.start + key) * p.dk_row + head * p.dk_head + 2 * c) = u32x2{round2<T>(dk[0], dk[1]), round2<T>(dk[2], dk[3])};
+    *reinterpret_cast<u32x2*>(p.dv + (k.start + key) * p.dv_row + head * p.dv_head + 2 * c) = u32x2{round2<T>(dv[0], dv[1]), round2<T>(dv[2], dv[3])};
 #endif
 }
 

@@ -415,16 +415,30 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     __shared__ __attribute__((aligned(1024))) char values[V_IN_LDS ? LV::BYTES : 16];
     __shared__ __attribute__((aligned(16))) float stats0[2 * STEP], stats1[2 * STEP];      // lse, delta of a step's rows
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const Block block = block_of(p, blockIdx.x);
+    // (WINDOW: the pieces of the first keys' tiles go first)
+    const int pieces = WINDOW ? p.slots * p.sink_tiles * p.Hkv : 0;
+    const bool of_piece = WINDOW && (int)blockIdx.x < pieces;
+    const Block block = of_piece ? Block{(int)blockIdx.x % p.Hkv, 0, 0} : block_of(p, blockIdx.x - pieces);
     const int head = block.head;
-    const Found f = find<KeyTiles<D, WINDOW>>(p, block.index);
+    Found f = {-1, 0, 1, {0, 0}, false};
+    Piece piece = {0, 0, 0, {0, 0}};
+    if (of_piece) {
+        const int slot = blockIdx.x / (p.Hkv * p.sink_tiles);
+        f.tile = blockIdx.x / p.Hkv % p.sink_tiles;
+        piece = find_piece<KeyTiles<D, WINDOW>, STEP>(p, f.tile, slot);
+        if (piece.seq < 0) return;
+        f.seq = piece.seq;
+        f.n = piece.n;
+    } else {
+        f = find<KeyTiles<D, WINDOW>>(p, block.index);
+    }
     if (f.seq < 0) {
         if (block.part) return;
         clear_rows<D>(p.dk, p.dk_row, p.dk_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f, nullptr);
         clear_rows<D>(p.dv, p.dv_row, p.dv_head, p.cu_k, p.n_seq, p.Tk, 1, head, kRows, f, nullptr);
         return;
     }
-    if (block.part >= f.parts) return;
+    if (block.part >= f.parts || (WINDOW && !of_piece && KeyTiles<D, WINDOW>{p}.pieces(f.n, f.tile))) return;
     const Range rq = rows_of_sequence(p.cu_q, f.seq, f.n.lq), rk = rows_of_sequence(p.cu_k, f.seq, f.n.lk);
     const int lq = rq.length > 0 ? rq.length : 0;
     const int key0 = f.tile * kRows, key = key0 + 32 * wave + (lane & 31);
@@ -438,7 +452,11 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     const int wave_first = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave)), wave_all = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave + 31));
     // steps of this part
     const int begin = tiles.first_step(f.n, f.tile), steps = tiles.end_step(f.n, f.tile) - begin;
-    const int t0 = begin + (int)((int64_t)block.part * steps / f.parts), n = begin + (int)((int64_t)(block.part + 1) * steps / f.parts);
+    int t0 = begin + (int)((int64_t)block.part * steps / f.parts), n = begin + (int)((int64_t)(block.part + 1) * steps / f.parts);
+    if (of_piece) {
+        t0 = begin + piece.index * p.piece;
+        if (piece.index + 1 < piece.count) n = t0 + p.piece;
+    }
 
     if constexpr (V_IN_LDS) {
         const auto vr = rows_of<D, kRows>(p.v + (rk.start + (int64_t)key0) * p.v_row + head * p.v_head, p.v_row, rk.length - key0);
@@ -591,8 +609,10 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
             dv[b] *= power_of_two(-kUpP);
         }
     }
-    if (f.parts > 1) {
-        float* const part = p.parts + (((int64_t)block.index * p.Hkv + head) * p.most_parts + block.part) * (2 * kRows * D) + (32 * wave + (lane & 31)) * D;
+    if (of_piece && until <= t0 * STEP) return;          // (no row of the piece sees the key, and none is added up for it)
+    if (f.parts > 1 || of_piece) {
+        float* const part = (of_piece ? p.pieces + (int64_t)blockIdx.x * (2 * kRows * D) : p.parts + (((int64_t)block.index * p.Hkv + head) * p.most_parts + block.part) * (2 * kRows * D)) +
+                            (32 * wave + (lane & 31)) * D;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -709,17 +729,37 @@ struct Cut { int64_t tiles; int parts, least; size_t bytes; };
 struct Window { int window = 0, sinks = 0; };
 int check_window(const cosmos_attn_ragged_desc* d, int64_t window, int64_t sinks) {
     if (window < 0 || sinks < 0) return COSMOS_ATTN_BAD_ARG;
+    // (a few thousand workgroups more than without)
+    if (window && ((d->Tq * (d->Hq / d->Hkv) + d->Tk) / kRows + d->n_seq + 1) * d->Hkv > kMostBlocks - 4096) return COSMOS_ATTN_UNSUPPORTED;
     return window && !d->causal ? COSMOS_ATTN_UNSUPPORTED : COSMOS_ATTN_OK;
 }
 Window window_of(const cosmos_attn_ragged_desc* d, int64_t window, int64_t sinks) {
     return window && window < d->Tk && sinks < d->Tk ? Window{(int)window, (int)sinks} : Window{};
 }
+// The first keys' tiles of dk and dv: pieces of three quarters of a window's steps, 1024 rows at least, and not more pieces than twice the workgroups that run at once (what they leave is 128 MB then).
+struct Pieces { int piece, slots, tiles; size_t bytes; };
+Pieces pieces_of(const cosmos_attn_ragged_desc* d, Window w) {
+    if (!w.window || !w.sinks || !d->Tq) return {};
+    const int step = row_step(d->D);
+    const int64_t group = d->Hq / d->Hkv, rows = d->Tq * group, tiles = (w.sinks + kRows - 1) / kRows, most = 4 * kNumCUs / (tiles * d->Hkv) + 1;
+    if (tiles * d->Hkv > 2 * kNumCUs) return {};         // (so many fill the chip as they are)
+    int64_t piece = 3 * ((int64_t)w.window + kRows) * group / (4 * step);
+    piece = piece > 1024 / step ? piece : 1024 / step;
+    piece = piece > rows / (step * most) ? piece : rows / (step * most) + 1;
+    if (piece > rows / (2 * step)) return {};            // (no sequence has two)
+    const int64_t slots = rows / (piece * step) + 1;
+    return {(int)piece, (int)slots, (int)tiles, (size_t)(slots * tiles * d->Hkv) * 2 * kRows * d->D * sizeof(float)};
+}
 Cut cut_of(const cosmos_attn_ragged_desc* d, int which, Window w) {
     const int step = row_step(d->D);
     const int64_t group = d->Hq / d->Hkv, rows = d->Tq * group, tiles = which == 2 ? most_tiles(d->Tk, d->n_seq) : most_tiles(rows, d->n_seq);
     int64_t longest = which == 2 ? (rows + step - 1) / step : (d->Tk + kStep - 1) / kStep;
-    if (w.window && !(which == 2 && w.sinks)) {       // (the first keys' tiles are as long as ever)
-        const int64_t seen = which == 2 ? ((int64_t)w.window + kRows) * group / step + 2 : ((int64_t)w.window + kRows / group + 1) / kStep + 2 + (w.sinks + kStep - 1) / kStep;
+    if (w.window) {
+        int64_t seen = which == 2 ? ((int64_t)w.window + kRows) * group / step + 2 : ((int64_t)w.window + kRows / group + 1) / kStep + 2 + (w.sinks + kStep - 1) / kStep;
+        if (which == 2 && w.sinks) {                  // (the first keys' tiles that are not cut into pieces)
+            const Pieces cut = pieces_of(d, w);
+            seen = !cut.piece ? longest : seen > 2 * cut.piece + 1 ? seen : 2 * cut.piece + 1;
+        }
         longest = seen < longest ? seen : longest;
     }
     const int least = which == 2 ? least_rows(d->D) / step : least_steps(d->D), parts = most_parts(tiles * d->Hkv, longest, least);
@@ -760,7 +800,7 @@ size_t backward_bytes(const cosmos_attn_ragged_desc* desc, int64_t window, int64
     if (check(desc, true) != COSMOS_ATTN_OK || check_window(desc, window, sinks) != COSMOS_ATTN_OK) return 0;
     const Window w = window_of(desc, window, sinks);
     const size_t a = cut_of(desc, 1, w).bytes, b = cut_of(desc, 2, w).bytes;
-    return up((size_t)desc->Tq * desc->Hq * sizeof(float)) + (a > b ? a : b);
+    return up((size_t)desc->Tq * desc->Hq * sizeof(float)) + up(a > b ? a : b) + pieces_of(desc, w).bytes;
 }
 int backward(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
     int st = check(desc, true);
@@ -775,19 +815,27 @@ int backward(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks,
     p.window = w.window; p.sinks = w.sinks;
     p.delta = (float*)workspace;
     p.parts = (float*)((char*)workspace + up((size_t)desc->Tq * desc->Hq * sizeof(float)));      // (of dq, then of dk and dv)
+    const Pieces pieces = pieces_of(desc, w);
+    p.piece = pieces.piece; p.slots = pieces.slots; p.sink_tiles = pieces.tiles;
+    p.pieces = (float*)((char*)workspace + wanted - pieces.bytes);
     return with_type(desc->dtype, desc->D, [&](auto* t, auto d) {
         constexpr int D = decltype(d)::value;
         typedef std::remove_pointer_t<decltype(t)> T;
         int done = COSMOS_ATTN_OK;
-        auto one = [&](const Cut& cut, auto kernel, auto join) {
+        auto one = [&](const Cut& cut, auto kernel, auto join, int64_t before = 0) {
             p.tiles = (int)cut.tiles; p.most_parts = cut.parts; p.least = cut.least;
-            if (done == COSMOS_ATTN_OK) done = launch(kernel, cut.tiles * p.Hkv * cut.parts, p, stream);
+            if (done == COSMOS_ATTN_OK) done = launch(kernel, before + cut.tiles * p.Hkv * cut.parts, p, stream);
             if (done == COSMOS_ATTN_OK && cut.parts > 1) done = launch(join, cut.tiles * p.Hkv * kJoinBlocks<D>, p, stream, kJoinThreads);
         };
         auto run = [&](auto windowed) {
             constexpr bool WINDOW = decltype(windowed)::value;
             if (desc->Tq) one(cut_of(desc, 1, w), ragged_dq_kernel<T, D, WINDOW>, ragged_join_kernel<T, D, 1, WINDOW>);
-            if (desc->Tk) one(cut_of(desc, 2, w), ragged_dkdv_kernel<T, D, WINDOW>, ragged_join_kernel<T, D, 2, WINDOW>);
+            if (!desc->Tk) return done;
+            const int64_t blocks = (int64_t)p.slots * p.sink_tiles * p.Hkv;
+            one(cut_of(desc, 2, w), ragged_dkdv_kernel<T, D, WINDOW>, ragged_join_kernel<T, D, 2, WINDOW>, blocks);
+            if constexpr (WINDOW) {
+                if (done == COSMOS_ATTN_OK && blocks) done = launch(ragged_pieces_kernel<T, D>, blocks * kJoinBlocks<D>, p, stream, kJoinThreads);
+            }
             return done;
         };
         return w.window ? run(Int<1>{}) : run(Int<0>{});

@@ -54,6 +54,30 @@ def test_tiles_that_are_cut(pkg, ragged_oracle, gpu, ql, kl, window, sinks):
     both(pkg, ragged_oracle, gpu, ql, kl, 2, 1, 64, BF16, window, sinks)
 
 
+@pytest.mark.parametrize("D, dtype", [(64, BF16), (64, FP16), (128, BF16), (128, FP16)])
+@pytest.mark.parametrize("ql, kl, window, sinks", [([2200], [2200], 10, 1), ([1100, 60, 2500], [1100, 60, 2500], 40, 4), ([2300, 1200], [2600, 900], 150, 129), ([3000], [2000], 30, 260), ([4100], [4100], 1500, 128)])
+def test_first_keys_in_pieces(pkg, ragged_oracle, gpu, ql, kl, window, sinks, D, dtype):
+    """Tiles of first keys that all rows see, cut into pieces of 1024 rows and more."""
+    both(pkg, ragged_oracle, gpu, ql, kl, 2, 1, D, dtype, window, sinks)
+
+
+def test_first_keys_in_pieces_of_many_sequences(pkg, ragged_oracle, gpu):
+    """Pieces that begin close to each other's ends, sequences of one piece and of none between, offsets that go back."""
+    lens = [1030, 1, 0, 2050, 511, 512, 1024, 513, 3] + [7] * 70 + [1500]
+    both(pkg, ragged_oracle, gpu, lens, lens, 2, 1, 64, BF16, 5, 2)
+    n = sum(lens)
+    q, k, v, g = (rows(n, h, 64, BF16, gpu, i) for i, h in enumerate((2, 1, 1, 2)))
+    at = cu(lens)
+    odd = at[:4] + [at[3] - 700, at[4]] + at[4:]           # one that begins inside of the one before, and the next one from there
+    on, once = offsets(odd, gpu), offsets(at, gpu)
+    o, lse = pkg.ragged_fwd(q, k, v, once, causal=True, window=5, sinks=2)
+    a = pkg.ragged_bwd(q, k, v, o, lse, g, once, causal=True, window=5, sinks=2)
+    b = pkg.ragged_bwd(q, k, v, o, lse, g, on, causal=True, window=5, sinks=2)
+    keep = torch.ones(n, dtype=torch.bool, device=gpu)
+    keep[at[3]:at[4]] = False
+    for x, y in zip(a, b):
+        assert torch.equal(x[keep], y[keep]) and y.isfinite().all()
+
 @pytest.mark.parametrize("n", [150, 300, 1100])
 def test_many_sequences(pkg, ragged_oracle, gpu, n):
     lens = [(7 * i * i) % 23 for i in range(n)]
