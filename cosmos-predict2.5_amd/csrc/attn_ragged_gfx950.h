@@ -525,8 +525,9 @@ inline int64_t most_tiles(int64_t rows, int n_seq) { return rows / kRows + n_seq
 // Parts that a tile may be cut into.  A call with fewer tiles than some rounds of workgroups ends with its longest tiles on a few compute units; one with more is dealt out evenly as it is.
 // (The workgroups of parts that a tile does not have end at once.)
 constexpr int64_t kFullGrid = 6 * kNumCUs;
-inline int most_parts(int64_t tiles, int64_t longest, int least) {
-    int64_t parts = (kFullGrid + tiles - 1) / tiles;
+// (WINDOW: tiles are of one length, so that there is nothing to deal out, and those that fill the chip once are left as they are.)
+inline int most_parts(int64_t tiles, int64_t longest, int least, bool window = false) {
+    int64_t parts = window ? kAtOnce / tiles : (kFullGrid + tiles - 1) / tiles;
     parts = parts < 16 ? parts : 16;
     const int64_t of_length = longest / least;
     parts = parts < of_length ? parts : of_length;

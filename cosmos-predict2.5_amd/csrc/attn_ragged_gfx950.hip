@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
                 s = mfma32(read_rows<V8>(kt + 32 * h * L::ROW, k_at[c]), qf[c], s);
                 g = mfma32(read_rows<V8>(vt + 32 * h * L::ROW, k_at[c]), gf[c], g);
             }
-            V8 df[2];
+            V8 df[2], dr[2];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], p.scale_log2, -lse2));
@@ -354,13 +354,25 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
                 u32x4 w;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = round2<T>(s[8 * c + 2 * i], s[8 * c + 2 * i + 1]);
+                if constexpr (WINDOW) {
+                    u32x4 x;
+                    asm("" : "+v"(w));          // (what the product takes)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = round2<T>(s[8 * c + 2 * i] - element<T>(w[i], 0), s[8 * c + 2 * i + 1] - element<T>(w[i], 1));
+                    dr[c] = __builtin_bit_cast(V8, x);
+                }
                 df[c] = __builtin_bit_cast(V8, w);
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) acc[b] = mfma32(read_channels<V8>(kt + (32 * h + 16 * c) * L::ROW, k_tr[b][0], k_tr[b][1]), df[c], acc[b]);
-            reads_ahead<4 * NB, 2 * NB, 8>();
+                for (int b = 0; b < NB; ++b) {
+                    const V8 kt8 = read_channels<V8>(kt + (32 * h + 16 * c) * L::ROW, k_tr[b][0], k_tr[b][1]);
+                    acc[b] = mfma32(kt8, df[c], acc[b]);
+                    if constexpr (WINDOW) acc[b] = mfma32(kt8, dr[c], acc[b]);
+                }
+            if constexpr (WINDOW) reads_ahead<4 * NB, 4 * NB, 8>();
+            else reads_ahead<4 * NB, 2 * NB, 8>();
         }
     };
     for (int t = t0; t < n; t += 2) {
@@ -762,7 +774,7 @@ Cut cut_of(const cosmos_attn_ragged_desc* d, int which, Window w) {
         }
         longest = seen < longest ? seen : longest;
     }
-    const int least = which == 2 ? least_rows(d->D) / step : least_steps(d->D), parts = most_parts(tiles * d->Hkv, longest, least);
+    const int least = which == 2 ? least_rows(d->D) / step : least_steps(d->D), parts = most_parts(tiles * d->Hkv, longest, least, w.window != 0);
     return {tiles, parts, least, parts > 1 ? (size_t)tiles * d->Hkv * parts * kRows * (which == 0 ? d->D + 2 : which * d->D) * sizeof(float) : 0};
 }
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
