@@ -31,6 +31,14 @@ struct ChunkParams : RaggedParams {
     int pages, page_shift;
 };
 
+// what was written to LDS is there and all reads have returned; then the workgroup meets, with loads to registers under way
+__device__ __forceinline__ void meet_in_lds() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);           // lgkmcnt 0 alone
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // ---- A workgroup: as ragged_fwd_kernel, with K and V out of pages.
 // 16 bits: rows go straight to LDS; what lies behind the last key, and runs that no row of the tile sees, come as zeros.  8 bits: codes are loaded into registers a step earlier, become exact
 // 16-bit values on their way to LDS, K's scales multiply the scores and V's the weights, before these are rounded.
@@ -76,14 +84,16 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
     auto at_step = [&](int u) { return WINDOW && u >= sink_steps ? u + gap : u; };
     const int t0 = (int)((int64_t)block.part * steps / f.parts), n = (int)((int64_t)(block.part + 1) * steps / f.parts);
 
-    const int* const table = p.table + f.seq * p.table_row;
+    // (of constant memory, so that the scalar unit looks up: a vector load's result in scalar registers is waited for at once, with all loads in front of it)
+    typedef const __attribute__((address_space(4))) int* Table;
+    const Table table = (Table)(uintptr_t)(p.table + f.seq * p.table_row);
     const int mask = (1 << p.page_shift) - 1;
     const char* const kh = p.side[0].pages + head * p.side[0].head;
     const char* const vh = p.side[1].pages + head * p.side[1].head;
     // this wavefront's run of step u: its first key, and whether some row of the tile sees some of it
     auto run_of = [&](int u) { return at_step(u) * kStep + RUN * wave; };
     auto is_seen = [&](int key) { return key < tile_end && (!WINDOW || key + RUN > tile_first || key < p.sinks); };
-    auto look_up = [&](int u) { const int key = run_of(u); return u < n && is_seen(key) ? __builtin_amdgcn_readfirstlane(table[key >> p.page_shift]) : 0; };
+    auto look_up = [&](int u) { const int key = run_of(u); return table[(u < n && is_seen(key) ? key : tile_end - 1) >> p.page_shift]; };      // (there is a key: t0 < n)
     // WINDOW: keys of a run that no row of the tile sees, beside others that are seen
     auto is_hidden = [&](int key) { return WINDOW && key < tile_first && key >= p.sinks; };
 
@@ -111,33 +121,35 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
     };
     // 8 bits: 16 codes to a lane, CODE_ROWS rows at a time
     constexpr int CODE_LANES = D / 16, CODE_ROWS = 64 / CODE_LANES, CODE_LOADS = RUN / CODE_ROWS;
-    u32x4 codes[2][CODES ? CODE_LOADS : 1];
-    float scale = 0.f;             // lanes 0 .. RUN - 1: of K's rows, RUN .. 2 RUN - 1: of V's
-    auto load_codes = [&](int u, int page) __attribute__((always_inline)) {
+    struct Codes {
+        u32x4 codes[2][CODES ? CODE_LOADS : 1];
+        float scale[2];            // of row lane % RUN
+        bool none;                 // its page is not there
+    };
+    int code_off[2][CODES ? CODE_LOADS : 1];
+    // (Without a condition around the loads, whatever is there: behind a branch the compiler waits for all that are under way.  A run that is not there has no bytes, and reads as zeros.)
+    auto load_codes = [&](Codes& to, int u, int page) __attribute__((always_inline)) {
         const int key0 = run_of(u);
         const bool seen = u < n && is_seen(key0), there = page >= 0 && page < p.pages;
-        const int64_t at = there ? page : 0;
-        scale = 0.f;
+        const int left = seen && there ? (tile_end - key0 < RUN ? tile_end - key0 : RUN) : 0;
+        const bool partly = WINDOW && key0 < tile_first && key0 + RUN > p.sinks;
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < CODE_LOADS; ++i) codes[s][i] = u32x4{0, 0, 0, 0};
-        if (!seen) return;
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s) {
+            const Side& side = p.side[s];
+            const int64_t at = there ? page : 0;
+            const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>((s ? vh : kh) + at * side.page + (key0 & mask) * side.row), 0, left > 0 ? (int)((left - 1) * side.row) + D : 0, 0x00020000);
+            const auto scales = __builtin_amdgcn_make_buffer_rsrc(side.scales + at * side.scale_page + head * side.scale_head + (key0 & mask), 0, 4 * left, 0x00020000);
 #pragma unroll
             for (int i = 0; i < CODE_LOADS; ++i) {
-                const int r = i * CODE_ROWS + lane / CODE_LANES;
-                if (there && key0 + r < tile_end && !is_hidden(key0 + r))
-                    codes[s][i] = *reinterpret_cast<const u32x4*>((s ? vh : kh) + at * p.side[s].page + ((key0 & mask) + r) * p.side[s].row + 16 * (lane % CODE_LANES));
+                const bool hidden = partly && is_hidden(key0 + i * CODE_ROWS + lane / CODE_LANES);
+                to.codes[s][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, hidden ? (int)0x80000000 : code_off[s][i], 0, 0));
             }
-        const int r = lane % RUN;
-        if (lane < 2 * RUN && key0 + r < tile_end && !is_hidden(key0 + r)) {
-            const Side& side = p.side[lane / RUN];
-            scale = there ? side.scales[at * side.scale_page + head * side.scale_head + (key0 & mask) + r] : lane < RUN ? NAN : 0.f;
+            to.scale[s] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(scales, partly && is_hidden(key0 + lane % RUN) ? (int)0x80000000 : 4 * (lane % RUN), 0, 0));
         }
+        to.none = seen && !there;
     };
-    auto keep_codes = [&](char* kt, char* vt, float* st) __attribute__((always_inline)) {
+    auto keep_codes = [&](const Codes& of, char* kt, char* vt, float* st) __attribute__((always_inline)) {
+        auto& codes = of.codes;
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -155,20 +167,34 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
                     *reinterpret_cast<u32x4*>(to + (((chunk + h) ^ L::mix(r)) << 4)) = w;
                 }
             }
-        if (lane < 2 * RUN) st[(lane / RUN) * kStep + RUN * wave + lane % RUN] = scale;
+        if (lane < 2 * RUN) st[(lane / RUN) * kStep + RUN * wave + lane % RUN] = lane >= RUN ? of.scale[1] : of.none ? NAN : of.scale[0];
     };
-    int page = look_up(t0);
+    Codes even, odd;               // of steps t0, t0 + 2, ..; of the others
+    int page = 0, page2 = 0;
     if constexpr (CODES) {
-        load_codes(t0, page);
-        page = look_up(t0 + 1);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < CODE_LOADS; ++i) code_off[s][i] = (i * CODE_ROWS + lane / CODE_LANES) * (int)p.side[s].row + 16 * (lane % CODE_LANES);
     } else {
 #pragma unroll
         for (int i = 0; i < L::LOADS; ++i) {
             k_off[i] = L::load_row(lane, 0, i) * (int)p.side[0].row + L::load_byte(lane, wave, i);
             v_off[i] = L::load_row(lane, 0, i) * (int)p.side[1].row + L::load_byte(lane, wave, i);
         }
-        if (t0 < n) bring(t0, page, tile0, tile1);
-        page = look_up(t0 + 1);
+    }
+    if (t0 < n) {
+        page = look_up(t0);
+        page2 = look_up(t0 + 1);
+        if constexpr (CODES) {
+            load_codes(even, t0, page);
+            load_codes(odd, t0 + 1, page2);
+            page = look_up(t0 + 2);
+            page2 = look_up(t0 + 3);
+        } else {
+            bring(t0, page, tile0, tile1);
+            page = page2;
+        }
     }
 
     // Q as an operand: channels 16 c + 8 half .. + 7 of this lane's row
@@ -296,20 +322,21 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
         if constexpr (D == 64) __builtin_amdgcn_s_setprio(0);
     };
     if constexpr (CODES) {
-        // a step's codes are on their way while the one before is computed
-        auto next = [&](int u, char* kt, char* vt, float* st) __attribute__((always_inline)) {
-            keep_codes(kt, vt, st);
-            load_codes(u + 1, page);
-            page = look_up(u + 2);
+        // A step's codes are on their way while the two before are computed, and go to LDS during the one before.  (One step ahead: two workgroups of a unit have half as many bytes under way, 46 single
+        // tokens of up to 8000 keys beside two pieces in e4m3 ... us instead of ...)
+        auto next = [&](Codes& codes, int& at, int u, char* kt, char* vt, float* st) __attribute__((always_inline)) {
+            keep_codes(codes, kt, vt, st);
+            load_codes(codes, u + 2, at);
+            at = look_up(u + 4);
         };
-        if (t0 < n) next(t0, tile0, tile1, scales0);
+        if (t0 < n) next(even, page, t0, tile0, tile1, scales0);
         for (int t = t0; t < n; t += 2) {
-            meet();
-            if (t + 1 < n) next(t + 1, tile2, tile3, scales1);
+            meet_in_lds();
+            if (t + 1 < n) next(odd, page2, t + 1, tile2, tile3, scales1);
             step(t, tile0, tile1, scales0);
             if (t + 1 == n) break;
-            meet();
-            if (t + 2 < n) next(t + 2, tile0, tile1, scales0);
+            meet_in_lds();
+            if (t + 2 < n) next(even, page, t + 2, tile0, tile1, scales0);
             step(t + 1, tile2, tile3, scales1);
         }
     } else {
