@@ -29,7 +29,281 @@ struct ChunkParams : RaggedParams {
     const int* table;
     int64_t table_row;
     int pages, page_shift;
+    int short_blocks;              // workgroups of short sequences, behind the tiles'
+    float* short_sums;             // what their parts leave: of part s of the i-th and key head h, at (i Hkv + h) short_parts + s
 };
+
+// ---- Sequences of few rows (a token or some, of which the query heads of a key head are 16 at most together): keys and values go by once, for a product or two, and what counts is how many bytes are
+// under way.  A wavefront has 32 of 128 keys to a step, straight from memory into registers, as in cache_attention_kernel; rows are the columns of 16 x 16 x 32 products.
+constexpr int kShortRows = 16, kShortStep = 128;
+template <int D> constexpr int kShortFloats = kShortRows * (D + 2);       // of a part: its rows' D sums, then max and sum of exponentials
+// the keys that a sequence's tokens see, in steps: those of the first keys and, behind the `gap` that none looks at, those from the first token's window on
+template <bool WINDOW> struct Seen {
+    int from, first, gap, steps;
+    __device__ __forceinline__ Seen(const RaggedParams& p, Lengths n) {
+        const int len = n.lk > 0 ? n.lk : 0;
+        from = WINDOW && len - n.lq + 1 > p.window ? len - n.lq + 1 - p.window : 0;
+        first = ((p.sinks < from ? p.sinks : from) + kShortStep - 1) / kShortStep;
+        gap = WINDOW && from / kShortStep > first ? from / kShortStep - first : 0;
+        steps = (len + kShortStep - 1) / kShortStep - gap;
+    }
+};
+template <bool WINDOW> struct ShortTiles {
+    const RaggedParams& p;
+    __device__ __forceinline__ int keys_of(int i) const { return RowTilesOf<WINDOW, true>{p}.keys_of(i); }
+    __device__ __forceinline__ Lengths lengths(int i) const { return RowTilesOf<WINDOW, true>{p}.lengths(i); }
+    __device__ __forceinline__ int count(Lengths n) const { return n.lq > 0 && (int64_t)n.lq * p.group <= p.short_rows; }
+    static __device__ __forceinline__ int at(int rank, int) { return rank; }
+    __device__ __forceinline__ int steps(Lengths n, int) const { return Seen<WINDOW>(p, n).steps; }
+    __device__ __forceinline__ int64_t all_steps(Lengths n, int) const { return steps(n, 0); }
+    __device__ __forceinline__ int most_parts() const { return p.short_parts; }
+    __device__ __forceinline__ int least() const { return p.short_least; }
+    static constexpr bool OF_KEYS = false, IN_PAGES = true;
+};
+__device__ __forceinline__ float over_quarters_max(float x) {
+    x = over_halves_max(x);
+    return fmaxf(x, __shfl_xor(x, 16));
+}
+// row r of the sequence that begins at `start`: o and lse from its sums
+template <typename T> __device__ __forceinline__ void store_row(const ChunkParams& p, int start, int head, int r, int c, const float (&f)[8], float top, float sum, bool bad) {
+    const int token = r / p.group, hq = head * p.group + (r - token * p.group);
+    float by = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum, lse = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f : sum == 0.f ? -INFINITY : sum;
+    if (bad) by = lse = NAN;
+    *reinterpret_cast<u32x4*>(p.o + (start + token) * p.o_row + hq * p.o_head + 2 * c) = u32x4{round2<T>(f[0] * by, f[1] * by), round2<T>(f[2] * by, f[3] * by), round2<T>(f[4] * by, f[5] * by), round2<T>(f[6] * by, f[7] * by)};
+    if (p.lse && c == 0) p.lse[(start + token) * p.lse_row + hq] = lse;
+}
+// sums: two halves, of two wavefronts each
+template <typename T, int KIND, int D, bool WINDOW>
+__device__ __forceinline__ void short_sequence(const ChunkParams& p, const Found& f, int head, int index, int part, float* sums01, float* sums23, float* stat) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef typename VecOf<T>::v8 V8;
+    constexpr bool CODES = KIND != SAME16;
+    constexpr int BYTES = CODES ? 1 : 2, NC = D / 32, NB = D / 16;       // NC: products of 32 channels; NB: of 16 channels of the output, channels of a lane of V
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g = lane >> 4;
+    const Range rq = rows_of_sequence(p.cu_q, f.seq, f.n.lq);
+    const int rows = rq.length * p.group, len = f.n.lk > 0 ? f.n.lk : 0;
+    const Seen<WINDOW> seen(p, f.n);
+    const int from = (int)((int64_t)part * seen.steps / f.parts), to = (int)((int64_t)(part + 1) * seen.steps / f.parts);
+    const int* const table = p.table + f.seq * p.table_row;
+    const char* const kh = p.side[0].pages + head * p.side[0].head;
+    const char* const vh = p.side[1].pages + head * p.side[1].head;
+    const int mask = (1 << p.page_shift) - 1;
+    // Q: row n16, the channels that this lane's K holds
+    const int row = n16 < rows ? n16 : rows - 1, token = row / p.group, row_end = len - (rq.length - 1 - token);      // row_end: keys that it sees
+    V8 qf[NC];
+    {
+        const char* const at = p.q + (rq.start + token) * p.q_row + (head * p.group + (row - token * p.group)) * p.q_head;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            u32x4 w = *reinterpret_cast<const u32x4*>(at + 2 * (CODES ? 64 * (c / 2) + 16 * g + 8 * (c % 2) : 32 * c + 8 * g));
+            w ^= p.flip;
+            qf[c] = __builtin_bit_cast(V8, w);
+        }
+    }
+    f32x4 acc[NB];
+    float m = kLowest, l = 0.f, R = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // Steps of 32 keys.  A step's K is loaded behind the products of the one before, its V behind that one's, and its pages are looked up a step earlier still.  Keys past the end are the last
+    // one's, keys that no token sees the first one that is looked back on.
+    constexpr int KLOADS = CODES ? NC / 2 : NC, VWORDS = NB * BYTES / 4;
+    const int most = len - 1, first_key = 32 * wave;
+    auto base_of = [&](int u) { return (WINDOW && u >= seen.first ? u + seen.gap : u) * kShortStep + first_key; };
+    auto is_seen = [&](int key) { return !WINDOW || key >= seen.from || key < p.sinks; };
+    int end = (len - first_key + kShortStep - 1) / kShortStep - seen.gap;
+    end = to < end ? to : end;
+    u32x4 kw[2][KLOADS];
+    unsigned vw[8][VWORDS];
+    float ks[8], vs[8];
+    // K: row n16 of key half u is key 8 (n16 / 4) + 4 u + n16 % 4, so that a lane's results of the two halves are those of 8 keys in order, 8 g .. 8 g + 7
+    auto k_key = [&](int t, int u) { const int key = base_of(t) + 8 * (n16 >> 2) + 4 * u + (n16 & 3); return key >= most ? most : is_seen(key) ? key : seen.from; };
+    // V: keys 8 g .. 8 g + 7, channels NB n16 .. NB n16 + NB - 1; 8 keys in order share a page
+    auto v_key = [&](int t) { const int key = base_of(t) + 8 * g; return key >= (most & ~7) ? most & ~7 : is_seen(key) || is_seen(key + 7) ? key : seen.from & ~7; };
+    int kp[2], vp;
+    bool none = false, none_next = false;      // the page of this lane's keys of the step, and of the next one, is not there
+    auto look_up = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) kp[u] = table[k_key(t, u) >> p.page_shift];
+        vp = table[v_key(t) >> p.page_shift];
+    };
+    auto is_there = [&](int page) { return page >= 0 && page < p.pages; };
+    auto load_k = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const char* const at = kh + (int64_t)(is_there(kp[u]) ? kp[u] : 0) * p.side[0].page + (k_key(t, u) & mask) * p.side[0].row + 16 * g;
+#pragma unroll
+            for (int c = 0; c < KLOADS; ++c) kw[u][c] = *reinterpret_cast<const u32x4*>(at + 64 * c);
+        }
+    };
+    auto load_v = [&](int t, int page) __attribute__((always_inline)) {
+        const int key8 = v_key(t), in8 = key8 & mask;
+        const char* const at = vh + page * p.side[1].page + in8 * p.side[1].row + NB * BYTES * n16;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) __builtin_memcpy(vw[i], __builtin_assume_aligned(at + (key8 + i < most ? i : most - key8) * p.side[1].row, 4 * VWORDS), 4 * VWORDS);
+        if constexpr (CODES) {
+            __builtin_memcpy(ks, __builtin_assume_aligned(p.side[0].scales + page * p.side[0].scale_page + head * p.side[0].scale_head + in8, 16), 32);
+            __builtin_memcpy(vs, __builtin_assume_aligned(p.side[1].scales + page * p.side[1].scale_page + head * p.side[1].scale_head + in8, 16), 32);
+        }
+    };
+    if (from < end) {
+        look_up(from);
+        load_k(from);
+        none = !is_there(vp);
+        load_v(from, none ? 0 : vp);
+        look_up(from + 1);
+    }
+    // (the last step loads nothing: a condition around the loads would have the compiler wait for all of them at the next use of any)
+    auto step = [&](int t, auto more) __attribute__((always_inline)) {
+        f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                u32x4 w;
+                if constexpr (CODES) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        w[2 * i] = code_pair<T, KIND, false>(kw[u][c / 2][2 * (c % 2) + i]);
+                        w[2 * i + 1] = code_pair<T, KIND, true>(kw[u][c / 2][2 * (c % 2) + i]);
+                    }
+                } else {
+                    w = kw[u][c];
+                }
+                s[u] = mfma16(__builtin_bit_cast(V8, w), qf[c], s[u]);
+            }
+        int vnext = 0;
+        if constexpr (decltype(more)::value) {
+            load_k(t + 1);
+            none_next = !is_there(vp);
+            vnext = none_next ? 0 : vp;
+            look_up(t + 2);
+        }
+        const int at = base_of(t) + 8 * g, left = row_end - at, out = left - p.window, in = p.sinks - at;
+        // keys that this lane's row sees; that some row does
+        auto counts = [&](int i) { return i < left && (!WINDOW || i >= out || i < in); };
+        auto any_sees = [&](int i) { return !none && i < len - at && (!WINDOW || i >= seen.from - at || i < in); };
+        float by[8];                            // what V's weights are multiplied with
+        if constexpr (CODES) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) by[i] = any_sees(i) ? vs[i] : 0.f;
+            if constexpr (__is_same(T, _Float16)) {
+                // (weights p scale in fp16 would leave its range where values are small: held relative to the largest scale so far, but for a factor of up to 64)
+                float top = by[0];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) top = fmaxf(top, by[i]);
+                if (__any(top > 64.f * R)) {
+                    top = fmaxf(fmaxf(R, over_quarters_max(top)), 0x1p-100f);
+                    const float f = R / top;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) acc[b] *= f;
+                    R = top;
+                }
+                const float over = R > 0.f ? 1.f / R : 1.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) by[i] *= over;
+            }
+        }
+        float x[8], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = s[i / 4][i % 4] * p.scale_log2;
+            if constexpr (CODES) x[i] *= ks[i];
+            x[i] = !counts(i) ? -INFINITY : none ? NAN : x[i];
+            top = fmaxf(top, x[i]);
+        }
+        if (__any(top > m + kMaxSlack)) {
+            top = fmaxf(m, over_quarters_max(top));
+            const float f = __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[b] *= f;
+        }
+        V8 pf;
+        {
+            u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(x[i] - m);
+                l += x[i];
+                if constexpr (CODES) x[i] *= by[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = round2<T>(x[2 * i], x[2 * i + 1]);
+            pf = __builtin_bit_cast(V8, w);
+        }
+        // rows that no token sees may hold anything, which a weight of 0 would make NaN
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < VWORDS; ++j) vw[i][j] = any_sees(i) ? vw[i][j] : 0u;
+        // output rows NB n + b, n = 0 .. 15: what lane n16 holds of V, transposed in its registers
+        unsigned vx[8][NB / 2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < VWORDS; ++j) {
+                if constexpr (CODES) {
+                    vx[i][2 * j] = code_pair<T, KIND, false>(vw[i][j]);
+                    vx[i][2 * j + 1] = code_pair<T, KIND, true>(vw[i][j]);
+                } else {
+                    vx[i][j] = vw[i][j];
+                }
+            }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            u32x4 vt;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vt[i] = __builtin_amdgcn_perm(vx[2 * i + 1][b / 2], vx[2 * i][b / 2], b % 2 ? 0x07060302u : 0x05040100u);
+            acc[b] = mfma16(__builtin_bit_cast(V8, vt), pf, acc[b]);
+        }
+        if constexpr (decltype(more)::value) {
+            load_v(t + 1, vnext);
+            none = none_next;
+        }
+    };
+    if (from < end) {
+        for (int t = from; t + 1 < end; ++t) step(t, Int<1>{});
+        step(end - 1, Int<0>{});
+    }
+    // ---- join the wavefronts: [wave][row][channel], and [wave][row] of max, sum
+    auto sums_of = [&](int w) { return (w < 2 ? sums01 : sums23) + (w & 1) * kShortRows * D; };
+    const float back = CODES && __is_same(T, _Float16) ? R : 1.f;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g == 0) {
+        stat[2 * (wave * kShortRows + n16)] = m;
+        stat[2 * (wave * kShortRows + n16) + 1] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int b = 0; b < NB; b += 4) *reinterpret_cast<f32x4*>(sums_of(wave) + n16 * D + NB * (4 * g + e) + b) = f32x4{acc[b][e], acc[b + 1][e], acc[b + 2][e], acc[b + 3][e]} * back;
+    __syncthreads();
+    constexpr int LANES = D / 8, AT_ONCE = kThreads / LANES;
+    for (int r = threadIdx.x / LANES; r < rows; r += AT_ONCE) {
+        const int c = 8 * (threadIdx.x % LANES);
+        float top = kLowest, sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[2 * (w * kShortRows + r)]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float by = __builtin_amdgcn_exp2f(stat[2 * (w * kShortRows + r)] - top);
+            sum += by * stat[2 * (w * kShortRows + r) + 1];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] += by * sums_of(w)[r * D + c + i];
+        }
+        if (f.parts == 1) {
+            store_row<T>(p, rq.start, head, r, c, o, top, sum, f.n.lk < 0);
+        } else {
+            float* const to_part = p.short_sums + (((int64_t)index * p.Hkv + head) * p.short_parts + part) * kShortFloats<D>;
+            *reinterpret_cast<f32x4*>(to_part + r * D + c) = f32x4{o[0], o[1], o[2], o[3]};
+            *reinterpret_cast<f32x4*>(to_part + r * D + c + 4) = f32x4{o[4], o[5], o[6], o[7]};
+            if (c == 0) { to_part[kShortRows * D + 2 * r] = top; to_part[kShortRows * D + 2 * r + 1] = sum; }
+        }
+    }
+#endif
+}
 
 // what was written to LDS is there and all reads have returned; then the workgroup meets, with loads to registers under way
 __device__ __forceinline__ void meet_in_lds() {
@@ -53,6 +327,13 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
     constexpr bool CODES = KIND != SAME16;
     LDS_TILES(L);
     __shared__ __attribute__((aligned(16))) float scales0[CODES ? 2 * kStep : 4], scales1[CODES ? 2 * kStep : 4];      // of a step's keys, then of its values
+    if ((int)blockIdx.x >= (int)gridDim.x - p.short_blocks) {
+        // (first come the first parts of all short sequences, then the second ones)
+        const int b = blockIdx.x - (gridDim.x - p.short_blocks), rest = b / p.Hkv, part = rest / p.n_seq, index = rest - part * p.n_seq;
+        const Found f = find<ShortTiles<WINDOW>>(p, index);
+        if (f.seq >= 0 && part < f.parts) short_sequence<T, KIND, D, WINDOW>(p, f, b - rest * p.Hkv, index, part, (float*)tile0, (float*)tile1, (float*)tile2);
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Block block = block_of(p, blockIdx.x);
     const int head = block.head;
@@ -378,19 +659,69 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
 #endif
 }
 
+// ---- what was cut: the parts added up, in their order.  A workgroup for each key head and tile's 32 rows, behind these one for each key head and short sequence.
+constexpr int kJoinRows = 32;
+template <typename T, int D, bool WINDOW>
+__global__ void __launch_bounds__(kThreads) cache_chunk_join_kernel(const ChunkParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int LANES = D / 8, AT_ONCE = kThreads / LANES, TILE_BLOCKS = kRows / kJoinRows;
+    const int tiles = p.most_parts > 1 ? p.tiles * p.Hkv * TILE_BLOCKS : 0, lane = threadIdx.x % LANES, c = 8 * lane;
+    const bool of_tile = (int)blockIdx.x < tiles;
+    const int b = of_tile ? blockIdx.x : blockIdx.x - tiles, head = b % p.Hkv, rest = b / p.Hkv, index = of_tile ? rest % p.tiles : rest, row0 = of_tile ? rest / p.tiles * kJoinRows : 0;
+    const Found f = of_tile ? find<RowTilesOf<WINDOW, true>>(p, index) : find<ShortTiles<WINDOW>>(p, index);
+    if (f.seq < 0 || f.parts <= 1) return;
+    const Range rq = rows_of_sequence(p.cu_q, f.seq, f.n.lq);
+    // (a part's rows lie apart: max and sum in front of a tile's D sums, behind all rows of a short one)
+    const int first = of_tile ? f.tile * kRows : 0, rows = rq.length * p.group - first, size = of_tile ? kPartFloats<D> : kShortFloats<D>;
+    const float* const sums = (of_tile ? p.parts + ((int64_t)index * p.Hkv + head) * p.most_parts * kPartFloats<D> + 2 : p.short_sums + ((int64_t)index * p.Hkv + head) * p.short_parts * kShortFloats<D>) + c;
+    const float* const stat = of_tile ? sums - c - 2 : sums - c + kShortRows * D;
+    const int row_floats = of_tile ? D + 2 : D, stat_floats = of_tile ? D + 2 : 2;
+    for (int r = row0 + threadIdx.x / LANES; r < rows && r < row0 + kJoinRows; r += AT_ONCE) {
+        float top = kLowest, sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = 0; s < f.parts; ++s) top = fmaxf(top, stat[s * size + r * stat_floats]);
+#pragma unroll 4
+        for (int s = 0; s < f.parts; ++s) {
+            const float* const at = sums + s * size + r * row_floats;
+            const f32x2 st = *reinterpret_cast<const f32x2*>(stat + s * size + r * stat_floats);
+            const float by = __builtin_amdgcn_exp2f(st[0] - top);
+            sum += by * st[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x2 x = *reinterpret_cast<const f32x2*>(at + 2 * i);
+                o[2 * i] += by * x[0];
+                o[2 * i + 1] += by * x[1];
+            }
+        }
+        store_row<T>(p, rq.start, head, first + r, c, o, top, sum, false);
+    }
+#endif
+}
+
 // ---- C ABI
-// tiles, and the parts that they may be cut into: as packed sequences of as many keys as a sequence may have
-struct Cut { int64_t tiles; int parts, least; size_t bytes; };
+// tiles, and the parts that they may be cut into: as packed sequences of as many keys as a sequence may have; short sequences as well
+constexpr int kLeastShort = 6;      // steps of a short sequence's part
+struct Cut { int64_t tiles; int parts, least, short_rows, short_parts, short_least; size_t bytes, short_bytes; };
 Cut cut_of(const cosmos_attn_cache_desc* d, Window w) {
     const int64_t group = d->Hq / d->Hkv, tiles = most_tiles(d->rows * group, d->B), most = (int64_t)d->width * d->page_size;
-    int64_t longest = (most + kStep - 1) / kStep;
-    if (w.window) {
-        const int64_t seen = ((int64_t)w.window + kRows / group + 1) / kStep + 2 + ((int64_t)w.sinks + kStep - 1) / kStep;
-        longest = seen < longest ? seen : longest;
+    auto steps_of = [&](int step, int64_t tokens) {
+        const int64_t all = (most + step - 1) / step, seen = ((int64_t)w.window + tokens) / step + 2 + ((int64_t)w.sinks + step - 1) / step;
+        return w.window && seen < all ? seen : all;
+    };
+    Cut c = {};
+    c.tiles = tiles;
+    c.least = least_steps(d->D);
+    c.parts = most_parts(tiles * d->Hkv, steps_of(kStep, kRows / group + 1), c.least);
+    c.bytes = c.parts > 1 ? (size_t)tiles * d->Hkv * c.parts * kRows * (d->D + 2) * sizeof(float) : 0;
+    if (group <= kShortRows && d->B) {
+        c.short_rows = kShortRows;
+        c.short_least = kLeastShort;
+        c.short_parts = most_parts((int64_t)d->B * d->Hkv, steps_of(kShortStep, kShortRows), c.short_least);
+        c.short_bytes = c.short_parts > 1 ? (size_t)d->B * d->Hkv * c.short_parts * kShortRows * (d->D + 2) * sizeof(float) : 0;
     }
-    const int least = least_steps(d->D), parts = most_parts(tiles * d->Hkv, longest, least);
-    return {tiles, parts, least, parts > 1 ? (size_t)tiles * d->Hkv * parts * kRows * (d->D + 2) * sizeof(float) : 0};
+    return c;
 }
+size_t workspace_of(const Cut& c) { return (c.bytes + 255) / 256 * 256 + c.short_bytes; }
 int check_chunk(const cosmos_attn_cache_desc* d, int64_t window, int64_t sinks) {
     int st = check(d);
     if (st != COSMOS_ATTN_OK) return st;
@@ -398,7 +729,7 @@ int check_chunk(const cosmos_attn_cache_desc* d, int64_t window, int64_t sinks) 
     if (d->Hq % d->Hkv) return COSMOS_ATTN_BAD_SHAPE;
     const int64_t group = d->Hq / d->Hkv;
     // (rows are 32-bit numbers, and so are the threads of a launch)
-    if (d->rows > kMost || d->rows * group > kMost / 2 || (d->rows * group / kRows + d->B + 1) * d->Hkv > kMostBlocks) return COSMOS_ATTN_UNSUPPORTED;
+    if (d->rows > kMost || d->rows * group > kMost / 2 || (d->rows * group / kRows + 2 * (int64_t)d->B + 1) * d->Hkv > kMostBlocks / 2) return COSMOS_ATTN_UNSUPPORTED;
     if (!d->rows) return COSMOS_ATTN_OK;
     if (!d->cu || (d->B && !d->lens)) return COSMOS_ATTN_BAD_ARG;
     if (d->q_stride[0] * 2 > kMostRowBytes || d->o_stride[0] * 2 > kMostRowBytes) return COSMOS_ATTN_BAD_STRIDE;
@@ -411,7 +742,7 @@ int check_chunk(const cosmos_attn_cache_desc* d, int64_t window, int64_t sinks) 
 extern "C" {
 
 size_t cosmos_attn_cache_chunk_workspace_bytes(const cosmos_attn_cache_desc* desc, int64_t window, int64_t sinks) {
-    return check_chunk(desc, window, sinks) == COSMOS_ATTN_OK && desc->rows ? cut_of(desc, window_of(desc, window, sinks)).bytes : 0;
+    return check_chunk(desc, window, sinks) == COSMOS_ATTN_OK && desc->rows ? workspace_of(cut_of(desc, window_of(desc, window, sinks))) : 0;
 }
 
 int cosmos_attn_cache_chunk(const cosmos_attn_cache_desc* desc, int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
@@ -419,8 +750,9 @@ int cosmos_attn_cache_chunk(const cosmos_attn_cache_desc* desc, int64_t window, 
     if (st != COSMOS_ATTN_OK || !desc->rows) return st;
     const Window w = window_of(desc, window, sinks);
     const Cut cut = cut_of(desc, w);
-    if (workspace_bytes < cut.bytes || (cut.bytes && !workspace)) return COSMOS_ATTN_WORKSPACE_TOO_SMALL;
-    if (cut.bytes && !aligned16(workspace)) return COSMOS_ATTN_BAD_STRIDE;
+    const size_t wanted = workspace_of(cut);
+    if (workspace_bytes < wanted || (wanted && !workspace)) return COSMOS_ATTN_WORKSPACE_TOO_SMALL;
+    if (wanted && !aligned16(workspace)) return COSMOS_ATTN_BAD_STRIDE;
     if (!device_is_whole_mi355x()) return COSMOS_ATTN_WRONG_DEVICE;
     const CacheParams c = params_of(desc);
     ChunkParams p = {};
@@ -434,6 +766,9 @@ int cosmos_attn_cache_chunk(const cosmos_attn_cache_desc* desc, int64_t window, 
     p.window = w.window; p.sinks = w.sinks;
     p.most_keys = desc->width * desc->page_size;
     p.parts = (float*)workspace;
+    p.short_rows = cut.short_rows; p.short_parts = cut.short_parts; p.short_least = cut.short_least;
+    p.short_blocks = cut.short_rows ? desc->B * desc->Hkv * cut.short_parts : 0;
+    p.short_sums = (float*)((char*)workspace + wanted - cut.short_bytes);
     p.scale = desc->sm_scale;
     p.scale_log2 = fmaxf(fabsf(desc->sm_scale) * 1.44269504088896341f, 1e-37f);      // (a masked score of -inf stays that)
     p.flip = signbit(desc->sm_scale) ? 0x80008000u : 0u;
@@ -444,9 +779,9 @@ int cosmos_attn_cache_chunk(const cosmos_attn_cache_desc* desc, int64_t window, 
         constexpr int D = decltype(dim)::value, K = decltype(kind)::value;
         auto run = [&](auto windowed) {
             constexpr bool WINDOW = decltype(windowed)::value;
-            const int done = launch(cache_chunk_kernel<T, K, D, WINDOW>, cut.tiles * p.Hkv * cut.parts, 0, p, stream);
-            if (done != COSMOS_ATTN_OK || cut.parts == 1) return done;
-            return launch(ragged_join_kernel<T, D, 0, WINDOW, true>, cut.tiles * p.Hkv * kJoinBlocks<D>, 0, (const RaggedParams&)p, stream, kJoinThreads);
+            const int done = launch(cache_chunk_kernel<T, K, D, WINDOW>, cut.tiles * p.Hkv * cut.parts + p.short_blocks, 0, p, stream);
+            const int64_t joins = (cut.parts > 1 ? cut.tiles * p.Hkv * (kRows / kJoinRows) : 0) + (cut.short_parts > 1 ? (int64_t)p.n_seq * p.Hkv : 0);
+            return done != COSMOS_ATTN_OK ? done : launch(cache_chunk_join_kernel<T, D, WINDOW>, joins, 0, p, stream);
         };
         return w.window ? run(Int<1>{}) : run(Int<0>{});
     });

@@ -21,6 +21,8 @@ struct RaggedParams {
     int window, sinks;             // keys that a row looks back on, its own among them; first keys that every row sees
     const int* lens;               // keys in pages: a sequence's number of them, which `most_keys` is the most of
     int most_keys;
+    int short_rows;                // sequences of so many rows and fewer are not cut into tiles (others have them)
+    int short_parts, short_least;  // parts that one of these may be cut into, steps of a part
     int64_t lse_row, lse_head;     // elements
     int piece, slots, sink_tiles;  // the first keys' tiles, dk and dv: steps of a piece, pieces that there may be, tiles of a sequence
     float* pieces;                 // of slot s, tile j and key head h, at (s sink_tiles + j) Hkv + h
@@ -187,8 +189,10 @@ template <bool KEYS, int ROWS, int STEP, bool WINDOW = false, bool PAGED = false
     __device__ __forceinline__ Lengths lengths(int i) const { return {range_of(p.cu_q, i, p.Tq).length, keys_of(i)}; }
     __device__ __forceinline__ int count(Lengths n) const {
         const int64_t rows = KEYS ? n.lk : (int64_t)n.lq * p.group;
-        return rows > 0 ? (int)((rows + ROWS - 1) / ROWS) : 0;
+        return rows > (PAGED ? p.short_rows : 0) ? (int)((rows + ROWS - 1) / ROWS) : 0;
     }
+    __device__ __forceinline__ int most_parts() const { return p.most_parts; }
+    __device__ __forceinline__ int least() const { return p.least; }
     static __device__ __forceinline__ int at(int rank, int tiles) { return KEYS ? rank : tiles - 1 - rank; }
     // first row that sees key j, in rows; (rounded up to steps where none does)
     __device__ __forceinline__ int first_row(Lengths n, int j) const {
@@ -286,10 +290,10 @@ template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Foun
             f.seq = base + at;
             f.n = {__builtin_amdgcn_readlane(n.lq, at), __builtin_amdgcn_readlane(n.lk, at)};
             f.tile = T.at(index - (before + __builtin_amdgcn_readlane(sum, at) - of), of);
-            if (p.most_parts <= 1) return true;
+            if (T.most_parts() <= 1) return true;
         }
         before += __builtin_amdgcn_readlane(sum, 63);
-        if (p.most_parts > 1) all += sum_of(share_of(n, tiles, (1 << 25) - 1));
+        if (T.most_parts() > 1) all += sum_of(share_of(n, tiles, (1 << 25) - 1));
         return false;
     };
     if (p.n_seq <= kFew) {
@@ -310,7 +314,7 @@ template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Foun
             const int tiles = T.count(n), sum = sums_up_to(tiles);
             const bool odd = __any(is_odd(mine, n));
             if (lane == 63) sums[turn][wave] = odd ? ODD : sum;
-            if (p.most_parts > 1) all += sum_of(share_of(n, tiles, (1 << 25) - 1));
+            if (T.most_parts() > 1) all += sum_of(share_of(n, tiles, (1 << 25) - 1));
             __syncthreads();
             int at = before + sum - tiles, past = before;
 #pragma unroll
@@ -322,7 +326,7 @@ template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Foun
             if (f.seq < 0 && index < past) {
                 if (index >= at && index < at + tiles) found = {mine, T.at(index - at, tiles), 1, n, false};
                 f.seq = 0;           // (it is in `found`)
-                if (p.most_parts <= 1) break;
+                if (T.most_parts() <= 1) break;
             }
             before = past;
         }
@@ -331,7 +335,7 @@ template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Foun
             __syncthreads();
             if (f.seq >= 0) {
                 f = {__builtin_amdgcn_readfirstlane(found.seq), __builtin_amdgcn_readfirstlane(found.tile), 1, {__builtin_amdgcn_readfirstlane(found.n.lq), __builtin_amdgcn_readfirstlane(found.n.lk)}, false};
-                if (p.most_parts <= 1) return f;
+                if (T.most_parts() <= 1) return f;
                 all = 0;
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) all += shares[w];
@@ -353,9 +357,9 @@ template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Foun
     if (f.seq < 0) { f.tile = index - before; return f; }
     const int64_t share = (all * p.Hkv + kAtOnce - 1) / kAtOnce;
     const int steps = T.steps(f.n, f.tile);
-    const int64_t wish = KEYS || share >= 2 * p.least ? 3 * share / 5 : 5 * share / 4;
-    const int per = wish > p.least ? (int)wish : p.least, parts = (steps + per - 1) / per;
-    f.parts = __builtin_amdgcn_readfirstlane(parts < 1 ? 1 : parts < p.most_parts ? parts : p.most_parts);
+    const int64_t wish = KEYS || share >= 2 * T.least() ? 3 * share / 5 : 5 * share / 4;
+    const int per = wish > T.least() ? (int)wish : T.least(), parts = (steps + per - 1) / per;
+    f.parts = __builtin_amdgcn_readfirstlane(parts < 1 ? 1 : parts < T.most_parts() ? parts : T.most_parts());
     return f;
 }
 // Of block `b`: the key head, the tile's place among all, the part.  Last parts first, which only long tiles have, and all tiles' first parts at the end, so that short tiles end the call.
