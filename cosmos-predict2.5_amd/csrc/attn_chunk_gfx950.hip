@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(kThreads) cache_chunk_join_kernel(const ChunkP
 
 // ---- C ABI
 // tiles, and the parts that they may be cut into: as packed sequences of as many keys as a sequence may have; short sequences as well
-constexpr int kLeastShort = 6;      // steps of a short sequence's part
+constexpr int kLeastTile = 4, kLeastShort = 6;      // steps of a part
 struct Cut { int64_t tiles; int parts, least, short_rows, short_parts, short_least; size_t bytes, short_bytes; };
 Cut cut_of(const cosmos_attn_cache_desc* d, Window w) {
     const int64_t group = d->Hq / d->Hkv, tiles = most_tiles(d->rows * group, d->B), most = (int64_t)d->width * d->page_size;
@@ -710,8 +710,8 @@ Cut cut_of(const cosmos_attn_cache_desc* d, Window w) {
     };
     Cut c = {};
     c.tiles = tiles;
-    c.least = least_steps(d->D);
-    c.parts = most_parts(tiles * d->Hkv, steps_of(kStep, kRows / group + 1), c.least);
+    c.least = kLeastTile;
+    c.parts = group <= kShortRows && d->rows * group <= kShortRows ? 1 : most_parts(tiles * d->Hkv, steps_of(kStep, kRows / group + 1), c.least, false, 4 * kNumCUs);
     c.bytes = c.parts > 1 ? (size_t)tiles * d->Hkv * c.parts * kRows * (d->D + 2) * sizeof(float) : 0;
     if (group <= kShortRows && d->B) {
         c.short_rows = kShortRows;

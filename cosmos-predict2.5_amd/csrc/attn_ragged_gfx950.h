@@ -357,8 +357,8 @@ template <typename Kind, int THREADS = kThreads> __device__ __forceinline__ Foun
     if (f.seq < 0) { f.tile = index - before; return f; }
     const int64_t share = (all * p.Hkv + kAtOnce - 1) / kAtOnce;
     const int steps = T.steps(f.n, f.tile);
-    const int64_t wish = KEYS || share >= 2 * T.least() ? 3 * share / 5 : 5 * share / 4;
-    const int per = wish > T.least() ? (int)wish : T.least(), parts = (steps + per - 1) / per;
+    const int64_t wish = !Kind::IN_PAGES && (KEYS || share >= 2 * T.least()) ? 3 * share / 5 : 5 * share / 4;
+    const int per = wish > T.least() ? (int)wish : T.least(), parts = Kind::IN_PAGES && steps <= 2 * T.least() ? 1 : (steps + per - 1) / per;
     f.parts = __builtin_amdgcn_readfirstlane(parts < 1 ? 1 : parts < T.most_parts() ? parts : T.most_parts());
     return f;
 }
@@ -530,8 +530,8 @@ inline int64_t most_tiles(int64_t rows, int n_seq) { return rows / kRows + n_seq
 // (The workgroups of parts that a tile does not have end at once.)
 constexpr int64_t kFullGrid = 6 * kNumCUs;
 // (WINDOW: tiles are of one length, so that there is nothing to deal out, and those that fill the chip once are left as they are.)
-inline int most_parts(int64_t tiles, int64_t longest, int least, bool window = false) {
-    int64_t parts = window ? kAtOnce / tiles : (kFullGrid + tiles - 1) / tiles;
+inline int most_parts(int64_t tiles, int64_t longest, int least, bool window = false, int64_t grid = kFullGrid) {
+    int64_t parts = window ? kAtOnce / tiles : (grid + tiles - 1) / tiles;
     parts = parts < 16 ? parts : 16;
     const int64_t of_length = longest / least;
     parts = parts < of_length ? parts : of_length;
