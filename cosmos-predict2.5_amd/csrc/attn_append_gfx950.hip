@@ -23,8 +23,8 @@ namespace {
 constexpr int kThreads = 256;
 #include "attn_cache_gfx950.h"
 
-// A share of the work: `heads` of each row, `each` of them to a group of lanes.
-struct Share { int heads, each, chunks; int64_t blocks; };
+// Of the queries, keys or values: heads of a row, and workgroups.
+struct Share { int heads; int64_t blocks; };
 struct AppendParams : CacheParams {
     Share share[3];               // queries, keys, values
     const float* freqs;           // [axes, pairs]
@@ -62,37 +62,36 @@ template <int LANES> __device__ __forceinline__ float row_sum(float v) {
     return LANES == 8 ? dpp_sum<0x141>(v) : v;      // row_half_mirror
 }
 
-// A lane has 16 channels of a row, two runs of 8, so that it has both of each of its 8 pairs; D / 16 lanes a row, and `each` heads of it one after the other, with one set of angles.  Workgroups
-// are the queries', the keys' or the values': which is theirs is the scalar unit's to find.
-constexpr int kMostEach = 4;
+// A lane has 16 channels of a row, two runs of 8, so that it has both of each of its 8 pairs; D / 16 lanes a row of a head.  Workgroups are the queries', the keys' or the values': which is theirs is
+// the scalar unit's to find.  A workgroup's few rows' cosines and sines are formed once, by all threads, and read from LDS, each lane its own 8.
+// Memory: 13069 rows of 32 + 8 + 8 heads to e4m3 with norms 63 us, 4.7 TB/s (a plain copy of the queries, norm and angles left out, 52, 5.6 TB/s: what is left are norms, turns and codes, the vector unit's); to
+// 16 bits 62 us, 5.1 TB/s.  Angles in each lane for four heads after each other 72 us, shared for four heads 70, two 65; keys and values alone 28, 26.6, 24 and 21 us: the fewer registers, the more
+// wavefronts there are.  Loads or stores past the caches: 65, but 25 % slower for 16 bits without norms.
 template <typename T, int KIND, int D, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int LANES = D / 16, GROUPS = kThreads / LANES;
+    __shared__ int position_of[GROUPS];                                                              // of the workgroup's rows
+    __shared__ __attribute__((aligned(16))) float cos_of[GROUPS * D / 2], sin_of[GROUPS * D / 2];    // [row][pair]
     int64_t block = blockIdx.x;
     int what = 0;                 // 0 queries, 1 keys, 2 values
     for (; what < 2 && block >= p.share[what].blocks; ++what) block -= p.share[what].blocks;
     const Share& share = p.share[what];
-    const int64_t unit = block * GROUPS, row0 = unit / share.chunks;
-    const unsigned u = (unsigned)(unit - row0 * share.chunks) + threadIdx.x / LANES, r = u / (unsigned)share.chunks;
+    const int64_t unit = block * GROUPS, row0 = unit / share.heads;
+    const unsigned u = (unsigned)(unit - row0 * share.heads) + threadIdx.x / LANES, r = u / (unsigned)share.heads;
     const int64_t row = row0 + r;
-    const int chunk = (int)(u - r * share.chunks), lane = threadIdx.x % LANES;
+    const int head = (int)(u - r * share.heads), lane = threadIdx.x % LANES;
     const bool in = row < p.rows;
     // where this lane's two runs of channels begin, and its first pair (none from p.pairs on)
     const bool turned = what < 2 && 8 * lane < p.pairs;
     const int c0 = INTERLEAVED ? 16 * lane : 8 * lane < p.pairs ? 8 * lane : 16 * lane, c1 = INTERLEAVED || 8 * lane >= p.pairs ? c0 + 8 : c0 + p.pairs;
     const char* from = what == 0 ? p.q : p.side[what - 1].packed;
     const int64_t from_row = what == 0 ? p.q_row : p.side[what - 1].packed_row, from_head = what == 0 ? p.q_head : p.side[what - 1].packed_head;
-    from += row * from_row;
-    u32x4 w[kMostEach][2];
-#pragma unroll
-    for (int i = 0; i < kMostEach; ++i) {
-        const int head = i * share.chunks + chunk;
-        w[i][0] = w[i][1] = u32x4{0, 0, 0, 0};
-        if (in && i < share.each && head < share.heads) {
-            w[i][0] = *reinterpret_cast<const u32x4*>(from + head * from_head + 2 * c0);
-            w[i][1] = *reinterpret_cast<const u32x4*>(from + head * from_head + 2 * c1);
-        }
+    from += row * from_row + head * from_head;
+    u32x4 w[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+    if (in) {
+        w[0] = *reinterpret_cast<const u32x4*>(from + 2 * c0);
+        w[1] = *reinterpret_cast<const u32x4*>(from + 2 * c1);
     }
     // the row's sequence and place
     Place at(p, p.cu ? last_below(p.cu, 0, p.B, row0) : (int)(row0 < p.B ? row0 : p.B), true);
@@ -108,25 +107,29 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendPara
         if (of && (position >> p.page_shift) < p.width) page = p.table[at.seq * p.table_row + (position >> p.page_shift)];
         there = page >= 0 && page < p.pages;
         const int place = position & ((1 << p.page_shift) - 1);
-        pages = side.pages + (int64_t)(there ? page : 0) * side.page + place * side.row;
-        if constexpr (KIND != SAME16) scales = side.scales + (int64_t)(there ? page : 0) * side.scale_page + place;
+        pages = side.pages + (int64_t)(there ? page : 0) * side.page + place * side.row + head * side.head;
+        if constexpr (KIND != SAME16) scales = side.scales + (int64_t)(there ? page : 0) * side.scale_page + head * side.scale_head + place;
     }
     float c[8], s[8], by[16];
-    if (turned) {
-        double angle[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) angle[j] = 0.0;
-        for (int a = 0; a < p.axes; ++a) {
-            const int n = p.positions ? of ? p.positions[row * p.positions_row + a] : 0 : position;
-            f32x4 f[2];
-            __builtin_memcpy(f, __builtin_assume_aligned(p.freqs + a * p.pairs + 8 * lane, 16), 32);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) angle[j] = __builtin_fma((double)n, (double)f[j / 4][j % 4], angle[j]);
+    if (what < 2 && p.pairs) {
+        const int first = (int)(unit - row0 * share.heads), rows = (first + GROUPS - 1) / share.heads + 1;      // the workgroup's, from row0 on
+        if (lane == 0) position_of[r] = position;
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * p.pairs; i += kThreads) {
+            const int at_row = i / p.pairs, pair = i - at_row * p.pairs;
+            double angle = 0.0;
+            for (int a = 0; a < p.axes; ++a) {
+                int n = position_of[at_row];
+                if (p.positions) n = row0 + at_row < p.rows ? p.positions[(row0 + at_row) * p.positions_row + a] : 0;
+                angle = __builtin_fma((double)n, (double)p.freqs[a * p.pairs + pair], angle);
+            }
+            const double turns = angle * 0.15915494309189533577;
+            turn((float)(turns - __builtin_rint(turns)), cos_of[i], sin_of[i]);
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const double turns = angle[j] * 0.15915494309189533577;
-            turn((float)(turns - __builtin_rint(turns)), c[j], s[j]);
+        __syncthreads();
+        if (turned) {
+            __builtin_memcpy(c, __builtin_assume_aligned(cos_of + r * p.pairs + 8 * lane, 16), 32);
+            __builtin_memcpy(s, __builtin_assume_aligned(sin_of + r * p.pairs + 8 * lane, 16), 32);
         }
     }
     const void* const weight = what < 2 ? p.weight[what] : nullptr;
@@ -143,69 +146,62 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendPara
             }
         }
     }
+    float x[16];
 #pragma unroll
-    for (int i = 0; i < kMostEach; ++i) {
-        const int head = i * share.chunks + chunk;
-        if (i >= share.each) break;
-        float x[16];
+    for (int j = 0; j < 8; ++j) {
+        x[2 * j] = low<T>(w[j / 4][j % 4]);
+        x[2 * j + 1] = high<T>(w[j / 4][j % 4]);
+    }
+    if (weight) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum = __builtin_fmaf(x[j], x[j], sum);
+        const float root = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<LANES>(sum), 1.f / D, p.eps));
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] *= root * by[j];
+    }
+    if (turned) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            x[2 * j] = low<T>(w[i][j / 4][j % 4]);
-            x[2 * j + 1] = high<T>(w[i][j / 4][j % 4]);
+            float& a = x[INTERLEAVED ? 2 * j : j];
+            float& b = x[INTERLEAVED ? 2 * j + 1 : 8 + j];
+            const float A = __builtin_fmaf(a, c[j], -(b * s[j])), B = __builtin_fmaf(b, c[j], a * s[j]);
+            a = A;
+            b = B;
         }
-        if (weight) {
-            float sum = 0.f;
+    }
+    if (what == 0 || KIND == SAME16) {
+        u32x4 y[2];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sum = __builtin_fmaf(x[j], x[j], sum);
-            const float root = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<LANES>(sum), 1.f / D, p.eps));
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] *= root * by[j];
+        for (int j = 0; j < 8; ++j) y[j / 4][j % 4] = round2<T>(x[2 * j], x[2 * j + 1]);
+        if (what == 0 && !of) y[0] = y[1] = u32x4{0, 0, 0, 0};
+        char* const to = what == 0 ? p.o + row * p.o_row + head * p.o_head : pages;
+        if (there || (what == 0 && in && p.fill)) {
+            *reinterpret_cast<u32x4*>(to + 2 * c0) = y[0];
+            *reinterpret_cast<u32x4*>(to + 2 * c1) = y[1];
         }
-        if (turned) {
+    } else {
+        // the largest magnitude: floats without their signs as whole numbers, in whose order NaN comes behind infinity and that behind all others
+        unsigned top = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float& a = x[INTERLEAVED ? 2 * j : j];
-                float& b = x[INTERLEAVED ? 2 * j + 1 : 8 + j];
-                const float A = __builtin_fmaf(a, c[j], -(b * s[j])), B = __builtin_fmaf(b, c[j], a * s[j]);
-                a = A;
-                b = B;
-            }
+        for (int j = 0; j < 16; ++j) { const unsigned b = __builtin_bit_cast(unsigned, x[j]) & 0x7FFFFFFFu; top = top > b ? top : b; }
+        top = row_max<LANES>(top);
+        // (a row of zeros: divided by 1; one that is not finite: codes of no meaning)
+        const float scale = top < 0x7F800000u ? __builtin_bit_cast(float, top) * (KIND == E4M3 ? 1.f / 448.f : 1.f / 127.f) : NAN;
+        const Divide over(scale > 0.f ? scale : 1.f);
+        if (__any(over.by != 1.f)) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] *= over.by;
         }
-        const bool writes = in && head < share.heads;
-        if (what == 0 || KIND == SAME16) {
-            u32x4 y[2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j / 4][j % 4] = round2<T>(x[2 * j], x[2 * j + 1]);
-            if (what == 0 && !of) y[0] = y[1] = u32x4{0, 0, 0, 0};
-            char* const to = what == 0 ? p.o + row * p.o_row + head * p.o_head : pages + head * p.side[what - 1].head;
-            if (writes && (there || (what == 0 && p.fill))) {
-                *reinterpret_cast<u32x4*>(to + 2 * c0) = y[0];
-                *reinterpret_cast<u32x4*>(to + 2 * c1) = y[1];
-            }
-        } else {
-            // the largest magnitude: floats without their signs as whole numbers, in whose order NaN comes behind infinity and that behind all others
-            unsigned top = 0;
+        for (int j = 0; j < 16; ++j) x[j] = over(x[j]);
+        u32x2 y[2];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) { const unsigned b = __builtin_bit_cast(unsigned, x[j]) & 0x7FFFFFFFu; top = top > b ? top : b; }
-            top = row_max<LANES>(top);
-            // (a row of zeros: divided by 1; one that is not finite: codes of no meaning)
-            const float scale = top < 0x7F800000u ? __builtin_bit_cast(float, top) * (KIND == E4M3 ? 1.f / 448.f : 1.f / 127.f) : NAN;
-            const Divide over(scale > 0.f ? scale : 1.f);
-            if (__any(over.by != 1.f)) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] *= over.by;
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = over(x[j]);
-            u32x2 y[2];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j / 2][j % 2] = code_word<KIND>(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
-            if (writes && there) {
-                char* const to = pages + head * p.side[what - 1].head;
-                *reinterpret_cast<u32x2*>(to + c0) = y[0];
-                *reinterpret_cast<u32x2*>(to + c1) = y[1];
-                if (lane == 0) scales[head * p.side[what - 1].scale_head] = scale;
-            }
+        for (int j = 0; j < 4; ++j) y[j / 2][j % 2] = code_word<KIND>(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+        if (there) {
+            *reinterpret_cast<u32x2*>(pages + c0) = y[0];
+            *reinterpret_cast<u32x2*>(pages + c1) = y[1];
+            if (lane == 0) *scales = scale;
         }
     }
 #endif
@@ -238,10 +234,7 @@ int check_append(const cosmos_attn_cache_desc* d, const cosmos_attn_cache_rope* 
 }
 Share share_of(const cosmos_attn_cache_desc* d, int heads) {
     const int groups = kThreads / (d->D / 16);
-    int each = kMostEach;
-    while (each > 1 && d->rows * ((heads + each - 1) / each) < 8 * kNumCUs * groups) each /= 2;
-    const int chunks = (heads + each - 1) / each;
-    return {heads, each, chunks, (d->rows * chunks + groups - 1) / groups};
+    return {heads, (d->rows * heads + groups - 1) / groups};
 }
 
 }  // namespace
@@ -255,7 +248,7 @@ int cosmos_attn_cache_append(const cosmos_attn_cache_desc* desc, const cosmos_at
     static_cast<CacheParams&>(p) = params_of(desc);
     p.q = (const char*)desc->q; p.o = (char*)desc->o; p.Hq = desc->Hq;
     p.q_row = 2 * desc->q_stride[0]; p.q_head = 2 * desc->q_stride[1]; p.o_row = 2 * desc->o_stride[0]; p.o_head = 2 * desc->o_stride[1];
-    p.share[0] = desc->q ? share_of(desc, desc->Hq) : Share{0, 1, 1, 0};
+    p.share[0] = desc->q ? share_of(desc, desc->Hq) : Share{1, 0};
     p.share[1] = p.share[2] = share_of(desc, desc->Hkv);
     const int64_t blocks = p.share[0].blocks + p.share[1].blocks + p.share[2].blocks;
     if (blocks > kMostBlocks) return COSMOS_ATTN_UNSUPPORTED;

@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
                 for (int i = 0; i < 8; ++i) by[i] *= over;
             }
         }
-        V8 pf[NR];
+        V8 pf[NR], pr[NR];       // (pr, WINDOW: what the weights' rounding leaves off, for which memory leaves the time)
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             float x[8], top = -INFINITY;
@@ -465,6 +465,13 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = round2<T>(x[2 * i], x[2 * i + 1]);
+            if constexpr (WINDOW) {
+                u32x4 rest;
+                asm("" : "+v"(w));       // (what the product takes)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rest[i] = round2<T>(x[2 * i] - low<T>(w[i]), x[2 * i + 1] - high<T>(w[i]));
+                pr[r] = __builtin_bit_cast(V8, rest);
+            }
             pf[r] = __builtin_bit_cast(V8, w);
         }
         // Past the end lie the last rows once more, whose infinite values with a weight of 0 would be NaN.  (The last step alone reaches there; a code's scale is what is infinite, or NaN, and is
@@ -494,7 +501,10 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attention_kernel(const Cach
 #pragma unroll
             for (int i = 0; i < 4; ++i) vt[i] = __builtin_amdgcn_perm(vx[2 * i + 1][b / 2], vx[2 * i][b / 2], b % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-            for (int r = 0; r < NR; ++r) acc[r][b] = mfma16(__builtin_bit_cast(V8, vt), pf[r], acc[r][b]);
+            for (int r = 0; r < NR; ++r) {
+                acc[r][b] = mfma16(__builtin_bit_cast(V8, vt), pf[r], acc[r][b]);
+                if constexpr (WINDOW) acc[r][b] = mfma16(__builtin_bit_cast(V8, vt), pr[r], acc[r][b]);
+            }
         }
         if constexpr (decltype(more)::value) load_v(t + 1, vnext);
     };

@@ -219,9 +219,9 @@ __device__ __forceinline__ void short_sequence(const ChunkParams& p, const Found
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[b] *= f;
         }
-        V8 pf;
+        V8 pf, pr;          // the weights, and what their rounding leaves off: there is time for both
         {
-            u32x4 w;
+            u32x4 w, rest;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 x[i] = __builtin_amdgcn_exp2f(x[i] - m);
@@ -230,7 +230,11 @@ __device__ __forceinline__ void short_sequence(const ChunkParams& p, const Found
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = round2<T>(x[2 * i], x[2 * i + 1]);
+            asm("" : "+v"(w));       // (what the product takes)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rest[i] = round2<T>(x[2 * i] - element<T>(w[i], 0), x[2 * i + 1] - element<T>(w[i], 1));
             pf = __builtin_bit_cast(V8, w);
+            pr = __builtin_bit_cast(V8, rest);
         }
         // rows that no token sees may hold anything, which a weight of 0 would make NaN
 #pragma unroll
@@ -256,6 +260,7 @@ __device__ __forceinline__ void short_sequence(const ChunkParams& p, const Found
 #pragma unroll
             for (int i = 0; i < 4; ++i) vt[i] = __builtin_amdgcn_perm(vx[2 * i + 1][b / 2], vx[2 * i][b / 2], b % 2 ? 0x07060302u : 0x05040100u);
             acc[b] = mfma16(__builtin_bit_cast(V8, vt), pf, acc[b]);
+            acc[b] = mfma16(__builtin_bit_cast(V8, vt), pr, acc[b]);
         }
         if constexpr (decltype(more)::value) {
             load_v(t + 1, vnext);
