@@ -657,8 +657,9 @@ int check_attention(const cosmos_attn_cache_desc* d) {
 }
 // Tables of few tiles: a workgroup for each sequence and head, and nothing to join, which a second launch would be for (333 keys of 4 heads: 6.3 us, as parts 5.8 and 3.8 for the join).  Of
 // some more tiles too where there are many workgroups (us, whole / as parts: 32 sequences of 1000 keys, 64 heads of 64 on 8, 13.9 / 20.2; 300 of them in int8 78 / 90; 128 of 2000 keys, 32 heads of 128 on
-// 8, 101 / 106; but 40 of them 70 / 68), up to lengths at which the longest alone takes some 20 us.
-constexpr int kWholeTiles = 4, kWholeManyTiles = 16, kMany = 32;       // kMany: workgroups to a tile of the table's
+// 8, 101 / 106; but 40 of them 70 / 68), up to lengths at which the longest alone takes some 20 us.  A window's tiles are all there are: six of them go whole (one token, 500 keys and 16 first ones,
+// a call with the host's part, us, 16 heads of 64 on 4 in fp16 11.2 / 13.3, 32 of 128 on 8 in int8 14.5 / 13.5; eight tiles 12.8 / 13.0 and 17.6 / 13.2).
+constexpr int kWholeTiles = 4, kWholeWindow = 6, kWholeManyTiles = 16, kMany = 32;       // kMany: workgroups to a tile of the table's
 struct Shape { int row_blocks, rows16, slots; bool whole; };
 Shape shape_of(const cosmos_attn_cache_desc* d, Window w) {
     const int group = d->Hq / d->Hkv, rows16 = group <= 16 ? 1 : 2, row_blocks = (group + 16 * rows16 - 1) / (16 * rows16);
@@ -668,7 +669,7 @@ Shape shape_of(const cosmos_attn_cache_desc* d, Window w) {
         capacity = seen < capacity ? seen : capacity;
     }
     const int64_t most = (int64_t)d->B * capacity;
-    if (capacity <= kWholeTiles || (capacity <= kWholeManyTiles && (int64_t)d->B * d->Hkv * row_blocks >= kMany * capacity)) return {row_blocks, rows16, 1, true};
+    if (capacity <= (w.window ? kWholeWindow : kWholeTiles) || (capacity <= kWholeManyTiles && (int64_t)d->B * d->Hkv * row_blocks >= kMany * capacity)) return {row_blocks, rows16, 1, true};
     // two workgroups a compute unit, if the tables hold that many tiles
     int64_t slots = 2 * kNumCUs / ((int64_t)d->Hkv * row_blocks);
     slots = slots < 1 ? 1 : slots;

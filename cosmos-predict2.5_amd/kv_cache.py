@@ -157,6 +157,42 @@ def _check_weight(weight: Optional[torch.Tensor], like: torch.Tensor, name: str)
     return weight if weight.stride(0) == 1 and weight.data_ptr() % 16 == 0 else weight.clone(memory_format=torch.contiguous_format)
 
 
+def _is_weight(x: Optional[torch.Tensor], D: int, device: int) -> bool:
+    return x is None or (x.dim() == 1 and x.shape[0] == D and x.get_device() == device and x.is_contiguous() and not x.data_ptr() & 15)
+
+
+def _append_as_it_is(cache, q, k, v, table, lens, cu, freqs, positions, interleaved, q_weight, k_weight, eps):
+    """:func:`cache_append` of tensors that can be taken as they are, all of it looked at once: None where something is to be converted, copied or refused.  (One new token: 11 us, 13 with
+    the checks one by one.)"""
+    if not (q.dim() == 3 == k.dim() and freqs.dim() <= 2 == table.dim()):
+        return None
+    device, dtype, D = cache._index, k.dtype, cache.head_dim
+    (rows, Hq, _), shape, (B, width) = q.shape, k.shape, table.shape
+    axes, pairs = freqs.shape if freqs.dim() == 2 else (1, freqs.shape[0] if freqs.dim() else 0)
+    pq, pk, pv, pf = q.data_ptr(), k.data_ptr(), v.data_ptr(), freqs.data_ptr()
+    if (dtype not in _DTYPES or shape != (rows, cache.heads, D) or v.shape != shape or q.shape[2] != D or q.dtype is not dtype or v.dtype is not dtype or freqs.dtype is not torch.float32
+            or not (q.get_device() == k.get_device() == v.get_device() == freqs.get_device() == device) or not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous() and freqs.is_contiguous())
+            or (pq | pk | pv | pf) & 15 or Hq < 1 or max(Hq, cache.heads) * D > 1 << 22 or pairs % 8 or 2 * pairs > D or axes < 1
+            or not plain_int32(table, 2, device) or table.stride()[0] < 0 or not plain_int32(lens, 1, device) or lens.shape[0] != B
+            or (rows != B if cu is None else not plain_int32(cu, 1, device) or cu.shape[0] != B + 1)
+            or (axes != 1 if positions is None else positions.shape != (rows, axes) or not plain_int32(positions, 2, device) or not positions.is_contiguous())
+            or not _is_weight(q_weight, D, device) or not _is_weight(k_weight, D, device)):
+        return None
+    weight_16 = 0
+    if q_weight is not None or k_weight is not None:
+        kinds = {w.dtype for w in (q_weight, k_weight) if w is not None}
+        if kinds != {torch.float32} and kinds != {dtype}:
+            return None
+        weight_16 = 0 if kinds == {torch.float32} else 1
+    part, o, own = cache._part(dtype), torch.empty_like(q), cache.heads * D
+    desc = part + _CALL_PART.pack(B, width, table.data_ptr(), table.stride()[0], lens.data_ptr(), 0 if cu is None else cu.data_ptr(), rows, pk, pv, own, D, own, D, 1, Hq, 0.0, 0, pq, o.data_ptr(),
+                                  Hq * D, D, Hq * D, D, 0)
+    rope = _ROPE.pack(pf, 0 if positions is None else positions.data_ptr(), axes, 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), pairs, axes,
+                      1 if interleaved else 0, weight_16, eps, 0)
+    on_device(device, _lib.load_library().cosmos_attn_cache_append, desc, rope)
+    return o
+
+
 def cache_append(
     cache: KVCache,
     q: Optional[torch.Tensor],
@@ -182,6 +218,10 @@ def cache_append(
     videos say; None: the token's place in its sequence.
     ``q_weight``, ``k_weight``: ``[D]`` of the RMS norm (``eps``) of each head's row in front of that; None: no norm.  All of it in fp32, rounded once: to the rows' type, or to the cache's 8 bits.
     Queries of no sequence, and of sequences whose ``lens`` is below their rows, become zeros (in ``out``: left as they are).  As in :func:`cache_write`, what has no place is not written."""
+    if q is not None and freqs is not None and out is None:
+        made = _append_as_it_is(cache, q, k, v, table, lens, cu, freqs, positions, interleaved, q_weight, k_weight, eps)
+        if made is not None:
+            return made
     k = _check_rows(k, "k", cache)
     v = _check_rows(v, "v", cache, k)
     assert k.shape == v.shape and k.shape[1] == cache.heads, "k and v must be [rows, heads, D] of the cache"
