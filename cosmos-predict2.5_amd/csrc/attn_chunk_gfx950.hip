@@ -34,7 +34,10 @@ struct ChunkParams : RaggedParams {
 };
 
 // ---- Sequences of few rows (a token or some, of which the query heads of a key head are 16 at most together): keys and values go by once, for a product or two, and what counts is how many bytes are
-// under way.  A wavefront has 32 of 128 keys to a step, straight from memory into registers, as in cache_attention_kernel; rows are the columns of 16 x 16 x 32 products.
+// under way.  A wavefront has 32 of 128 keys to a step, straight from memory into registers, as in cache_attention_kernel; rows are the columns of 16 x 16 x 32 products.  In the tiles' launch, behind
+// these: 46 single tokens of 1 to 7939 keys beside pieces of 512 and 300 tokens, 16 heads of 128 on 8 in e4m3, 107 us; as tiles of 128 rows with 2 live ones 145.  (The single tokens alone 61 us, 4.1 TB/s, where
+// cache_attention_kernel's three wavefronts on a SIMD take 46; the pieces alone 61.  Tiles and short sequences alternating, 119; first the short ones, 120.  What these bound each other by is the
+// vector unit, which both need for codes.)
 constexpr int kShortRows = 16, kShortStep = 128;
 template <int D> constexpr int kShortFloats = kShortRows * (D + 2);       // of a part: its rows' D sums, then max and sum of exponentials
 // the keys that a sequence's tokens see, in steps: those of the first keys and, behind the `gap` that none looks at, those from the first token's window on
@@ -318,7 +321,9 @@ __device__ __forceinline__ void meet_in_lds() {
     asm volatile("" ::: "memory");
 }
 
-// ---- A workgroup: as ragged_fwd_kernel, with K and V out of pages.
+// ---- A workgroup: as ragged_fwd_kernel, with K and V out of pages.  2048 tokens on 16384 positions, 32 heads of 128 on 8: 500 us, 1.0 PFLOP/s, in 8 bits 595 to 620 (codes' conversions are 8 %, scales 11 % of that, measured
+// without them; what bounds it is as there, a fragment from LDS to each product).  A call of few tiles is as long as its longest part: a step of 64 keys takes 1.1 us in 16 bits and 1.7 in 8, all of it one chain.
+// Hence parts of 4 steps at least, if there are more than 8 (64 tokens on 1280 positions, 8 heads on 2, us, bf16 / int8: whole 30 / 42, parts of 8 and more 24 / 30, of 6 21 / 26, of 4 18 / 21, with 5 for the second launch).
 // 16 bits: rows go straight to LDS; what lies behind the last key, and runs that no row of the tile sees, come as zeros.  8 bits: codes are loaded into registers a step earlier, become exact
 // 16-bit values on their way to LDS, K's scales multiply the scores and V's the weights, before these are rounded.
 // A page that is not there: its keys are NaN, for the rows that see them.
@@ -370,7 +375,8 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
     auto at_step = [&](int u) { return WINDOW && u >= sink_steps ? u + gap : u; };
     const int t0 = (int)((int64_t)block.part * steps / f.parts), n = (int)((int64_t)(block.part + 1) * steps / f.parts);
 
-    // (of constant memory, so that the scalar unit looks up: a vector load's result in scalar registers is waited for at once, with all loads in front of it)
+    // (of constant memory, so that the scalar unit looks up: a vector load's result in scalar registers is waited for at once, with all loads in front of it; 160 -> 145 us, and 2048 + 512 + 77 tokens on
+    // 16384, 9001 and 1301 positions in bf16 717 -> 653)
     typedef const __attribute__((address_space(4))) int* Table;
     const Table table = (Table)(uintptr_t)(p.table + f.seq * p.table_row);
     const int mask = (1 << p.page_shift) - 1;
@@ -608,8 +614,8 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
         if constexpr (D == 64) __builtin_amdgcn_s_setprio(0);
     };
     if constexpr (CODES) {
-        // A step's codes are on their way while the two before are computed, and go to LDS during the one before.  (One step ahead: two workgroups of a unit have half as many bytes under way, 46 single
-        // tokens of up to 8000 keys beside two pieces in e4m3 ... us instead of ...)
+        // A step's codes are on their way while the two before are computed, and go to LDS during the one before.  (One step ahead two workgroups of a unit have half as many bytes under way: the pieces and
+        // single tokens above, then all as tiles, 189 us, two steps ahead 160.)
         auto next = [&](Codes& codes, int& at, int u, char* kt, char* vt, float* st) __attribute__((always_inline)) {
             keep_codes(codes, kt, vt, st);
             load_codes(codes, u + 2, at);
@@ -664,7 +670,8 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
 #endif
 }
 
-// ---- what was cut: the parts added up, in their order.  A workgroup for each key head and tile's 32 rows, behind these one for each key head and short sequence.
+// ---- what was cut: the parts added up, in their order.  A workgroup for each key head and tile's 32 rows, behind these one for each key head and short sequence.  (256 threads: most workgroups find
+// nothing to do, and 1024 threads each of them take two rounds of the chip; 62 tiles of 8 heads, few of them cut, 10 us instead of 20.)
 constexpr int kJoinRows = 32;
 template <typename T, int D, bool WINDOW>
 __global__ void __launch_bounds__(kThreads) cache_chunk_join_kernel(const ChunkParams p) {
@@ -716,6 +723,7 @@ Cut cut_of(const cosmos_attn_cache_desc* d, Window w) {
     Cut c = {};
     c.tiles = tiles;
     c.least = kLeastTile;
+    // (no list of exactly the parts that there are: the search for it takes 4 us more in each workgroup)
     c.parts = group <= kShortRows && d->rows * group <= kShortRows ? 1 : most_parts(tiles * d->Hkv, steps_of(kStep, kRows / group + 1), c.least, false, 4 * kNumCUs);
     c.bytes = c.parts > 1 ? (size_t)tiles * d->Hkv * c.parts * kRows * (d->D + 2) * sizeof(float) : 0;
     if (group <= kShortRows && d->B) {
