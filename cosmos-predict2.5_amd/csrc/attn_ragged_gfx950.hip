@@ -830,6 +830,7 @@ int backward(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks,
     const Window w = window_of(desc, window, sinks);
     RaggedParams p = params_of(desc);
     p.window = w.window; p.sinks = w.sinks;
+    if (w.window == 1 && !w.sinks) p.scale = 0.f;       // (a row that sees one key has the weight 1 on it, whatever its score: dq and dk are 0, and not what roundings of dP and delta leave)
     p.delta = (float*)workspace;
     p.parts = (float*)((char*)workspace + up((size_t)desc->Tq * desc->Hq * sizeof(float)));      // (of dq, then of dk and dv)
     const Pieces pieces = pieces_of(desc, w);

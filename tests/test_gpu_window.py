@@ -110,6 +110,24 @@ def test_hidden_scores_that_are_large(pkg, ragged_oracle, gpu):
     assert all(x.isfinite().all() for x in (dq, dk, dv))
 
 
+@pytest.mark.parametrize("D, dtype", [(64, FP16), (128, BF16)])
+def test_one_key_to_a_row(pkg, gpu, D, dtype):
+    """Its weight is 1: o is its value, dv its rows' gradients, and nothing depends on scores."""
+    q, k, v, g = (rows(300, h, D, dtype, gpu, i) for i, h in enumerate((4, 2, 2, 4)))
+    on = offsets([0, 100, 101, 300], gpu)
+    rest = torch.empty_like(q)
+    o, lse = pkg.ragged_fwd(q, k, v, on, causal=True, rest=rest, window=1)
+    # (a weight of 1 to within fp32's exponential, 1e-5: the score, some 10, is rounded once more where the row's largest is taken off it)
+    of = v.repeat_interleave(2, 1)
+    assert torch.equal(o, of) and (rest.double().abs() <= 1e-5 * of.double().abs() + 2.0 ** -24).all()
+    dq, dk, dv = pkg.ragged_bwd(q, k, v, o, lse, g, on, causal=True, rest=rest, window=1)
+    want = g.double().reshape(300, 2, 2, D).sum(2)
+    assert (dq == 0).all() and (dk == 0).all()
+    # (such a weight as an operand and the result are rounded once each)
+    u, size = torch.finfo(dtype).eps / 2, g.double().abs().reshape(300, 2, 2, D).sum(2)
+    assert ((dv.double() - want).abs() <= u * want.abs() + (u + 1e-5) * size + 2.0 ** -24).all()
+
+
 def test_a_window_that_hides_nothing(pkg, gpu):
     """As long as there are keys: the results of the call without it."""
     q, k, v, g = (rows(300, h, 128, BF16, gpu, i) for i, h in enumerate((4, 2, 2, 4)))
