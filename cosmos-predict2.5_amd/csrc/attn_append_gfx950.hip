@@ -35,9 +35,10 @@ struct AppendParams : CacheParams {
     float eps;
 };
 
-// cos and sin of 2 pi r, |r| <= 1/2: the nearest quarter turn off, then Taylor's series on pi/4 to either side (their remainders are below 2^-30)
-__device__ __forceinline__ void turn(float r, float& c, float& s) {
-    const float quarter = rintf(4.f * r), x = __builtin_fmaf(-0.25f, quarter, r) * 6.28318530717958648f, y = x * x;
+// cos and sin of an angle: the nearest quarter turn off, in 64 bits (in 32 the rest would be off by as much as a rounding of 1), then Taylor's series on pi/4 to either side (their remainders are below 2^-30)
+__device__ __forceinline__ void turn(double angle, float& c, float& s) {
+    const double quarters = angle * 0.63661977236758134308, whole = __builtin_rint(quarters);
+    const float x = (float)((quarters - whole) * 1.57079632679489661923), y = x * x;
     float cx = __builtin_fmaf(y, -1.f / 3628800.f, 1.f / 40320.f);
     cx = __builtin_fmaf(y, cx, -1.f / 720.f);
     cx = __builtin_fmaf(y, cx, 1.f / 24.f);
@@ -47,7 +48,7 @@ __device__ __forceinline__ void turn(float r, float& c, float& s) {
     sx = __builtin_fmaf(y, sx, 1.f / 120.f);
     sx = __builtin_fmaf(y, sx, -1.f / 6.f);
     sx = __builtin_fmaf(y * x, sx, x);
-    const int q = (int)quarter;
+    const int q = (int)(int64_t)whole;
     const float a = q & 1 ? sx : cx, b = q & 1 ? cx : sx;
     c = (q + 1) & 2 ? -a : a;
     s = q & 2 ? -b : b;
@@ -123,8 +124,7 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendPara
                 if (p.positions) n = row0 + at_row < p.rows ? p.positions[(row0 + at_row) * p.positions_row + a] : 0;
                 angle = __builtin_fma((double)n, (double)p.freqs[a * p.pairs + pair], angle);
             }
-            const double turns = angle * 0.15915494309189533577;
-            turn((float)(turns - __builtin_rint(turns)), cos_of[i], sin_of[i]);
+            turn(angle, cos_of[i], sin_of[i]);
         }
         __syncthreads();
         if (turned) {
@@ -156,7 +156,9 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const AppendPara
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) sum = __builtin_fmaf(x[j], x[j], sum);
-        const float root = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<LANES>(sum), 1.f / D, p.eps));
+        const float mean = __builtin_fmaf(row_sum<LANES>(sum), 1.f / D, p.eps);
+        float root = __builtin_amdgcn_rsqf(mean);
+        if (mean > 0.f && mean < INFINITY) root = __builtin_fmaf(0.5f * root, __builtin_fmaf(-mean * root, root, 1.f), root);      // (a step of Newton's: the instruction is good to one unit in the last place)
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] *= root * by[j];
     }
