@@ -4,7 +4,7 @@
 // A row x of a query's or key's head, at position p:
 //     n = x rsqrt(mean(x^2) + eps) w  (with a weight),   a_i = sum_axes p_axis freq_axis,i,   (u, v) -> (u cos a_i - v sin a_i, v cos a_i + u sin a_i)
 // for its R pairs of channels, (i, i + R) or (2 i, 2 i + 1); what lies behind 2 R channels is not turned.  All of it in fp32, rounded once: to the 16-bit type, or as a code of 8 bits with its row's scale.
-// Angles are formed in 64 bits, in turns, and reduced there: at position 10^6 an angle in fp32 is off by 0.06.  Positions are the rows' places in their sequences, or given, several axes to a row.
+// Angles are formed in 64 bits, in quarters of a turn, and reduced there: at position 10^6 an angle in fp32 is off by 0.06.  Positions are the rows' places in their sequences, or given, several axes to a row.
 #include <hip/hip_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
