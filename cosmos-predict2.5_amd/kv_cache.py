@@ -164,11 +164,11 @@ def _is_weight(x: Optional[torch.Tensor], D: int, device: int) -> bool:
 def _append_as_it_is(cache, q, k, v, table, lens, cu, freqs, positions, interleaved, q_weight, k_weight, eps):
     """:func:`cache_append` of tensors that can be taken as they are, all of it looked at once: None where something is to be converted, copied or refused.  (One new token: 11 us, 13 with
     the checks one by one.)"""
-    if not (q.dim() == 3 == k.dim() and freqs.dim() <= 2 == table.dim()):
+    if not (q.dim() == 3 == k.dim() and 1 <= freqs.dim() <= 2 == table.dim()):
         return None
     device, dtype, D = cache._index, k.dtype, cache.head_dim
     (rows, Hq, _), shape, (B, width) = q.shape, k.shape, table.shape
-    axes, pairs = freqs.shape if freqs.dim() == 2 else (1, freqs.shape[0] if freqs.dim() else 0)
+    axes, pairs = freqs.shape if freqs.dim() == 2 else (1, freqs.shape[0])
     pq, pk, pv, pf = q.data_ptr(), k.data_ptr(), v.data_ptr(), freqs.data_ptr()
     if (dtype not in _DTYPES or shape != (rows, cache.heads, D) or v.shape != shape or q.shape[2] != D or q.dtype is not dtype or v.dtype is not dtype or freqs.dtype is not torch.float32
             or not (q.get_device() == k.get_device() == v.get_device() == freqs.get_device() == device) or not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous() and freqs.is_contiguous())
@@ -213,7 +213,7 @@ def cache_append(
     """New tokens, packed as for :func:`cache_write`: keys are normalised and turned by their positions and written with their values; returns the queries, normalised and turned, ``[rows, Hq, D]``
     (``q`` None: None; ``out``, which may be ``q``, takes them).
 
-    ``freqs``: fp32 ``[R]`` or ``[axes, R]``, radians a position, for R pairs of channels (a multiple of 8, ``2 R <= D``): ``(i, i + R)``, or with ``interleaved`` ``(2 i, 2 i + 1)``; the channels behind
+    ``freqs``: ``[R]`` or ``[axes, R]``, fp32 (others are rounded to it), radians a position, for R pairs of channels (a multiple of 8, ``2 R <= D``): ``(i, i + R)``, or with ``interleaved`` ``(2 i, 2 i + 1)``; the channels behind
     are not turned (None: none are).  The angle of pair i is ``sum_a positions[row, a] * freqs[a, i]``, formed in 64 bits; ``positions``: whole numbers ``[rows]`` or ``[rows, axes]``, of images and
     videos say; None: the token's place in its sequence.
     ``q_weight``, ``k_weight``: ``[D]`` of the RMS norm (``eps``) of each head's row in front of that; None: no norm.  All of it in fp32, rounded once: to the rows' type, or to the cache's 8 bits.

@@ -255,3 +255,34 @@ def test_a_layer_piece_by_piece_and_token_by_token(pkg, ragged_oracle, gpu, dtyp
         got = pkg.cache_read(cache, table[i:i + 1], offsets([0, done[i]], gpu), done[i], dtype=dtype)[0]
         y = ragged_oracle.turned(k[i][:done[i]], w[1], 1e-6, torch.arange(done[i])[:, None], freqs[:].cpu().reshape(1, -1), False)
         near(got, *held(ragged_oracle, *y, kind, dtype), "k")
+
+
+@pytest.mark.parametrize("kind", [BF16, INT8])
+def test_two_streams_at_once(pkg, gpu, kind):
+    """Two layers' steps, each on its own cache, together what they are one after the other: nothing is shared between calls."""
+    page, Hq, Hkv, D, lens, new = 16, 8, 2, 128, [900, 700, 40], [300, 1, 16]
+    table, pages = tables(lens, page, gpu)
+    freqs, on, at = freqs_of(64).to(gpu), offsets(cu(new), gpu), offsets(lens, gpu)
+    w = torch.ones(D, device=gpu)
+
+    def layer(seed):
+        cache = empty(pkg, pages, Hkv, page, D, kind, gpu)
+        k, v = (rows(sum(lens), Hkv, D, BF16, gpu, seed + i) for i in range(2))
+        pkg.cache_write(cache, k, v, table, at, offsets(cu(lens), gpu))
+        return cache, rows(sum(new), Hq, D, BF16, gpu, seed + 2), k[:sum(new)] * 2, v[:sum(new)] * 2
+
+    def step(cache, q, k, v):
+        q = pkg.cache_append(cache, q, k, v, table, at, on, freqs=freqs, q_weight=w, k_weight=w)
+        return q, *pkg.cache_attention(q, cache, table, at, need_lse=True, cu=on), *pkg.cache_attention(q, cache, table, at, need_lse=True, cu=on, window=200, sinks=4)
+
+    layers = [layer(10), layer(20)]
+    want = [step(*x) for x in layers]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in layers]
+    for _ in range(5):
+        got = []
+        for stream, x in zip(streams, layers):
+            with torch.cuda.stream(stream):
+                got.append(step(*x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))

@@ -138,3 +138,15 @@ def test_refusals_of_append(pkg, monkeypatch):
     ]:
         with pytest.raises(error):
             pkg.cache_append(cache, *args, table, lens, **{"freqs": freqs, **over})
+
+
+def test_freqs_without_a_dim_are_refused(pkg, monkeypatch):
+    """(by what looks at all arguments at once as well)"""
+    def no_launch(*a):
+        raise AssertionError("launched")
+
+    monkeypatch.setattr(pkg.kv_cache, "on_device", no_launch)
+    new = lambda *shape, dtype=torch.bfloat16: on(torch.zeros(shape, dtype=dtype))
+    cache = pkg.KVCache(new(5, 2, 16, 64), new(5, 2, 16, 64))
+    with pytest.raises(AssertionError, match="freqs must be"):
+        pkg.cache_append(cache, new(3, 4, 64), new(3, 2, 64), new(3, 2, 64), new(3, 2, dtype=torch.int32), new(3, dtype=torch.int32), freqs=new(dtype=torch.float32))
