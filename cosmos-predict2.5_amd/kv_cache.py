@@ -302,6 +302,28 @@ def _workspace_bytes(Hkv: int, D: int, page_size: int, B: int, width: int, Hq: i
     return (lib.cosmos_attn_cache_window_workspace_bytes if rows < 0 else lib.cosmos_attn_cache_chunk_workspace_bytes)(part + call, window, sinks)
 
 
+def _attention_as_it_is(q, cache, table, lens, sm_scale, need_lse, cu, window, sinks):
+    """:func:`cache_attention` of tensors that can be taken as they are, all of it looked at once: None where something is to be converted, copied or refused.  (One new
+    token: 9.9 us, 11.1 with the checks one by one.)"""
+    if not q.dim() == 3 == 1 + table.dim():
+        return None
+    device, dtype, D, pq = cache._index, q.dtype, cache.head_dim, q.data_ptr()
+    (rows, Hq, of), (B, width) = q.shape, table.shape
+    if (dtype not in _DTYPES or of != D or q.get_device() != device or not q.is_contiguous() or pq & 15 or Hq < 1 or Hq % cache.heads or Hq * D > 1 << 22
+            or not plain_int32(table, 2, device) or not plain_int32(lens, 1, device) or lens.shape[0] != B
+            or (rows != B if cu is None else not plain_int32(cu, 1, device) or cu.shape[0] != B + 1)):
+        return None
+    part, o, row = cache._part(dtype), torch.empty_like(q), Hq * D
+    lse = q.new_empty((rows, Hq), dtype=torch.float32) if need_lse else None
+    desc = part + _CALL_PART.pack(B, width, table.data_ptr(), table.stride()[0], lens.data_ptr(), 0 if cu is None else cu.data_ptr(), rows, 0, 0, 0, 0, 0, 0, _lib.FILL_ALL, Hq,
+                                  D ** -0.5 if sm_scale is None else sm_scale, 0, pq, o.data_ptr(), row, D, row, D, 0 if lse is None else lse.data_ptr())
+    ws_bytes = _workspace_bytes(cache.heads, D, cache.page_size, B, width, Hq, window, sinks, -1 if cu is None else rows)
+    workspace = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    lib = _lib.load_library()
+    on_device(device, lib.cosmos_attn_cache_window if cu is None else lib.cosmos_attn_cache_chunk, desc, window, sinks, 0 if workspace is None else workspace.data_ptr(), ws_bytes)
+    return o, lse
+
+
 def cache_attention(
     q: torch.Tensor,
     cache: KVCache,
@@ -323,6 +345,10 @@ def cache_attention(
     A token that sees nothing (``lens[i] == 0``, or below its rows): o = 0, lse = -inf.  A length that the table does not hold: NaN.  A page outside of the cache: NaN for the tokens that see it.
     ``out``: a tensor for o."""
     window, sinks = checked_window(window, sinks)
+    if out is None:
+        made = _attention_as_it_is(q, cache, table, lens, sm_scale, need_lse, cu, window, sinks)
+        if made is not None:
+            return made
     q = _check_rows(q, "q", cache)
     rows, Hq, D = q.shape
     assert Hq >= 1 and Hq % cache.heads == 0, "q must be [rows, Hq, D], Hq a multiple of the cache's heads"
