@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
 // ---- backward, first kernel: delta and dq.  The forward's rows and tiles, with P from lse, dP^T = V dO^T beside S^T, and dQ^T = K^T dS^T.  Matrix unit busy 65 % at 1.7 GHz (8192 positions, 32
 // heads of 128 on 8): three products to an exponential, under the power limit.
 // WINDOW: what rounding dS leaves off is a second operand of the last product, whose other one is there already.  dq's error is then 1.03 of its own rounding instead of 1.46 (dS sums to zero over a row, so
-// that its errors are larger next to dq than next to dS), for 12 to 16 % of this kernel.
+// that its errors are larger next to dq than next to dS), for 12 to 16 % of this kernel.  (Its reads are left to the compiler: in the order of the others 1157 instead of 1150 us for a whole pass.)
 template <typename T, int D, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -375,8 +375,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
                     acc[b] = mfma32(kt8, df[c], acc[b]);
                     if constexpr (WINDOW) acc[b] = mfma32(kt8, dr[c], acc[b]);
                 }
-            if constexpr (WINDOW) reads_ahead<4 * NB, 4 * NB, 8>();
-            else reads_ahead<4 * NB, 2 * NB, 8>();
+            if constexpr (!WINDOW) reads_ahead<4 * NB, 2 * NB, 8>();
         }
     };
     for (int t = t0; t < n; t += 2) {
