@@ -670,16 +670,17 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
 #endif
 }
 
-// ---- what was cut: the parts added up, in their order.  A workgroup for each key head and tile's 32 rows, behind these one for each key head and short sequence.  (256 threads: most workgroups find
-// nothing to do, and 1024 threads each of them take two rounds of the chip; 62 tiles of 8 heads, few of them cut, 10 us instead of 20.)
+// ---- what was cut: the parts added up, in their order.  A workgroup for each key head and short sequence, behind these one for each key head and tile's 32 rows.  (256 threads: most workgroups find
+// nothing to do, and 1024 threads each of them take two rounds of the chip; 62 tiles of 8 heads, few of them cut, 9 us instead of 20, and 10.4 with those that find nothing in between.  16 rows each: 9.8.)
 constexpr int kJoinRows = 32;
 template <typename T, int D, bool WINDOW>
 __global__ void __launch_bounds__(kThreads) cache_chunk_join_kernel(const ChunkParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int LANES = D / 8, AT_ONCE = kThreads / LANES, TILE_BLOCKS = kRows / kJoinRows;
-    const int tiles = p.most_parts > 1 ? p.tiles * p.Hkv * TILE_BLOCKS : 0, lane = threadIdx.x % LANES, c = 8 * lane;
-    const bool of_tile = (int)blockIdx.x < tiles;
-    const int b = of_tile ? blockIdx.x : blockIdx.x - tiles, head = b % p.Hkv, rest = b / p.Hkv, index = of_tile ? rest % p.tiles : rest, row0 = of_tile ? rest / p.tiles * kJoinRows : 0;
+    // (short sequences', then the tiles' in their order: what there is none of comes last)
+    const int shorts = p.short_parts > 1 ? p.n_seq * p.Hkv : 0, lane = threadIdx.x % LANES, c = 8 * lane;
+    const bool of_tile = (int)blockIdx.x >= shorts;
+    const int b = of_tile ? blockIdx.x - shorts : blockIdx.x, head = b % p.Hkv, rest = b / p.Hkv, index = of_tile ? rest / TILE_BLOCKS : rest, row0 = of_tile ? rest % TILE_BLOCKS * kJoinRows : 0;
     const Found f = of_tile ? find<RowTilesOf<WINDOW, true>>(p, index) : find<ShortTiles<WINDOW>>(p, index);
     if (f.seq < 0 || f.parts <= 1) return;
     const Range rq = rows_of_sequence(p.cu_q, f.seq, f.n.lq);
