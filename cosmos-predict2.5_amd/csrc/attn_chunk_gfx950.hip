@@ -35,7 +35,7 @@ struct ChunkParams : RaggedParams {
 
 // ---- Sequences of few rows (a token or some, of which the query heads of a key head are 16 at most together): keys and values go by once, for a product or two, and what counts is how many bytes are
 // under way.  A wavefront has 32 of 128 keys to a step, straight from memory into registers, as in cache_attention_kernel; rows are the columns of 16 x 16 x 32 products.  In the tiles' launch, behind
-// these: 46 single tokens of 1 to 7939 keys beside pieces of 512 and 300 tokens, 16 heads of 128 on 8 in e4m3, 107 us; as tiles of 128 rows with 2 live ones 145.  (The single tokens alone 61 us, 4.1 TB/s, where
+// these: 46 single tokens of 1 to 7939 keys beside pieces of 512 and 300 tokens, 16 heads of 128 on 8 in e4m3, 105 us; as tiles of 128 rows with 2 live ones 145.  (The single tokens alone 61 us, 4.1 TB/s, where
 // cache_attention_kernel's three wavefronts on a SIMD take 46; the pieces alone 61.  Tiles and short sequences alternating, 119; first the short ones, 120.  What these bound each other by is the
 // vector unit, which both need for codes.)
 constexpr int kShortRows = 16, kShortStep = 128;
