@@ -188,9 +188,9 @@ __device__ __forceinline__ void short_sequence(const ChunkParams& p, const Found
         float by[8];                            // what V's weights are multiplied with
         if constexpr (CODES) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) by[i] = any_sees(i) ? vs[i] : 0.f;
+            for (int i = 0; i < 8; ++i) by[i] = counts(i) ? vs[i] : 0.f;
             if constexpr (__is_same(T, _Float16)) {
-                // (weights p scale in fp16 would leave its range where values are small: held relative to the largest scale so far, but for a factor of up to 64)
+                // (weights p scale in fp16 would leave its range where values are small: held relative to the largest scale so far of the keys that this lane's row sees, but for a factor of up to 64)
                 float top = by[0];
 #pragma unroll
                 for (int i = 1; i < 8; ++i) top = fmaxf(top, by[i]);
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
     float m = kLowest, l = 0.f;       // (l: of this lane's half of the keys)
-    float R = 0.f;                    // fp16 and codes: what weights are relative to, the largest scale of V so far but for a factor of 64
+    float R = 0.f;                    // fp16 and codes: what weights are relative to, the largest scale of V so far that this lane's row sees, but for a factor of 64
 
     auto step = [&](int u, const char* kt, const char* vt, const float* st) __attribute__((always_inline)) {
         const int key0 = at_step(u) * kStep;
@@ -564,14 +564,19 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
         }
         float over = 1.f;
         if constexpr (CODES && __is_same(T, _Float16)) {
-            // weights p scale in fp16 would leave its range where values are small
-            float most = 0.f;
+            // Weights p scale in fp16 would leave its range where values are small.  (A row's own keys alone say what they are relative to: those of a later token, whose values may be 2^25 times as large,
+            // would make all of an earlier one's weights 0.  Steps in which no key is masked need not ask.)
+            auto most_of = [&](auto masked) __attribute__((always_inline)) {
+                float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const f32x4 by = *reinterpret_cast<const f32x4*>(st + kStep + 8 * i + 4 * half);
+                for (int i = 0; i < 8; ++i) {
+                    const f32x4 by = *reinterpret_cast<const f32x4*>(st + kStep + 8 * i + 4 * half);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) most = fmaxf(most, by[j]);
-            }
+                    for (int j = 0; j < 4; ++j) top = fmaxf(top, decltype(masked)::value && s[i / 4][4 * (i % 4) + j] == -INFINITY ? 0.f : by[j]);
+                }
+                return top;
+            };
+            float most = key0 + kStep > wave_all || behind ? most_of(Int<1>{}) : most_of(Int<0>{});
             if (__any(most > 64.f * R)) {
                 most = fmaxf(fmaxf(R, over_halves_max(most)), 0x1p-100f);      // (far below what fp16 holds, and its reciprocal is a number)
                 const float by = R / most;
@@ -592,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
                 f32x4 by[2];
                 if constexpr (CODES) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) by[i] = *reinterpret_cast<const f32x4*>(st + kStep + 32 * h + 16 * c + 8 * i + 4 * half) * over;
+                    for (int i = 0; i < 2; ++i) by[i] = *reinterpret_cast<const f32x4*>(st + kStep + 32 * h + 16 * c + 8 * i + 4 * half);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -601,8 +606,9 @@ __global__ void __launch_bounds__(kThreads, 2) cache_chunk_kernel(const ChunkPar
                     l += a;
                     l += b;
                     if constexpr (CODES) {
-                        a *= by[i / 2][2 * (i % 2)];
-                        b *= by[i / 2][2 * (i % 2) + 1];
+                        // (the factor first: a masked weight of 0 stays that beside a scale that is far above the row's own)
+                        a = a * over * by[i / 2][2 * (i % 2)];
+                        b = b * over * by[i / 2][2 * (i % 2) + 1];
                     }
                     w[i] = round2<T>(a, b);
                 }
