@@ -3,7 +3,7 @@
 // Sequence i has the rows cu_q[i] .. cu_q[i + 1] - 1 of q and the rows cu_k[i] .. of k and v.  With c the scale, t and j counted from the sequence's start, Lq and Lk its lengths:
 //     s_tj = c q_t k_j,   visible: j <= t + Lk - Lq (causal, aligned at the ends) or all,   p = exp(s - lse),   o_t = sum_j p_tj v_j,   lse_t = log sum_j exp(s_tj)
 //     dp_tj = do_t v_j,   delta_t = sum_d do_t o_t,   ds = p (dp - delta),   dq_t = c sum_j ds_tj k_j,   dk_j = c sum_t ds_tj q_t,   dv_j = sum_t p_tj do_t
-// A row that sees no key: o = 0, lse = -inf, no gradient.
+// A row that sees no key: o = 0, lse = -inf, no gradient.  A row that sees one: ds = 0.
 //
 // Grouped heads.  The `group` query heads of a key head are rows of one matrix: row r of sequence i and key head h is token r / group, query head h group + r % group.  A tile of
 // rows then shares K and V among the heads, few tokens still fill a tile, a causal tile's diagonal is `group` times shorter, and the sums over the group that dk and dv need
@@ -302,6 +302,8 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
         const float x = p.lse[stat];
         lse2 = x == -INFINITY ? INFINITY : x * 1.44269504088896341f;
         if (half == 0 && block.part == 0) p.delta[stat] = delta;
+        // (a row that sees one key has the weight 1 on it whatever its score: dS is 0, and not what the roundings of dP and delta leave)
+        if (end - (WINDOW && from > p.sinks ? from - p.sinks : 0) == 1) lse2 = INFINITY;
     }
     const float lse0 = lse2;
     if constexpr (kNarrow<T>) lse2 -= kUp;      // (P is not needed but for dS: 2^up is part of its exponent)
@@ -466,6 +468,9 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     const int wave_until = WINDOW ? __builtin_amdgcn_readfirstlane(tiles.end_row(f.n, wave_key < p.sinks ? 0 : wave_key + 31)) : 0,
               wave_least = WINDOW ? __builtin_amdgcn_readfirstlane(tiles.end_row(f.n, wave_key < p.sinks && p.sinks < wave_key + 32 ? p.sinks : wave_key)) : 0;
     const int wave_first = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave)), wave_all = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave + 31));
+    // Rows that see one key have no dS: all that see this tile's, or those of the first position, which see the first key alone (`alone`: one behind them, in the wavefront that has that key).
+    const bool only = rk.length == 1 || (WINDOW && p.window == 1 && !p.sinks);
+    const int alone = wave_key == 0 && (WINDOW || p.causal) && lq >= rk.length ? (lq - rk.length + 1) * p.group : 0;
     // steps of this part
     const int begin = tiles.first_step(f.n, f.tile), steps = tiles.end_step(f.n, f.tile) - begin;
     int t0 = begin + (int)((int64_t)block.part * steps / f.parts), n = begin + (int)((int64_t)(block.part + 1) * steps / f.parts);
@@ -567,6 +572,11 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
             }
             V8 pf[2], df[2];
             g *= s;
+            if (row0 + 32 * h < alone) {
+                const int left = lane & 31 ? 0 : alone - row0 - 32 * h - 4 * half;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) g[e] = 8 * (e >> 2) + (e & 3) >= left ? g[e] : g[e] * 0.f;
+            }
             if constexpr (kNarrow<T>) {
                 g *= up;
                 const float top = largest(g);
@@ -617,6 +627,10 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
         step(t + 1, tile2, tile3, stats1);
     }
     if (!live) return;
+    if (only) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) dk[b] *= 0.f;
+    }
     if constexpr (kNarrow<T>) {
         const float back = power_of_two(1 - kUpP - __builtin_amdgcn_frexp_expf(up));      // (of a power of two: the exponent and one)
 #pragma unroll
@@ -829,7 +843,6 @@ int backward(const cosmos_attn_ragged_desc* desc, int64_t window, int64_t sinks,
     const Window w = window_of(desc, window, sinks);
     RaggedParams p = params_of(desc);
     p.window = w.window; p.sinks = w.sinks;
-    if (w.window == 1 && !w.sinks) p.scale = 0.f;       // (a row that sees one key has the weight 1 on it, whatever its score: dq and dk are 0, and not what roundings of dP and delta leave)
     p.delta = (float*)workspace;
     p.parts = (float*)((char*)workspace + up((size_t)desc->Tq * desc->Hq * sizeof(float)));      // (of dq, then of dk and dv)
     const Pieces pieces = pieces_of(desc, w);
