@@ -297,13 +297,14 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
         delta = over_halves_sum(delta);
     }
     const int64_t stat = (int64_t)hq * p.Tq + rq.start + token;
+    // A row that sees one key has the weight 1 on it whatever its score, and dS = 0, not what the roundings of dP and delta leave.  Here it has no P; its delta for the second kernel is its dP (below),
+    // whose products that kernel adds up in the same order: their difference is 0.
+    const bool one = end - (WINDOW && from > p.sinks ? from - p.sinks : 0) == 1, some = __any(one);
     float lse2 = INFINITY;            // (P = 0 where there is no row, or nothing that it sees)
     if (live) {
         const float x = p.lse[stat];
-        lse2 = x == -INFINITY ? INFINITY : x * 1.44269504088896341f;
-        if (half == 0 && block.part == 0) p.delta[stat] = delta;
-        // (a row that sees one key has the weight 1 on it whatever its score: dS is 0, and not what the roundings of dP and delta leave)
-        if (end - (WINDOW && from > p.sinks ? from - p.sinks : 0) == 1) lse2 = INFINITY;
+        lse2 = x == -INFINITY || one ? INFINITY : x * 1.44269504088896341f;
+        if (half == 0 && block.part == 0 && !one) p.delta[stat] = delta;
     }
     const float lse0 = lse2;
     if constexpr (kNarrow<T>) lse2 -= kUp;      // (P is not needed but for dS: 2^up is part of its exponent)
@@ -340,6 +341,13 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
             if (masked)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = 32 * h + 8 * (e >> 2) + (e & 3) < left ? s[e] : 0.f;
+            if (some) {                             // (the one key is the last that the row sees)
+                const int last = left - 1 - 32 * h;
+                float dp = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) dp = 8 * (e >> 2) + (e & 3) == last ? g[e] : dp;
+                if (one && last >= 0 && last < 32 && !(last & 4)) p.delta[stat] = dp;
+            }
             if (behind) {
                 const int out = from - key0 - 4 * half, in = p.sinks - key0 - 4 * half;
 #pragma unroll
@@ -468,9 +476,6 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
     const int wave_until = WINDOW ? __builtin_amdgcn_readfirstlane(tiles.end_row(f.n, wave_key < p.sinks ? 0 : wave_key + 31)) : 0,
               wave_least = WINDOW ? __builtin_amdgcn_readfirstlane(tiles.end_row(f.n, wave_key < p.sinks && p.sinks < wave_key + 32 ? p.sinks : wave_key)) : 0;
     const int wave_first = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave)), wave_all = __builtin_amdgcn_readfirstlane(tiles.first_row(f.n, key0 + 32 * wave + 31));
-    // Rows that see one key have no dS: all that see this tile's, or those of the first position, which see the first key alone (`alone`: one behind them, in the wavefront that has that key).
-    const bool only = rk.length == 1 || (WINDOW && p.window == 1 && !p.sinks);
-    const int alone = wave_key == 0 && (WINDOW || p.causal) && lq >= rk.length ? (lq - rk.length + 1) * p.group : 0;
     // steps of this part
     const int begin = tiles.first_step(f.n, f.tile), steps = tiles.end_step(f.n, f.tile) - begin;
     int t0 = begin + (int)((int64_t)block.part * steps / f.parts), n = begin + (int)((int64_t)(block.part + 1) * steps / f.parts);
@@ -572,11 +577,6 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
             }
             V8 pf[2], df[2];
             g *= s;
-            if (row0 + 32 * h < alone) {
-                const int left = lane & 31 ? 0 : alone - row0 - 32 * h - 4 * half;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) g[e] = 8 * (e >> 2) + (e & 3) >= left ? g[e] : g[e] * 0.f;
-            }
             if constexpr (kNarrow<T>) {
                 g *= up;
                 const float top = largest(g);
@@ -627,10 +627,6 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dkdv_kernel(const RaggedPa
         step(t + 1, tile2, tile3, stats1);
     }
     if (!live) return;
-    if (only) {
-#pragma unroll
-        for (int b = 0; b < NB; ++b) dk[b] *= 0.f;
-    }
     if constexpr (kNarrow<T>) {
         const float back = power_of_two(1 - kUpP - __builtin_amdgcn_frexp_expf(up));      // (of a power of two: the exponent and one)
 #pragma unroll
