@@ -215,7 +215,7 @@ int check_rope(const cosmos_attn_cache_desc* d, const cosmos_attn_cache_rope* r)
     if (!r || r->pairs < 0 || r->axes < 1 || !(r->eps >= 0.f && r->eps <= 3.0e38f)) return COSMOS_ATTN_BAD_ARG;
     if (r->pairs % 8 || 2 * (int64_t)r->pairs > d->D) return COSMOS_ATTN_BAD_SHAPE;
     if (r->axes > kMostAxes) return COSMOS_ATTN_UNSUPPORTED;
-    if (r->pairs && (!r->freqs || (r->axes > 1 && !r->positions))) return COSMOS_ATTN_BAD_ARG;
+    if (r->pairs && (!r->freqs || (r->axes > 1 && d->rows && !r->positions))) return COSMOS_ATTN_BAD_ARG;
     if (!aligned16(r->freqs) || !aligned16(r->q_weight) || !aligned16(r->k_weight) || (reinterpret_cast<uintptr_t>(r->positions) & 3) || r->positions_stride < 0) return COSMOS_ATTN_BAD_STRIDE;
     return COSMOS_ATTN_OK;
 }
