@@ -254,6 +254,12 @@ int cosmos_attn_cache_append(const cosmos_attn_cache_desc* desc, const cosmos_at
     p.share[1] = p.share[2] = share_of(desc, desc->Hkv);
     const int64_t blocks = p.share[0].blocks + p.share[1].blocks + p.share[2].blocks;
     if (blocks > kMostBlocks) return COSMOS_ATTN_UNSUPPORTED;
+    if (desc->q) {
+        // (keys or values that queries have been written over would be what another workgroup reads)
+        const Packed o = {desc->o, desc->o_stride, desc->Hq};
+        if (check_in_place(desc, desc->rows) != COSMOS_ATTN_OK || meet_in_memory(o, {desc->k_rows, desc->k_rows_stride, desc->Hkv}, desc->rows, desc->D) ||
+            meet_in_memory(o, {desc->v_rows, desc->v_rows_stride, desc->Hkv}, desc->rows, desc->D)) return COSMOS_ATTN_BAD_ARG;
+    }
     if (!device_is_whole_mi355x()) return COSMOS_ATTN_WRONG_DEVICE;
     p.freqs = rope->freqs; p.positions = rope->positions; p.positions_row = rope->positions_stride;
     p.weight[0] = rope->q_weight; p.weight[1] = rope->k_weight; p.weight_16 = rope->weight_16 != 0;

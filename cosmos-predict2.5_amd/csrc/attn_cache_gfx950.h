@@ -158,6 +158,30 @@ int check_out(const void* at, const int64_t* stride, int64_t rows, int heads, in
     const bool by_row = rows <= 1 || stride[0] >= (heads - 1) * stride[1] + D, by_head = heads <= 1 || stride[1] >= (rows - 1) * stride[0] + D;
     return by_row || by_head ? COSMOS_ATTN_OK : COSMOS_ATTN_BAD_STRIDE;
 }
+// Rows of D 16-bit elements, [rows, heads]: do two such tensors have an element in common?  Of different row strides they are taken to where their extents meet.
+struct Packed { const void* at; const int64_t* stride; int heads; };
+bool meet_in_memory(Packed a, Packed b, int64_t rows, int D) {
+    const bool one_row = rows <= 1;
+    auto extent = [&](Packed x) { return (__int128)(one_row ? 0 : rows - 1) * x.stride[0] + (__int128)(x.heads - 1) * x.stride[1] + D; };
+    const __int128 between = ((__int128)reinterpret_cast<uintptr_t>(b.at) - (__int128)reinterpret_cast<uintptr_t>(a.at)) / 2;      // elements from a's first row to b's (of 16-byte steps)
+    if (between >= extent(a) || -between >= extent(b)) return false;
+    if (!one_row && a.stride[0] != b.stride[0]) return true;
+    const int64_t step = one_row ? 0 : a.stride[0];
+    for (int i = 0; i < a.heads; ++i)
+        for (int j = 0; j < b.heads; ++j) {
+            const __int128 d = between + (__int128)j * b.stride[1] - (__int128)i * a.stride[1];
+            // some row of b, `n` rows behind one of a, is less than a row's D elements from it
+            const __int128 n = step ? -d / step : 0;
+            for (__int128 k = n - 1; k <= n + 1; ++k)
+                if (k < rows && -k < rows && d + k * step < D && -(d + k * step) < D) return true;
+        }
+    return false;
+}
+// Queries and the output of as many rows and heads: apart, or the same rows, which a lane (a workgroup) has read before it writes them.
+int check_in_place(const cosmos_attn_cache_desc* d, int64_t rows) {
+    const bool same = d->o == d->q && (rows <= 1 || d->o_stride[0] == d->q_stride[0]) && (d->Hq <= 1 || d->o_stride[1] == d->q_stride[1]);
+    return same || !meet_in_memory({d->o, d->o_stride, d->Hq}, {d->q, d->q_stride, d->Hq}, rows, d->D) ? COSMOS_ATTN_OK : COSMOS_ATTN_BAD_ARG;
+}
 int check_scale(const float* at, const int64_t* stride) {
     if (!at) return COSMOS_ATTN_BAD_ARG;
     return aligned16(at) && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[0] >= 0 && stride[1] >= 0 ? COSMOS_ATTN_OK : COSMOS_ATTN_BAD_STRIDE;

@@ -653,7 +653,8 @@ int check_attention(const cosmos_attn_cache_desc* d) {
     // (tiles of all sequences are counted in 32 bits)
     if ((int64_t)d->B * (((int64_t)d->width * d->page_size + kTile - 1) / kTile) > kMost / 2 || (int64_t)d->B * d->Hq > kMostBlocks / 2) return COSMOS_ATTN_UNSUPPORTED;
     st = check_rows(d->q, d->q_stride);
-    return st != COSMOS_ATTN_OK ? st : check_out(d->o, d->o_stride, d->B, d->Hq, d->D);
+    if (st == COSMOS_ATTN_OK) st = check_out(d->o, d->o_stride, d->B, d->Hq, d->D);
+    return st != COSMOS_ATTN_OK ? st : check_in_place(d, d->B);
 }
 // Tables of few tiles: a workgroup for each sequence and head, and nothing to join, which a second launch would be for (333 keys of 4 heads: 6.3 us, as parts 5.8 and 3.8 for the join).  Of
 // some more tiles too where there are many workgroups (us, whole / as parts: 32 sequences of 1000 keys, 64 heads of 64 on 8, 13.9 / 20.2; 300 of them in int8 78 / 90; 128 of 2000 keys, 32 heads of 128 on

@@ -755,7 +755,8 @@ int check_chunk(const cosmos_attn_cache_desc* d, int64_t window, int64_t sinks) 
     if (!d->cu || (d->B && !d->lens)) return COSMOS_ATTN_BAD_ARG;
     if (d->q_stride[0] * 2 > kMostRowBytes || d->o_stride[0] * 2 > kMostRowBytes) return COSMOS_ATTN_BAD_STRIDE;
     st = check_rows(d->q, d->q_stride);
-    return st != COSMOS_ATTN_OK ? st : check_out(d->o, d->o_stride, d->rows, d->Hq, d->D);
+    if (st == COSMOS_ATTN_OK) st = check_out(d->o, d->o_stride, d->rows, d->Hq, d->D);
+    return st != COSMOS_ATTN_OK ? st : check_in_place(d, d->rows);
 }
 
 }  // namespace

@@ -211,7 +211,7 @@ def cache_append(
     out: Optional[torch.Tensor] = None,
 ) -> Optional[torch.Tensor]:
     """New tokens, packed as for :func:`cache_write`: keys are normalised and turned by their positions and written with their values; returns the queries, normalised and turned, ``[rows, Hq, D]``
-    (``q`` None: None; ``out``, which may be ``q``, takes them).
+    (``q`` None: None; ``out`` takes them: memory of its own, or ``q`` itself; one that lies over ``k``, ``v`` or other rows of ``q`` is refused).
 
     ``freqs``: ``[R]`` or ``[axes, R]``, fp32 (others are rounded to it), radians a position, for R pairs of channels (a multiple of 8, ``2 R <= D``): ``(i, i + R)``, or with ``interleaved`` ``(2 i, 2 i + 1)``; the channels behind
     are not turned (None: none are).  The angle of pair i is ``sum_a positions[row, a] * freqs[a, i]``, formed in 64 bits; ``positions``: whole numbers ``[rows]`` or ``[rows, axes]``, of images and
@@ -343,7 +343,7 @@ def cache_attention(
     ``window``: a token sees that many last positions, its own among them, and those below ``sinks``; pages that no token of a sequence sees are not looked up, whatever the table says of them.
 
     A token that sees nothing (``lens[i] == 0``, or below its rows): o = 0, lse = -inf.  A length that the table does not hold: NaN.  A page outside of the cache: NaN for the tokens that see it.
-    ``out``: a tensor for o."""
+    ``out``: a tensor for o, of its own memory or ``q`` itself."""
     window, sinks = checked_window(window, sinks)
     if out is None:
         made = _attention_as_it_is(q, cache, table, lens, sm_scale, need_lse, cu, window, sinks)

@@ -516,7 +516,7 @@ COSMOS_ATTN_API int cosmos_attn_cache_chunk(const cosmos_attn_cache_desc *desc, 
 
 /*
  * cosmos_attn_cache_append: cosmos_attn_cache_write of keys that are normalised and turned by their positions first, and of their values, with the queries of the same tokens in the same pass.
- * q, o [rows, Hq, D] (o may be q; q NULL: no queries), k_rows, v_rows [rows, Hkv, D]; lens, cu, table as in cosmos_attn_cache_write.  A row x of a head of q or k becomes
+ * q, o [rows, Hq, D] (o may be q itself, and has no other memory in common with q, k_rows or v_rows: refused; q NULL: no queries), k_rows, v_rows [rows, Hkv, D]; lens, cu, table as in cosmos_attn_cache_write.  A row x of a head of q or k becomes
  *     x rsqrt(mean(x^2) + eps) w                                   where there is a weight w
  *     (u, v) -> (u cos a_i - v sin a_i, v cos a_i + u sin a_i)     for `pairs` pairs of channels, (i, i + pairs) or with `interleaved` (2 i, 2 i + 1);   a_i = sum over axes of position * freqs[axis][i]
  * in fp32 (angles in 64 bits), rounded once, to `dtype` or to the cache's codes.  The position is the token's place in its sequence, or positions[row][axis].
