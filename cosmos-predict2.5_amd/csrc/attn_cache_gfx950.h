@@ -117,9 +117,10 @@ struct Place {
     __device__ __forceinline__ bool has(const CacheParams& p, int row) const { return seq < p.B && start >= 0 && row >= start && row < end && end <= p.rows; }
 };
 
-// x / s as IEEE division rounds it, for |x / s| up to some hundreds: x r corrected by the remainder, which fma gives exactly (Markstein's division), with r = 1 / s good to an ulp.  (That one
-// correction is enough has been seen for all there is: a 16-bit x has 2^7 or 2^10 significands and s, which follows from another one, as many.)  Rows whose scale would leave the range
-// in which all of that is exact are multiplied with a power of two first, as their scale is.
+// x / s as IEEE division rounds it, for fp32 numbers with |x / s| up to some hundreds: x r corrected by the remainder (Markstein's division), with r = 1 / s corrected by its own.  With the nearest r, which this
+// is for each of the 2^23 significands of s (the instruction is good to one unit), that is 3 units times 2^-24 off at most before its rounding; of quotients that close to the middle of two numbers there are
+// 29 million, and all of them come out right.  (tests/test_host_division.py has the bound and how to find them.)  Rows whose scale would leave the range in which all of that is exact are multiplied
+// with a power of two first, as their scale is.
 struct Divide {
     float s, r, by;
     __device__ __forceinline__ explicit Divide(float scale) {
