@@ -31,7 +31,7 @@ struct AppendParams : CacheParams {
     const int* positions;         // [rows, axes], or null: places in the sequences
     int64_t positions_row;
     const void* weight[2];        // of queries, of keys: fp32, or 16 bits; null: no norm
-    int Hq, pairs, axes, weight_16;
+    int pairs, axes, weight_16;
     float eps;
 };
 
@@ -248,7 +248,7 @@ int cosmos_attn_cache_append(const cosmos_attn_cache_desc* desc, const cosmos_at
     if (st != COSMOS_ATTN_OK || !desc->rows) return st;
     AppendParams p = {};
     static_cast<CacheParams&>(p) = params_of(desc);
-    p.q = (const char*)desc->q; p.o = (char*)desc->o; p.Hq = desc->Hq;
+    p.q = (const char*)desc->q; p.o = (char*)desc->o;
     p.q_row = 2 * desc->q_stride[0]; p.q_head = 2 * desc->q_stride[1]; p.o_row = 2 * desc->o_stride[0]; p.o_head = 2 * desc->o_stride[1];
     p.share[0] = desc->q ? share_of(desc, desc->Hq) : Share{1, 0};
     p.share[1] = p.share[2] = share_of(desc, desc->Hkv);

@@ -257,7 +257,6 @@ constexpr int kAtOnce = 2 * kNumCUs;      // workgroups
 constexpr int least_steps(int D) { return D == 128 ? 12 : 24; }
 constexpr int least_rows(int D) { return D == 128 ? 512 : 2048; }       // (of dk and dv, in rows)
 template <bool WINDOW, bool PAGED = false> using RowTilesOf = Tiles<false, kRows, kStep, WINDOW, PAGED>;
-typedef RowTilesOf<false> RowTiles;
 // of dk and dv
 constexpr int row_step(int D) { return D == 128 ? 32 : 64; }
 template <int D, bool WINDOW = false> using KeyTiles = Tiles<true, kRows, row_step(D), WINDOW>;
@@ -439,13 +438,13 @@ constexpr float kLowest = -3.0e38f;      // a max that no score has moved yet: e
 // of 16 wavefronts instead of two, 37 us.)
 constexpr int kJoinThreads = 1024;
 template <int D> constexpr int kJoinBlocks = kRows * (D / 4) / kJoinThreads;      // of a tile
-template <typename T, int D, int WHICH, bool WINDOW = false, bool PAGED = false>
+template <typename T, int D, int WHICH, bool WINDOW = false>
 __global__ void __launch_bounds__(kJoinThreads) __attribute__((amdgpu_num_sgpr(80))) ragged_join_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr bool KEYS = WHICH == 2;
     constexpr int LANES = D / 4, AT_ONCE = kJoinThreads / LANES;
     const int head = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv % p.tiles;
-    const Found f = find<std::conditional_t<KEYS, KeyTiles<D, WINDOW>, RowTilesOf<WINDOW, PAGED>>, kJoinThreads>(p, index);
+    const Found f = find<std::conditional_t<KEYS, KeyTiles<D, WINDOW>, RowTilesOf<WINDOW>>, kJoinThreads>(p, index);
     if (f.seq < 0 || f.parts <= 1) return;
     if constexpr (KEYS && WINDOW) {
         if (KeyTiles<D, WINDOW>{p}.pieces(f.n, f.tile)) return;
