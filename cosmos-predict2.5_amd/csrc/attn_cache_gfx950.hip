@@ -658,9 +658,17 @@ int check_attention(const cosmos_attn_cache_desc* d) {
 }
 // Tables of few tiles: a workgroup for each sequence and head, and nothing to join, which a second launch would be for (333 keys of 4 heads: 6.3 us, as parts 5.8 and 3.8 for the join).  Of
 // some more tiles too where there are many workgroups (us, whole / as parts: 32 sequences of 1000 keys, 64 heads of 64 on 8, 13.9 / 20.2; 300 of them in int8 78 / 90; 128 of 2000 keys, 32 heads of 128 on
-// 8, 101 / 106; but 40 of them 70 / 68), up to lengths at which the longest alone takes some 20 us.  A window's tiles are all there are: six of them go whole (one token, 500 keys and 16 first ones,
-// a call with the host's part, us, 16 heads of 64 on 4 in fp16 11.2 / 13.3, 32 of 128 on 8 in int8 14.5 / 13.5; eight tiles 12.8 / 13.0 and 17.6 / 13.2).
-constexpr int kWholeTiles = 4, kWholeWindow = 6, kWholeManyTiles = 16, kMany = 32;       // kMany: workgroups to a tile of the table's
+// 8, 101 / 106; but 40 of them 70 / 68), up to lengths at which the longest alone takes some 20 us.
+// A window's tiles are all there are, and a workgroup for each sequence and head goes through them in 3.4 to 4.2 us and 1 to 1.9 us a tile, by head dim, codes and rows.  Parts and their join take 8.2 to 9.9 us (12.5 with
+// two blocks of rows) of the device, a captured step's time, and 13 for the host of a call by itself, to whose 8.6 a single launch is hidden.  The limit lies between where the one and the other is made up for:
+// 6.5 us of tiles (captured / by itself, us, whole against parts, 1 to 16 sequences, 1 to 8 heads of keys: head dim 64 in 16 bits 6 tiles 9.7 / 10.8 against 8.9 / 13.0, 8 tiles 11.8 / 12.9 against 8.9 / 13.0;
+// int8 5 tiles 10.2 / 11.3 against 8.9 / 13.2; head dim 128 in 16 bits 5 tiles 10.0 / 10.9 against 9.6 / 13.2, in int8 4 tiles 10.1 / 11.0 against 9.7 / 13.2, 6 tiles 13.3 / 14.3 against 9.8 / 13.1, with 32 query
+// heads to one of keys 3 tiles 11.1 / 12.0 against 12.2 / 13.8, 5 tiles 15.1 / 15.9 against 12.4 / 14.0).
+constexpr int kWholeTiles = 4, kWholeManyTiles = 16, kMany = 32;       // kMany: workgroups to a tile of the table's
+constexpr int kWholeWindow = 650;                                      // hundredths of a microsecond
+int tile_time(const cosmos_attn_cache_desc* d, int rows16) {
+    return (d->D == 64 ? 100 : 120) + (d->kind == COSMOS_ATTN_CACHE_SAME ? 0 : d->kind == COSMOS_ATTN_CACHE_E4M3 ? 15 : 30) + (rows16 == 1 ? 0 : 25);
+}
 struct Shape { int row_blocks, rows16, slots; bool whole; };
 Shape shape_of(const cosmos_attn_cache_desc* d, Window w) {
     const int group = d->Hq / d->Hkv, rows16 = group <= 16 ? 1 : 2, row_blocks = (group + 16 * rows16 - 1) / (16 * rows16);
@@ -670,7 +678,7 @@ Shape shape_of(const cosmos_attn_cache_desc* d, Window w) {
         capacity = seen < capacity ? seen : capacity;
     }
     const int64_t most = (int64_t)d->B * capacity;
-    if (capacity <= (w.window ? kWholeWindow : kWholeTiles) || (capacity <= kWholeManyTiles && (int64_t)d->B * d->Hkv * row_blocks >= kMany * capacity)) return {row_blocks, rows16, 1, true};
+    if ((w.window ? capacity * tile_time(d, rows16) <= kWholeWindow : capacity <= kWholeTiles) || (capacity <= kWholeManyTiles && (int64_t)d->B * d->Hkv * row_blocks >= kMany * capacity)) return {row_blocks, rows16, 1, true};
     // two workgroups a compute unit, if the tables hold that many tiles
     int64_t slots = 2 * kNumCUs / ((int64_t)d->Hkv * row_blocks);
     slots = slots < 1 ? 1 : slots;

@@ -294,9 +294,9 @@ def cache_read(cache: KVCache, table: torch.Tensor, cu: torch.Tensor, rows: int,
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(Hkv: int, D: int, page_size: int, B: int, width: int, Hq: int, window: int = 0, sinks: int = 0, rows: int = -1) -> int:
-    """What the library asks for, which follows from sizes alone (addresses are never dereferenced).  `rows`: of a call with offsets."""
-    part = _CACHE_PART.pack(_lib.ABI_VERSION, _lib.DTYPE_BF16, _lib.CACHE_SAME, Hkv, D, page_size, 1, 16, 16, *(page_size * Hkv * D, page_size * D, D) * 2, 0, 0, 0, 0, 0, 0)
+def _workspace_bytes(Hkv: int, D: int, page_size: int, B: int, width: int, Hq: int, window: int = 0, sinks: int = 0, rows: int = -1, kind: int = _lib.CACHE_SAME) -> int:
+    """What the library asks for, which follows from sizes and the cache's kind alone (addresses are never dereferenced).  `rows`: of a call with offsets."""
+    part = _CACHE_PART.pack(_lib.ABI_VERSION, _lib.DTYPE_BF16, kind, Hkv, D, page_size, 1, 16, 16, *(page_size * Hkv * D, page_size * D, D) * 2, 16, 16, 0, 0, 0, 0)
     call = _CALL_PART.pack(B, width, 16, width, 16, 16, max(rows, 0), 0, 0, 0, 0, 0, 0, 0, Hq, 1.0, 0, 16, 16, Hq * D, D, Hq * D, D, 0)
     lib = _lib.load_library()
     return (lib.cosmos_attn_cache_window_workspace_bytes if rows < 0 else lib.cosmos_attn_cache_chunk_workspace_bytes)(part + call, window, sinks)
@@ -317,7 +317,7 @@ def _attention_as_it_is(q, cache, table, lens, sm_scale, need_lse, cu, window, s
     lse = q.new_empty((rows, Hq), dtype=torch.float32) if need_lse else None
     desc = part + _CALL_PART.pack(B, width, table.data_ptr(), table.stride()[0], lens.data_ptr(), 0 if cu is None else cu.data_ptr(), rows, 0, 0, 0, 0, 0, 0, _lib.FILL_ALL, Hq,
                                   D ** -0.5 if sm_scale is None else sm_scale, 0, pq, o.data_ptr(), row, D, row, D, 0 if lse is None else lse.data_ptr())
-    ws_bytes = _workspace_bytes(cache.heads, D, cache.page_size, B, width, Hq, window, sinks, -1 if cu is None else rows)
+    ws_bytes = _workspace_bytes(cache.heads, D, cache.page_size, B, width, Hq, window, sinks, -1 if cu is None else rows, cache.kind)
     workspace = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     lib = _lib.load_library()
     on_device(device, lib.cosmos_attn_cache_window if cu is None else lib.cosmos_attn_cache_chunk, desc, window, sinks, 0 if workspace is None else workspace.data_ptr(), ws_bytes)
@@ -367,7 +367,7 @@ def cache_attention(
             raise ValueError("out: rows of 16-byte steps are written in place, this view cannot be")
         o = out
     lse = q.new_empty((rows, Hq), dtype=torch.float32) if need_lse else None
-    ws_bytes = _workspace_bytes(cache.heads, D, cache.page_size, B, table.shape[1], Hq, window, sinks, -1 if cu is None else rows)
+    ws_bytes = _workspace_bytes(cache.heads, D, cache.page_size, B, table.shape[1], Hq, window, sinks, -1 if cu is None else rows, cache.kind)
     workspace = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     desc = part + _call(table, lens.data_ptr(), 0 if cu is None else cu.data_ptr(), rows, 0, 0, (0, 0), (0, 0), _lib.FILL_ALL if out is None else _lib.FILL_LSE, Hq,
                         D ** -0.5 if sm_scale is None else sm_scale, q.data_ptr(), o.data_ptr(), q.stride()[:2], o.stride()[:2], 0 if lse is None else lse.data_ptr())
