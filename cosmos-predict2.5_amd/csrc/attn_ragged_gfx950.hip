@@ -762,7 +762,8 @@ int check_window(const cosmos_attn_ragged_desc* d, int64_t window, int64_t sinks
 Window window_of(const cosmos_attn_ragged_desc* d, int64_t window, int64_t sinks) {
     return window && window < d->Tk && sinks < d->Tk ? Window{(int)window, (int)sinks} : Window{};
 }
-// The first keys' tiles of dk and dv: pieces of three quarters of a window's steps, 1024 rows at least, and not more pieces than twice the workgroups that run at once (what they leave is 128 MB then).
+// The first keys' tiles of dk and dv: pieces of three quarters of a window's steps, 1024 rows at least, and about as many pieces at most as twice the workgroups that run at once (each tile may have one more:
+// 1536, and what they leave is 192 MiB, at most).
 struct Pieces { int piece, slots, tiles; size_t bytes; };
 Pieces pieces_of(const cosmos_attn_ragged_desc* d, Window w) {
     if (!w.window || !w.sinks || !d->Tq) return {};

@@ -104,8 +104,8 @@ def dequantise(codes, scale):
 
 def turned(x, weight, eps, positions, freqs, interleaved):
     """(y, bound): rows [n, heads, D] normalised (weight None: not) and turned, positions [n, axes] and freqs [axes, pairs], in 64 bits; how far arithmetic in fp32 may be from it.
-    The norm: D + 2 roundings of a sum under a root, its own two and the product's: (D + 2) / 2 + 4.  cos and sin: an angle in turns is rounded to fp32 below 1/2, 2^-26 of a turn, 2 pi 2^-26 < 2^-23;
-    the series and their last steps another 2^-23; formed in 64 bits it is off by 2^-52 of itself.  Two products and a sum: 3."""
+    The norm: D + 2 roundings of a sum under a root, its own two and the product's: (D + 2) / 2 + 4.  cos and sin: the angle, reduced to an eighth of a turn in 64 bits, is
+    rounded to fp32 below 1, 2^-25; the series, their remainders of 2^-29 and their last steps less than 2^-23: 2^-22 in all; formed in 64 bits the angle is off by 2^-52 of itself (2^-50 below: of several axes too).  Two products and a sum: 3."""
     x = x.double().cpu()
     off = torch.zeros(x.shape[:2] + (1,), dtype=torch.float64)
     if weight is not None:
