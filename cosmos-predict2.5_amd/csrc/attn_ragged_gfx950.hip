@@ -296,10 +296,23 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
         }
         delta = over_halves_sum(delta);
     }
+    // A row that sees one key has the weight 1 on it whatever its score, and dS = 0, not what the roundings of dP and delta leave.  Here it has no P; its delta for the second kernel is its
+    // dP, the same products of 16 channels in the same order as there, so that their difference is 0.  (In front of the loop: in either kernel's loop a few registers more cost 2 to 9 %.)
+    const bool one = end - (WINDOW && from > p.sinks ? from - p.sinks : 0) == 1;
+    const unsigned long long ones = __ballot(one);
+    if (ones && block.part == 0) {
+        // (the last key that it sees; the wavefront's lie behind each other, from the first such row's on)
+        const int base = __builtin_amdgcn_readlane(end, __builtin_ctzll(ones)) - 1, at = base + (lane & 31), own = end - 1 - base - 4 * half;
+        const char* const va = vp + (int64_t)(at < lk ? at : lk - 1) * p.v_row + 16 * half;
+        f32x16 g = f32x16{};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) g = mfma32(__builtin_bit_cast(V8, *reinterpret_cast<const u32x4*>(va + 32 * c)), gf[c], g);
+        float dp = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp = 8 * (e >> 2) + (e & 3) == own ? g[e] : dp;
+        if (one && own >= 0 && !(own & 4)) p.delta[(int64_t)hq * p.Tq + rq.start + token] = dp;
+    }
     const int64_t stat = (int64_t)hq * p.Tq + rq.start + token;
-    // A row that sees one key has the weight 1 on it whatever its score, and dS = 0, not what the roundings of dP and delta leave.  Here it has no P; its delta for the second kernel is its dP (below),
-    // whose products that kernel adds up in the same order: their difference is 0.
-    const bool one = end - (WINDOW && from > p.sinks ? from - p.sinks : 0) == 1, some = __any(one);
     float lse2 = INFINITY;            // (P = 0 where there is no row, or nothing that it sees)
     if (live) {
         const float x = p.lse[stat];
@@ -341,13 +354,6 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
             if (masked)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = 32 * h + 8 * (e >> 2) + (e & 3) < left ? s[e] : 0.f;
-            if (some) {                             // (the one key is the last that the row sees)
-                const int last = left - 1 - 32 * h;
-                float dp = 0.f;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) dp = 8 * (e >> 2) + (e & 3) == last ? g[e] : dp;
-                if (one && last >= 0 && last < 32 && !(last & 4)) p.delta[stat] = dp;
-            }
             if (behind) {
                 const int out = from - key0 - 4 * half, in = p.sinks - key0 - 4 * half;
 #pragma unroll
