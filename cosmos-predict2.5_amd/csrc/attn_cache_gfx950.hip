@@ -151,7 +151,7 @@ constexpr int kTile = 128;           // keys: 32 of each wavefront
 constexpr float kLowest = -3.0e38f;
 
 // WINDOW: the token at the end of n keys sees those from n - window on and the first ones.  Its tiles are those of the first keys and, behind the `gap` that it does not look at, those of the
-// window (64 sequences of up to 30000 keys, 4096 and the first 4, 32 heads of 128 on 8 in int8: 62 us, 4.6 TB/s): tile u is tile u, or from `first` on u + gap.  Keys between are not read, nor are their pages looked up: what they hold, and what the table says of them, may be anything.
+// window (64 sequences of up to 30000 keys, 4096 and the first 4, 32 heads of 128 on 8 in int8: 68 us a call, the kernel 58, 4.9 TB/s): tile u is tile u, or from `first` on u + gap.  Keys between are not read, nor are their pages looked up: what they hold, and what the table says of them, may be anything.
 struct Gap {
     int from, first, gap;       // the first key that is looked back on
     __device__ __forceinline__ Gap(const CacheParams& p, int n) {

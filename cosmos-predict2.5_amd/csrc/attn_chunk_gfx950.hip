@@ -322,7 +322,7 @@ __device__ __forceinline__ void meet_in_lds() {
 }
 
 // ---- A workgroup: as ragged_fwd_kernel, with K and V out of pages.  2048 tokens on 16384 positions, 32 heads of 128 on 8: 500 us, 1.0 PFLOP/s, in 8 bits 595 to 620 (codes' conversions are 8 %, scales 11 % of that, measured
-// without them; what bounds it is as there, a fragment from LDS to each product).  A call of few tiles is as long as its longest part: a step of 64 keys takes 1.1 us in 16 bits and 1.7 in 8, all of it one chain.
+// without them; the matrix unit is busy 55 % of the time, as there with two wavefronts on a SIMD, whose maxima and exponentials it waits for).  A call of few tiles is as long as its longest part: a step of 64 keys takes 1.1 us in 16 bits and 1.7 in 8, all of it one chain.
 // Hence parts of 4 steps at least, if there are more than 8 (64 tokens on 1280 positions, 8 heads on 2, us, bf16 / int8: whole 30 / 42, parts of 8 and more 24 / 30, of 6 21 / 26, of 4 18 / 21, with 5 for the second launch).
 // 16 bits: rows go straight to LDS; what lies behind the last key, and runs that no row of the tile sees, come as zeros.  8 bits: codes are loaded into registers a step earlier, become exact
 // 16-bit values on their way to LDS, K's scales multiply the scores and V's the weights, before these are rounded.

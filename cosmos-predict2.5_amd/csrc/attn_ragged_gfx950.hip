@@ -34,10 +34,11 @@ namespace {
 
 // ---- forward.  A workgroup: kRows rows of one sequence and key head; a wavefront 32 of them, one a lane and its other half: S^T = K Q^T has the keys in registers, so that the softmax
 // needs one exchange between the halves, and P^T, rounded, is the next product's operand where it lies.  Two workgroups a compute unit (head dim 64: four), so that one's products and another's
-// exponentials go on beside each other.  16384 causal positions, 16 heads of 128 on 4: 950 to 1000 us, 1.1 to 1.15 PFLOP/s, the matrix unit busy 63 % of the time at 1.8 GHz: every product of
-// 32 x 32 x 16 has a fragment from LDS to itself, which a stream of such products alone runs at 1.09 to 1.15 PFLOP/s with.  Head dim 64: 8192 positions, 16 heads, 297 us, 0.92 PFLOP/s (causal 187,
+// exponentials go on beside each other.  16384 causal positions, 16 heads of 128 on 4: 950 to 1000 us, 1.1 to 1.15 PFLOP/s, the matrix unit busy 63 % of the time at 1.8 GHz.  (Not
+// all that a fragment from LDS to each product of 32 x 32 x 16 allows: the forward of sequences of one length, attn_fwd_jvp_gfx950.hip, has come to 1.3 that way, with three wavefronts on a SIMD, no max in front
+// of the exponentials and the softmax between the products.  Here are two, and 32 maxima and an exchange between the halves in every step.)  Head dim 64: 8192 positions, 16 heads, 297 us, 0.92 PFLOP/s (causal 187,
 // 0.73).  Short calls end with their longest tiles: 12 causal prompts of 1 to 2048 positions, 32 heads on 8, 125 us, 0.77 PFLOP/s, 84 % of the units busy.
-// WINDOW: 16384 + 5000 + 1777 + 1 positions, 1024 keys and the first 4, 16 heads on 4, 225 us, 0.81 PFLOP/s of what is seen (all of it 1.1): a tile of 32 tokens has 18.5 steps of 64 keys for 16 that each row
+// WINDOW: 16384 + 5000 + 1777 + 1 positions, 1024 keys and the first 4, 16 heads on 4, 232 us, 0.79 PFLOP/s of what is seen (all of it 1.1): a tile of 32 tokens has 18.5 steps of 64 keys for 16 that each row
 // sees, of which one holds the 4 first keys.
 template <typename T, int D, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedParams p) {
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_fwd_kernel(const RaggedPar
 // ---- backward, first kernel: delta and dq.  The forward's rows and tiles, with P from lse, dP^T = V dO^T beside S^T, and dQ^T = K^T dS^T.  Matrix unit busy 65 % at 1.7 GHz (8192 positions, 32
 // heads of 128 on 8): three products to an exponential, under the power limit.
 // WINDOW: what rounding dS leaves off is a second operand of the last product, whose other one is there already.  dq's error is then 1.03 of its own rounding instead of 1.46 (dS sums to zero over a row, so
-// that its errors are larger next to dq than next to dS), for 12 to 16 % of this kernel.  (Its reads are left to the compiler: in the order of the others 1157 instead of 1150 us for a whole pass.)
+// that its errors are larger next to dq than next to dS), for 12 to 16 % of this kernel.  (Its reads are left to the compiler: in the order of the others a pass takes as long.)
 template <typename T, int D, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 2) ragged_dq_kernel(const RaggedPara
 // LDS at 128: with both in registers there are too many for two wavefronts on a SIMD, whose matrix products and other arithmetic go on beside each other (head dim 64, 1560 + 880 + 390 positions,
 // 16 heads, us, dq with it, V in LDS / in registers: 95 / 87).  Matrix unit busy 51 % at 1.8 GHz (8192 positions, 32 heads of 128 on 8); what it waits for are reads from LDS, four to a product
 // of K's and V's side, for which no more registers are free to be ahead (two wavefronts a SIMD have 256 each, all taken).  With dq 1.12 PFLOP/s of seven products.
-// WINDOW: 12728 positions, 1024 keys and the first 4, 32 heads on 8, 475 to 570 us by the clock; before the first keys' tiles were cut into pieces 1146.
+// WINDOW: 12728 positions, 1024 keys and the first 4, 32 heads on 8, 481 us (least 464); before the first keys' tiles were cut into pieces 1146.
 // (64 keys and half of a step's rows to a wavefront, one on a SIMD with all 512 registers, so that every fragment of Q and dO feeds two products: as fast on 8192 positions, 10 to 20 % slower on 512 to
 // 4096 and on prompts of mixed lengths, where a tile's start and end then have no other workgroup beside them.)
 template <typename T, int D, bool WINDOW>

@@ -162,7 +162,7 @@ def _is_weight(x: Optional[torch.Tensor], D: int, device: int) -> bool:
 
 
 def _append_as_it_is(cache, q, k, v, table, lens, cu, freqs, positions, interleaved, q_weight, k_weight, eps):
-    """:func:`cache_append` of tensors that can be taken as they are, all of it looked at once: None where something is to be converted, copied or refused.  (One new token: 11 us, 13 with
+    """:func:`cache_append` of tensors that can be taken as they are, all of it looked at once: None where something is to be converted, copied or refused.  (One new token: 9.6 us, 13 with
     the checks one by one.)"""
     if not (q.dim() == 3 == k.dim() and 1 <= freqs.dim() <= 2 == table.dim()):
         return None
@@ -214,7 +214,7 @@ def cache_append(
     (``q`` None: None; ``out`` takes them: memory of its own, or ``q`` itself; one that lies over ``k``, ``v`` or other rows of ``q`` is refused).
 
     ``freqs``: ``[R]`` or ``[axes, R]``, fp32 (others are rounded to it), radians a position, for R pairs of channels (a multiple of 8, ``2 R <= D``): ``(i, i + R)``, or with ``interleaved`` ``(2 i, 2 i + 1)``; the channels behind
-    are not turned (None: none are).  The angle of pair i is ``sum_a positions[row, a] * freqs[a, i]``, formed in 64 bits; ``positions``: whole numbers ``[rows]`` or ``[rows, axes]``, of images and
+    are not turned (None: none are).  The angle of pair i is ``sum_a positions[row, a] * freqs[a, i]``, formed in 64 bits; ``positions``: whole numbers of 32 bits, ``[rows]`` or ``[rows, axes]``, of images and
     videos say; None: the token's place in its sequence.
     ``q_weight``, ``k_weight``: ``[D]`` of the RMS norm (``eps``) of each head's row in front of that; None: no norm.  All of it in fp32, rounded once: to the rows' type, or to the cache's 8 bits.
     Queries of no sequence, and of sequences whose ``lens`` is below their rows, become zeros (in ``out``: left as they are).  As in :func:`cache_write`, what has no place is not written."""
@@ -339,7 +339,7 @@ def cache_attention(
     """``(o, lse)``: attention of one token of each sequence, ``q [B, Hq, D]``, over the first ``lens[i]`` positions that its row of ``table`` holds; ``lse``: fp32 ``[B, Hq]``.
 
     ``cu``: of the sequences' last tokens, packed, ``q [rows, Hq, D]``: sequence i's are the rows ``cu[i] .. cu[i + 1] - 1`` and its last positions of ``lens[i]``, whose keys and values are in the
-    cache already; each sees the positions up to its own.  ``lse``: ``[rows, Hq]``.  Offsets as in :func:`ragged_fwd`; rows of no sequence become zeros, and -inf (in ``out``: left as they are).
+    cache already; each sees the positions up to its own; keys and values that it does not see have to be finite where another token of its sequence in the call sees them.  ``lse``: ``[rows, Hq]``.  Offsets as in :func:`ragged_fwd`; rows of no sequence become zeros, and -inf (in ``out``: left as they are).
     ``window``: a token sees that many last positions, its own among them, and those below ``sinks``; pages that no token of a sequence sees are not looked up, whatever the table says of them.
 
     A token that sees nothing (``lens[i] == 0``, or below its rows): o = 0, lse = -inf.  A length that the table does not hold: NaN.  A page outside of the cache: NaN for the tokens that see it.
