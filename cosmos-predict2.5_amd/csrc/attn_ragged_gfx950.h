@@ -530,7 +530,7 @@ inline int64_t most_tiles(int64_t rows, int n_seq) { return rows / kRows + n_seq
 // (The workgroups of parts that a tile does not have end at once.)
 constexpr int64_t kFullGrid = 6 * kNumCUs;
 // (WINDOW: tiles are of one length, so that there is nothing to deal out, and those that fill the chip once are left as they are: forward and gradients of 12728 positions, window 1024, 32 heads on 8,
-// 1110 us, cut by the rule of the others 1210.)
+// 1110 us, cut by the rule of the others 1210, both before dS had a second operand in dq.)
 inline int most_parts(int64_t tiles, int64_t longest, int least, bool window = false, int64_t grid = kFullGrid) {
     int64_t parts = window ? kAtOnce / tiles : (grid + tiles - 1) / tiles;
     parts = parts < 16 ? parts : 16;
