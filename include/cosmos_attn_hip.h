@@ -466,7 +466,8 @@ COSMOS_ATTN_API int cosmos_attn_ragged_window_bwd(const cosmos_attn_ragged_desc 
  * cosmos_attn_cache_read: the first cu[i + 1] - cu[i] positions of sequence i to the rows cu[i] .. of k_rows and v_rows, code * scale rounded to `dtype`; rows of no sequence are left as
  *     they are, or with `fill` become zeros.
  * cosmos_attn_cache_attention: o[i] = softmax(sm_scale q[i] K^T) V over the first lens[i] positions, q, o [B, Hq, D], query head h on key head h / (Hq / Hkv); lse [B, Hq] fp32 or NULL.
- *     lens[i] == 0: o = 0, lse = -inf.  The workspace holds sums of the sequences that several workgroups share; the bytes follow from the sizes alone.
+ *     lens[i] == 0: o = 0, lse = -inf.  The workspace holds sums of the sequences that several workgroups share; the bytes follow from the sizes alone.  o may be q itself, and has no other memory in common
+ *     with it (refused).  fp16 over 8 bits: each key's weight times its values is good to 2^-25 of the largest value that the token sees, beside its roundings.
  */
 enum cosmos_attn_cache_kind { COSMOS_ATTN_CACHE_SAME = 0, COSMOS_ATTN_CACHE_E4M3 = 1, COSMOS_ATTN_CACHE_INT8 = 2 };
 typedef struct cosmos_attn_cache_desc {
@@ -502,12 +503,12 @@ COSMOS_ATTN_API int cosmos_attn_cache_attention(const cosmos_attn_cache_desc *de
 
 /*
  * cosmos_attn_cache_window: cosmos_attn_cache_attention where the token, at position lens[i] - 1, sees the last `window` positions, its own among them, and those below `sinks` (window 0: all).
- *     Pages without a position that is seen are not looked up: their entries of the table may be anything.
+ *     Pages without a position that is seen are not looked up: their entries of the table may be anything.  The workspace's bytes follow from the sizes, the window and the cache's kind.
  * cosmos_attn_cache_chunk: attention of several tokens of each sequence, q, o [rows, Hq, D]; sequence i's are the rows cu[i] .. cu[i + 1] - 1, its last positions of lens[i], written before the call.
  *     The token at position p sees the positions j <= p, with a window those with j > p - window or j < sinks; pages that none of a sequence's tokens sees are not looked up.  lse [rows, Hq]
  *     fp32 or NULL.  A row that sees nothing (lens[i] below its rows): o = 0, lse = -inf.  A length below 0 or that the table does not hold: NaN; a page outside of the cache: NaN for the rows
  *     that see it.  Rows of no sequence as `fill` says (enum cosmos_attn_ragged_fill); offsets as in cosmos_attn_ragged.  Values that a row does not see have to be finite where another row of its
- *     sequence in the call sees them.
+ *     sequence in the call sees them.  o and q, and fp16 over 8 bits, as in cosmos_attn_cache_attention.
  */
 COSMOS_ATTN_API size_t cosmos_attn_cache_window_workspace_bytes(const cosmos_attn_cache_desc *desc, int64_t window, int64_t sinks);
 COSMOS_ATTN_API int cosmos_attn_cache_window(const cosmos_attn_cache_desc *desc, int64_t window, int64_t sinks, void *workspace, size_t workspace_bytes, void *stream);
