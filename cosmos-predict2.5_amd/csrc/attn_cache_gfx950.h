@@ -166,14 +166,18 @@ bool meet_in_memory(Packed a, Packed b, int64_t rows, int D) {
     auto extent = [&](Packed x) { return (__int128)(one_row ? 0 : rows - 1) * x.stride[0] + (__int128)(x.heads - 1) * x.stride[1] + D; };
     const __int128 between = ((__int128)reinterpret_cast<uintptr_t>(b.at) - (__int128)reinterpret_cast<uintptr_t>(a.at)) / 2;      // elements from a's first row to b's (of 16-byte steps)
     if (between >= extent(a) || -between >= extent(b)) return false;
-    if (!one_row && a.stride[0] != b.stride[0]) return true;
-    const int64_t step = one_row ? 0 : a.stride[0];
+    if (extent(a) >> 62 || extent(b) >> 62 || (!one_row && a.stride[0] != b.stride[0])) return true;
+    const int64_t step = one_row ? 0 : a.stride[0], d0 = (int64_t)between, ea = (a.heads - 1) * a.stride[1] + D, eb = (b.heads - 1) * b.stride[1] + D;
+    // parts of wider rows, the most frequent case: b's lies between a's and the next row's
+    if (step > 0) {
+        const int64_t in = (d0 % step + step) % step;
+        if (in >= ea && in + eb <= step) return false;
+    }
     for (int i = 0; i < a.heads; ++i)
         for (int j = 0; j < b.heads; ++j) {
-            const __int128 d = between + (__int128)j * b.stride[1] - (__int128)i * a.stride[1];
-            // some row of b, `n` rows behind one of a, is less than a row's D elements from it
-            const __int128 n = step ? -d / step : 0;
-            for (__int128 k = n - 1; k <= n + 1; ++k)
+            const int64_t d = d0 + j * b.stride[1] - i * a.stride[1], n = step ? -d / step : 0;
+            // some row of b, `k` rows behind one of a, is less than a row's D elements from it
+            for (int64_t k = n - 1; k <= n + 1; ++k)
                 if (k < rows && -k < rows && d + k * step < D && -(d + k * step) < D) return true;
         }
     return false;
